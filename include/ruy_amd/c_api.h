@@ -44,6 +44,10 @@ enum {
   RUYAMD_DTYPE_I32 = 4,
   RUYAMD_DTYPE_F32 = 5,
   RUYAMD_DTYPE_F64 = 6,
+  /* 16-bit floating point: bfloat16 and IEEE half. Operands and destinations of
+   * ruyamd_mul_grouped, ruyamd_mul_grouped_depth and ruyamd_mul_int4 only. */
+  RUYAMD_DTYPE_BF16 = 7,
+  RUYAMD_DTYPE_F16 = 8,
 };
 
 /* Values of ruy::CachePolicy (ruy/matrix.h:117-122). */
@@ -94,6 +98,10 @@ enum {
                                   one, v_mfma_i32_16x16x64_i8 for 2..16 */
   RUYAMD_KERNEL_I8I16_MFMA = 5,/* int8 x int16 as two int8 MFMA planes */
   RUYAMD_KERNEL_F32_GEMV = 6,  /* fp32 skinny kernels, narrow side <= 16 */
+  RUYAMD_KERNEL_GROUPED_MFMA = 7,   /* grouped products on tiles, matrix cores */
+  RUYAMD_KERNEL_GROUPED_STREAM = 8, /* grouped products of a few columns a group:
+                                       every weight read once, matrix cores */
+  RUYAMD_KERNEL_INT4_STREAM = 9,    /* 4-bit weights, read once, matrix cores */
 };
 
 /* Type-erased, non-owning matrix view: the fields of ruy::Matrix<T>
@@ -198,6 +206,102 @@ RUYAMD_API int ruyamd_mul_no_alloc(ruyamd_ctx* ctx, const ruyamd_mat* lhs,
                                    const ruyamd_mat* rhs,
                                    const ruyamd_mul_params* params,
                                    const ruyamd_mat* dst);
+
+/* ---- Products for layers of experts (no counterpart in the reference) ----
+ *
+ * A layer of experts multiplies every token by the weight matrix of the expert
+ * that the token was sent to. With the tokens sorted by expert these are
+ * products whose columns, or in the weights' gradients whose depth, are dealt
+ * to groups of any size, and the sizes are known on the device only. */
+
+/* Group g has the columns (ruyamd_mul_grouped, ruyamd_mul_int4) or the depth
+ * positions (ruyamd_mul_grouped_depth) [offsets[g], offsets[g + 1]).
+ * `offsets` is device memory, count + 1 values that do not decrease, each
+ * between 0 and the number of columns (of depth positions); they are read when
+ * the call's kernels run. Kernels hold every value to that range and take a
+ * group that would end before it begins for an empty one, so other values give
+ * other results but no access outside the caller's matrices. */
+typedef struct ruyamd_groups {
+  const int32_t* offsets;
+  int32_t count;         /* 1 .. 65536 */
+  int32_t reserved;
+  int64_t matrix_stride; /* elements from one group's matrix (lhs, or dst of
+                            ruyamd_mul_grouped_depth) to the next one's; 0: one
+                            right behind the other */
+  int64_t bias_stride;   /* values from one group's bias to the next one's; 0:
+                            one right behind the other */
+} ruyamd_groups;
+
+/* dst[:, c] = clamp(lhs_g * rhs[:, c] + bias_g) for every column c of every
+ * group g; columns that belong to no group are left as they are. `lhs`
+ * describes the first group's matrix, the others lie groups->matrix_stride
+ * apart. Any storage order, stride and alignment.
+ *
+ * Types: lhs and rhs both bfloat16, both half or both fp32; dst their type or
+ * fp32; accum_dtype fp32. Products are exact, sums are fp32, and the result is
+ * rounded once, when it is stored. `params`: bias (fp32, one value to each row of
+ * dst, or NULL), clamp_min, clamp_max. Multipliers, zero points and a bias to each
+ * column are refused. Cache policies are not looked at.
+ *
+ * Every buffer is device memory. No memory is allocated and nothing is kept from
+ * one call to the next; a call may be recorded into a graph. It returns when dst
+ * is complete, or once it is enqueued after ruyamd_ctx_set_synchronous(ctx, 0).
+ *
+ * The gradient of the columns of rhs is this product with lhs's storage order
+ * exchanged (and its rows with its columns) and the gradient of dst as rhs. */
+RUYAMD_API int ruyamd_mul_grouped(ruyamd_ctx* ctx, const ruyamd_mat* lhs,
+                                  const ruyamd_mat* rhs,
+                                  const ruyamd_groups* groups,
+                                  const ruyamd_mul_params* params,
+                                  const ruyamd_mat* dst);
+
+/* dst_g = clamp(lhs[:, range of g] * rhs[range of g, :]) for every group g: the
+ * gradient of every group's matrix from the gradient of dst (lhs) and the
+ * transposed columns (rhs) of ruyamd_mul_grouped. A group without depth gets
+ * the (clamped) product of nothing, zeros. `dst` describes the first group's
+ * matrix, the others lie groups->matrix_stride apart. Types, memory and calls as
+ * above; there is no bias (its gradient is this product with a column of ones
+ * as rhs). */
+RUYAMD_API int ruyamd_mul_grouped_depth(ruyamd_ctx* ctx, const ruyamd_mat* lhs,
+                                        const ruyamd_mat* rhs,
+                                        const ruyamd_groups* groups,
+                                        const ruyamd_mul_params* params,
+                                        const ruyamd_mat* dst);
+
+/* Weights of 4 bits by rows: the value at (r, c) is
+ *   (q(r, c) - zero_point(r, c / group_size)) * scale(r, c / group_size)
+ * where q(r, c) is the low (c even) or high (c odd) half of byte
+ * data[r * row_bytes + c / 2], an unsigned number, scale(r, i) is
+ * scales[r * scale_stride + i] and zero_point(r, i) is
+ * zero_points[r * scale_stride + i], or 8 without zero points. */
+typedef struct ruyamd_int4_mat {
+  const void* data;
+  const void* scales;         /* of scale_dtype: fp32, bfloat16 or half */
+  const uint8_t* zero_points; /* 0 .. 15, or NULL */
+  int32_t rows;
+  int32_t cols;
+  int32_t group_size;   /* a multiple of 32, or at least cols */
+  int32_t row_bytes;    /* from a row to the next; 0: (cols + 1) / 2 */
+  int32_t scale_stride; /* values from a row to the next; 0: as many as a row has */
+  uint8_t scale_dtype;
+  uint8_t reserved[3];
+  int64_t matrix_bytes;         /* from a group's data to the next one's and */
+  int64_t scales_matrix_stride; /* its scales and zero points (values); 0: one
+                                   right behind the other */
+} ruyamd_int4_mat;
+
+/* dst = clamp(lhs * rhs + bias) with 4-bit weights and a few columns, such as
+ * the tokens of a decoding step: every weight is read once to each 16 to 64
+ * columns. With `groups` (not NULL) there is a weight matrix to each group, as
+ * in ruyamd_mul_grouped (whose matrix_stride is not looked at here). rhs:
+ * bfloat16, half or fp32, any order; dst its type or fp32; products with the
+ * whole-numbered part of the weights are exact, sums are fp32, a group's scale is
+ * applied to its sum. Parameters, memory and calls as in ruyamd_mul_grouped. */
+RUYAMD_API int ruyamd_mul_int4(ruyamd_ctx* ctx, const ruyamd_int4_mat* lhs,
+                               const ruyamd_mat* rhs,
+                               const ruyamd_groups* groups,
+                               const ruyamd_mul_params* params,
+                               const ruyamd_mat* dst);
 
 /* Stream control. By default a context owns a stream and every ruyamd_mul
  * synchronises it before returning, which is ruy::Mul's contract

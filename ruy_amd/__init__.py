@@ -10,6 +10,7 @@ _API_NAMES = (
     "Order", "CachePolicy", "ChannelDimension", "Path", "Layout", "Matrix",
     "MulParams", "Context", "RuyAmdError", "mul", "make_simple_layout",
     "offset", "storage_elements",
+    "Groups", "Int4Matrix", "mul_grouped", "mul_grouped_depth", "mul_int4",
 )
 
 

@@ -32,6 +32,7 @@ lib = C.CDLL(LIB_PATH)
 _ctx = C.c_void_p
 _matp = C.POINTER(S.Mat)
 _parp = C.POINTER(S.MulParamsStruct)
+_grpp = C.POINTER(S.Groups)
 
 PROTOTYPES = {
     "ruyamd_ctx_create": (C.c_int, [C.POINTER(C.c_void_p)]),
@@ -39,6 +40,9 @@ PROTOTYPES = {
     "ruyamd_mul": (C.c_int, [_ctx, _matp, _matp, _parp, _matp]),
     "ruyamd_mul_batch": (C.c_int, [_ctx, C.c_int, _matp, _matp, _parp, _matp]),
     "ruyamd_mul_no_alloc": (C.c_int, [_ctx, _matp, _matp, _parp, _matp]),
+    "ruyamd_mul_grouped": (C.c_int, [_ctx, _matp, _matp, _grpp, _parp, _matp]),
+    "ruyamd_mul_grouped_depth": (C.c_int, [_ctx, _matp, _matp, _grpp, _parp, _matp]),
+    "ruyamd_mul_int4": (C.c_int, [_ctx, C.POINTER(S.Int4Mat), _matp, _grpp, _parp, _matp]),
     "ruyamd_ctx_set_stream": (C.c_int, [_ctx, C.c_void_p]),
     "ruyamd_ctx_set_synchronous": (C.c_int, [_ctx, C.c_int]),
     "ruyamd_ctx_synchronize": (C.c_int, [_ctx]),

@@ -126,7 +126,8 @@ class MulParams:
 
     def __init__(self, accum_dtype, dst_dtype):
         self.accum_dtype, self.dst_dtype = accum_dtype, dst_dtype
-        fp_dst = dst_dtype in (S.F32, S.F64)
+        # (bfloat16 and half: destinations of mul_grouped, mul_grouped_depth, mul_int4.)
+        fp_dst = dst_dtype in (S.F32, S.F64, S.BF16, S.F16)
         if fp_dst != (accum_dtype in (S.F32, S.F64)):
             raise ValueError("floating-point Dst requires floating-point Accum and vice versa")
         if not fp_dst and accum_dtype != S.I32:
@@ -224,6 +225,43 @@ class MulParams:
         p.channel_dimension = self.channel_dimension
         p.perchannel_buffers_capacity_rounding_log2 = self._rounding_log2
         return p
+
+
+class Groups:
+    """ruyamd_groups: the columns (or depth positions) of a product dealt to
+    `count` groups, group g from offsets[g] up to offsets[g + 1]. `offsets`:
+    int32 device memory; strides of 0: one group's matrix (bias) right behind
+    the other's."""
+
+    def __init__(self, offsets, count, matrix_stride=0, bias_stride=0):
+        self.offsets, self.count = offsets, count
+        self.matrix_stride, self.bias_stride = matrix_stride, bias_stride
+
+    def to_struct(self):
+        g = S.Groups()
+        g.offsets, g.count = _address(self.offsets), self.count
+        g.matrix_stride, g.bias_stride = self.matrix_stride, self.bias_stride
+        return g
+
+
+class Int4Matrix:
+    """ruyamd_int4_mat: 4-bit weights by rows, two to a byte, with a scale (and
+    a zero point, 8 without them) to every `group_size` columns of a row."""
+
+    def __init__(self, rows, cols, group_size, data, scales, scale_dtype, zero_points=None, row_bytes=0,
+                 scale_stride=0, matrix_bytes=0, scales_matrix_stride=0):
+        self.rows, self.cols, self.group_size = rows, cols, group_size
+        self.data, self.scales, self.scale_dtype, self.zero_points = data, scales, scale_dtype, zero_points
+        self.row_bytes, self.scale_stride = row_bytes, scale_stride
+        self.matrix_bytes, self.scales_matrix_stride = matrix_bytes, scales_matrix_stride
+
+    def to_struct(self):
+        m = S.Int4Mat()
+        m.data, m.scales, m.zero_points = _address(self.data), _address(self.scales), _address(self.zero_points)
+        m.rows, m.cols, m.group_size = self.rows, self.cols, self.group_size
+        m.row_bytes, m.scale_stride, m.scale_dtype = self.row_bytes, self.scale_stride, self.scale_dtype
+        m.matrix_bytes, m.scales_matrix_stride = self.matrix_bytes, self.scales_matrix_stride
+        return m
 
 
 class RuyAmdError(RuntimeError):
@@ -392,5 +430,41 @@ def mul(lhs, rhs, mul_params, context, dst):
     context._check(lib.ruyamd_mul(context._h, C.byref(l), C.byref(r), C.byref(p), C.byref(d)))
 
 
+def _call_with_groups(which, lhs, rhs, groups, mul_params, context, dst):
+    """ruyamd_mul_grouped, ruyamd_mul_grouped_depth or ruyamd_mul_int4 (`which` 0, 1, 2)."""
+    rc = native.mul_with_groups(which, lhs, rhs, groups, mul_params, context._address, dst) if native else None
+    if rc is not None:
+        if rc:
+            context._check(rc)
+        return
+    # As in mul: what the native path does not take.
+    if mul_params.dst_dtype != dst.dtype:
+        raise ValueError("MulParams DstScalar does not match the destination matrix")
+    l, r, d = lhs.to_struct(), rhs.to_struct(), dst.to_struct()
+    p = mul_params.to_struct()
+    g = C.byref(groups.to_struct()) if groups is not None else None
+    context._check(_WITH_GROUPS[which](context._h, C.byref(l), C.byref(r), g, C.byref(p), C.byref(d)))
+
+
+_WITH_GROUPS = (lib.ruyamd_mul_grouped, lib.ruyamd_mul_grouped_depth, lib.ruyamd_mul_int4)
+
+
+def mul_grouped(lhs, rhs, groups, mul_params, context, dst):
+    """dst[:, c] = clamp(lhs of c's group * rhs[:, c] + bias) (ruyamd_mul_grouped)."""
+    _call_with_groups(0, lhs, rhs, groups, mul_params, context, dst)
+
+
+def mul_grouped_depth(lhs, rhs, groups, mul_params, context, dst):
+    """dst of g = clamp(lhs[:, range of g] * rhs[range of g, :]) (ruyamd_mul_grouped_depth)."""
+    _call_with_groups(1, lhs, rhs, groups, mul_params, context, dst)
+
+
+def mul_int4(lhs, rhs, mul_params, context, dst, groups=None):
+    """dst = clamp(lhs * rhs + bias) with an Int4Matrix for lhs, or one to each
+    of `groups` (ruyamd_mul_int4)."""
+    _call_with_groups(2, lhs, rhs, groups, mul_params, context, dst)
+
+
 if native:
+    native.bind_with_groups([C.cast(f, C.c_void_p).value for f in _WITH_GROUPS], Groups, Int4Matrix)
     native.bind(C.cast(lib.ruyamd_mul, C.c_void_p).value, Matrix, Layout, MulParams)

@@ -25,10 +25,19 @@ PyTypeObject* matrix_type = nullptr;
 PyTypeObject* layout_type = nullptr;
 PyTypeObject* params_type = nullptr;
 
+template <typename Lhs>
+using GroupedFunction = int (*)(ruyamd_ctx*, const Lhs*, const ruyamd_mat*, const ruyamd_groups*,
+                                const ruyamd_mul_params*, const ruyamd_mat*);
+uintptr_t grouped_functions[3] = {};  // ruyamd_mul_grouped, ruyamd_mul_grouped_depth, ruyamd_mul_int4
+PyTypeObject* groups_type = nullptr;
+PyTypeObject* int4_type = nullptr;
+
 #define RUYAMD_NAMES(X)                                                                                        \
   X(dtype) X(data) X(layout) X(zero_point) X(cache_policy) X(rows) X(cols) X(stride) X(order) X(data_ptr)      \
   X(ctypes) X(bias) X(_perchannel) X(_mf) X(_me) X(_mf_pc) X(_me_pc) X(clamp_min) X(clamp_max) X(accum_dtype) \
-  X(dst_dtype) X(channel_dimension) X(_rounding_log2)
+  X(dst_dtype) X(channel_dimension) X(_rounding_log2) X(offsets) X(count) X(matrix_stride) X(bias_stride)      \
+  X(group_size) X(scales) X(scale_dtype) X(zero_points) X(row_bytes) X(scale_stride) X(matrix_bytes)          \
+  X(scales_matrix_stride)
 #define RUYAMD_DECLARE(name) PyObject* name_##name;
 RUYAMD_NAMES(RUYAMD_DECLARE)
 
@@ -191,6 +200,113 @@ PyObject* Mul(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return PyLong_FromLong(rc);
 }
 
+Outcome Groups(PyObject* object, ruyamd_groups* g) {
+  if (Py_TYPE(object) != groups_type) return kNotHandled;
+  const Ref dict = DictOf(object);
+  const Ref offsets = Field(dict, name_offsets);
+  uint64_t count, matrix_stride, bias_stride;
+  if (!offsets || !Integer(dict, name_count, &count) || !Integer(dict, name_matrix_stride, &matrix_stride) ||
+      !Integer(dict, name_bias_stride, &bias_stride))
+    return kNotHandled;
+  g->count = static_cast<int32_t>(count);
+  g->reserved = 0;
+  g->matrix_stride = static_cast<int64_t>(matrix_stride);
+  g->bias_stride = static_cast<int64_t>(bias_stride);
+  void* address = nullptr;
+  if (Outcome o = Address(offsets, &address)) return o;
+  g->offsets = static_cast<const int32_t*>(address);
+  return kDone;
+}
+
+Outcome Int4(PyObject* object, ruyamd_int4_mat* m) {
+  if (Py_TYPE(object) != int4_type) return kNotHandled;
+  const Ref dict = DictOf(object);
+  const Ref data = Field(dict, name_data);
+  const Ref scales = Field(dict, name_scales);
+  const Ref zero_points = Field(dict, name_zero_points);
+  uint64_t rows, cols, group_size, row_bytes, scale_stride, scale_dtype, matrix_bytes, scales_matrix_stride;
+  if (!data || !scales || !zero_points || !Integer(dict, name_rows, &rows) || !Integer(dict, name_cols, &cols) ||
+      !Integer(dict, name_group_size, &group_size) || !Integer(dict, name_row_bytes, &row_bytes) ||
+      !Integer(dict, name_scale_stride, &scale_stride) || !Integer(dict, name_scale_dtype, &scale_dtype) ||
+      !Integer(dict, name_matrix_bytes, &matrix_bytes) ||
+      !Integer(dict, name_scales_matrix_stride, &scales_matrix_stride))
+    return kNotHandled;
+  std::memset(m, 0, sizeof(*m));
+  m->rows = static_cast<int32_t>(rows);
+  m->cols = static_cast<int32_t>(cols);
+  m->group_size = static_cast<int32_t>(group_size);
+  m->row_bytes = static_cast<int32_t>(row_bytes);
+  m->scale_stride = static_cast<int32_t>(scale_stride);
+  m->scale_dtype = static_cast<uint8_t>(scale_dtype);
+  m->matrix_bytes = static_cast<int64_t>(matrix_bytes);
+  m->scales_matrix_stride = static_cast<int64_t>(scales_matrix_stride);
+  void* address = nullptr;
+  if (Outcome o = Address(data, &address)) return o;
+  m->data = address;
+  if (Outcome o = Address(scales, &address)) return o;
+  m->scales = address;
+  if (Outcome o = Address(zero_points, &address)) return o;
+  m->zero_points = static_cast<const uint8_t*>(address);
+  return kDone;
+}
+
+// mul_with_groups(which, lhs, rhs, groups, mul_params, context address, dst): as
+// Mul, of the function number `which`.
+PyObject* MulWithGroups(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  const long which = count == 7 && PyLong_Check(args[0]) ? PyLong_AsLong(args[0]) : -1;
+  if (which < 0 || which > 2 || !grouped_functions[which]) {
+    PyErr_SetString(PyExc_TypeError,
+                    "mul_with_groups(which, lhs, rhs, groups, mul_params, context address, dst)");
+    return nullptr;
+  }
+  ruyamd_mat lhs, rhs, dst;
+  ruyamd_int4_mat int4;
+  ruyamd_groups groups;
+  ruyamd_mul_params params;
+  uint64_t dst_dtype = 0;
+  const bool has_groups = args[3] != Py_None;
+  Outcome o = Params(args[4], &params, &dst_dtype);
+  if (o == kDone) o = which == 2 ? Int4(args[1], &int4) : Matrix(args[1], &lhs);
+  if (o == kDone) o = Matrix(args[2], &rhs);
+  if (o == kDone && has_groups) o = Groups(args[3], &groups);
+  if (o == kDone) o = Matrix(args[6], &dst);
+  if (o == kError) return nullptr;
+  if (o == kNotHandled || dst_dtype != dst.dtype || !PyLong_Check(args[5])) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  ruyamd_ctx* ctx = reinterpret_cast<ruyamd_ctx*>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLongMask(args[5])));
+  const ruyamd_groups* g = has_groups ? &groups : nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  if (which == 2)
+    rc = reinterpret_cast<GroupedFunction<ruyamd_int4_mat>>(grouped_functions[2])(ctx, &int4, &rhs, g, &params, &dst);
+  else
+    rc = reinterpret_cast<GroupedFunction<ruyamd_mat>>(grouped_functions[which])(ctx, &lhs, &rhs, g, &params, &dst);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// bind_with_groups([addresses of the three functions], Groups, Int4Matrix)
+PyObject* BindWithGroups(PyObject*, PyObject* args) {
+  PyObject *addresses, *groups, *int4;
+  if (!PyArg_ParseTuple(args, "O!O!O!", &PyList_Type, &addresses, &PyType_Type, &groups, &PyType_Type, &int4))
+    return nullptr;
+  if (PyList_GET_SIZE(addresses) != 3) {
+    PyErr_SetString(PyExc_ValueError, "three addresses");
+    return nullptr;
+  }
+  for (int i = 0; i < 3; ++i) {
+    const unsigned long long address = PyLong_AsUnsignedLongLong(PyList_GET_ITEM(addresses, i));
+    if (PyErr_Occurred()) return nullptr;
+    grouped_functions[i] = static_cast<uintptr_t>(address);
+  }
+  for (PyObject* t : {groups, int4}) Py_INCREF(t);
+  groups_type = reinterpret_cast<PyTypeObject*>(groups);
+  int4_type = reinterpret_cast<PyTypeObject*>(int4);
+  Py_RETURN_NONE;
+}
+
 // bind(address of ruyamd_mul, Matrix, Layout, MulParams)
 PyObject* Bind(PyObject*, PyObject* args) {
   unsigned long long address = 0;
@@ -208,6 +324,9 @@ PyObject* Bind(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     {"mul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Mul)), METH_FASTCALL, nullptr},
     {"bind", Bind, METH_VARARGS, nullptr},
+    {"mul_with_groups", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(MulWithGroups)), METH_FASTCALL,
+     nullptr},
+    {"bind_with_groups", BindWithGroups, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
