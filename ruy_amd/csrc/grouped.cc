@@ -131,8 +131,13 @@ int Run(ruyamd_ctx* ctx, grouped::Call* call, const grouped::Int4* weights) {
   }
   ctx->capturing = status == hipStreamCaptureStatusActive;
   const bool timed = ctx->TimingBegin();
-  const hipError_t launched = grouped::LaunchGeneric(ctx->stream, *call, weights);
-  ctx->last_kernel = RUYAMD_KERNEL_GENERIC;
+  hipError_t launched = hipSuccess;
+  if (!ctx->force_generic && !weights && grouped::LaunchTiles(ctx->stream, *call, &launched)) {
+    ctx->last_kernel = RUYAMD_KERNEL_GROUPED_MFMA;
+  } else {
+    launched = grouped::LaunchGeneric(ctx->stream, *call, weights);
+    ctx->last_kernel = RUYAMD_KERNEL_GENERIC;
+  }
   if (timed) ctx->TimingEnd();
   const bool wait = ctx->synchronous && !ctx->capturing;
   ctx->capturing = false;

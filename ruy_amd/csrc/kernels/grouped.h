@@ -50,6 +50,10 @@ struct Int4 {
 // tested against it, and it takes what they do not.)
 hipError_t LaunchGeneric(hipStream_t stream, const Call& call, const Int4* weights);
 
+// Tiles of the destination on the matrix cores (grouped_gemm.h). False: the call is
+// not one for this kernel, and nothing was launched.
+bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status);
+
 }  // namespace grouped
 }  // namespace ruyamd
 

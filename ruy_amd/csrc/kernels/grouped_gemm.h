@@ -1,0 +1,477 @@
+// Grouped products on tiles of the destination, on the matrix cores.
+//
+// A workgroup makes one tile of one group's product: kTileM x kTileN elements,
+// the M side the one along which the destination is contiguous. Each operand
+// comes in steps of 128 bytes of depth (64 values of 16 bits, 32 of 32) through
+// LDS, in the order in which it lies in memory: runs along the depth (kPlain) or
+// along the tile's side (kAcross, such as the weights in a token gradient and both
+// operands of a weight gradient). Fragments of the latter come out of LDS through
+// the transposing reads of gfx950, so no operand is ever copied for its order.
+#ifndef RUY_AMD_CSRC_KERNELS_GROUPED_GEMM_H_
+#define RUY_AMD_CSRC_KERNELS_GROUPED_GEMM_H_
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+#include <utility>
+
+#include "granule.h"
+#include "grouped_device.h"
+
+namespace ruyamd {
+namespace grouped {
+
+using granule::v4i;
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+enum class Runs { kPlain, kAcross };
+
+// One side of the product as a workgroup's tile sees it.
+struct Side {
+  const void* data = nullptr;
+  int64_t pitch = 0;         // values from a run to the next
+  int64_t group_stride = 0;  // values from a group's matrix to the next one's
+  int count = 0;             // rows (columns) of the side, over all groups where they are dealt
+};
+
+struct GemmArgs {
+  Dealt dealt;
+  Side m, n;
+  void* dst;
+  int64_t dst_m_stride, dst_n_stride, dst_group_stride;
+  const int32_t* offsets;
+  int groups, depth;  // depth: over all groups where it is dealt
+  const float* bias;  // one value to each place of the M side
+  int64_t bias_stride;
+  float clamp_min, clamp_max;
+  int dst_f32;
+  int vector_stores;  // 4 values of the destination's M side lie side by side, aligned
+};
+
+// f(std::integral_constant<int, 0>()), ..., f(std::integral_constant<int, N - 1>()).
+template <class F, int... Is>
+__device__ __forceinline__ void StaticForEach(F&& f, std::integer_sequence<int, Is...>) {
+  (f(std::integral_constant<int, Is>()), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void StaticFor(F&& f) {
+  StaticForEach(f, std::make_integer_sequence<int, N>());
+}
+
+// 64 lanes x 16 bytes from the lanes' offsets to 1024 bytes of LDS, on their way
+// until vmcnt says otherwise. Offsets at or past the end of `rsrc` bring zeros.
+__device__ __forceinline__ void LoadToLds(uint32_t lds, uint32_t voffset, v4i rsrc) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(voffset), "s"(rsrc)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void WaitVmcnt() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void Barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// What a lane's offset is set to for zeros; offsets inside a tile stay below it.
+constexpr uint32_t kNothing = 0x80000000u;
+__device__ __forceinline__ v4i Resource(const char* base) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  v4i r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(a & 0xffffffffu));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>((a >> 32) & 0xffffu));
+  r[2] = static_cast<int>(kNothing);
+  r[3] = 0x00020000;
+  return r;
+}
+
+template <int kType>
+struct Element {
+  static constexpr int kBytes = kType == RUYAMD_DTYPE_F32 ? 4 : 2;
+  static constexpr int kDepth = 128 / kBytes;     // depth positions to a step
+  static constexpr int kGranule = 16 / kBytes;    // values to 16 bytes
+};
+
+// Two fragments of 16 bytes: 16 rows x 16 columns x 4 granules of depth.
+template <int kType>
+__device__ __forceinline__ void Mma(const v4i& a, const v4i& b, v4f& acc) {
+  if constexpr (kType == RUYAMD_DTYPE_BF16) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), acc, 0, 0, 0);
+  } else if constexpr (kType == RUYAMD_DTYPE_F16) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(a[e]), __int_as_float(b[e]), acc, 0, 0, 0);
+  }
+}
+
+// One side of the tile: how it is laid out in LDS, loaded and read. `kRows` rows
+// of the tile in `kWaveRows`-row pieces, one to a wave, of kBlocks blocks of 16.
+template <int kType, Runs kRuns, int kRows, int kBlocks, bool kPermuted, int kWaves>
+struct TileSide {
+  using E = Element<kType>;
+  static constexpr int kBytes = kRows * 128;                 // in LDS, per step
+  static constexpr int kLoads = kBytes / 1024 / kWaves;      // per wave and step
+  static constexpr int kRunGranules = kRuns == Runs::kPlain ? 8 : kRows / E::kGranule;
+  static constexpr int kRunsPerLoad = 64 / kRunGranules;     // (0: a run takes several loads)
+  static constexpr int kWaveRows = 16 * kBlocks;
+  static_assert(kBytes % (1024 * kWaves) == 0, "");
+
+  // Row of the wave's piece that lane l (mod 16) holds of block b. Where the rows
+  // are permuted a lane of the accumulators has 4 * kBlocks consecutive ones.
+  static __device__ __forceinline__ int RowOf(int b, int l) {
+    return kPermuted ? (l >> 2) * 4 * kBlocks + b * 4 + (l & 3) : b * 16 + l;
+  }
+
+  // Granule g of run r is stored in slot g ^ Key(r): lanes that read LDS together
+  // then reach all banks.
+  static __device__ __forceinline__ int Key(int r) {
+    if constexpr (kRuns == Runs::kPlain) {
+      if constexpr (kPermuted) return ((r >> 1) & 1) | ((r / (4 * kBlocks)) & 3) << 1;
+      return (r >> 1) & 7;
+    } else if constexpr (E::kBytes == 2) {
+      // Reads of 4 consecutive runs of each of 4 groups of 8, 32 bytes of each.
+      return (((r & 3) | ((r >> 3) & 3) << 2) << 1) & (kRunGranules - 1);
+    } else {
+      return (r >> 2) & 3;
+    }
+  }
+
+  // Where load number n of a wave puts what lane `lane` brings: run and granule.
+  static __device__ __forceinline__ int RunOf(int n, int wave, int lane) {
+    return ((n * kWaves + wave) * 64 + lane) / kRunGranules;
+  }
+  static __device__ __forceinline__ int GranuleOf(int n, int wave, int lane) {
+    return (((n * kWaves + wave) * 64 + lane) % kRunGranules) ^ Key(RunOf(n, wave, lane));
+  }
+
+  // The fragment of block b and depth half kk (0, 1) from the side's LDS; `piece`: the wave's.
+  static __device__ __forceinline__ v4i Fragment(const char* lds, int piece, int b, int kk, int lane) {
+    const int l = lane & 15, q = lane >> 4;
+    if constexpr (kRuns == Runs::kPlain) {
+      const int r = piece * kWaveRows + RowOf(b, l);
+      return *reinterpret_cast<const v4i*>(lds + r * 128 + (((kk * 4 + q) ^ Key(r)) << 4));
+    } else if constexpr (E::kBytes == 2) {
+      // (A read hands lane l of 16 the l-th column of the 4 runs x 16 values
+      // that the 16 lanes point at, 4 values each.)
+      v4s half[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int run = kk * 32 + q * 8 + h * 4 + (l >> 2);
+        const int at = piece * kWaveRows + RowOf(b, (l & 3) * 4);
+        const char* p = lds + run * (kRows * 2) + (((at >> 3) ^ Key(run)) << 4) + (at & 7) * 2;
+        half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) v4s*)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
+      }
+      return __builtin_bit_cast(v4i, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      v4i f;
+      const int at = piece * kWaveRows + RowOf(b, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int run = kk * 16 + q * 4 + e;
+        f[e] = *reinterpret_cast<const int*>(lds + run * (kRows * 4) + (((at >> 2) ^ Key(run)) << 4) + (at & 3) * 4);
+      }
+      return f;
+    }
+  }
+};
+
+// The range of a group that is the same for the whole wave, in scalar registers.
+__device__ __forceinline__ Range UniformRangeOf(const int32_t* offsets, int group, int total) {
+  const Range r = RangeOf(offsets, group, total);
+  return {__builtin_amdgcn_readfirstlane(r.begin), __builtin_amdgcn_readfirstlane(r.count)};
+}
+
+// The tile a workgroup makes: its group, and which along either side.
+struct TileOf {
+  int group, m, n;
+};
+
+// Tiles of groups whose columns are dealt: how many a group has is known here only.
+// Workgroups go round the eight XCDs one by one; each XCD gets a contiguous
+// run of the tiles, so that what its L2 holds serves several of them. Tiles of a
+// group go in bands of kBand along the N side.
+constexpr int kBand = 8;
+template <int kTileN>
+__device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int columns, int tiles_m, TileOf* tile,
+                                         Range* range) {
+  const int lane = threadIdx.x & 63;
+  const auto tiles_of = [&](int g) __attribute__((always_inline)) {
+    if (g >= groups) return 0;
+    return (RangeOf(offsets, g, columns).count + kTileN - 1) / kTileN;
+  };
+  int total = 0, first = 0;
+  for (int g = lane; g < groups; g += 64) {
+    const int tiles = tiles_of(g);
+    total += tiles;
+    if (g == lane) first = tiles;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+  total = __builtin_amdgcn_readfirstlane(total);
+  // (int64_t: tiles of many groups times those of many rows.)
+  const int64_t all = int64_t(total) * tiles_m, per_xcd = (all + 7) / 8;
+  const int64_t place = blockIdx.x >> 3;
+  const int64_t t = int64_t(blockIdx.x & 7) * per_xcd + place;
+  if (place >= per_xcd || t >= all) return false;
+  int64_t before = 0;
+  for (int g0 = 0;; g0 += 64) {
+    const int tiles = g0 == 0 ? first : tiles_of(g0 + lane);
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    const uint64_t past = __ballot((before + upto) * tiles_m > t);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int mine = __builtin_amdgcn_readfirstlane(__shfl(tiles, at));
+      const int64_t group_first = (before + __builtin_amdgcn_readfirstlane(__shfl(upto, at)) - mine) * tiles_m;
+      int in_group = static_cast<int>(t - group_first);
+      const int band = in_group / (kBand * tiles_m), width = min(kBand, mine - band * kBand);
+      in_group -= band * kBand * tiles_m;
+      tile->group = __builtin_amdgcn_readfirstlane(g0 + at);
+      tile->m = __builtin_amdgcn_readfirstlane(in_group / width);
+      tile->n = __builtin_amdgcn_readfirstlane(band * kBand + in_group % width);
+      break;
+    }
+    before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+  }
+  *range = UniformRangeOf(offsets, tile->group, columns);
+  return true;
+}
+
+// kDirect: every run of both operands begins at a multiple of 16 bytes and is a
+// whole number of granules, so that tiles go to LDS without passing through
+// registers. Otherwise they are read 16 bytes a lane from wherever they begin, the
+// granule in which a run ends put in its place (granule.h), and written to LDS.
+template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect>
+__global__ __launch_bounds__(64 * kWavesM * kWavesN) void GroupedGemmKernel(GemmArgs p) {
+  using E = Element<kType>;
+  constexpr int kWaves = kWavesM * kWavesN;
+  constexpr int kTileM = kWavesM * kBlocksM * 16, kTileN = kWavesN * kBlocksN * 16;
+  using M = TileSide<kType, kRunsM, kTileM, kBlocksM, kRunsM == Runs::kPlain, kWaves>;
+  using N = TileSide<kType, kRunsN, kTileN, kBlocksN, false, kWaves>;
+  constexpr int kStage = M::kBytes + N::kBytes;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_m = wave % kWavesM, wave_n = wave / kWavesM;
+  const int tiles_m = (p.m.count + kTileM - 1) / kTileM;
+
+  TileOf tile;
+  Range range;
+  const bool columns = p.dealt == Dealt::kColumns;
+  if (columns) {
+    if (!FindTile<kTileN>(p.offsets, p.groups, p.n.count, tiles_m, &tile, &range)) return;
+  } else {
+    const int tiles_n = (p.n.count + kTileN - 1) / kTileN;
+    const int64_t all = int64_t(p.groups) * tiles_m * tiles_n, per_xcd = (all + 7) / 8, place = blockIdx.x >> 3;
+    const int64_t t = int64_t(blockIdx.x & 7) * per_xcd + place;
+    if (place >= per_xcd || t >= all) return;
+    tile.group = static_cast<int>(t / (tiles_m * tiles_n));
+    int in_group = static_cast<int>(t - int64_t(tile.group) * tiles_m * tiles_n);
+    const int band = in_group / (kBand * tiles_m), width = min(kBand, tiles_n - band * kBand);
+    in_group -= band * kBand * tiles_m;
+    tile.m = in_group / width;
+    tile.n = band * kBand + in_group % width;
+    range = UniformRangeOf(p.offsets, tile.group, p.depth);
+  }
+  const int rows_m = p.m.count, rows_n = columns ? range.count : p.n.count;
+  const int depth = columns ? p.depth : range.count;
+  const int m0 = tile.m * kTileM, n0 = tile.n * kTileN;
+  const int here_m = min(kTileM, rows_m - m0), here_n = min(kTileN, rows_n - n0);
+
+  // The first value of each side's part of the operand.
+  const auto base_of = [&](const Side& s, Runs runs, int first, bool dealt_rows) __attribute__((always_inline)) {
+    int64_t at = columns ? (dealt_rows ? 0 : tile.group * s.group_stride) : 0;
+    int64_t row = first, k = 0;
+    if (columns && dealt_rows) row += range.begin;
+    if (!columns) k = range.begin;
+    at += runs == Runs::kPlain ? row * s.pitch + k : k * s.pitch + row;
+    return static_cast<const char*>(s.data) + at * E::kBytes;
+  };
+  const char* base_m = base_of(p.m, kRunsM, m0, false);
+  const char* base_n = base_of(p.n, kRunsN, n0, true);
+
+  const int steps = (depth + E::kDepth - 1) / E::kDepth;
+
+  v4f acc[kBlocksM][kBlocksN] = {};
+  const auto compute = [&](auto stage) __attribute__((always_inline)) {
+    const char* const side_m = lds + stage * kStage;
+    const char* const side_n = side_m + M::kBytes;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      v4i a[kBlocksM], b[kBlocksN];
+#pragma unroll
+      for (int i = 0; i < kBlocksM; ++i) a[i] = M::Fragment(side_m, wave_m, i, kk, lane);
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j) b[j] = N::Fragment(side_n, wave_n, j, kk, lane);
+#pragma unroll
+      for (int i = 0; i < kBlocksM; ++i)
+#pragma unroll
+        for (int j = 0; j < kBlocksN; ++j) Mma<kType>(a[i], b[j], acc[i][j]);
+    }
+  };
+
+  if constexpr (kDirect) {
+    const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    uint32_t off_m[M::kLoads], off_n[N::kLoads];
+    // A lane's offset of load n, and its first depth position. What lies beyond
+    // the tile's side is read from the side's last row (granule): it ends up
+    // in rows of the tile that are not stored.
+    const auto offset_of = [&](auto side, int n, int here, Runs runs, int64_t pitch) __attribute__((always_inline)) {
+      using T = decltype(side);
+      const int run = T::RunOf(n, wave, lane), granule = T::GranuleOf(n, wave, lane);
+      if (runs == Runs::kPlain)
+        return static_cast<uint32_t>(min(run, here - 1) * pitch * E::kBytes) + granule * 16;
+      return static_cast<uint32_t>(run * pitch * E::kBytes) + min(granule, here / E::kGranule - 1) * 16;
+    };
+    const auto depth_of = [&](auto side, int n, Runs runs) __attribute__((always_inline)) {
+      using T = decltype(side);
+      return runs == Runs::kPlain ? T::GranuleOf(n, wave, lane) * E::kGranule : T::RunOf(n, wave, lane);
+    };
+#pragma unroll
+    for (int n = 0; n < M::kLoads; ++n) off_m[n] = offset_of(M(), n, here_m, kRunsM, p.m.pitch);
+#pragma unroll
+    for (int n = 0; n < N::kLoads; ++n) off_n[n] = offset_of(N(), n, here_n, kRunsN, p.n.pitch);
+    const int64_t step_m = (kRunsM == Runs::kPlain ? 1 : p.m.pitch) * 128;
+    const int64_t step_n = (kRunsN == Runs::kPlain ? 1 : p.n.pitch) * 128;
+    const auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+      const v4i rsrc_m = Resource(base_m + s * step_m), rsrc_n = Resource(base_n + s * step_n);
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_base + stage * kStage + wave * 1024);
+      const int left = depth - s * E::kDepth;
+      if (left >= E::kDepth) {
+#pragma unroll
+        for (int n = 0; n < M::kLoads; ++n) LoadToLds(to + n * kWaves * 1024, off_m[n], rsrc_m);
+#pragma unroll
+        for (int n = 0; n < N::kLoads; ++n) LoadToLds(to + M::kBytes + n * kWaves * 1024, off_n[n], rsrc_n);
+      } else {  // the last, partial step: zeros past the depth
+#pragma unroll
+        for (int n = 0; n < M::kLoads; ++n)
+          LoadToLds(to + n * kWaves * 1024, depth_of(M(), n, kRunsM) < left ? off_m[n] : kNothing, rsrc_m);
+#pragma unroll
+        for (int n = 0; n < N::kLoads; ++n)
+          LoadToLds(to + M::kBytes + n * kWaves * 1024, depth_of(N(), n, kRunsN) < left ? off_n[n] : kNothing, rsrc_n);
+      }
+    };
+    if (steps > 0) issue(0, 0);
+    // A step's loads have landed in every wave, and every wave is done with
+    // the other half of LDS, when all have passed the barrier in front of it.
+    const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
+      WaitVmcnt<0>();
+      Barrier();
+      if (s + 1 < steps) issue(s + 1, 1 - stage);
+      compute(stage);
+    };
+    for (int s = 0; s < steps; s += 2) {
+      step(s, std::integral_constant<int, 0>());
+      if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
+    }
+  } else {
+    // A granule of a run of `length` values that begins at `run`, from place `at`
+    // on, zeros past its end.
+    const auto load = [&](const char* run, int at, int length) __attribute__((always_inline)) -> v4i {
+      const int bytes = length * E::kBytes, k = at * E::kBytes;
+      if (k >= bytes) return v4i{0, 0, 0, 0};
+      if (bytes < 16) return granule::LoadGranule<true>(reinterpret_cast<const uint8_t*>(run), k, bytes);
+      const v4i x = granule::LoadGranule<false>(reinterpret_cast<const uint8_t*>(run), k, bytes);
+      return k + 16 <= bytes ? x : granule::PlaceGranule(x, k, bytes);
+    };
+    const auto side_load = [&](auto side, int n, const char* base, Runs runs, int64_t pitch, int here, int s) __attribute__((always_inline)) -> v4i {
+      using T = decltype(side);
+      const int run = T::RunOf(n, wave, lane), granule = T::GranuleOf(n, wave, lane);
+      const int k0 = s * E::kDepth;
+      if (runs == Runs::kPlain)
+        return load(base + min(run, here - 1) * pitch * E::kBytes, k0 + granule * E::kGranule, depth);
+      if (k0 + run >= depth) return v4i{0, 0, 0, 0};
+      return load(base + (k0 + run) * pitch * E::kBytes, granule * E::kGranule, here);
+    };
+    v4i held_m[M::kLoads], held_n[N::kLoads];
+    const auto fetch = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < M::kLoads; ++n) held_m[n] = side_load(M(), n, base_m, kRunsM, p.m.pitch, here_m, s);
+#pragma unroll
+      for (int n = 0; n < N::kLoads; ++n) held_n[n] = side_load(N(), n, base_n, kRunsN, p.n.pitch, here_n, s);
+    };
+    const auto put = [&](int stage) __attribute__((always_inline)) {
+      char* to = lds + stage * kStage + (wave * 64 + lane) * 16;
+#pragma unroll
+      for (int n = 0; n < M::kLoads; ++n) *reinterpret_cast<v4i*>(to + n * kWaves * 1024) = held_m[n];
+#pragma unroll
+      for (int n = 0; n < N::kLoads; ++n) *reinterpret_cast<v4i*>(to + M::kBytes + n * kWaves * 1024) = held_n[n];
+    };
+    if (steps > 0) {
+      fetch(0);
+      put(0);
+    }
+    const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
+      __syncthreads();
+      if (s + 1 < steps) fetch(s + 1);
+      compute(stage);
+      if (s + 1 < steps) put(1 - stage);
+    };
+    for (int s = 0; s < steps; s += 2) {
+      step(s, std::integral_constant<int, 0>());
+      if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
+    }
+  }
+
+  // Write-back. Lane l holds column l % 16 of each block of the N side and 4
+  // rows (l / 16) * 4 .. of each block of the M side.
+  const int l = lane & 15, q = lane >> 4;
+  const bool f32 = p.dst_f32 != 0, whole = p.vector_stores != 0 && here_m == kTileM;
+  const int64_t group_at = columns ? 0 : tile.group * p.dst_group_stride;
+  const int first_n = columns ? range.begin + n0 : n0;
+  const float* bias = p.bias ? p.bias + tile.group * p.bias_stride + m0 : nullptr;
+#pragma unroll
+  for (int i = 0; i < kBlocksM; ++i) {
+    const int m = wave_m * M::kWaveRows + M::RowOf(i, q * 4);  // (and the three behind it)
+    float add[4] = {};
+    if (bias)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add[e] = m + e < here_m ? bias[m + e] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kBlocksN; ++j) {
+      const int n = wave_n * N::kWaveRows + j * 16 + l;
+      if (n >= here_n) continue;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = Clamp(acc[i][j][e] + add[e], p.clamp_min, p.clamp_max);
+      const int64_t at = group_at + (m0 + m) * p.dst_m_stride + int64_t(first_n + n) * p.dst_n_stride;
+      if (whole) {
+        if (f32) {
+          *reinterpret_cast<v4f*>(static_cast<float*>(p.dst) + at) = v4f{v[0], v[1], v[2], v[3]};
+        } else if constexpr (kType == RUYAMD_DTYPE_BF16) {
+          typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<v4bf*>(static_cast<__bf16*>(p.dst) + at) =
+              v4bf{static_cast<__bf16>(v[0]), static_cast<__bf16>(v[1]), static_cast<__bf16>(v[2]), static_cast<__bf16>(v[3])};
+        } else if constexpr (kType == RUYAMD_DTYPE_F16) {
+          typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<v4h*>(static_cast<_Float16*>(p.dst) + at) =
+              v4h{static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]),
+                  static_cast<_Float16>(v[3])};
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (m + e < here_m) StoreFloat(p.dst, f32 ? RUYAMD_DTYPE_F32 : kType, at + e * p.dst_m_stride, v[e]);
+      }
+    }
+  }
+}
+
+}  // namespace grouped
+}  // namespace ruyamd
+
+#endif  // RUY_AMD_CSRC_KERNELS_GROUPED_GEMM_H_
