@@ -132,7 +132,9 @@ int Run(ruyamd_ctx* ctx, grouped::Call* call, const grouped::Int4* weights) {
   ctx->capturing = status == hipStreamCaptureStatusActive;
   const bool timed = ctx->TimingBegin();
   hipError_t launched = hipSuccess;
-  if (!ctx->force_generic && !weights && grouped::LaunchTiles(ctx->stream, *call, &launched)) {
+  if (!ctx->force_generic && grouped::LaunchStream(ctx->stream, *call, weights, &launched)) {
+    ctx->last_kernel = weights ? RUYAMD_KERNEL_INT4_STREAM : RUYAMD_KERNEL_GROUPED_STREAM;
+  } else if (!ctx->force_generic && !weights && grouped::LaunchTiles(ctx->stream, *call, &launched)) {
     ctx->last_kernel = RUYAMD_KERNEL_GROUPED_MFMA;
   } else {
     launched = grouped::LaunchGeneric(ctx->stream, *call, weights);

@@ -54,6 +54,10 @@ hipError_t LaunchGeneric(hipStream_t stream, const Call& call, const Int4* weigh
 // not one for this kernel, and nothing was launched.
 bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status);
 
+// Every weight read once (grouped_stream.h): 4-bit weights, and others by rows against a
+// few columns a group. False as above.
+bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hipError_t* status);
+
 }  // namespace grouped
 }  // namespace ruyamd
 

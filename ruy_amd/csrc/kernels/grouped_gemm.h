@@ -167,8 +167,7 @@ struct TileSide {
         const int run = kk * 32 + q * 8 + h * 4 + (l >> 2);
         const int at = piece * kWaveRows + RowOf(b, (l & 3) * 4);
         const char* p = lds + run * (kRows * 2) + (((at >> 3) ^ Key(run)) << 4) + (at & 7) * 2;
-        half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) v4s*)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
+        half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p);
       }
       return __builtin_bit_cast(v4i, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
