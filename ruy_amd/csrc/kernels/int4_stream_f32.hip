@@ -4,8 +4,8 @@
 namespace ruyamd {
 namespace grouped {
 
-hipError_t LaunchStreamInt4F32(hipStream_t stream, const StreamArgs& args, unsigned blocks, int waves, int rows, int cols) {
-  return LaunchStreamType<true, RUYAMD_DTYPE_F32>(stream, args, blocks, waves, rows, cols);
+hipError_t LaunchStreamInt4F32(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
+  return LaunchStreamInt4<RUYAMD_DTYPE_F32>(stream, args, plan);
 }
 
 }  // namespace grouped
