@@ -194,59 +194,63 @@ struct TileOf {
   int group, m, n;
 };
 
+// The sum of the lanes' values up to and with each lane's own.
+__device__ __forceinline__ int InclusiveSum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // from 1, 2, 4, 8 lanes below in its row of 16,
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);  // the last lane of row 0 (2) to row 1 (3),
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);  // of row 1 to rows 2 and 3
+  return v;
+}
+
 // Tiles of groups whose columns are dealt: how many a group has is known here only.
 // Workgroups go round the eight XCDs one by one; each XCD gets a contiguous
 // run of the tiles, so that what its L2 holds serves several of them. Tiles of a
 // group go in bands of kBand along the N side.
 constexpr int kBand = 8;
-template <int kTileN>
-__device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int columns, int tiles_m, TileOf* tile,
-                                         Range* range) {
+__device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int columns, int tile_n, int tiles_m,
+                                         TileOf* tile, Range* range) {
   const int lane = threadIdx.x & 63;
-  const auto tiles_of = [&](int g) __attribute__((always_inline)) {
-    if (g >= groups) return 0;
-    return (RangeOf(offsets, g, columns).count + kTileN - 1) / kTileN;
+  struct Lane {
+    int begin, count, tiles;
   };
-  int total = 0, first = 0;
-  for (int g = lane; g < groups; g += 64) {
-    const int tiles = tiles_of(g);
-    total += tiles;
-    if (g == lane) first = tiles;
+  // What lane l knows of group g0 + l.
+  const auto look = [&](int g) __attribute__((always_inline)) -> Lane {
+    if (g >= groups) return {0, 0, 0};
+    const Range r = RangeOf(offsets, g, columns);
+    return {r.begin, r.count, (r.count + tile_n - 1) / tile_n};
+  };
+  Lane mine = look(lane);
+  int upto = InclusiveSum(mine.tiles), total = __builtin_amdgcn_readlane(upto, 63);
+  if (groups > 64) {  // (the total first: the XCDs' shares go by it)
+    for (int g0 = 64; g0 < groups; g0 += 64) total += __builtin_amdgcn_readlane(InclusiveSum(look(g0 + lane).tiles), 63);
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-  total = __builtin_amdgcn_readfirstlane(total);
   // (int64_t: tiles of many groups times those of many rows.)
   const int64_t all = int64_t(total) * tiles_m, per_xcd = (all + 7) / 8;
   const int64_t place = blockIdx.x >> 3;
   const int64_t t = int64_t(blockIdx.x & 7) * per_xcd + place;
   if (place >= per_xcd || t >= all) return false;
   int64_t before = 0;
-  for (int g0 = 0;; g0 += 64) {
-    const int tiles = g0 == 0 ? first : tiles_of(g0 + lane);
-    int upto = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
-    }
+  for (int g0 = 0;;) {
     const uint64_t past = __ballot((before + upto) * tiles_m > t);
     if (past) {
       const int at = __builtin_ctzll(past);
-      const int mine = __builtin_amdgcn_readfirstlane(__shfl(tiles, at));
-      const int64_t group_first = (before + __builtin_amdgcn_readfirstlane(__shfl(upto, at)) - mine) * tiles_m;
+      const int tiles = __builtin_amdgcn_readlane(mine.tiles, at);
+      const int64_t group_first = (before + __builtin_amdgcn_readlane(upto, at) - tiles) * tiles_m;
       int in_group = static_cast<int>(t - group_first);
-      const int band = in_group / (kBand * tiles_m), width = min(kBand, mine - band * kBand);
+      const int band = in_group / (kBand * tiles_m), width = min(kBand, tiles - band * kBand);
       in_group -= band * kBand * tiles_m;
-      tile->group = __builtin_amdgcn_readfirstlane(g0 + at);
-      tile->m = __builtin_amdgcn_readfirstlane(in_group / width);
-      tile->n = __builtin_amdgcn_readfirstlane(band * kBand + in_group % width);
-      break;
+      *tile = {g0 + at, in_group / width, band * kBand + in_group % width};
+      *range = {__builtin_amdgcn_readlane(mine.begin, at), __builtin_amdgcn_readlane(mine.count, at)};
+      return true;
     }
-    before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+    before += __builtin_amdgcn_readlane(upto, 63);
+    g0 += 64;
+    mine = look(g0 + lane);
+    upto = InclusiveSum(mine.tiles);
   }
-  *range = UniformRangeOf(offsets, tile->group, columns);
-  return true;
 }
 
 // kDirect: every run of both operands begins at a multiple of 16 bytes and is a
@@ -272,7 +276,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void GroupedGemmKernel(Gemm
   Range range;
   const bool columns = p.dealt == Dealt::kColumns;
   if (columns) {
-    if (!FindTile<kTileN>(p.offsets, p.groups, p.n.count, tiles_m, &tile, &range)) return;
+    if (!FindTile(p.offsets, p.groups, p.n.count, kTileN, tiles_m, &tile, &range)) return;
   } else {
     const int tiles_n = (p.n.count + kTileN - 1) / kTileN;
     const int64_t all = int64_t(p.groups) * tiles_m * tiles_n, per_xcd = (all + 7) / 8, place = blockIdx.x >> 3;

@@ -12,9 +12,9 @@
 // have through LDS. The tokens are put into LDS first, as the matrix instructions want
 // them: all of their depth where that fits, slab by slab otherwise (kSlabs).
 //
-// 4-bit weights. (16 + q) is what is left of a 16-bit float of exponent 4 with the four bits of q
-// put at the top of its mantissa, so eight of them take eight instructions. Half: 16 + zero is
-// then taken away, exactly (packed, half an instruction a weight). bfloat16 has no such
+// 4-bit weights. The four bits of q put into the mantissa of a 16-bit float of some exponent
+// make 2^e + q (half: 1024 + q, bfloat16: 16 + q), two at a time. Half: 1024 + zero is
+// then taken away, exactly and packed: 9 instructions to 8 weights. bfloat16 has no such
 // instruction: the product is formed with 16 + q, and (16 + zero) * sum(x), whose sums come from
 // the matrix cores as well (a product with ones), is taken away from every group's sum. fp32 tokens
 // are three bf16 rows each that add up to them (float_parts.h), so that every product is exact.
@@ -34,21 +34,26 @@ struct StreamArgs {
   Call c;
   Int4 w;
   int tiles_m;       // workgroups along the rows
-  int depth_waves;   // waves that deal out the depth
+  int depth_waves;   // waves that deal out the depth (a power of two)
+  int row_waves;     // waves along the rows (a power of two; kSlabs: RowWaves)
   int pitch;         // bytes from a token in LDS to the next
   int slab_bytes;    // of one of the two buffers (kSlabs)
+  int tokens;        // to a workgroup, at most
+  int scale_shift;   // Scaling::kWide: logarithm of the depth positions to a scale
 };
 
 // LDS that a workgroup of these kernels may take.
 constexpr int kStreamLds = 144 << 10;
 
-// How weights of each kind and their tokens come.
-template <bool kInt4, int kType>
+// How weights of each kind and their tokens come. A wave takes 128 bytes of every row
+// at a time, a whole line of the caches (4-bit weights slab by slab: 64, half the tokens
+// in LDS).
+template <bool kInt4, int kType, bool kSlabs>
 struct Stream {
   static constexpr int kBytes = kType == RUYAMD_DTYPE_F32 ? 4 : 2;
-  static constexpr int kChunk = kInt4 ? 128 : 128 / kBytes;  // depth positions that a wave takes at a time
-  static constexpr int kWeightLoads = kInt4 ? 1 : 2;         // of 16 bytes to a row and chunk
-  static constexpr int kSteps = kInt4 ? 4 : 2;               // products of a fragment of 16 bytes of tokens
+  static constexpr int kChunk = kInt4 ? (kSlabs ? 128 : 256) : 128 / kBytes;  // depth positions
+  static constexpr int kWeightLoads = kInt4 && kSlabs ? 1 : 2;  // of 16 bytes to a row and chunk
+  static constexpr int kSteps = (kInt4 ? 4 : 1) * kWeightLoads; // products of a fragment of 16 bytes of tokens
   static constexpr bool kParts = kInt4 && kType == RUYAMD_DTYPE_F32;
   static constexpr int kTokens = kParts ? 5 : 16;            // to 16 rows of a matrix instruction
   static constexpr int kUnit = kInt4 ? 8 : 16 / kBytes;      // depth positions put into LDS at a time
@@ -60,23 +65,25 @@ typedef uint32_t u32_unaligned __attribute__((aligned(1)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef v2i v2i_unaligned __attribute__((aligned(1)));
 
-// Groups of 4-bit weights, by their size: 128 and its multiples, or one for a whole
+// Groups of 4-bit weights, by their size: a power of two from 128 on, or one for a whole
 // row (kWide); 64; 32; any other multiple of 32.
 enum class Scaling { kWide, k64, k32, kAny };
 
-// Waves along the rows of a workgroup.
+// Waves along the rows of a workgroup of the kernels that go slab by slab.
 constexpr int RowWaves(bool slabs, int cols) { return slabs && cols > 1 ? 2 : 1; }
 
-template <bool kInt4, int kType, int kRows, int kCols, Scaling kScaling, bool kSlabs>
+// (kF32Scales, kZeroPoints: as template arguments since a load that depends on a branch
+// has the wave wait for all its loads, where it should wait for a chunk's: 16384 x 16384 half,
+// one token, 37 us with branches, FIGURE without.)
+template <bool kInt4, int kType, int kRows, int kCols, Scaling kScaling, bool kSlabs, bool kF32Scales, bool kZeroPoints>
 __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
-  using T = Stream<kInt4, kType>;
-  constexpr int kWorkTokens = T::kTokens * kCols;
+  using T = Stream<kInt4, kType, kSlabs>;
+  constexpr int kMostTokens = T::kTokens * kCols;
   constexpr int kRowWaves = RowWaves(kSlabs, kCols);
-  constexpr int kWorkRows = 16 * kRows * kRowWaves;
-  constexpr int kDepth = 2;  // chunks of weights held by a wave
   // Scales to a chunk, steps to a scale.
-  constexpr int kScales = !kInt4 || kScaling == Scaling::kWide ? 1 : kScaling == Scaling::k64 ? 2 : 4;
-  constexpr int kStepsToScale = T::kSteps / kScales;
+  constexpr int kScales =
+      T::kWeightLoads * (!kInt4 || kScaling == Scaling::kWide ? 1 : kScaling == Scaling::k64 ? 2 : 4);
+  constexpr int kStepsToScale = kInt4 ? T::kSteps / kScales : 1;
   constexpr bool kScalesSideBySide = kScaling == Scaling::k64 || kScaling == Scaling::k32;
   constexpr bool kHalf = kType == RUYAMD_DTYPE_F16;
   constexpr int kMmaType = kHalf ? RUYAMD_DTYPE_F16 : RUYAMD_DTYPE_BF16;  // of 4-bit weights
@@ -85,24 +92,25 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   const Int4& w = args.w;
   const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int depth_waves = args.depth_waves;
-  const int depth_wave = kRowWaves == 1 ? wave : wave / kRowWaves, row_wave = kRowWaves == 1 ? 0 : wave % kRowWaves;
+  const int depth_waves = args.depth_waves, row_waves = kSlabs ? kRowWaves : args.row_waves;
+  const int depth_wave = wave >> __builtin_ctz(row_waves), row_wave = wave & (row_waves - 1);
+  const int work_rows = 16 * kRows * row_waves;
 
   TileOf tile;
   Range range;
   if (c.offsets) {
-    if (!FindTile<kWorkTokens>(c.offsets, c.groups, c.n, args.tiles_m, &tile, &range)) return;
+    if (!FindTile(c.offsets, c.groups, c.n, args.tokens, args.tiles_m, &tile, &range)) return;
   } else {
-    const int tiles_n = (c.n + kWorkTokens - 1) / kWorkTokens;
+    const int tiles_n = (c.n + args.tokens - 1) / args.tokens;
     const int64_t all = int64_t(tiles_n) * args.tiles_m, per_xcd = (all + 7) / 8, place = blockIdx.x >> 3;
     const int64_t t = int64_t(blockIdx.x & 7) * per_xcd + place;
     if (place >= per_xcd || t >= all) return;
     tile = {0, static_cast<int>(t / tiles_n), static_cast<int>(t % tiles_n)};
     range = {0, c.n};
   }
-  const int row0 = tile.m * kWorkRows, token0 = tile.n * kWorkTokens;
-  const int tokens = min(kWorkTokens, range.count - token0);
-  const int chunks = (c.k + T::kChunk - 1) / T::kChunk;
+  const int row0 = tile.m * work_rows, token0 = tile.n * args.tokens;
+  const int tokens = min(args.tokens, range.count - token0);
+  const int chunks = (c.k + T::kChunk - 1) / T::kChunk, whole_chunks = c.k / T::kChunk;
 
   // Where this lane's rows of weights begin. (Rows past the last are the last one
   // again; their results are not stored.)
@@ -120,63 +128,79 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   }
   const int row_bytes = kInt4 ? (c.k + 1) / 2 : c.k * T::kBytes;
   const int row_scale_count = kInt4 ? (c.k + w.group_size - 1) / w.group_size : 0;
-  const bool f32_scales = w.scale_type == RUYAMD_DTYPE_F32;
 
   struct Held {
     v4i weights[kRows][T::kWeightLoads];
-    uint32_t scales[kRows][kScales], zeros[kRows][kScalesSideBySide ? 1 : kScales];
+    uint32_t scales[kRows][kScales], zeros[kRows][kScalesSideBySide ? (kScales + 3) / 4 : kScales];
   };
   // Loads never reach past the end of a row (which has 16 bytes and, side by side,
   // kScales scales at least): what would is read from its last bytes, and moved to
   // where it belongs by Place.
+  // (Scales first: a wave that waits for its weights then waits for all of a chunk, and
+  // for next to nothing of the one behind it, whether there are zero points or not.)
   const auto load = [&](int chunk, Held& h) __attribute__((always_inline)) {
+    if constexpr (kInt4) {
+      if constexpr (kScalesSideBySide) {
+        const int at = min(chunk * kScales, row_scale_count - kScales);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          v4i x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+          if constexpr (kF32Scales) {
+            const float* p = static_cast<const float*>(w.scales) + row_scales[r] + at;
+            if constexpr (kScales == 2) {
+              const v2i both = *reinterpret_cast<const v2i_unaligned*>(p);
+              x = v4i{both[0], both[1], 0, 0};
+            } else {
+              x = *reinterpret_cast<const granule::v4i_unaligned*>(p);
+              if constexpr (kScales == 8) y = *reinterpret_cast<const granule::v4i_unaligned*>(p + 4);
+            }
+          } else {
+            const uint16_t* p = static_cast<const uint16_t*>(w.scales) + row_scales[r] + at;
+            if constexpr (kScales == 2) {
+              x[0] = *reinterpret_cast<const u32_unaligned*>(p);
+            } else if constexpr (kScales == 4) {
+              const v2i both = *reinterpret_cast<const v2i_unaligned*>(p);
+              x = v4i{both[0], both[1], 0, 0};
+            } else {
+              x = *reinterpret_cast<const granule::v4i_unaligned*>(p);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < kScales; ++g) h.scales[r][g] = g < 4 ? x[g & 3] : y[g & 3];
+#pragma unroll
+          for (int g = 0; g < (kScales + 3) / 4; ++g) h.zeros[r][g] = 0x08080808u;
+          if constexpr (kZeroPoints) {
+            const uint8_t* p = w.zero_points + row_scales[r] + at;
+            if constexpr (kScales == 2) h.zeros[r][0] = p[0] | p[1] << 8;
+#pragma unroll
+            for (int g = 0; g < kScales / 4; ++g) h.zeros[r][g] = reinterpret_cast<const u32_unaligned*>(p)[g];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kScales; ++g) {
+          const int k = min(chunk * T::kChunk + g * (T::kChunk / kScales), c.k - 1);
+          const int at = kScaling == Scaling::kWide ? k >> args.scale_shift : k / w.group_size;
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            if constexpr (kF32Scales)
+              h.scales[r][g] = static_cast<const uint32_t*>(w.scales)[row_scales[r] + at];
+            else
+              h.scales[r][g] = static_cast<const uint16_t*>(w.scales)[row_scales[r] + at];
+            h.zeros[r][g] = kZeroPoints ? w.zero_points[row_scales[r] + at] : 8;
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < T::kWeightLoads; ++i) {
       const int at = min(chunk * (T::kWeightLoads * 64) + i * 64 + q * 16, row_bytes - 16);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) h.weights[r][i] = *reinterpret_cast<const granule::v4i_unaligned*>(row_data[r] + at);
     }
-    if constexpr (kInt4) {
-      if constexpr (kScalesSideBySide) {
-        const int at = min(chunk * kScales, row_scale_count - kScales);
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          if (f32_scales) {
-            const float* p = static_cast<const float*>(w.scales) + row_scales[r] + at;
-#pragma unroll
-            for (int g = 0; g < kScales; ++g) h.scales[r][g] = __float_as_uint(p[g]);
-          } else {
-            const uint16_t* p = static_cast<const uint16_t*>(w.scales) + row_scales[r] + at;
-            if constexpr (kScales == 4) {
-              const v2i both = *reinterpret_cast<const v2i_unaligned*>(p);
-              h.scales[r][0] = both[0];
-              h.scales[r][1] = both[1];
-            } else {
-              h.scales[r][0] = *reinterpret_cast<const u32_unaligned*>(p);
-            }
-          }
-          h.zeros[r][0] = 0x08080808u;
-          if (w.zero_points) {
-            const uint8_t* p = w.zero_points + row_scales[r] + at;
-            h.zeros[r][0] = kScales == 4 ? *reinterpret_cast<const u32_unaligned*>(p) : p[0] | p[1] << 8;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int g = 0; g < kScales; ++g) {
-          const int at = w.group_size == 128 ? chunk : min(chunk * 128 + g * 32, c.k - 1) / w.group_size;
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            h.scales[r][g] = f32_scales ? static_cast<const uint32_t*>(w.scales)[row_scales[r] + at]
-                                        : static_cast<const uint16_t*>(w.scales)[row_scales[r] + at];
-            h.zeros[r][g] = w.zero_points ? w.zero_points[row_scales[r] + at] : 8;
-          }
-        }
-      }
-    }
   };
   const auto place = [&](int chunk, Held& h) __attribute__((always_inline)) {
-    if ((chunk + 1) * T::kChunk <= c.k) return;
+    if (chunk < whole_chunks) return;
 #pragma unroll
     for (int i = 0; i < T::kWeightLoads; ++i) {
       const int at = chunk * (T::kWeightLoads * 64) + i * 64 + q * 16;
@@ -188,43 +212,60 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           h.zeros[r][0] >>= 8;
-          if (f32_scales) {
+          if constexpr (kScales == 8) {
+            h.zeros[r][0] |= h.zeros[r][1] << 24;
+            h.zeros[r][1] >>= 8;
+          }
+          if constexpr (kF32Scales) {
 #pragma unroll
             for (int g = 0; g < kScales; ++g) h.scales[r][g] = g + 1 < kScales ? h.scales[r][g + 1] : 0;
           } else {
-            h.scales[r][0] >>= 16;
-            if constexpr (kScales == 4) {
-              h.scales[r][0] |= h.scales[r][1] << 16;
-              h.scales[r][1] >>= 16;
-            }
+#pragma unroll
+            for (int g = 0; g < kScales / 2; ++g)
+              h.scales[r][g] = h.scales[r][g] >> 16 | (g + 1 < kScales / 2 ? h.scales[r][g + 1] << 16 : 0);
           }
         }
     }
   };
-  const auto scale_of = [&](const Held& h, int r, int g) __attribute__((always_inline)) -> float {
-    if (f32_scales) return __uint_as_float(h.scales[r][g]);
-    const uint32_t bits = kScalesSideBySide ? h.scales[r][g / 2] >> (16 * (g & 1)) & 0xffffu : h.scales[r][g];
-    if (w.scale_type == RUYAMD_DTYPE_BF16) return __uint_as_float(bits << 16);
-    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+  const bool bf16_scales = w.scale_type == RUYAMD_DTYPE_BF16;
+  const auto scales_of = [&](const Held& h, float (&scale)[kRows][kScales]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int g = 0; g < kScales; ++g) {
+        if constexpr (kF32Scales) {
+          scale[r][g] = __uint_as_float(h.scales[r][g]);
+        } else {
+          const uint32_t bits = kScalesSideBySide ? h.scales[r][g / 2] >> (16 * (g & 1)) : h.scales[r][g];
+          const float as_half = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+          const float as_bf16 = __uint_as_float(bits << 16);
+          scale[r][g] = bf16_scales ? as_bf16 : as_half;
+        }
+      }
   };
   const auto zero_of = [&](const Held& h, int r, int g) __attribute__((always_inline)) -> uint32_t {
-    return kScalesSideBySide ? h.zeros[r][0] >> (8 * g) & 0xffu : h.zeros[r][g];
+    return kScalesSideBySide ? h.zeros[r][g / 4] >> (8 * (g & 3)) & 0xffu : h.zeros[r][g];
   };
 
   // Unit u of a token (kUnit values from depth position u * kUnit on), zeros past the depth.
   struct Unit {
     v4i x[T::kUnitLoads];
   };
+  const uint8_t* const token_data =
+      static_cast<const uint8_t*>(c.rhs) + (int64_t(range.begin) + token0) * c.rhs_cs * T::kBytes;
+  // (One inside the depth, of tokens whose values lie side by side.)
+  const auto fetch_inside = [&](int token, int u) __attribute__((always_inline)) -> Unit {
+    Unit unit;
+    const uint8_t* p = token_data + (token * c.rhs_cs + u * T::kUnit) * T::kBytes;
+#pragma unroll
+    for (int i = 0; i < T::kUnitLoads; ++i) unit.x[i] = reinterpret_cast<const granule::v4i_unaligned*>(p)[i];
+    return unit;
+  };
   const auto fetch = [&](int token, int u) __attribute__((always_inline)) -> Unit {
     Unit unit;
     const int k = u * T::kUnit;
-    const uint8_t* p = static_cast<const uint8_t*>(c.rhs) +
-                       ((int64_t(range.begin) + token0 + token) * c.rhs_cs + k * c.rhs_rs) * T::kBytes;
-    if (c.rhs_rs == 1 && k + T::kUnit <= c.k) {
-#pragma unroll
-      for (int i = 0; i < T::kUnitLoads; ++i) unit.x[i] = reinterpret_cast<const granule::v4i_unaligned*>(p)[i];
-      return unit;
-    }
+    if (c.rhs_rs == 1 && k + T::kUnit <= c.k) return fetch_inside(token, u);
+    const uint8_t* p = token_data + (token * c.rhs_cs + k * c.rhs_rs) * T::kBytes;
     // One value after the other, each pushed in behind those before it.
 #pragma unroll
     for (int i = 0; i < T::kUnitLoads; ++i) {
@@ -297,17 +338,32 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 
   v4f acc[kRows][kCols] = {};
 
-  // 16 + q of the eight values of a word, in that order.
+  // What the eight values of a word are taken apart with. (Held in registers: as constants
+  // in the instructions they would each take one more.)
+  uint32_t low_mask = kHalf ? 0x000F000Fu : 0x00780078u, high_mask = 0x00F000F0u, sixteenth = 0x2C002C00u;
+  uint32_t exponent = kHalf ? 0x64006400u : 0x41804180u;
+  asm("" : "+s"(low_mask));
+  asm("" : "+s"(high_mask));
+  asm("" : "+s"(sixteenth));
+  asm("" : "+v"(exponent));
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+  const auto halves = [](uint32_t x) __attribute__((always_inline)) -> v2h { return __builtin_bit_cast(v2h, x); };
+  const auto bits = [](v2h x) __attribute__((always_inline)) -> int { return __builtin_bit_cast(int, x); };
+  // Half: q - zero, in the order 0 4 1 5 2 6 3 7. 1024 + q (its four bits lowest in the mantissa) less 1024 + zero, or
+  // 1024 + 16 q (one place further up) sixteenths less 64 + zero; all exact.
+  const auto less_zero = [&](uint32_t x, uint32_t zero) __attribute__((always_inline)) -> v4i {
+    const uint32_t low = 0x6400u | zero, high = 0xD400u | zero << 4;  // 1024 + zero, -(64 + zero)
+    const v2h away_low = halves(low | low << 16), away_high = halves(high | high << 16);
+    const uint32_t y = x >> 8;
+    return v4i{bits(halves((x & low_mask) | exponent) - away_low),
+               bits(__builtin_elementwise_fma(halves((x & high_mask) | exponent), halves(sixteenth), away_high)),
+               bits(halves((y & low_mask) | exponent) - away_low),
+               bits(__builtin_elementwise_fma(halves((y & high_mask) | exponent), halves(sixteenth), away_high))};
+  };
+  // bfloat16: 16 + q, in that order.
   const auto sixteen_and = [&](uint32_t x) __attribute__((always_inline)) -> v4i {
-    constexpr uint32_t kSixteen = kHalf ? 0x4C004C00u : 0x41804180u, kMask = kHalf ? 0x03C003C0u : 0x00780078u;
-    constexpr int kUp = kHalf ? 6 : 3;
-    v4i out;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int shift = kUp - 4 * e;
-      out[e] = static_cast<int>(((shift >= 0 ? x << (shift & 31) : x >> (-shift & 31)) & kMask) | kSixteen);
-    }
-    return out;
+    return v4i{static_cast<int>((x << 3 & low_mask) | exponent), static_cast<int>((x >> 1 & low_mask) | exponent),
+               static_cast<int>((x >> 5 & low_mask) | exponent), static_cast<int>((x >> 9 & low_mask) | exponent)};
   };
   // 16-byte pieces of four lanes to pieces of a 4-byte word each: word j of the
   // lane with q holds what bytes j * 16 + q * 4 .. of the row's 64 held. A step's 32 depth positions are
@@ -332,7 +388,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   };
   // The unit of a chunk that step j of this lane takes.
   const auto unit_of = [&](int j) __attribute__((always_inline)) -> int {
-    return kInt4 && kScaling == Scaling::kWide ? q * 4 + j : j * 4 + q;
+    return kInt4 && kScaling == Scaling::kWide ? j / 4 * 16 + q * 4 + j % 4 : j * 4 + q;
   };
 
   // `at`: the chunk's place in the tokens' rows.
@@ -347,9 +403,13 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
           for (int r = 0; r < kRows; ++r) Mma<kType>(x, h.weights[r][j], acc[r][t]);
         }
     } else {
-      v4i words[kRows];
+      v4i words[kRows][T::kWeightLoads];
+      float scale[kRows][kScales];
+      scales_of(h, scale);
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) words[r] = exchange(h.weights[r][0]);
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < T::kWeightLoads; ++i) words[r][i] = exchange(h.weights[r][i]);
 #pragma unroll
       for (int g = 0; g < kScales; ++g) {
         v4f sum[kRows][kCols] = {};
@@ -368,18 +428,13 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
           }
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
-            v4i b = sixteen_and(words[r][j]);
-            if constexpr (kHalf) {
-              const auto sixteen_and_zero = static_cast<uint16_t>(0x4C00u | zero_of(h, r, g) << 6);
-              b = __builtin_bit_cast(v4i, __builtin_bit_cast(v8h, b) - __builtin_bit_cast(_Float16, sixteen_and_zero));
-            }
+            const v4i b = kHalf ? less_zero(words[r][j / 4][j % 4], zero_of(h, r, g)) : sixteen_and(words[r][j / 4][j % 4]);
 #pragma unroll
             for (int t = 0; t < kCols; ++t) Mma<kMmaType>(x[t], b, sum[r][t]);
           }
         }
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          const float scale = scale_of(h, r, g);
           const float away = -16.0f - static_cast<float>(zero_of(h, r, g));
 #pragma unroll
           for (int t = 0; t < kCols; ++t)
@@ -387,44 +442,84 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
             for (int e = 0; e < 4; ++e) {
               float v = sum[r][t][e];
               if constexpr (!kHalf) v = __builtin_fmaf(away, ones[t][e], v);
-              acc[r][t][e] = __builtin_fmaf(scale, v, acc[r][t][e]);
+              acc[r][t][e] = __builtin_fmaf(scale[r][g], v, acc[r][t][e]);
             }
         }
       }
     }
   };
 
-  Held held[kDepth];
-  StaticFor<kDepth>([&](auto d) __attribute__((always_inline)) {
-    const int chunk = depth_wave + d * depth_waves;
-    if (chunk < chunks) load(chunk, held[d]);
-  });
   constexpr int kLdsChunk = T::kChunkUnits * 16;
-  const int iterations = (chunks + depth_waves - 1) / depth_waves;
-  // Units of a slab that a thread puts into LDS.
-  constexpr int kPieces = (kWorkTokens * T::kChunkUnits + 64 * kRowWaves - 1) / (64 * kRowWaves);
-  Unit pieces[kSlabs ? kPieces : 1];
-  const int slab_units = depth_waves * T::kChunkUnits, unit_bits = __builtin_ctz(slab_units);  // (a power of two)
-  const auto fetch_slab = [&](int slab) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int n = i * blockDim.x + threadIdx.x;
-      if (n < tokens * slab_units) pieces[i] = fetch(n >> unit_bits, slab * slab_units + (n & (slab_units - 1)));
-    }
+  // Turns of this wave's main loop, a whole chunk each; the slabs' turns are those of all
+  // waves. What is left of the depth comes behind the loop.
+  const int turns = kSlabs ? whole_chunks / depth_waves
+                           : (whole_chunks - depth_wave + depth_waves - 1) / depth_waves;
+  // The depth begins at another place in every 16 * kRows rows and goes round: rows
+  // often lie a power of two apart, and whoever goes through theirs side by side, from
+  // the same place on, asks the same few memory channels.
+  const int first_turn = turns > 0 ? (kSlabs ? tile.m : tile.m * row_waves + row_wave) % turns : 0;
+  const auto place_of = [&](int turn) __attribute__((always_inline)) -> int {  // (past the last: the last)
+    const int at = min(turn, turns - 1) + first_turn;
+    return at < turns ? at : at - turns;
   };
-  const auto put_slab = [&](int buffer) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int n = i * blockDim.x + threadIdx.x;
-      if (n < tokens * slab_units)
-        put(pieces[i], lds + buffer * args.slab_bytes + row_in_lds(n >> unit_bits) * args.pitch +
-                           (n & (slab_units - 1)) * 16);
-    }
-  };
+  // The loop's loads are issued whatever comes (past the end once more the last chunk):
+  // a load that may or may not have been issued is one for which everything is waited for.
+  Held held[2];
+  if (turns > 0) {
+    load(depth_wave + place_of(0) * depth_waves, held[0]);
+    load(depth_wave + place_of(1) * depth_waves, held[1]);
+  }
   if constexpr (kSlabs) {
-    fetch_slab(0);
-    put_slab(0);
-    if (iterations > 1) fetch_slab(1);
+    const int slab_units = depth_waves * T::kChunkUnits, unit_bits = __builtin_ctz(slab_units);  // (a power of two)
+    constexpr int kPieces = (kMostTokens * T::kChunkUnits + 64 * kRowWaves - 1) / (64 * kRowWaves);
+    Unit pieces[kPieces];
+    // (Tokens past the last are the last one again.)
+    const auto fetch_slab = [&](int slab) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int n = i * blockDim.x + threadIdx.x, token = min(n >> unit_bits, tokens - 1);
+        pieces[i] = fetch_inside(token, slab * slab_units + (n & (slab_units - 1)));
+      }
+    };
+    const auto put_slab = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int n = i * blockDim.x + threadIdx.x, token = min(n >> unit_bits, tokens - 1);
+        put(pieces[i], lds + buffer * args.slab_bytes + row_in_lds(token) * args.pitch + (n & (slab_units - 1)) * 16);
+      }
+    };
+    if (turns > 0) {
+      fetch_slab(place_of(0));
+      put_slab(0);
+      fetch_slab(place_of(1));
+      const auto turn = [&](int n, auto d) __attribute__((always_inline)) {
+        // Slab n is there, and slab n - 1 no longer read, when all have come here.
+        __syncthreads();
+        put_slab(1 - d);
+        fetch_slab(place_of(n + 2));
+        use(held[d], lds + d * args.slab_bytes + depth_wave * kLdsChunk);
+        load(depth_wave + place_of(n + 2) * depth_waves, held[d]);
+      };
+      for (int n = 0;;) {
+        turn(n, std::integral_constant<int, 0>());
+        if (++n == turns) break;
+        turn(n, std::integral_constant<int, 1>());
+        if (++n == turns) break;
+      }
+    }
+    const int done = turns * depth_waves, left = chunks - done;
+    if (left > 0) {
+      __syncthreads();
+      const int units = left * T::kChunkUnits;
+      for (int n = threadIdx.x; n < tokens * units; n += blockDim.x)
+        put(fetch(n / units, done * T::kChunkUnits + n % units), lds + row_in_lds(n / units) * args.pitch + n % units * 16);
+      __syncthreads();
+      if (depth_wave < left) {
+        load(done + depth_wave, held[0]);
+        place(done + depth_wave, held[0]);
+        use(held[0], lds + depth_wave * kLdsChunk);
+      }
+    }
   } else {
     const int units = chunks * T::kChunkUnits;
     for (int n0 = threadIdx.x; n0 < tokens * units; n0 += 4 * blockDim.x) {
@@ -441,22 +536,23 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
       }
     }
     __syncthreads();
-  }
-  for (int i = 0; i < iterations; i += kDepth) {
-    StaticFor<kDepth>([&](auto d) __attribute__((always_inline)) {
-      const int n = i + d, chunk = depth_wave + n * depth_waves;
-      if (kSlabs && n < iterations) {
-        // Slab n is there, and slab n - 1 no longer read, when all have come here.
-        __syncthreads();
-        if (n + 1 < iterations) put_slab((n + 1) & 1);
-        if (n + 2 < iterations) fetch_slab(n + 2);
+    if (turns > 0) {
+      const auto turn = [&](int n, auto d) __attribute__((always_inline)) {
+        use(held[d], lds + (depth_wave + place_of(n) * depth_waves) * kLdsChunk);
+        load(depth_wave + place_of(n + 2) * depth_waves, held[d]);
+      };
+      for (int n = 0;;) {
+        turn(n, std::integral_constant<int, 0>());
+        if (++n == turns) break;
+        turn(n, std::integral_constant<int, 1>());
+        if (++n == turns) break;
       }
-      if (chunk < chunks) {
-        place(chunk, held[d]);
-        use(held[d], kSlabs ? lds + (n & 1) * args.slab_bytes + depth_wave * kLdsChunk : lds + chunk * kLdsChunk);
-        if (chunk + kDepth * depth_waves < chunks) load(chunk + kDepth * depth_waves, held[d]);
-      }
-    });
+    }
+    if (whole_chunks < chunks && whole_chunks % depth_waves == depth_wave) {
+      load(whole_chunks, held[0]);
+      place(whole_chunks, held[0]);
+      use(held[0], lds + whole_chunks * kLdsChunk);
+    }
   }
 
   if constexpr (kInt4 && !kHalf) {
@@ -478,8 +574,12 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         Held h;
         load(chunk, h);
         place(chunk, h);
+        float scale[kRows][kScales];
+        scales_of(h, scale);
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) h.weights[r][0] = exchange(h.weights[r][0]);
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int i = 0; i < T::kWeightLoads; ++i) h.weights[r][i] = exchange(h.weights[r][i]);
 #pragma unroll
         for (int g = 0; g < kScales; ++g) {
 #pragma unroll 1
@@ -492,7 +592,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
               const Unit x = fetch(token, chunk * T::kChunkUnits + unit_of(j));
 #pragma unroll
               for (int r = 0; r < kRows; ++r) {
-                const uint32_t word = h.weights[r][0][0];
+                const uint32_t word = h.weights[r][g * kStepsToScale / 4][0];
                 const int zero = static_cast<int>(zero_of(h, r, g));
                 float v[8];
 #pragma unroll
@@ -508,16 +608,15 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
                                  float_parts::RoundPair(v[2], v[6]), float_parts::RoundPair(v[3], v[7])};
                   Mma<kMmaType>(in_word_order(x.x[0]), b, sum);
                 }
-                const float scale = scale_of(h, r, g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[r][t][e] = __builtin_fmaf(scale, sum[e], acc[r][t][e]);
+                for (int e = 0; e < 4; ++e) acc[r][t][e] = __builtin_fmaf(scale[r][g], sum[e], acc[r][t][e]);
               }
             }
             // (The next step's word in the place of this one's.)
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
-              const v4i x = h.weights[r][0];
-              h.weights[r][0] = v4i{x[1], x[2], x[3], 0};
+              v4i& x = h.weights[r][g * kStepsToScale / 4];
+              x = v4i{x[1], x[2], x[3], 0};
             }
           }
         }
@@ -537,7 +636,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
       for (int e = 0; e < 4; ++e) partial[((wave * kRows + r) * 4 + e) * 64 + lane] = acc[r][t][e];
     __syncthreads();
     // Value number v: row v % 16 of a block of 16, token v / 16 % 16, block v / 256.
-    for (int v = threadIdx.x; v < kWorkRows * T::kTokens; v += blockDim.x) {
+    for (int v = threadIdx.x; v < work_rows * T::kTokens; v += blockDim.x) {
       const int row = v % 16, token = v / 16 % T::kTokens, r = v / (16 * T::kTokens);
       const int m = row0 + r * 16 + row, n = token0 + t * T::kTokens + token;
       if (m >= c.m || n >= token0 + tokens) continue;
@@ -546,7 +645,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
       for (int s = 0; s < (T::kParts ? 3 : 1); ++s) {
         const int at = T::kParts ? token * 3 + s : token;  // row of the accumulators' block
         const float* from = partial + (r * 4 + at % 4) * 64 + at / 4 * 16 + row;
-        for (int i = 0; i < depth_waves; ++i) sum += from[i * kRowWaves * kRows * 256];
+        for (int i = 0; i < depth_waves; ++i) sum += from[i * row_waves * kRows * 256];
       }
       if (c.bias) sum += c.bias[tile.group * c.bias_stride + m];
       StoreFloat(c.dst, c.dst_type, m * c.dst_rs + (int64_t(range.begin) + n) * c.dst_cs,
@@ -565,9 +664,9 @@ struct StreamPlan {
   unsigned lds_bytes;
 };
 
-template <bool kInt4, int kType, int kRows, int kCols, Scaling kScaling, bool kSlabs>
+template <bool kInt4, int kType, int kRows, int kCols, Scaling kScaling, bool kSlabs, bool kF32Scales, bool kZeroPoints>
 hipError_t LaunchStreamKernel(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
-  auto* const kernel = &GroupedStreamKernel<kInt4, kType, kRows, kCols, kScaling, kSlabs>;
+  auto* const kernel = &GroupedStreamKernel<kInt4, kType, kRows, kCols, kScaling, kSlabs, kF32Scales, kZeroPoints>;
   static const hipError_t attribute = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, kStreamLds);
   if (attribute != hipSuccess) return attribute;
@@ -575,38 +674,54 @@ hipError_t LaunchStreamKernel(hipStream_t stream, const StreamArgs& args, const 
   return hipGetLastError();
 }
 
-template <bool kInt4, int kType, Scaling kScaling, int kRows>
-hipError_t LaunchStreamRows(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
-  if constexpr (kInt4 && kRows == 1) {
-    if (plan.cols == 4) return LaunchStreamKernel<kInt4, kType, 1, 4, kScaling, true>(stream, args, plan);
-  }
-  if constexpr (kRows <= 2) {
-    if (plan.cols == 2) return LaunchStreamKernel<kInt4, kType, kRows, 2, kScaling, true>(stream, args, plan);
-  }
-  if (plan.slabs) return LaunchStreamKernel<kInt4, kType, kRows, 1, kScaling, true>(stream, args, plan);
-  return LaunchStreamKernel<kInt4, kType, kRows, 1, kScaling, false>(stream, args, plan);
+template <int kType, Scaling kScaling, bool kF32Scales, bool kZeroPoints>
+hipError_t LaunchStreamInt4Of(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
+  if (plan.cols == 4)
+    return LaunchStreamKernel<true, kType, 1, 4, kScaling, true, kF32Scales, kZeroPoints>(stream, args, plan);
+  if (plan.cols == 2)
+    return LaunchStreamKernel<true, kType, 1, 2, kScaling, true, kF32Scales, kZeroPoints>(stream, args, plan);
+  if (plan.slabs)
+    return LaunchStreamKernel<true, kType, 1, 1, kScaling, true, kF32Scales, kZeroPoints>(stream, args, plan);
+  if constexpr (kScaling != Scaling::kAny)
+    if (plan.rows == 2)
+      return LaunchStreamKernel<true, kType, 2, 1, kScaling, false, kF32Scales, kZeroPoints>(stream, args, plan);
+  return LaunchStreamKernel<true, kType, 1, 1, kScaling, false, kF32Scales, kZeroPoints>(stream, args, plan);
 }
 
-template <bool kInt4, int kType, Scaling kScaling>
+template <int kType, Scaling kScaling>
 hipError_t LaunchStreamScaling(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
-  if constexpr (!kInt4)
-    if (plan.rows == 4) return LaunchStreamRows<kInt4, kType, kScaling, 4>(stream, args, plan);
-  if (plan.rows == 2) return LaunchStreamRows<kInt4, kType, kScaling, 2>(stream, args, plan);
-  return LaunchStreamRows<kInt4, kType, kScaling, 1>(stream, args, plan);
+  if (args.w.scale_type == RUYAMD_DTYPE_F32) {
+    if (args.w.zero_points) return LaunchStreamInt4Of<kType, kScaling, true, true>(stream, args, plan);
+    return LaunchStreamInt4Of<kType, kScaling, true, false>(stream, args, plan);
+  }
+  if (args.w.zero_points) return LaunchStreamInt4Of<kType, kScaling, false, true>(stream, args, plan);
+  return LaunchStreamInt4Of<kType, kScaling, false, false>(stream, args, plan);
 }
 
 template <int kType>
 hipError_t LaunchStreamInt4(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
   switch (plan.scaling) {
     case Scaling::kWide:
-      return LaunchStreamScaling<true, kType, Scaling::kWide>(stream, args, plan);
+      return LaunchStreamScaling<kType, Scaling::kWide>(stream, args, plan);
     case Scaling::k64:
-      return LaunchStreamScaling<true, kType, Scaling::k64>(stream, args, plan);
+      return LaunchStreamScaling<kType, Scaling::k64>(stream, args, plan);
     case Scaling::k32:
-      return LaunchStreamScaling<true, kType, Scaling::k32>(stream, args, plan);
+      return LaunchStreamScaling<kType, Scaling::k32>(stream, args, plan);
     default:
-      return LaunchStreamRows<true, kType, Scaling::kAny, 1>(stream, args, plan);
+      return LaunchStreamScaling<kType, Scaling::kAny>(stream, args, plan);
   }
+}
+
+// Weights in the tokens' type.
+template <int kType>
+hipError_t LaunchStreamFloat(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
+  if (plan.cols == 2)
+    return LaunchStreamKernel<false, kType, 1, 2, Scaling::kWide, true, false, false>(stream, args, plan);
+  if (plan.slabs)
+    return LaunchStreamKernel<false, kType, 1, 1, Scaling::kWide, true, false, false>(stream, args, plan);
+  if (plan.rows == 2)
+    return LaunchStreamKernel<false, kType, 2, 1, Scaling::kWide, false, false, false>(stream, args, plan);
+  return LaunchStreamKernel<false, kType, 1, 1, Scaling::kWide, false, false, false>(stream, args, plan);
 }
 
 // (Each in a file of its own.)

@@ -1,6 +1,7 @@
 // The streaming kernels of weights in the tokens' own type, and the choice of a
 // streaming kernel.
 #include "grouped_stream.h"
+#include <cstdlib>
 
 namespace ruyamd {
 namespace grouped {
@@ -20,38 +21,58 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   const int64_t per_group = (call.n + busy - 1) / busy;
   if (!int4 && per_group > 32) return false;
   StreamPlan plan;
-  plan.cols = per_group <= block_tokens ? 1 : per_group <= 2 * block_tokens ? 2 : 4;
-  if (!int4) plan.cols = min(plan.cols, 2);
 
-  const int chunk = int4 ? 128 : 128 / bytes;              // depth positions
-  const int chunk_bytes = int4 ? 256 : 128;                // of a token in LDS
-  const int chunks = (call.k + chunk - 1) / chunk;
+  // Tokens of all depth in LDS where 16 of them (or as many as there are) fit, and
+  // slab by slab otherwise; tokens whose values do not lie side by side as many as fit.
+  const int depth_to_chunk = int4 ? 256 : 128 / bytes;
+  const int64_t whole_pitch = int64_t((call.k + depth_to_chunk - 1) / depth_to_chunk) * (int4 ? 512 : 128) + 16;
+  const int64_t room = 128 << 10;
+  const int64_t fit = room / (whole_pitch * rows_to_token);
+  const int64_t to_group = call.offsets ? block_tokens : call.n;  // (a group may have many more than others)
+  if (call.rhs_rs != 1) {
+    if (fit == 0) return false;
+    plan.cols = 1;
+    plan.slabs = false;
+  } else {
+    plan.cols = per_group <= block_tokens ? 1 : per_group <= 2 * block_tokens || !int4 ? 2 : 4;
+    plan.slabs = plan.cols > 1 || min(to_group, int64_t(block_tokens)) > fit;
+  }
+  const int chunk = int4 && plan.slabs ? 128 : depth_to_chunk, chunks = (call.k + chunk - 1) / chunk;
+  const int chunk_bytes = int4 ? 2 * chunk : 128;  // of a token in LDS
+  args.tokens = static_cast<int>(plan.slabs ? plan.cols * block_tokens : min(fit, int64_t(block_tokens)));
+
   plan.scaling = Scaling::kWide;
-  if (int4 && weights->group_size < call.k && weights->group_size % 128) {
-    const int scales = (call.k + weights->group_size - 1) / weights->group_size;
-    plan.scaling = weights->group_size == 64 && scales >= 2   ? Scaling::k64
-                   : weights->group_size == 32 && scales >= 4 ? Scaling::k32
-                                                              : Scaling::kAny;
+  args.scale_shift = 31;
+  if (int4 && weights->group_size < call.k) {
+    const int size = weights->group_size, scales = (call.k + size - 1) / size;
+    args.scale_shift = __builtin_ctz(size);
+    plan.scaling = size >= 128 && (size & (size - 1)) == 0 ? Scaling::kWide
+                   : size == 64 && scales >= chunk / 64    ? Scaling::k64
+                   : size == 32 && scales >= chunk / 32    ? Scaling::k32
+                                                           : Scaling::kAny;
   }
 
-  // Tokens of all depth in LDS where they fit.
-  const int64_t most = min(int64_t(block_tokens), call.offsets ? int64_t(block_tokens) : int64_t(call.n)) * rows_to_token;
-  const int64_t whole_pitch = int64_t(chunks) * chunk_bytes + 16;
-  plan.slabs = plan.cols > 1 || most * whole_pitch > (128 << 10);
-
-  const int row_waves = RowWaves(plan.slabs, plan.cols);
-  plan.rows = plan.cols > 2 ? 1 : plan.cols > 1 || int4 ? 2 : 4;
-  if (plan.scaling == Scaling::kAny) plan.rows = 1;
+  // Waves: 16 to a CU if the rows give them, 8 to a workgroup, along the rows first, then
+  // along the depth.
+  int row_waves = RowWaves(plan.slabs, plan.cols), depth_waves = 8 / row_waves;
+  plan.rows = plan.slabs || plan.scaling == Scaling::kAny ? 1 : 2;
+  if (const char* e = getenv("S_ROWS")) if (plan.rows == 2) plan.rows = atoi(e);
   while (plan.rows > 1 && (call.m + 16 * plan.rows * row_waves - 1) / (16 * plan.rows * row_waves) * busy < call.compute_units)
     plan.rows /= 2;
-  int depth_waves = 8 / row_waves;
+  if (!plan.slabs) {
+    const int64_t units = (call.m + 16 * plan.rows - 1) / (16 * plan.rows) * busy;
+    int per_cu = 16;
+    if (const char* e = getenv("S_WAVES")) per_cu = atoi(e);
+    while (depth_waves > 1 && units * depth_waves > int64_t(per_cu) * call.compute_units) depth_waves /= 2;
+    row_waves = 8 / depth_waves;
+  }
   while (depth_waves > 1 && chunks < depth_waves) depth_waves /= 2;
   plan.waves = depth_waves * row_waves;
   args.depth_waves = depth_waves;
+  args.row_waves = row_waves;
   const int work_rows = 16 * plan.rows * row_waves;
   args.tiles_m = (call.m + work_rows - 1) / work_rows;
-  const int64_t work_tokens = plan.cols * block_tokens;
-  const int64_t slots = call.offsets ? call.n / work_tokens + busy : (call.n + work_tokens - 1) / work_tokens;
+  const int64_t slots = call.offsets ? call.n / args.tokens + busy : (call.n + args.tokens - 1) / args.tokens;
   const int64_t blocks = (slots * args.tiles_m + 7) / 8 * 8;
   if (blocks > 0x7fffffff) return false;
   plan.blocks = static_cast<unsigned>(blocks);
@@ -64,7 +85,7 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   } else {
     args.pitch = static_cast<int>(whole_pitch);
     args.slab_bytes = 0;
-    lds = most * whole_pitch;
+    lds = min(int64_t(args.tokens), to_group) * rows_to_token * whole_pitch;
   }
   const int64_t sums = int64_t(plan.waves) * plan.rows * 1024;
   plan.lds_bytes = static_cast<unsigned>(lds > sums ? lds : sums);
@@ -74,9 +95,9 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
               : call.type == RUYAMD_DTYPE_F16 ? LaunchStreamInt4F16(stream, args, plan)
                                               : LaunchStreamInt4F32(stream, args, plan);
   } else {
-    *status = call.type == RUYAMD_DTYPE_BF16  ? LaunchStreamScaling<false, RUYAMD_DTYPE_BF16, Scaling::kWide>(stream, args, plan)
-              : call.type == RUYAMD_DTYPE_F16 ? LaunchStreamScaling<false, RUYAMD_DTYPE_F16, Scaling::kWide>(stream, args, plan)
-                                              : LaunchStreamScaling<false, RUYAMD_DTYPE_F32, Scaling::kWide>(stream, args, plan);
+    *status = call.type == RUYAMD_DTYPE_BF16  ? LaunchStreamFloat<RUYAMD_DTYPE_BF16>(stream, args, plan)
+              : call.type == RUYAMD_DTYPE_F16 ? LaunchStreamFloat<RUYAMD_DTYPE_F16>(stream, args, plan)
+                                              : LaunchStreamFloat<RUYAMD_DTYPE_F32>(stream, args, plan);
   }
   return true;
 }
