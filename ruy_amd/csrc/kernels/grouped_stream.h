@@ -40,10 +40,12 @@ struct StreamArgs {
   int slab_bytes;    // of one of the two buffers (kSlabs)
   int tokens;        // to a workgroup, at most
   int scale_shift;   // Scaling::kWide: logarithm of the depth positions to a scale
+  int scales_at, scale_pitch;  // scales of 4-bit weights in LDS: bytes, values from a row to the next
+  int zeros_at, zero_pitch;    // and their zero points
 };
 
 // LDS that a workgroup of these kernels may take.
-constexpr int kStreamLds = 144 << 10;
+constexpr int kStreamLds = 156 << 10;
 
 // How weights of each kind and their tokens come. A wave takes 128 bytes of every row
 // at a time, a whole line of the caches (4-bit weights slab by slab: 64, half the tokens
@@ -72,19 +74,17 @@ enum class Scaling { kWide, k64, k32, kAny };
 // Waves along the rows of a workgroup of the kernels that go slab by slab.
 constexpr int RowWaves(bool slabs, int cols) { return slabs && cols > 1 ? 2 : 1; }
 
-// (kF32Scales, kZeroPoints: as template arguments since a load that depends on a branch
-// has the wave wait for all its loads, where it should wait for a chunk's: 16384 x 16384 half,
-// one token, 37 us with branches, FIGURE without.)
-template <bool kInt4, int kType, int kRows, int kCols, Scaling kScaling, bool kSlabs, bool kF32Scales, bool kZeroPoints>
+template <bool kInt4, int kType, int kCols, Scaling kScaling, bool kSlabs, bool kZeroPoints>
 __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   using T = Stream<kInt4, kType, kSlabs>;
   constexpr int kMostTokens = T::kTokens * kCols;
   constexpr int kRowWaves = RowWaves(kSlabs, kCols);
+  constexpr int kRows = 1;  // blocks of 16 rows to a wave
   // Scales to a chunk, steps to a scale.
   constexpr int kScales =
       T::kWeightLoads * (!kInt4 || kScaling == Scaling::kWide ? 1 : kScaling == Scaling::k64 ? 2 : 4);
   constexpr int kStepsToScale = kInt4 ? T::kSteps / kScales : 1;
-  constexpr bool kScalesSideBySide = kScaling == Scaling::k64 || kScaling == Scaling::k32;
+  constexpr bool kScalesInLds = kInt4 && kScaling != Scaling::kAny;
   constexpr bool kHalf = kType == RUYAMD_DTYPE_F16;
   constexpr int kMmaType = kHalf ? RUYAMD_DTYPE_F16 : RUYAMD_DTYPE_BF16;  // of 4-bit weights
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -128,67 +128,24 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   }
   const int row_bytes = kInt4 ? (c.k + 1) / 2 : c.k * T::kBytes;
   const int row_scale_count = kInt4 ? (c.k + w.group_size - 1) / w.group_size : 0;
+  const bool f32_scales = w.scale_type == RUYAMD_DTYPE_F32;
 
   struct Held {
     v4i weights[kRows][T::kWeightLoads];
-    uint32_t scales[kRows][kScales], zeros[kRows][kScalesSideBySide ? (kScales + 3) / 4 : kScales];
+    uint32_t scales[kScalesInLds ? 1 : kRows][kScales], zeros[kScalesInLds ? 1 : kRows][kScales];  // (Scaling::kAny)
   };
-  // Loads never reach past the end of a row (which has 16 bytes and, side by side,
-  // kScales scales at least): what would is read from its last bytes, and moved to
-  // where it belongs by Place.
-  // (Scales first: a wave that waits for its weights then waits for all of a chunk, and
-  // for next to nothing of the one behind it, whether there are zero points or not.)
+  // Loads never reach past the end of a row (which has 16 bytes at least): what would is
+  // read from its last bytes, and moved to where it belongs by Place.
   const auto load = [&](int chunk, Held& h) __attribute__((always_inline)) {
-    if constexpr (kInt4) {
-      if constexpr (kScalesSideBySide) {
-        const int at = min(chunk * kScales, row_scale_count - kScales);
+    if constexpr (kInt4 && !kScalesInLds) {
+#pragma unroll
+      for (int g = 0; g < kScales; ++g) {
+        const int at = min(chunk * T::kChunk + g * (T::kChunk / kScales), c.k - 1) / w.group_size;
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          v4i x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-          if constexpr (kF32Scales) {
-            const float* p = static_cast<const float*>(w.scales) + row_scales[r] + at;
-            if constexpr (kScales == 2) {
-              const v2i both = *reinterpret_cast<const v2i_unaligned*>(p);
-              x = v4i{both[0], both[1], 0, 0};
-            } else {
-              x = *reinterpret_cast<const granule::v4i_unaligned*>(p);
-              if constexpr (kScales == 8) y = *reinterpret_cast<const granule::v4i_unaligned*>(p + 4);
-            }
-          } else {
-            const uint16_t* p = static_cast<const uint16_t*>(w.scales) + row_scales[r] + at;
-            if constexpr (kScales == 2) {
-              x[0] = *reinterpret_cast<const u32_unaligned*>(p);
-            } else if constexpr (kScales == 4) {
-              const v2i both = *reinterpret_cast<const v2i_unaligned*>(p);
-              x = v4i{both[0], both[1], 0, 0};
-            } else {
-              x = *reinterpret_cast<const granule::v4i_unaligned*>(p);
-            }
-          }
-#pragma unroll
-          for (int g = 0; g < kScales; ++g) h.scales[r][g] = g < 4 ? x[g & 3] : y[g & 3];
-#pragma unroll
-          for (int g = 0; g < (kScales + 3) / 4; ++g) h.zeros[r][g] = 0x08080808u;
-          if constexpr (kZeroPoints) {
-            const uint8_t* p = w.zero_points + row_scales[r] + at;
-            if constexpr (kScales == 2) h.zeros[r][0] = p[0] | p[1] << 8;
-#pragma unroll
-            for (int g = 0; g < kScales / 4; ++g) h.zeros[r][g] = reinterpret_cast<const u32_unaligned*>(p)[g];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int g = 0; g < kScales; ++g) {
-          const int k = min(chunk * T::kChunk + g * (T::kChunk / kScales), c.k - 1);
-          const int at = kScaling == Scaling::kWide ? k >> args.scale_shift : k / w.group_size;
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            if constexpr (kF32Scales)
-              h.scales[r][g] = static_cast<const uint32_t*>(w.scales)[row_scales[r] + at];
-            else
-              h.scales[r][g] = static_cast<const uint16_t*>(w.scales)[row_scales[r] + at];
-            h.zeros[r][g] = kZeroPoints ? w.zero_points[row_scales[r] + at] : 8;
-          }
+          h.scales[r][g] = f32_scales ? static_cast<const uint32_t*>(w.scales)[row_scales[r] + at]
+                                      : static_cast<const uint16_t*>(w.scales)[row_scales[r] + at];
+          h.zeros[r][g] = kZeroPoints ? w.zero_points[row_scales[r] + at] : 8;
         }
       }
     }
@@ -207,44 +164,60 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) h.weights[r][i] = granule::PlaceGranule(h.weights[r][i], at, row_bytes);
     }
-    if constexpr (kInt4 && kScalesSideBySide) {
-      for (int past = (chunk + 1) * kScales - row_scale_count; past > 0; --past)
+  };
+  // A scale's bits, read as its type, as a number.
+  const auto as_float = [&](uint32_t bits) __attribute__((always_inline)) -> float {
+    const float as_half = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+    const float as_bf16 = __uint_as_float(bits << 16), as_is = __uint_as_float(bits);
+    return f32_scales ? as_is : w.scale_type == RUYAMD_DTYPE_BF16 ? as_bf16 : as_half;
+  };
+  // Scales and zero points of a workgroup's rows are put into LDS first, as numbers and zeros behind
+  // the last. (Where they lie they are 2 bytes of a line that has gone from the caches when the
+  // next 2 are wanted: 16384 x 16384 half, one token, 36 us with scales read
+  // where they lie, 29.7 with these.)
+  const float* const lds_scales = reinterpret_cast<const float*>(lds + args.scales_at);
+  const uint8_t* const lds_zeros = reinterpret_cast<const uint8_t*>(lds + args.zeros_at);
+  const auto put_scales = [&]() __attribute__((always_inline)) {
+    if constexpr (kScalesInLds) {
+      const int padded = chunks * kScales, all_waves = depth_waves * row_waves;
+      float* const to = reinterpret_cast<float*>(lds + args.scales_at);
+      uint8_t* const zeros_to = reinterpret_cast<uint8_t*>(lds + args.zeros_at);
+      constexpr int kAtOnce = 4;
+      for (int row = wave * kAtOnce; row < work_rows; row += all_waves * kAtOnce)
+        for (int g = lane; g < padded; g += 64) {
+          uint32_t bits[kAtOnce], zeros[kAtOnce];
+          // (A scale that several chunks share is there several times.)
+          const int at = kScaling == Scaling::kWide ? static_cast<int>(int64_t(g) * 128 >> args.scale_shift) : g;
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          h.zeros[r][0] >>= 8;
-          if constexpr (kScales == 8) {
-            h.zeros[r][0] |= h.zeros[r][1] << 24;
-            h.zeros[r][1] >>= 8;
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t from = tile.group * w.scales_matrix_stride + min(row0 + row + i, c.m - 1) * w.scale_stride + at;
+            bits[i] = zeros[i] = 0;
+            if (at < row_scale_count) {
+              bits[i] = f32_scales ? static_cast<const uint32_t*>(w.scales)[from] : static_cast<const uint16_t*>(w.scales)[from];
+              if constexpr (kZeroPoints) zeros[i] = w.zero_points[from];
+            }
           }
-          if constexpr (kF32Scales) {
 #pragma unroll
-            for (int g = 0; g < kScales; ++g) h.scales[r][g] = g + 1 < kScales ? h.scales[r][g + 1] : 0;
-          } else {
-#pragma unroll
-            for (int g = 0; g < kScales / 2; ++g)
-              h.scales[r][g] = h.scales[r][g] >> 16 | (g + 1 < kScales / 2 ? h.scales[r][g + 1] << 16 : 0);
+          for (int i = 0; i < kAtOnce; ++i) {
+            to[(row + i) * args.scale_pitch + g] = as_float(bits[i]);
+            if constexpr (kZeroPoints) zeros_to[(row + i) * args.zero_pitch + g] = static_cast<uint8_t>(zeros[i]);
           }
         }
     }
   };
-  const bool bf16_scales = w.scale_type == RUYAMD_DTYPE_BF16;
-  const auto scales_of = [&](const Held& h, float (&scale)[kRows][kScales]) __attribute__((always_inline)) {
+  const auto scales_of = [&](const Held& h, int chunk, float (&scale)[kRows][kScales], uint32_t (&zero)[kRows][kScales])
+                             __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int r = 0; r < kRows; ++r) {
+      const int row = (row_wave * kRows + r) * 16 + l;
 #pragma unroll
       for (int g = 0; g < kScales; ++g) {
-        if constexpr (kF32Scales) {
-          scale[r][g] = __uint_as_float(h.scales[r][g]);
-        } else {
-          const uint32_t bits = kScalesSideBySide ? h.scales[r][g / 2] >> (16 * (g & 1)) : h.scales[r][g];
-          const float as_half = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
-          const float as_bf16 = __uint_as_float(bits << 16);
-          scale[r][g] = bf16_scales ? as_bf16 : as_half;
-        }
+        scale[r][g] = kScalesInLds ? lds_scales[row * args.scale_pitch + chunk * kScales + g] : as_float(h.scales[r][g]);
+        zero[r][g] = 8;
+        if constexpr (kZeroPoints)
+          zero[r][g] = kScalesInLds ? lds_zeros[row * args.zero_pitch + chunk * kScales + g] : h.zeros[r][g];
       }
-  };
-  const auto zero_of = [&](const Held& h, int r, int g) __attribute__((always_inline)) -> uint32_t {
-    return kScalesSideBySide ? h.zeros[r][g / 4] >> (8 * (g & 3)) & 0xffu : h.zeros[r][g];
+    }
   };
 
   // Unit u of a token (kUnit values from depth position u * kUnit on), zeros past the depth.
@@ -264,31 +237,28 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   const auto fetch = [&](int token, int u) __attribute__((always_inline)) -> Unit {
     Unit unit;
     const int k = u * T::kUnit;
-    if (c.rhs_rs == 1 && k + T::kUnit <= c.k) return fetch_inside(token, u);
+    constexpr int kValues = 16 / T::kBytes;
+    if (c.rhs_rs == 1) {
+      const uint8_t* p = token_data + token * c.rhs_cs * T::kBytes;
+#pragma unroll
+      for (int i = 0; i < T::kUnitLoads; ++i) {
+        const int at = (k + i * kValues) * T::kBytes;
+        unit.x[i] = granule::PlaceGranule(granule::LoadGranule<false>(p, at, c.k * T::kBytes), at, c.k * T::kBytes);
+      }
+      return unit;
+    }
     const uint8_t* p = token_data + (token * c.rhs_cs + k * c.rhs_rs) * T::kBytes;
-    // One value after the other, each pushed in behind those before it.
 #pragma unroll
     for (int i = 0; i < T::kUnitLoads; ++i) {
-      constexpr int kValues = 16 / T::kBytes;
       v4i x = {0, 0, 0, 0};
-#pragma unroll 1
+#pragma unroll
       for (int e = 0; e < kValues; ++e) {
-        uint32_t v = 0;
         const int at = i * kValues + e;
-        if (k + at < c.k) {
-          if constexpr (T::kBytes == 4)
-            v = *reinterpret_cast<const uint32_t*>(p + at * c.rhs_rs * 4);
-          else
-            v = *reinterpret_cast<const uint16_t*>(p + at * c.rhs_rs * 2);
-        }
-        if constexpr (T::kBytes == 4) {
-          x = v4i{x[1], x[2], x[3], static_cast<int>(v)};
-        } else {
-          x = v4i{static_cast<int>(__builtin_amdgcn_alignbyte(x[1], x[0], 2)),
-                  static_cast<int>(__builtin_amdgcn_alignbyte(x[2], x[1], 2)),
-                  static_cast<int>(__builtin_amdgcn_alignbyte(x[3], x[2], 2)),
-                  static_cast<int>(__builtin_amdgcn_alignbyte(v, x[3], 2))};
-        }
+        if (k + at >= c.k) continue;
+        if constexpr (T::kBytes == 4)
+          x[e] = *reinterpret_cast<const int*>(p + at * c.rhs_rs * 4);
+        else
+          x[e / 2] |= static_cast<int>(uint32_t(*reinterpret_cast<const uint16_t*>(p + at * c.rhs_rs * 2)) << (16 * (e & 1)));
       }
       unit.x[i] = x;
     }
@@ -392,7 +362,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   };
 
   // `at`: the chunk's place in the tokens' rows.
-  const auto use = [&](const Held& h, const char* at) __attribute__((always_inline)) {
+  const auto use = [&](const Held& h, int chunk, const char* at) __attribute__((always_inline)) {
     if constexpr (!kInt4) {
 #pragma unroll
       for (int j = 0; j < T::kSteps; ++j)
@@ -405,7 +375,8 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
     } else {
       v4i words[kRows][T::kWeightLoads];
       float scale[kRows][kScales];
-      scales_of(h, scale);
+      uint32_t zero[kRows][kScales];
+      scales_of(h, chunk, scale, zero);
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
@@ -428,14 +399,14 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
           }
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
-            const v4i b = kHalf ? less_zero(words[r][j / 4][j % 4], zero_of(h, r, g)) : sixteen_and(words[r][j / 4][j % 4]);
+            const v4i b = kHalf ? less_zero(words[r][j / 4][j % 4], zero[r][g]) : sixteen_and(words[r][j / 4][j % 4]);
 #pragma unroll
             for (int t = 0; t < kCols; ++t) Mma<kMmaType>(x[t], b, sum[r][t]);
           }
         }
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          const float away = -16.0f - static_cast<float>(zero_of(h, r, g));
+          const float away = -16.0f - static_cast<float>(zero[r][g]);
 #pragma unroll
           for (int t = 0; t < kCols; ++t)
 #pragma unroll
@@ -456,19 +427,25 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
                            : (whole_chunks - depth_wave + depth_waves - 1) / depth_waves;
   // The depth begins at another place in every 16 * kRows rows and goes round: rows
   // often lie a power of two apart, and whoever goes through theirs side by side, from
-  // the same place on, asks the same few memory channels.
-  const int first_turn = turns > 0 ? (kSlabs ? tile.m : tile.m * row_waves + row_wave) % turns : 0;
+  // the same place on, asks the same few memory channels. (Places by a multiplicative hash; one after
+  // the other they meet again at some row lengths. 16384 rows of 8 KiB read alone, 4 waves
+  // along the depth: the same place 28 us, one after the other 33, hashed 25.7.)
+  const uint32_t unit = (static_cast<uint32_t>(tile.group) * args.tiles_m + tile.m) * row_waves + (kSlabs ? 0 : row_wave);
+  const int first_turn = turns > 0 ? static_cast<int>((unit * 2654435761u >> 12) % static_cast<uint32_t>(turns)) : 0;
   const auto place_of = [&](int turn) __attribute__((always_inline)) -> int {  // (past the last: the last)
     const int at = min(turn, turns - 1) + first_turn;
     return at < turns ? at : at - turns;
   };
   // The loop's loads are issued whatever comes (past the end once more the last chunk):
   // a load that may or may not have been issued is one for which everything is waited for.
-  Held held[2];
+  Held held[2], last;
+  const bool has_last = !kSlabs && whole_chunks < chunks && (whole_chunks & (depth_waves - 1)) == depth_wave;
+  if (has_last) load(whole_chunks, last);
   if (turns > 0) {
     load(depth_wave + place_of(0) * depth_waves, held[0]);
     load(depth_wave + place_of(1) * depth_waves, held[1]);
   }
+  put_scales();
   if constexpr (kSlabs) {
     const int slab_units = depth_waves * T::kChunkUnits, unit_bits = __builtin_ctz(slab_units);  // (a power of two)
     constexpr int kPieces = (kMostTokens * T::kChunkUnits + 64 * kRowWaves - 1) / (64 * kRowWaves);
@@ -497,7 +474,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         __syncthreads();
         put_slab(1 - d);
         fetch_slab(place_of(n + 2));
-        use(held[d], lds + d * args.slab_bytes + depth_wave * kLdsChunk);
+        use(held[d], depth_wave + place_of(n) * depth_waves, lds + d * args.slab_bytes + depth_wave * kLdsChunk);
         load(depth_wave + place_of(n + 2) * depth_waves, held[d]);
       };
       for (int n = 0;;) {
@@ -517,7 +494,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
       if (depth_wave < left) {
         load(done + depth_wave, held[0]);
         place(done + depth_wave, held[0]);
-        use(held[0], lds + depth_wave * kLdsChunk);
+        use(held[0], done + depth_wave, lds + depth_wave * kLdsChunk);
       }
     }
   } else {
@@ -538,7 +515,8 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
     __syncthreads();
     if (turns > 0) {
       const auto turn = [&](int n, auto d) __attribute__((always_inline)) {
-        use(held[d], lds + (depth_wave + place_of(n) * depth_waves) * kLdsChunk);
+        const int chunk = depth_wave + place_of(n) * depth_waves;
+        use(held[d], chunk, lds + chunk * kLdsChunk);
         load(depth_wave + place_of(n + 2) * depth_waves, held[d]);
       };
       for (int n = 0;;) {
@@ -548,10 +526,9 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         if (++n == turns) break;
       }
     }
-    if (whole_chunks < chunks && whole_chunks % depth_waves == depth_wave) {
-      load(whole_chunks, held[0]);
-      place(whole_chunks, held[0]);
-      use(held[0], lds + whole_chunks * kLdsChunk);
+    if (has_last) {
+      place(whole_chunks, last);
+      use(last, whole_chunks, lds + whole_chunks * kLdsChunk);
     }
   }
 
@@ -575,7 +552,8 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         load(chunk, h);
         place(chunk, h);
         float scale[kRows][kScales];
-        scales_of(h, scale);
+        uint32_t zero[kRows][kScales];
+        scales_of(h, chunk, scale, zero);
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
 #pragma unroll
@@ -593,10 +571,9 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
               for (int r = 0; r < kRows; ++r) {
                 const uint32_t word = h.weights[r][g * kStepsToScale / 4][0];
-                const int zero = static_cast<int>(zero_of(h, r, g));
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>(word >> (4 * e) & 15) - zero);
+                for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>(word >> (4 * e) & 15) - static_cast<int>(zero[r][g]));
                 v4f sum = {0, 0, 0, 0};
                 if constexpr (T::kParts) {
 #pragma unroll
@@ -658,15 +635,15 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 struct StreamPlan {
   unsigned blocks;
   int waves;
-  int rows, cols;  // kRows and kCols of the kernel
+  int cols;  // kCols of the kernel
   bool slabs;
   Scaling scaling;
   unsigned lds_bytes;
 };
 
-template <bool kInt4, int kType, int kRows, int kCols, Scaling kScaling, bool kSlabs, bool kF32Scales, bool kZeroPoints>
+template <bool kInt4, int kType, int kCols, Scaling kScaling, bool kSlabs, bool kZeroPoints>
 hipError_t LaunchStreamKernel(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
-  auto* const kernel = &GroupedStreamKernel<kInt4, kType, kRows, kCols, kScaling, kSlabs, kF32Scales, kZeroPoints>;
+  auto* const kernel = &GroupedStreamKernel<kInt4, kType, kCols, kScaling, kSlabs, kZeroPoints>;
   static const hipError_t attribute = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, kStreamLds);
   if (attribute != hipSuccess) return attribute;
@@ -674,28 +651,21 @@ hipError_t LaunchStreamKernel(hipStream_t stream, const StreamArgs& args, const 
   return hipGetLastError();
 }
 
-template <int kType, Scaling kScaling, bool kF32Scales, bool kZeroPoints>
+template <int kType, Scaling kScaling, bool kZeroPoints>
 hipError_t LaunchStreamInt4Of(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
   if (plan.cols == 4)
-    return LaunchStreamKernel<true, kType, 1, 4, kScaling, true, kF32Scales, kZeroPoints>(stream, args, plan);
+    return LaunchStreamKernel<true, kType, 4, kScaling, true, kZeroPoints>(stream, args, plan);
   if (plan.cols == 2)
-    return LaunchStreamKernel<true, kType, 1, 2, kScaling, true, kF32Scales, kZeroPoints>(stream, args, plan);
+    return LaunchStreamKernel<true, kType, 2, kScaling, true, kZeroPoints>(stream, args, plan);
   if (plan.slabs)
-    return LaunchStreamKernel<true, kType, 1, 1, kScaling, true, kF32Scales, kZeroPoints>(stream, args, plan);
-  if constexpr (kScaling != Scaling::kAny)
-    if (plan.rows == 2)
-      return LaunchStreamKernel<true, kType, 2, 1, kScaling, false, kF32Scales, kZeroPoints>(stream, args, plan);
-  return LaunchStreamKernel<true, kType, 1, 1, kScaling, false, kF32Scales, kZeroPoints>(stream, args, plan);
+    return LaunchStreamKernel<true, kType, 1, kScaling, true, kZeroPoints>(stream, args, plan);
+  return LaunchStreamKernel<true, kType, 1, kScaling, false, kZeroPoints>(stream, args, plan);
 }
 
 template <int kType, Scaling kScaling>
 hipError_t LaunchStreamScaling(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
-  if (args.w.scale_type == RUYAMD_DTYPE_F32) {
-    if (args.w.zero_points) return LaunchStreamInt4Of<kType, kScaling, true, true>(stream, args, plan);
-    return LaunchStreamInt4Of<kType, kScaling, true, false>(stream, args, plan);
-  }
-  if (args.w.zero_points) return LaunchStreamInt4Of<kType, kScaling, false, true>(stream, args, plan);
-  return LaunchStreamInt4Of<kType, kScaling, false, false>(stream, args, plan);
+  if (args.w.zero_points) return LaunchStreamInt4Of<kType, kScaling, true>(stream, args, plan);
+  return LaunchStreamInt4Of<kType, kScaling, false>(stream, args, plan);
 }
 
 template <int kType>
@@ -716,12 +686,10 @@ hipError_t LaunchStreamInt4(hipStream_t stream, const StreamArgs& args, const St
 template <int kType>
 hipError_t LaunchStreamFloat(hipStream_t stream, const StreamArgs& args, const StreamPlan& plan) {
   if (plan.cols == 2)
-    return LaunchStreamKernel<false, kType, 1, 2, Scaling::kWide, true, false, false>(stream, args, plan);
+    return LaunchStreamKernel<false, kType, 2, Scaling::kWide, true, false>(stream, args, plan);
   if (plan.slabs)
-    return LaunchStreamKernel<false, kType, 1, 1, Scaling::kWide, true, false, false>(stream, args, plan);
-  if (plan.rows == 2)
-    return LaunchStreamKernel<false, kType, 2, 1, Scaling::kWide, false, false, false>(stream, args, plan);
-  return LaunchStreamKernel<false, kType, 1, 1, Scaling::kWide, false, false, false>(stream, args, plan);
+    return LaunchStreamKernel<false, kType, 1, Scaling::kWide, true, false>(stream, args, plan);
+  return LaunchStreamKernel<false, kType, 1, Scaling::kWide, false, false>(stream, args, plan);
 }
 
 // (Each in a file of its own.)

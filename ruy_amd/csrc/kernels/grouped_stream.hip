@@ -1,7 +1,6 @@
 // The streaming kernels of weights in the tokens' own type, and the choice of a
 // streaming kernel.
 #include "grouped_stream.h"
-#include <cstdlib>
 
 namespace ruyamd {
 namespace grouped {
@@ -28,7 +27,9 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   const int64_t whole_pitch = int64_t((call.k + depth_to_chunk - 1) / depth_to_chunk) * (int4 ? 512 : 128) + 16;
   const int64_t room = 128 << 10;
   const int64_t fit = room / (whole_pitch * rows_to_token);
-  const int64_t to_group = call.offsets ? block_tokens : call.n;  // (a group may have many more than others)
+  // (A group may have more than its share: room for four times as many, which several
+  // workgroups then read the weights for where it has more still.)
+  const int64_t to_group = call.offsets ? min(int64_t(block_tokens), 4 * per_group) : call.n;
   if (call.rhs_rs != 1) {
     if (fit == 0) return false;
     plan.cols = 1;
@@ -39,56 +40,74 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   }
   const int chunk = int4 && plan.slabs ? 128 : depth_to_chunk, chunks = (call.k + chunk - 1) / chunk;
   const int chunk_bytes = int4 ? 2 * chunk : 128;  // of a token in LDS
-  args.tokens = static_cast<int>(plan.slabs ? plan.cols * block_tokens : min(fit, int64_t(block_tokens)));
+  args.tokens = static_cast<int>(plan.slabs ? plan.cols * block_tokens : min(fit, min(int64_t(block_tokens), to_group)));
 
   plan.scaling = Scaling::kWide;
   args.scale_shift = 31;
   if (int4 && weights->group_size < call.k) {
-    const int size = weights->group_size, scales = (call.k + size - 1) / size;
+    const int size = weights->group_size;
     args.scale_shift = __builtin_ctz(size);
     plan.scaling = size >= 128 && (size & (size - 1)) == 0 ? Scaling::kWide
-                   : size == 64 && scales >= chunk / 64    ? Scaling::k64
-                   : size == 32 && scales >= chunk / 32    ? Scaling::k32
+                   : size == 64                            ? Scaling::k64
+                   : size == 32                            ? Scaling::k32
                                                            : Scaling::kAny;
   }
 
-  // Waves: 16 to a CU if the rows give them, 8 to a workgroup, along the rows first, then
-  // along the depth.
+  // Waves: 8 to a workgroup, and 16 to a CU if the rows give them, along the rows first, then
+  // along the depth; fewer rows where what goes with them into LDS is too much. (16384 x
+  // 16384, one token: 16 waves to a CU 29.7 us, 8 30.7, 4 48. Two blocks of 16 rows to a wave
+  // are no faster anywhere, and slower where there are few rows.)
   int row_waves = RowWaves(plan.slabs, plan.cols), depth_waves = 8 / row_waves;
-  plan.rows = plan.slabs || plan.scaling == Scaling::kAny ? 1 : 2;
-  if (const char* e = getenv("S_ROWS")) if (plan.rows == 2) plan.rows = atoi(e);
-  while (plan.rows > 1 && (call.m + 16 * plan.rows * row_waves - 1) / (16 * plan.rows * row_waves) * busy < call.compute_units)
-    plan.rows /= 2;
   if (!plan.slabs) {
-    const int64_t units = (call.m + 16 * plan.rows - 1) / (16 * plan.rows) * busy;
-    int per_cu = 16;
-    if (const char* e = getenv("S_WAVES")) per_cu = atoi(e);
-    while (depth_waves > 1 && units * depth_waves > int64_t(per_cu) * call.compute_units) depth_waves /= 2;
+    const int64_t units = (int64_t(call.m) + 15) / 16 * busy;
+    while (depth_waves > 1 && units * depth_waves > int64_t(16) * call.compute_units) depth_waves /= 2;
     row_waves = 8 / depth_waves;
   }
   while (depth_waves > 1 && chunks < depth_waves) depth_waves /= 2;
+  const int padded_scales = chunks * (chunk / (plan.scaling == Scaling::kWide ? 128 : plan.scaling == Scaling::k64 ? 64 : 32));
+  // (Odd numbers of words: 16 rows side by side reach 16 banks.)
+  args.scale_pitch = padded_scales | 1;
+  args.zero_pitch = ((padded_scales + 3) / 4 | 1) * 4;
+  int64_t tokens_lds = 0, scales_lds = 0, zeros_lds = 0;
+  int work_rows = 0;
+  for (;;) {
+    work_rows = 16 * row_waves;
+    if (plan.slabs) {
+      args.pitch = depth_waves * chunk_bytes + 16;
+      args.slab_bytes = 16 * plan.cols * args.pitch;
+      tokens_lds = 2 * args.slab_bytes;
+    } else {
+      args.pitch = static_cast<int>(whole_pitch);
+      args.slab_bytes = 0;
+      tokens_lds = int64_t(args.tokens) * rows_to_token * whole_pitch;
+    }
+    if (int4 && plan.scaling != Scaling::kAny) {
+      scales_lds = int64_t(work_rows) * args.scale_pitch * 4;
+      zeros_lds = weights->zero_points ? int64_t(work_rows) * args.zero_pitch : 0;
+    }
+    if (tokens_lds + scales_lds + zeros_lds <= kStreamLds) break;
+    if (!plan.slabs && row_waves > 1) {
+      row_waves /= 2;
+      if (depth_waves * 2 <= chunks) depth_waves *= 2;
+    } else if (plan.slabs && depth_waves > 1) {
+      depth_waves /= 2;
+    } else {
+      plan.scaling = Scaling::kAny;
+      scales_lds = zeros_lds = 0;
+    }
+  }
+  args.scales_at = static_cast<int>(tokens_lds);
+  args.zeros_at = static_cast<int>(tokens_lds + scales_lds);
   plan.waves = depth_waves * row_waves;
   args.depth_waves = depth_waves;
   args.row_waves = row_waves;
-  const int work_rows = 16 * plan.rows * row_waves;
   args.tiles_m = (call.m + work_rows - 1) / work_rows;
+  const int64_t lds = tokens_lds + scales_lds + zeros_lds, sums = int64_t(plan.waves) * 1024;
+  plan.lds_bytes = static_cast<unsigned>(lds > sums ? lds : sums);
   const int64_t slots = call.offsets ? call.n / args.tokens + busy : (call.n + args.tokens - 1) / args.tokens;
   const int64_t blocks = (slots * args.tiles_m + 7) / 8 * 8;
   if (blocks > 0x7fffffff) return false;
   plan.blocks = static_cast<unsigned>(blocks);
-
-  int64_t lds;
-  if (plan.slabs) {
-    args.pitch = depth_waves * chunk_bytes + 16;
-    args.slab_bytes = 16 * plan.cols * args.pitch;
-    lds = 2 * args.slab_bytes;
-  } else {
-    args.pitch = static_cast<int>(whole_pitch);
-    args.slab_bytes = 0;
-    lds = min(int64_t(args.tokens), to_group) * rows_to_token * whole_pitch;
-  }
-  const int64_t sums = int64_t(plan.waves) * plan.rows * 1024;
-  plan.lds_bytes = static_cast<unsigned>(lds > sums ? lds : sums);
 
   if (int4) {
     *status = call.type == RUYAMD_DTYPE_BF16  ? LaunchStreamInt4Bf16(stream, args, plan)
