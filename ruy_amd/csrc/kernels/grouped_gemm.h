@@ -114,9 +114,10 @@ __device__ __forceinline__ void Mma(const v4i& a, const v4i& b, v4f& acc) {
 
 // One side of the tile: how it is laid out in LDS, loaded and read. `kRows` rows
 // of the tile in `kWaveRows`-row pieces, one to a wave, of kBlocks blocks of 16.
-template <int kType, Runs kRuns, int kRows, int kBlocks, bool kPermuted, int kWaves>
+template <int kType, Runs kRuns, int kTileRows, int kBlocks, bool kPermuted, int kWaves>
 struct TileSide {
   using E = Element<kType>;
+  static constexpr int kRows = kTileRows;
   static constexpr int kBytes = kRows * 128;                 // in LDS, per step
   static constexpr int kLoads = kBytes / 1024 / kWaves;      // per wave and step
   static constexpr int kRunGranules = kRuns == Runs::kPlain ? 8 : kRows / E::kGranule;
@@ -258,7 +259,9 @@ __device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int
 // registers. Otherwise they are read 16 bytes a lane from wherever they begin, the
 // granule in which a run ends put in its place (granule.h), and written to LDS.
 template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect>
-__global__ __launch_bounds__(64 * kWavesM * kWavesN) void GroupedGemmKernel(GemmArgs p) {
+// (At least two waves to a SIMD: with more registers than that leaves it the compiler puts the accumulators into the
+// second register file and moves them there and back on every step.)
+__global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(GemmArgs p) {
   using E = Element<kType>;
   constexpr int kWaves = kWavesM * kWavesN;
   constexpr int kTileM = kWavesM * kBlocksM * 16, kTileN = kWavesN * kBlocksN * 16;
@@ -382,51 +385,90 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN) void GroupedGemmKernel(Gemm
       if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
     }
   } else {
-    // A granule of a run of `length` values that begins at `run`, from place `at`
-    // on, zeros past its end.
-    const auto load = [&](const char* run, int at, int length) __attribute__((always_inline)) -> v4i {
-      const int bytes = length * E::kBytes, k = at * E::kBytes;
-      if (k >= bytes) return v4i{0, 0, 0, 0};
-      if (bytes < 16) return granule::LoadGranule<true>(reinterpret_cast<const uint8_t*>(run), k, bytes);
-      const v4i x = granule::LoadGranule<false>(reinterpret_cast<const uint8_t*>(run), k, bytes);
-      return k + 16 <= bytes ? x : granule::PlaceGranule(x, k, bytes);
+    // A granule is read where it lies, or, where it would reach past the end of its
+    // run, from the run's last 16 bytes (a run has as many); Put then moves it to its place and
+    // zeroes what lies past the depth. (What lies past the tile's sides
+    // ends up in rows of the tile that are not stored.)
+    struct Place {
+      const char* run;
+      int at, length;  // in bytes, of the run
     };
-    const auto side_load = [&](auto side, int n, const char* base, Runs runs, int64_t pitch, int here, int s) __attribute__((always_inline)) -> v4i {
+    const auto place_of = [&](auto side, int n, const Side& from, Runs runs, bool dealt_rows, int first, int here, int s)
+                              __attribute__((always_inline)) -> Place {
       using T = decltype(side);
-      const int run = T::RunOf(n, wave, lane), granule = T::GranuleOf(n, wave, lane);
-      const int k0 = s * E::kDepth;
-      if (runs == Runs::kPlain)
-        return load(base + min(run, here - 1) * pitch * E::kBytes, k0 + granule * E::kGranule, depth);
-      if (k0 + run >= depth) return v4i{0, 0, 0, 0};
-      return load(base + (k0 + run) * pitch * E::kBytes, granule * E::kGranule, here);
+      const int run = T::RunOf(n, wave, lane), granule = T::GranuleOf(n, wave, lane), k0 = s * E::kDepth;
+      const int64_t row = first + (columns && dealt_rows ? range.begin : 0), k = columns ? 0 : range.begin;
+      const int64_t group = columns && !dealt_rows ? tile.group * from.group_stride : 0;
+      Place p2;
+      int64_t runs_from;
+      if (runs == Runs::kPlain) {
+        runs_from = row + min(run, here - 1);
+        p2.at = static_cast<int>(k) + k0 + granule * E::kGranule;
+        p2.length = p.depth;
+      } else {
+        runs_from = k + min(k0 + run, depth - 1);
+        p2.at = static_cast<int>(row) + granule * E::kGranule;
+        p2.length = from.count;
+      }
+      p2.run = static_cast<const char*>(from.data) + (group + runs_from * from.pitch) * E::kBytes;
+      p2.at *= E::kBytes;
+      p2.length *= E::kBytes;
+      return p2;
+    };
+    const auto load = [](const Place& from) __attribute__((always_inline)) -> v4i {
+      return *reinterpret_cast<const granule::v4i_unaligned*>(from.run + min(from.at, from.length - 16));
     };
     v4i held_m[M::kLoads], held_n[N::kLoads];
     const auto fetch = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int n = 0; n < M::kLoads; ++n) held_m[n] = side_load(M(), n, base_m, kRunsM, p.m.pitch, here_m, s);
+      for (int n = 0; n < M::kLoads; ++n) held_m[n] = load(place_of(M(), n, p.m, kRunsM, false, m0, here_m, s));
 #pragma unroll
-      for (int n = 0; n < N::kLoads; ++n) held_n[n] = side_load(N(), n, base_n, kRunsN, p.n.pitch, here_n, s);
+      for (int n = 0; n < N::kLoads; ++n) held_n[n] = load(place_of(N(), n, p.n, kRunsN, true, n0, here_n, s));
     };
-    const auto put = [&](int stage) __attribute__((always_inline)) {
+    const auto put_side = [&](auto side, v4i* held, int loads, const Side& from, Runs runs, bool dealt_rows, int first,
+                              int here, int s, char* to) __attribute__((always_inline)) {
+      using T = decltype(side);
+      const int k0 = s * E::kDepth;
+      const bool depth_ends = k0 + E::kDepth > depth;
+      const int64_t row = first + (columns && dealt_rows ? range.begin : 0);
+      const bool run_ends = runs == Runs::kAcross && row + T::kRows > from.count;
+      // (Both the same for the whole workgroup.)
+      if (depth_ends || run_ends) {
+#pragma unroll
+        for (int n = 0; n < T::kLoads; ++n) {
+          const Place where = place_of(side, n, from, runs, dealt_rows, first, here, s);
+          v4i x = granule::PlaceGranule(held[n], where.at, where.length);
+          const int run = T::RunOf(n, wave, lane), granule = T::GranuleOf(n, wave, lane);
+          const int left = runs == Runs::kPlain ? depth - k0 - granule * E::kGranule : depth - k0 - run;  // values, or runs
+          const int bytes = runs == Runs::kPlain ? left * E::kBytes : left > 0 ? 16 : 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] &= static_cast<int>(granule::LowBytes(bytes - 4 * e));
+          held[n] = x;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < T::kLoads; ++n) *reinterpret_cast<v4i*>(to + n * kWaves * 1024) = held[n];
+    };
+    const auto put = [&](int s, int stage) __attribute__((always_inline)) {
       char* to = lds + stage * kStage + (wave * 64 + lane) * 16;
-#pragma unroll
-      for (int n = 0; n < M::kLoads; ++n) *reinterpret_cast<v4i*>(to + n * kWaves * 1024) = held_m[n];
-#pragma unroll
-      for (int n = 0; n < N::kLoads; ++n) *reinterpret_cast<v4i*>(to + M::kBytes + n * kWaves * 1024) = held_n[n];
+      put_side(M(), held_m, M::kLoads, p.m, kRunsM, false, m0, here_m, s, to);
+      put_side(N(), held_n, N::kLoads, p.n, kRunsN, true, n0, here_n, s, to + M::kBytes);
     };
     if (steps > 0) {
       fetch(0);
-      put(0);
+      put(0, 0);
     }
     const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
       __syncthreads();
-      if (s + 1 < steps) fetch(s + 1);
+      fetch(min(s + 1, steps - 1));
       compute(stage);
-      if (s + 1 < steps) put(1 - stage);
+      put(min(s + 1, steps - 1), 1 - stage);
     };
-    for (int s = 0; s < steps; s += 2) {
-      step(s, std::integral_constant<int, 0>());
-      if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
+    for (int s = 0;;) {
+      if (s == steps) break;
+      step(s++, std::integral_constant<int, 0>());
+      if (s == steps) break;
+      step(s++, std::integral_constant<int, 1>());
     }
   }
 

@@ -1,35 +1,45 @@
 // Launches of the tiled kernel of grouped products.
 #include "grouped_gemm.h"
+#include <cstdlib>
 
 namespace ruyamd {
 namespace grouped {
 namespace {
 
+struct Grid {
+  unsigned blocks;
+  int tile;
+};
+
+// Four waves, two along either side; `tile` destination elements a side, 128 or 64.
 template <int kType, Runs kRunsM, Runs kRunsN, bool kDirect>
-void LaunchOne(hipStream_t stream, const GemmArgs& args, unsigned blocks) {
-  hipLaunchKernelGGL((GroupedGemmKernel<kType, kRunsM, kRunsN, 2, 2, 4, 4, kDirect>), dim3(blocks), dim3(256), 0, stream,
-                     args);
+void LaunchOne(hipStream_t stream, const GemmArgs& args, const Grid& grid) {
+  if (grid.tile == 128)
+    hipLaunchKernelGGL((GroupedGemmKernel<kType, kRunsM, kRunsN, 2, 2, 4, 4, kDirect>), dim3(grid.blocks), dim3(256), 0,
+                       stream, args);
+  else
+    hipLaunchKernelGGL((GroupedGemmKernel<kType, kRunsM, kRunsN, 2, 2, 2, 2, kDirect>), dim3(grid.blocks), dim3(256), 0,
+                       stream, args);
 }
 
 template <int kType, bool kDirect>
-void LaunchRuns(hipStream_t stream, const GemmArgs& args, Runs m, Runs n, unsigned blocks) {
-  if (m == Runs::kPlain && n == Runs::kPlain) return LaunchOne<kType, Runs::kPlain, Runs::kPlain, kDirect>(stream, args, blocks);
-  if (m == Runs::kPlain) return LaunchOne<kType, Runs::kPlain, Runs::kAcross, kDirect>(stream, args, blocks);
-  if (n == Runs::kPlain) return LaunchOne<kType, Runs::kAcross, Runs::kPlain, kDirect>(stream, args, blocks);
-  LaunchOne<kType, Runs::kAcross, Runs::kAcross, kDirect>(stream, args, blocks);
+void LaunchRuns(hipStream_t stream, const GemmArgs& args, Runs m, Runs n, const Grid& grid) {
+  if (m == Runs::kPlain && n == Runs::kPlain) return LaunchOne<kType, Runs::kPlain, Runs::kPlain, kDirect>(stream, args, grid);
+  if (m == Runs::kPlain) return LaunchOne<kType, Runs::kPlain, Runs::kAcross, kDirect>(stream, args, grid);
+  if (n == Runs::kPlain) return LaunchOne<kType, Runs::kAcross, Runs::kPlain, kDirect>(stream, args, grid);
+  LaunchOne<kType, Runs::kAcross, Runs::kAcross, kDirect>(stream, args, grid);
 }
 
 template <bool kDirect>
-void LaunchType(hipStream_t stream, const GemmArgs& args, int type, Runs m, Runs n, unsigned blocks) {
-  if (type == RUYAMD_DTYPE_BF16) return LaunchRuns<RUYAMD_DTYPE_BF16, kDirect>(stream, args, m, n, blocks);
-  if (type == RUYAMD_DTYPE_F16) return LaunchRuns<RUYAMD_DTYPE_F16, kDirect>(stream, args, m, n, blocks);
-  LaunchRuns<RUYAMD_DTYPE_F32, kDirect>(stream, args, m, n, blocks);
+void LaunchType(hipStream_t stream, const GemmArgs& args, int type, Runs m, Runs n, const Grid& grid) {
+  if (type == RUYAMD_DTYPE_BF16) return LaunchRuns<RUYAMD_DTYPE_BF16, kDirect>(stream, args, m, n, grid);
+  if (type == RUYAMD_DTYPE_F16) return LaunchRuns<RUYAMD_DTYPE_F16, kDirect>(stream, args, m, n, grid);
+  LaunchRuns<RUYAMD_DTYPE_F32, kDirect>(stream, args, m, n, grid);
 }
 
 }  // namespace
 
 bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
-  constexpr int kTile = 128;
   const int bytes = call.type == RUYAMD_DTYPE_F32 ? 4 : 2, granule = 16 / bytes;
   const bool columns = call.dealt == Dealt::kColumns;
   // The M side is the one along which dst is contiguous. (Columns that are dealt
@@ -62,8 +72,8 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
   a.dst_n_stride = swapped ? call.dst_rs : call.dst_cs;
 
   // Offsets inside a tile are 31 bits.
-  if (a.m.pitch > (int64_t(1) << 31) / (bytes * kTile) - 128 || a.n.pitch > (int64_t(1) << 31) / (bytes * kTile) - 128)
-    return false;
+  const int64_t longest = (int64_t(1) << 31) / (bytes * 128) - 128;
+  if (a.m.pitch > longest || a.n.pitch > longest) return false;
   const auto aligned = [&](const Side& s, Runs runs, bool dealt_rows) {
     if (reinterpret_cast<uintptr_t>(s.data) % 16 || s.pitch % granule || s.group_stride % granule) return false;
     // Runs along the depth end and, where it is dealt, begin anywhere.
@@ -71,19 +81,30 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
     return !(columns && dealt_rows) && s.count % granule == 0;
   };
   const bool direct = aligned(a.m, runs_m, false) && aligned(a.n, runs_n, true);
+  // Runs that the registers' way reads have 16 bytes at least.
+  const auto long_enough = [&](const Side& s, Runs runs) { return (runs == Runs::kPlain ? call.k : s.count) >= granule; };
+  if (!direct && !(long_enough(a.m, runs_m) && long_enough(a.n, runs_n))) return false;
   const int dst_bytes = a.dst_f32 ? 4 : 2;
   a.vector_stores = a.dst_m_stride == 1 && reinterpret_cast<uintptr_t>(a.dst) % (4 * dst_bytes) == 0 &&
                     a.dst_n_stride % 4 == 0 && a.dst_group_stride % 4 == 0;
 
-  const int64_t tiles_m = (int64_t(a.m.count) + kTile - 1) / kTile;
-  const int64_t tiles_n =
-      columns ? a.n.count / kTile + min(call.groups, a.n.count) : ((int64_t(a.n.count) + kTile - 1) / kTile) * call.groups;
-  const int64_t blocks = (tiles_m * tiles_n + 7) / 8 * 8;
+  const auto blocks_of = [&](int tile) {
+    const int64_t tiles_m = (int64_t(a.m.count) + tile - 1) / tile;
+    const int64_t tiles_n = columns ? a.n.count / tile + min(call.groups, a.n.count)
+                                    : ((int64_t(a.n.count) + tile - 1) / tile) * call.groups;
+    return (tiles_m * tiles_n + 7) / 8 * 8;
+  };
+  Grid grid;
+  grid.tile = blocks_of(128) >= 2 * call.compute_units ? 128 : 64;
+  const char* e = getenv("G_TILE");
+  if (e) grid.tile = atoi(e);
+  const int64_t blocks = blocks_of(grid.tile);
   if (blocks > 0x7fffffff) return false;
+  grid.blocks = static_cast<unsigned>(blocks);
   if (direct)
-    LaunchType<true>(stream, a, call.type, runs_m, runs_n, static_cast<unsigned>(blocks));
+    LaunchType<true>(stream, a, call.type, runs_m, runs_n, grid);
   else
-    LaunchType<false>(stream, a, call.type, runs_m, runs_n, static_cast<unsigned>(blocks));
+    LaunchType<false>(stream, a, call.type, runs_m, runs_n, grid);
   *status = hipGetLastError();
   return true;
 }
