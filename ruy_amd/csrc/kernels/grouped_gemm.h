@@ -123,6 +123,7 @@ struct TileSide {
   static constexpr int kRunGranules = kRuns == Runs::kPlain ? 8 : kRows / E::kGranule;
   static constexpr int kRunsPerLoad = 64 / kRunGranules;     // (0: a run takes several loads)
   static constexpr int kWaveRows = 16 * kBlocks;
+  static constexpr int kReads = kRuns == Runs::kPlain ? 1 : E::kBytes == 2 ? 2 : 4;  // of LDS, for a fragment
   static_assert(kBytes % (1024 * kWaves) == 0, "");
 
   // Row of the wave's piece that lane l (mod 16) holds of block b. Where the rows
@@ -258,7 +259,7 @@ __device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int
 // whole number of granules, so that tiles go to LDS without passing through
 // registers. Otherwise they are read 16 bytes a lane from wherever they begin, the
 // granule in which a run ends put in its place (granule.h), and written to LDS.
-template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect>
+template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages>
 // (At least two waves to a SIMD: with more registers than that leaves it the compiler puts the accumulators into the
 // second register file and moves them there and back on every step.)
 __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(GemmArgs p) {
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
   using M = TileSide<kType, kRunsM, kTileM, kBlocksM, kRunsM == Runs::kPlain, kWaves>;
   using N = TileSide<kType, kRunsN, kTileN, kBlocksN, false, kWaves>;
   constexpr int kStage = M::kBytes + N::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+  extern __shared__ __attribute__((aligned(16))) char lds[];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -313,21 +314,31 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
   const int steps = (depth + E::kDepth - 1) / E::kDepth;
 
   v4f acc[kBlocksM][kBlocksN] = {};
-  const auto compute = [&](auto stage) __attribute__((always_inline)) {
+  struct Fragments {
+    v4i m[kBlocksM], n[kBlocksN];
+  };
+  const auto read = [&](int stage, int kk, Fragments& f) __attribute__((always_inline)) {
     const char* const side_m = lds + stage * kStage;
-    const char* const side_n = side_m + M::kBytes;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      v4i a[kBlocksM], b[kBlocksN];
+    for (int j = 0; j < kBlocksN; ++j) f.n[j] = N::Fragment(side_m + M::kBytes, wave_n, j, kk, lane);
 #pragma unroll
-      for (int i = 0; i < kBlocksM; ++i) a[i] = M::Fragment(side_m, wave_m, i, kk, lane);
+    for (int i = 0; i < kBlocksM; ++i) f.m[i] = M::Fragment(side_m, wave_m, i, kk, lane);
+  };
+  const auto multiply = [&](const Fragments& f) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < kBlocksN; ++j) b[j] = N::Fragment(side_n, wave_n, j, kk, lane);
+    for (int i = 0; i < kBlocksM; ++i)
 #pragma unroll
-      for (int i = 0; i < kBlocksM; ++i)
-#pragma unroll
-        for (int j = 0; j < kBlocksN; ++j) Mma<kType>(a[i], b[j], acc[i][j]);
-    }
+      for (int j = 0; j < kBlocksN; ++j) Mma<kType>(f.m[i], f.n[j], acc[i][j]);
+  };
+  // The reads of one half of a step between the products of the other.
+  const auto interleave = [&]() __attribute__((always_inline)) {
+    constexpr int kReads = M::kReads * kBlocksM + N::kReads * kBlocksN;
+    constexpr int kProducts = kBlocksM * kBlocksN * (E::kBytes == 4 ? 4 : 1);
+    constexpr int kEach = kProducts / kReads > 0 ? kProducts / kReads : 1;
+    StaticFor<(kReads < kProducts ? kReads : kProducts)>([](auto) __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kReads / kProducts > 0 ? kReads / kProducts : 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+    });
   };
 
   if constexpr (kDirect) {
@@ -371,18 +382,43 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
           LoadToLds(to + M::kBytes + n * kWaves * 1024, depth_of(N(), n, kRunsN) < left ? off_n[n] : kNothing, rsrc_n);
       }
     };
-    if (steps > 0) issue(0, 0);
-    // A step's loads have landed in every wave, and every wave is done with
-    // the other half of LDS, when all have passed the barrier in front of it.
-    const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
-      WaitVmcnt<0>();
+    // Steps are on their way to LDS up to kStages ahead. (Past the last the last one again, to
+    // where nobody reads any more: the number of loads on their way is then always the same.)
+    //
+    // The two halves of a step's depth take turns: while the matrix cores have one, the fragments of the
+    // other come out of LDS. In the middle of a step every wave has all of its fragments in registers
+    // and waits for the loads of the next one and for the other waves: from there on the
+    // next step can be read, and this one's LDS be loaded into again.
+    constexpr int kLoads = M::kLoads + N::kLoads;
+    if (steps > 0) {
+      StaticFor<kStages>([&](auto d) __attribute__((always_inline)) { issue(min(int(d), steps - 1), d); });
+      WaitVmcnt<(kStages - 1) * kLoads>();
       Barrier();
-      if (s + 1 < steps) issue(s + 1, 1 - stage);
-      compute(stage);
-    };
-    for (int s = 0; s < steps; s += 2) {
-      step(s, std::integral_constant<int, 0>());
-      if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
+      Fragments first, second;
+      read(0, 0, first);
+      const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
+        read(stage, 1, second);
+        multiply(first);
+        interleave();
+        WaitVmcnt<(kStages - 2) * kLoads>();
+        Barrier();
+        issue(min(s + kStages, steps - 1), stage);
+        read((stage + 1) % kStages, 0, first);
+        multiply(second);
+        interleave();
+      };
+      for (int s = 0;;) {
+        step(s, std::integral_constant<int, 0>());
+        if (++s == steps) break;
+        step(s, std::integral_constant<int, 1>());
+        if (++s == steps) break;
+        if constexpr (kStages > 2) {
+          step(s, std::integral_constant<int, 2>());
+          if (++s == steps) break;
+        }
+      }
+      // (LDS may be another workgroup's once this one has ended.)
+      WaitVmcnt<0>();
     }
   } else {
     // A granule is read where it lies, or, where it would reach past the end of its
@@ -461,7 +497,11 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
     const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
       __syncthreads();
       fetch(min(s + 1, steps - 1));
-      compute(stage);
+      Fragments first, second;
+      read(stage, 0, first);
+      read(stage, 1, second);
+      multiply(first);
+      multiply(second);
       put(min(s + 1, steps - 1), 1 - stage);
     };
     for (int s = 0;;) {

@@ -8,18 +8,30 @@ namespace {
 
 struct Grid {
   unsigned blocks;
-  int tile;
+  int m, n;  // destination elements to a tile
 };
 
-// Four waves, two along either side; `tile` destination elements a side, 128 or 64.
+template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages>
+void LaunchKernel(hipStream_t stream, const GemmArgs& args, unsigned blocks) {
+  constexpr int kLds = kStages * (kWavesM * kBlocksM + kWavesN * kBlocksN) * 16 * 128;
+  auto* const kernel = &GroupedGemmKernel<kType, kRunsM, kRunsN, kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect, kStages>;
+  static const hipError_t attribute = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  (void)attribute;  // (a launch that needs it fails)
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWavesM * kWavesN), kLds, stream, args);
+}
+
 template <int kType, Runs kRunsM, Runs kRunsN, bool kDirect>
 void LaunchOne(hipStream_t stream, const GemmArgs& args, const Grid& grid) {
-  if (grid.tile == 128)
-    hipLaunchKernelGGL((GroupedGemmKernel<kType, kRunsM, kRunsN, 2, 2, 4, 4, kDirect>), dim3(grid.blocks), dim3(256), 0,
-                       stream, args);
+  if constexpr (kDirect) {
+    if (grid.m == 256 && grid.n == 256)
+      return LaunchKernel<kType, kRunsM, kRunsN, 2, 4, 8, 4, true, 2>(stream, args, grid.blocks);
+    if (grid.m == 256) return LaunchKernel<kType, kRunsM, kRunsN, 4, 2, 4, 4, true, 3>(stream, args, grid.blocks);
+  }
+  if (grid.m == 128)
+    LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 4, 4, kDirect, 2>(stream, args, grid.blocks);
   else
-    hipLaunchKernelGGL((GroupedGemmKernel<kType, kRunsM, kRunsN, 2, 2, 2, 2, kDirect>), dim3(grid.blocks), dim3(256), 0,
-                       stream, args);
+    LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 2, 2, kDirect, 2>(stream, args, grid.blocks);
 }
 
 template <int kType, bool kDirect>
@@ -88,17 +100,16 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
   a.vector_stores = a.dst_m_stride == 1 && reinterpret_cast<uintptr_t>(a.dst) % (4 * dst_bytes) == 0 &&
                     a.dst_n_stride % 4 == 0 && a.dst_group_stride % 4 == 0;
 
-  const auto blocks_of = [&](int tile) {
-    const int64_t tiles_m = (int64_t(a.m.count) + tile - 1) / tile;
-    const int64_t tiles_n = columns ? a.n.count / tile + min(call.groups, a.n.count)
-                                    : ((int64_t(a.n.count) + tile - 1) / tile) * call.groups;
+  const auto blocks_of = [&](int tile_m, int tile_n) {
+    const int64_t tiles_m = (int64_t(a.m.count) + tile_m - 1) / tile_m;
+    const int64_t tiles_n = columns ? a.n.count / tile_n + min(call.groups, a.n.count)
+                                    : ((int64_t(a.n.count) + tile_n - 1) / tile_n) * call.groups;
     return (tiles_m * tiles_n + 7) / 8 * 8;
   };
   Grid grid;
-  grid.tile = blocks_of(128) >= 2 * call.compute_units ? 128 : 64;
-  const char* e = getenv("G_TILE");
-  if (e) grid.tile = atoi(e);
-  const int64_t blocks = blocks_of(grid.tile);
+  grid.m = grid.n = blocks_of(128, 128) >= 2 * call.compute_units ? 128 : 64;
+  if (const char* e = getenv("G_TILE")) { grid.m = atoi(e) / 1000; grid.n = atoi(e) % 1000; if (!direct && grid.m > 128) grid.m = grid.n = 128; }
+  const int64_t blocks = blocks_of(grid.m, grid.n);
   if (blocks > 0x7fffffff) return false;
   grid.blocks = static_cast<unsigned>(blocks);
   if (direct)
