@@ -49,7 +49,6 @@ struct GemmArgs {
   int64_t bias_stride;
   float clamp_min, clamp_max;
   int dst_f32;
-  int vector_stores;  // 4 values of the destination's M side lie side by side, aligned
 };
 
 // f(std::integral_constant<int, 0>()), ..., f(std::integral_constant<int, N - 1>()).
@@ -127,16 +126,16 @@ struct TileSide {
   static_assert(kBytes % (1024 * kWaves) == 0, "");
 
   // Row of the wave's piece that lane l (mod 16) holds of block b. Where the rows
-  // are permuted a lane of the accumulators has 4 * kBlocks consecutive ones.
+  // are permuted, a lane's accumulators of two blocks are of 8 consecutive ones.
   static __device__ __forceinline__ int RowOf(int b, int l) {
-    return kPermuted ? (l >> 2) * 4 * kBlocks + b * 4 + (l & 3) : b * 16 + l;
+    return kPermuted ? (b >> 1) * 32 + (l >> 2) * 8 + (b & 1) * 4 + (l & 3) : b * 16 + l;
   }
 
   // Granule g of run r is stored in slot g ^ Key(r): lanes that read LDS together
   // then reach all banks.
   static __device__ __forceinline__ int Key(int r) {
     if constexpr (kRuns == Runs::kPlain) {
-      if constexpr (kPermuted) return ((r >> 1) & 1) | ((r / (4 * kBlocks)) & 3) << 1;
+      if constexpr (kPermuted) return ((r >> 1) & 1) | ((r >> 3) & 3) << 1;
       return (r >> 1) & 7;
     } else if constexpr (E::kBytes == 2) {
       // Reads of 4 consecutive runs of each of 4 groups of 8, 32 bytes of each.
@@ -184,6 +183,20 @@ struct TileSide {
     }
   }
 };
+
+// Two values rounded to a 16-bit type, in one register.
+template <int kType>
+__device__ __forceinline__ int RoundPair(float x, float y) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const v2f both = {x, y};
+  if constexpr (kType == RUYAMD_DTYPE_BF16) {
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, __builtin_convertvector(both, v2bf));
+  } else {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, __builtin_convertvector(both, v2h));
+  }
+}
 
 // The range of a group that is the same for the whole wave, in scalar registers.
 __device__ __forceinline__ Range UniformRangeOf(const int32_t* offsets, int group, int total) {
@@ -513,44 +526,84 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
   }
 
   // Write-back. Lane l holds column l % 16 of each block of the N side and 4
-  // rows (l / 16) * 4 .. of each block of the M side.
+  // rows (l / 16) * 4 .. of each block of the M side; blocks go in pairs, 8 rows one after the other
+  // to a lane. (Those of 16 bits of unpermuted blocks are exchanged between neighbouring rows of 16 lanes for
+  // that.) A store takes any address its type allows.
   const int l = lane & 15, q = lane >> 4;
-  const bool f32 = p.dst_f32 != 0, whole = p.vector_stores != 0 && here_m == kTileM;
+  const bool f32 = p.dst_f32 != 0;
   const int64_t group_at = columns ? 0 : tile.group * p.dst_group_stride;
   const int first_n = columns ? range.begin + n0 : n0;
   const float* bias = p.bias ? p.bias + tile.group * p.bias_stride + m0 : nullptr;
+  constexpr bool kPermuted = kRunsM == Runs::kPlain;
+  typedef __attribute__((aligned(2))) v4i v4i_of_2;
+  typedef __attribute__((aligned(4))) v4f v4f_of_4;
+  const auto store = [&](int m, int64_t column, float v) __attribute__((always_inline)) {
+    if (m < here_m) StoreFloat(p.dst, f32 ? RUYAMD_DTYPE_F32 : kType, column + (m0 + m) * p.dst_m_stride, v);
+  };
 #pragma unroll
-  for (int i = 0; i < kBlocksM; ++i) {
-    const int m = wave_m * M::kWaveRows + M::RowOf(i, q * 4);  // (and the three behind it)
-    float add[4] = {};
+  for (int i = 0; i < kBlocksM; i += 2) {
+    const int rows[2] = {wave_m * M::kWaveRows + M::RowOf(i, q * 4), wave_m * M::kWaveRows + M::RowOf(i + 1, q * 4)};
+    float add[2][4] = {};
     if (bias)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) add[e] = m + e < here_m ? bias[m + e] : 0.0f;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) add[h][e] = rows[h] + e < here_m ? bias[rows[h] + e] : 0.0f;
 #pragma unroll
     for (int j = 0; j < kBlocksN; ++j) {
       const int n = wave_n * N::kWaveRows + j * 16 + l;
-      if (n >= here_n) continue;
-      float v[4];
+      const int64_t column = group_at + int64_t(first_n + n) * p.dst_n_stride;
+      float v[2][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = Clamp(acc[i][j][e] + add[e], p.clamp_min, p.clamp_max);
-      const int64_t at = group_at + (m0 + m) * p.dst_m_stride + int64_t(first_n + n) * p.dst_n_stride;
-      if (whole) {
-        if (f32) {
-          *reinterpret_cast<v4f*>(static_cast<float*>(p.dst) + at) = v4f{v[0], v[1], v[2], v[3]};
-        } else if constexpr (kType == RUYAMD_DTYPE_BF16) {
-          typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
-          *reinterpret_cast<v4bf*>(static_cast<__bf16*>(p.dst) + at) =
-              v4bf{static_cast<__bf16>(v[0]), static_cast<__bf16>(v[1]), static_cast<__bf16>(v[2]), static_cast<__bf16>(v[3])};
-        } else if constexpr (kType == RUYAMD_DTYPE_F16) {
-          typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-          *reinterpret_cast<v4h*>(static_cast<_Float16*>(p.dst) + at) =
-              v4h{static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]),
-                  static_cast<_Float16>(v[3])};
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[h][e] = Clamp(acc[i + h][j][e] + add[h][e], p.clamp_min, p.clamp_max);
+      if (p.dst_m_stride != 1) {
+        if (n < here_n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store(rows[h] + e, column, v[h][e]);
+        continue;
+      }
+      if (f32 || kType == RUYAMD_DTYPE_F32) {
+        if (n >= here_n) continue;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (rows[h] + 4 <= here_m)
+            *reinterpret_cast<v4f_of_4*>(static_cast<float*>(p.dst) + column + m0 + rows[h]) =
+                v4f{v[h][0], v[h][1], v[h][2], v[h][3]};
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store(rows[h] + e, column, v[h][e]);
         }
-      } else {
+        continue;
+      }
+      if constexpr (kType != RUYAMD_DTYPE_F32) {
+        v4i packed;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (m + e < here_m) StoreFloat(p.dst, f32 ? RUYAMD_DTYPE_F32 : kType, at + e * p.dst_m_stride, v[e]);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) packed[2 * h + e] = RoundPair<kType>(v[h][2 * e], v[h][2 * e + 1]);
+        int m = rows[0];
+        if constexpr (!kPermuted) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const auto both = __builtin_amdgcn_permlane16_swap(packed[e], packed[2 + e], false, false);
+            packed[e] = both[0];
+            packed[2 + e] = both[1];
+          }
+          m = wave_m * M::kWaveRows + (i + (q & 1)) * 16 + (q >> 1) * 8;
+        }
+        if (n >= here_n) continue;
+        uint16_t* const to = static_cast<uint16_t*>(p.dst) + column + m0 + m;
+        if (m + 8 <= here_m) {
+          *reinterpret_cast<v4i_of_2*>(to) = packed;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (m + e < here_m) to[e] = static_cast<uint16_t>(static_cast<uint32_t>(packed[e / 2]) >> (16 * (e & 1)));
+        }
       }
     }
   }

@@ -92,14 +92,10 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
     if (runs == Runs::kPlain) return columns && call.k % granule == 0;
     return !(columns && dealt_rows) && s.count % granule == 0;
   };
-  const bool direct = aligned(a.m, runs_m, false) && aligned(a.n, runs_n, true);
+  const bool direct = !getenv("G_NODIRECT") && aligned(a.m, runs_m, false) && aligned(a.n, runs_n, true);
   // Runs that the registers' way reads have 16 bytes at least.
   const auto long_enough = [&](const Side& s, Runs runs) { return (runs == Runs::kPlain ? call.k : s.count) >= granule; };
   if (!direct && !(long_enough(a.m, runs_m) && long_enough(a.n, runs_n))) return false;
-  const int dst_bytes = a.dst_f32 ? 4 : 2;
-  a.vector_stores = a.dst_m_stride == 1 && reinterpret_cast<uintptr_t>(a.dst) % (4 * dst_bytes) == 0 &&
-                    a.dst_n_stride % 4 == 0 && a.dst_group_stride % 4 == 0;
-
   const auto blocks_of = [&](int tile_m, int tile_n) {
     const int64_t tiles_m = (int64_t(a.m.count) + tile_m - 1) / tile_m;
     const int64_t tiles_n = columns ? a.n.count / tile_n + min(call.groups, a.n.count)
