@@ -429,6 +429,10 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
           step(s, std::integral_constant<int, 2>());
           if (++s == steps) break;
         }
+        if constexpr (kStages > 3) {
+          step(s, std::integral_constant<int, 3>());
+          if (++s == steps) break;
+        }
       }
       // (LDS may be another workgroup's once this one has ended.)
       WaitVmcnt<0>();
@@ -467,15 +471,20 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
     const auto load = [](const Place& from) __attribute__((always_inline)) -> v4i {
       return *reinterpret_cast<const granule::v4i_unaligned*>(from.run + min(from.at, from.length - 16));
     };
-    v4i held_m[M::kLoads], held_n[N::kLoads];
-    const auto fetch = [&](int s) __attribute__((always_inline)) {
-#pragma unroll
-      for (int n = 0; n < M::kLoads; ++n) held_m[n] = load(place_of(M(), n, p.m, kRunsM, false, m0, here_m, s));
-#pragma unroll
-      for (int n = 0; n < N::kLoads; ++n) held_n[n] = load(place_of(N(), n, p.n, kRunsN, true, n0, here_n, s));
+    // Steps held in registers on their way: two of the small tile's.
+    constexpr int kSets = kBlocksM == 2 ? 2 : 1;
+    struct Set {
+      v4i m[M::kLoads], n[N::kLoads];
     };
-    const auto put_side = [&](auto side, v4i* held, int loads, const Side& from, Runs runs, bool dealt_rows, int first,
-                              int here, int s, char* to) __attribute__((always_inline)) {
+    Set held[kSets];
+    const auto fetch = [&](int s, Set& set) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < M::kLoads; ++n) set.m[n] = load(place_of(M(), n, p.m, kRunsM, false, m0, here_m, s));
+#pragma unroll
+      for (int n = 0; n < N::kLoads; ++n) set.n[n] = load(place_of(N(), n, p.n, kRunsN, true, n0, here_n, s));
+    };
+    const auto put_side = [&](auto side, v4i* held, const Side& from, Runs runs, bool dealt_rows, int first, int here, int s,
+                              char* to) __attribute__((always_inline)) {
       using T = decltype(side);
       const int k0 = s * E::kDepth;
       const bool depth_ends = k0 + E::kDepth > depth;
@@ -498,24 +507,28 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
 #pragma unroll
       for (int n = 0; n < T::kLoads; ++n) *reinterpret_cast<v4i*>(to + n * kWaves * 1024) = held[n];
     };
-    const auto put = [&](int s, int stage) __attribute__((always_inline)) {
+    const auto put = [&](int s, int stage, Set& set) __attribute__((always_inline)) {
       char* to = lds + stage * kStage + (wave * 64 + lane) * 16;
-      put_side(M(), held_m, M::kLoads, p.m, kRunsM, false, m0, here_m, s, to);
-      put_side(N(), held_n, N::kLoads, p.n, kRunsN, true, n0, here_n, s, to + M::kBytes);
+      put_side(M(), set.m, p.m, kRunsM, false, m0, here_m, s, to);
+      put_side(N(), set.n, p.n, kRunsN, true, n0, here_n, s, to + M::kBytes);
     };
+    // (Steps past the last are the last one again, to where nobody reads.)
     if (steps > 0) {
-      fetch(0);
-      put(0, 0);
+      fetch(0, held[0]);
+      if constexpr (kSets == 2) fetch(min(1, steps - 1), held[1]);
+      put(0, 0, held[0]);
+      fetch(min(kSets, steps - 1), held[0]);
     }
     const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
       __syncthreads();
-      fetch(min(s + 1, steps - 1));
       Fragments first, second;
       read(stage, 0, first);
       read(stage, 1, second);
       multiply(first);
       multiply(second);
-      put(min(s + 1, steps - 1), 1 - stage);
+      Set& next = held[(stage + 1) % kSets];
+      put(min(s + 1, steps - 1), 1 - stage, next);
+      fetch(min(s + 1 + kSets, steps - 1), next);
     };
     for (int s = 0;;) {
       if (s == steps) break;

@@ -1,15 +1,35 @@
 // Launches of the tiled kernel of grouped products.
 #include "grouped_gemm.h"
-#include <cstdlib>
+
+#include <algorithm>
+#include <cmath>
 
 namespace ruyamd {
 namespace grouped {
 namespace {
 
+enum class Tile { k64x64, k128x128, k256x128, k256x256 };
+
 struct Grid {
   unsigned blocks;
-  int m, n;  // destination elements to a tile
+  Tile tile;
 };
+
+// A tile's sizes, the workgroups that a CU runs side by side, and how long one step
+// of all of them takes, with operands straight to LDS, through registers, and fp32 (0: there is no such
+// kernel). Measured, us: bfloat16, 8 x 4096 x 2048 x 8192 in 544 / 160 / 160 / 96 steps of every CU
+// 265 / 181 / 167 / 171, 16 x 1683 x 3968 x 6400 194 / 147 / 133 / 116.
+struct TileCost {
+  Tile tile;
+  int m, n, per_cu;
+  float direct, through, f32;
+};
+constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 2, 0.48f, 0.6f, 1.05f},
+                               {Tile::k128x128, 128, 128, 2, 1.08f, 0, 3.9f},
+                               {Tile::k256x128, 256, 128, 1, 1.0f, 0, 0},
+                               {Tile::k256x256, 256, 256, 1, 1.68f, 0, 0}};
+// What a workgroup does before its first step and after its last, in steps.
+constexpr float kFixedSteps = 6;
 
 template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages>
 void LaunchKernel(hipStream_t stream, const GemmArgs& args, unsigned blocks) {
@@ -21,17 +41,19 @@ void LaunchKernel(hipStream_t stream, const GemmArgs& args, unsigned blocks) {
   hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWavesM * kWavesN), kLds, stream, args);
 }
 
+// (Eight waves on the larger tiles, four on the others.)
 template <int kType, Runs kRunsM, Runs kRunsN, bool kDirect>
 void LaunchOne(hipStream_t stream, const GemmArgs& args, const Grid& grid) {
-  if constexpr (kDirect) {
-    if (grid.m == 256 && grid.n == 256)
+  if constexpr (kDirect && kType != RUYAMD_DTYPE_F32) {
+    if (grid.tile == Tile::k256x256)
       return LaunchKernel<kType, kRunsM, kRunsN, 2, 4, 8, 4, true, 2>(stream, args, grid.blocks);
-    if (grid.m == 256) return LaunchKernel<kType, kRunsM, kRunsN, 4, 2, 4, 4, true, 3>(stream, args, grid.blocks);
+    if (grid.tile == Tile::k256x128)
+      return LaunchKernel<kType, kRunsM, kRunsN, 4, 2, 4, 4, true, 3>(stream, args, grid.blocks);
   }
-  if (grid.m == 128)
-    LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 4, 4, kDirect, 2>(stream, args, grid.blocks);
-  else
-    LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 2, 2, kDirect, 2>(stream, args, grid.blocks);
+  if constexpr (kDirect)
+    if (grid.tile == Tile::k128x128)
+      return LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 4, 4, true, 2>(stream, args, grid.blocks);
+  LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 2, 2, kDirect, kDirect ? 4 : 2>(stream, args, grid.blocks);
 }
 
 template <int kType, bool kDirect>
@@ -92,20 +114,32 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
     if (runs == Runs::kPlain) return columns && call.k % granule == 0;
     return !(columns && dealt_rows) && s.count % granule == 0;
   };
-  const bool direct = !getenv("G_NODIRECT") && aligned(a.m, runs_m, false) && aligned(a.n, runs_n, true);
+  const bool direct = aligned(a.m, runs_m, false) && aligned(a.n, runs_n, true);
   // Runs that the registers' way reads have 16 bytes at least.
   const auto long_enough = [&](const Side& s, Runs runs) { return (runs == Runs::kPlain ? call.k : s.count) >= granule; };
   if (!direct && !(long_enough(a.m, runs_m) && long_enough(a.n, runs_n))) return false;
-  const auto blocks_of = [&](int tile_m, int tile_n) {
-    const int64_t tiles_m = (int64_t(a.m.count) + tile_m - 1) / tile_m;
-    const int64_t tiles_n = columns ? a.n.count / tile_n + min(call.groups, a.n.count)
-                                    : ((int64_t(a.n.count) + tile_n - 1) / tile_n) * call.groups;
-    return (tiles_m * tiles_n + 7) / 8 * 8;
-  };
+  // The tile that the CUs would be done with first. (How many tiles the groups' columns
+  // make is known on the device only: here every group that can have a column ends with half a tile.)
+  const int64_t busy = columns ? min(call.groups, a.n.count) : call.groups;
+  const float group_depth = columns ? call.k : float(call.k) / call.groups;
+  const float steps = group_depth * bytes / 128 + 0.5f + kFixedSteps;
   Grid grid;
-  grid.m = grid.n = blocks_of(128, 128) >= 2 * call.compute_units ? 128 : 64;
-  if (const char* e = getenv("G_TILE")) { grid.m = atoi(e) / 1000; grid.n = atoi(e) % 1000; if (!direct && grid.m > 128) grid.m = grid.n = 128; }
-  const int64_t blocks = blocks_of(grid.m, grid.n);
+  int64_t blocks = 0;
+  float best = 0;
+  for (const TileCost& t : kTiles) {
+    const float step = !direct ? t.through : call.type == RUYAMD_DTYPE_F32 ? t.f32 : t.direct;
+    if (step == 0) continue;
+    const int64_t tiles_m = (int64_t(a.m.count) + t.m - 1) / t.m;
+    const int64_t most_n = columns ? a.n.count / t.n + busy : ((int64_t(a.n.count) + t.n - 1) / t.n) * busy;
+    const float tiles_n = columns ? std::max(float(busy), float(a.n.count) / t.n + 0.5f * busy) : most_n;
+    const float rounds = std::ceil(tiles_m * tiles_n / (t.per_cu * call.compute_units) - 0.05f);
+    const float time = std::max(1.0f, rounds) * steps * step;
+    if (blocks == 0 || time < best) {
+      best = time;
+      grid.tile = t.tile;
+      blocks = (tiles_m * most_n + 7) / 8 * 8;
+    }
+  }
   if (blocks > 0x7fffffff) return false;
   grid.blocks = static_cast<unsigned>(blocks);
   if (direct)

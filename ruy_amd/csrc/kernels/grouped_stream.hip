@@ -35,7 +35,7 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
     plan.cols = 1;
     plan.slabs = false;
   } else {
-    plan.cols = per_group <= block_tokens ? 1 : per_group <= 2 * block_tokens || !int4 ? 2 : 4;
+    plan.cols = per_group <= block_tokens ? 1 : 2;
     plan.slabs = plan.cols > 1 || min(to_group, int64_t(block_tokens)) > fit;
   }
   const int chunk = int4 && plan.slabs ? 128 : depth_to_chunk, chunks = (call.k + chunk - 1) / chunk;
