@@ -291,8 +291,8 @@ typedef struct ruyamd_int4_mat {
 } ruyamd_int4_mat;
 
 /* dst = clamp(lhs * rhs + bias) with 4-bit weights and a few columns, such as
- * the tokens of a decoding step: every weight is read once to each 16 to 64
- * columns. With `groups` (not NULL) there is a weight matrix to each group, as
+ * the tokens of a decoding step: every weight is read once to each 16 to 32
+ * columns of a group (5 to 10 fp32 ones). With `groups` (not NULL) there is a weight matrix to each group, as
  * in ruyamd_mul_grouped (whose matrix_stride is not looked at here). rhs:
  * bfloat16, half or fp32, any order; dst its type or fp32; products with the
  * whole-numbered part of the weights are exact, sums are fp32, a group's scale is
@@ -378,7 +378,9 @@ RUYAMD_API void ruyamd_ctx_force_generic_kernel(ruyamd_ctx* ctx, int force);
  * tile_cols destination elements (256x256, 128x128, 128x64, 64x128 or 64x64;
  * plane columns count for int8 x int16) instead of the one their timing model
  * picks, where the kernel has that tile, also for products that would run on the
- * kernel for small ones instead; 0, 0 restores the model's choice.
+ * kernel for small ones instead; 0, 0 restores the model's choice. (Grouped
+ * products: 256x256, 256x128, 128x128 or 64x64, rows along dst's contiguous dimension,
+ * and no streaming kernel for matrices of bfloat16, half or fp32.)
  * depth_parts, looked at with the 256x256 tile forced on int8 data: not 0 =
  * split the depth over that many workgroups per tile (2, 4 or 8; 1: over none;
  * rounded down to what leaves no part without a depth step) instead of what

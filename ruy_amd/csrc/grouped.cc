@@ -124,6 +124,8 @@ int Run(ruyamd_ctx* ctx, grouped::Call* call, const grouped::Int4* weights) {
   }
   if (call->m == 0 || call->n == 0) return RUYAMD_OK;
   call->compute_units = ctx->multiprocessor_count;
+  call->forced_tile_rows = ctx->forced_tile_rows;
+  call->forced_tile_cols = ctx->forced_tile_cols;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {
     (void)hipGetLastError();

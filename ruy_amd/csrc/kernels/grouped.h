@@ -34,6 +34,7 @@ struct Call {
   int64_t bias_stride = 0;
   float clamp_min = 0, clamp_max = 0;
   int compute_units = 0;
+  int forced_tile_rows = 0, forced_tile_cols = 0;  // 0: the fastest one
 };
 
 // The 4-bit left-hand operand of a call (lhs, lhs_rs and lhs_cs of which are unused).

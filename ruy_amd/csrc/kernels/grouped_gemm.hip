@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <iterator>
 
 namespace ruyamd {
 namespace grouped {
@@ -126,9 +127,12 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
   Grid grid;
   int64_t blocks = 0;
   float best = 0;
+  const auto step_of = [&](const TileCost& t) { return !direct ? t.through : call.type == RUYAMD_DTYPE_F32 ? t.f32 : t.direct; };
+  const auto forced = [&](const TileCost& t) { return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols; };
+  const bool force = std::any_of(std::begin(kTiles), std::end(kTiles), [&](const TileCost& t) { return forced(t) && step_of(t) != 0; });
   for (const TileCost& t : kTiles) {
-    const float step = !direct ? t.through : call.type == RUYAMD_DTYPE_F32 ? t.f32 : t.direct;
-    if (step == 0) continue;
+    const float step = step_of(t);
+    if (step == 0 || (force && !forced(t))) continue;
     const int64_t tiles_m = (int64_t(a.m.count) + t.m - 1) / t.m;
     const int64_t most_n = columns ? a.n.count / t.n + busy : ((int64_t(a.n.count) + t.n - 1) / t.n) * busy;
     const float tiles_n = columns ? std::max(float(busy), float(a.n.count) / t.n + 0.5f * busy) : most_n;

@@ -449,19 +449,16 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   if constexpr (kSlabs) {
     const int slab_units = depth_waves * T::kChunkUnits, unit_bits = __builtin_ctz(slab_units);  // (a power of two)
     constexpr int kPieces = (kMostTokens * T::kChunkUnits + 64 * kRowWaves - 1) / (64 * kRowWaves);
-    struct Slab {
-      Unit pieces[kPieces];
-    };
-    Slab ahead[2];  // slabs on their way: one turn's, and the next one's
+    Unit pieces[kPieces];  // the next slab, on its way
     // (Tokens past the last are the last one again.)
-    const auto fetch_slab = [&](int slab, Unit (&pieces)[kPieces]) __attribute__((always_inline)) {
+    const auto fetch_slab = [&](int slab) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int n = i * blockDim.x + threadIdx.x, token = min(n >> unit_bits, tokens - 1);
         pieces[i] = fetch_inside(token, slab * slab_units + (n & (slab_units - 1)));
       }
     };
-    const auto put_slab = [&](int buffer, const Unit (&pieces)[kPieces]) __attribute__((always_inline)) {
+    const auto put_slab = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int n = i * blockDim.x + threadIdx.x, token = min(n >> unit_bits, tokens - 1);
@@ -469,15 +466,14 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
       }
     };
     if (turns > 0) {
-      fetch_slab(place_of(0), ahead[0].pieces);
-      fetch_slab(place_of(1), ahead[1].pieces);
-      put_slab(0, ahead[0].pieces);
-      fetch_slab(place_of(2), ahead[0].pieces);
+      fetch_slab(place_of(0));
+      put_slab(0);
+      fetch_slab(place_of(1));
       const auto turn = [&](int n, auto d) __attribute__((always_inline)) {
         // Slab n is there, and slab n - 1 no longer read, when all have come here.
         __syncthreads();
-        put_slab(1 - d, ahead[1 - d].pieces);
-        fetch_slab(place_of(n + 3), ahead[1 - d].pieces);
+        put_slab(1 - d);
+        fetch_slab(place_of(n + 2));
         use(held[d], depth_wave + place_of(n) * depth_waves, lds + d * args.slab_bytes + depth_wave * kLdsChunk);
         load(depth_wave + place_of(n + 2) * depth_waves, held[d]);
       };

@@ -7,7 +7,7 @@ namespace grouped {
 
 bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hipError_t* status) {
   const bool int4 = weights != nullptr;
-  if (!int4 && (call.dealt != Dealt::kColumns || call.lhs_cs != 1)) return false;
+  if (!int4 && (call.dealt != Dealt::kColumns || call.lhs_cs != 1 || call.forced_tile_rows)) return false;
   // (A row has 16 bytes at least, and what a lane has of one ends before 2^31.)
   if (call.k < 32 || call.k > (1 << 28)) return false;
   StreamArgs args;
@@ -53,14 +53,18 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
                                                            : Scaling::kAny;
   }
 
-  // Waves: 8 to a workgroup, and 16 to a CU if the rows give them, along the rows first, then
-  // along the depth; fewer rows where what goes with them into LDS is too much. (16384 x
-  // 16384, one token: 16 waves to a CU 29.7 us, 8 30.7, 4 48. Two blocks of 16 rows to a wave
-  // are no faster anywhere, and slower where there are few rows.)
+  // Waves: 8 to a workgroup, along the depth as long as that makes no more than 16 to a CU
+  // (of weights in 16 or 32 bits 64), along the rows otherwise; fewer rows where what goes with
+  // them into LDS is too much. (bfloat16, 64 x 4096x2048, one or two tokens each: 64 waves to a CU
+  // 40.6 us, 16 44.0. 4-bit, 64 x 1024x2048: 24.0 and 20.5; 16384 x 16384, one token: 32.2 and
+  // 31.3, with 4 waves to a workgroup 40, with 2 59. Two blocks of 16 rows to a wave are no
+  // faster anywhere, and slower where there are few rows.)
   int row_waves = RowWaves(plan.slabs, plan.cols), depth_waves = 8 / row_waves;
   if (!plan.slabs) {
     const int64_t units = (int64_t(call.m) + 15) / 16 * busy;
-    while (depth_waves > 1 && units * depth_waves > int64_t(16) * call.compute_units) depth_waves /= 2;
+    const int64_t most = int64_t(int4 ? 16 : 64) * call.compute_units;
+    depth_waves = 8;
+    while (depth_waves > 1 && units * depth_waves > most) depth_waves /= 2;
     row_waves = 8 / depth_waves;
   }
   while (depth_waves > 1 && chunks < depth_waves) depth_waves /= 2;

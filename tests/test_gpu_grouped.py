@@ -732,3 +732,80 @@ def test_offsets_of_values_beyond_32_bits(context, kernel):
     api.mul_int4(int4, rhs.matrix(), params_of(S.F32), context, dst.matrix(), api.Groups(table, 2))
     for i, at in enumerate((slice(0, 5), slice(5, 20))):
         assert torch.equal(dst.view()[:, at].double(), R.int4_values(q[i], scales[i], None, m, k, 128) @ x[:, at])
+
+
+# --- Every kernel, wherever the rules that choose would draw their lines -----
+
+TILES = [(64, 64), (128, 128), (256, 128), (256, 256)]
+
+
+@pytest.fixture(params=TILES, ids=str)
+def tile(request, context):
+    context.force_tile(*request.param)
+    yield request.param
+    context.force_tile()
+
+
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+@pytest.mark.parametrize("orders", [(a, b, d) for a in (ROW, COL) for b in (ROW, COL) for d in (ROW, COL)], ids=str)
+def test_every_tile_with_columns(context, tile, type_, orders):
+    """Depths of one step and less, of as many as a workgroup has buffers for, and of
+    more; groups that are empty, of one column, of more than a tile."""
+    for m, k, n in [(8, 8, 8), (264, 64, 72), (136, 128, 296), (520, 200, 560), (312, 712, 40)]:
+        offsets = [0, n // 8, n // 8, n // 8 + 1, n // 4, n]
+        run_columns(context, type_, type_, m, k, n, offsets, orders, bias=True, low=-50.0, seed=m)
+        assert context.last_kernel_name() == "grouped_mfma"
+
+
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+@pytest.mark.parametrize("orders", [(a, b, d) for a in (ROW, COL) for b in (ROW, COL) for d in (ROW, COL)], ids=str)
+def test_every_tile_with_depth(context, tile, type_, orders):
+    for m, n, depth in [(8, 8, 8), (264, 72, 64), (136, 520, 360), (560, 312, 1000)]:
+        offsets = [0, depth // 8, depth // 8, depth // 8 + 1, depth // 4, depth]
+        run_depth(context, type_, S.F32, m, n, depth, offsets, orders, seed=m)
+        assert context.last_kernel_name() == "grouped_mfma"
+
+
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+def test_every_tile_with_ordinary_values(context, tile, type_):
+    run_columns(context, type_, type_, 520, 1032, 600, [0, 5, 300, 600], bias=True, whole=False)
+    run_depth(context, type_, type_, 264, 520, 1500, [0, 333, 334, 1500], whole=False)
+
+
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+def test_kernels_are_the_ones_meant(context, type_):
+    run_columns(context, type_, type_, 256, 512, 8, [0, 3, 3, 8])
+    assert context.last_kernel_name() == "grouped_stream"
+    # All columns in one of many groups: several workgroups read its weights.
+    run_columns(context, type_, type_, 80, 520, 60, [0] * 7 + [60] * 14)
+    assert context.last_kernel_name() == "grouped_stream"
+    # Tokens slab by slab.
+    run_columns(context, type_, type_, 80, 9000, 20, [0, 20])
+    assert context.last_kernel_name() == "grouped_stream"
+    run_columns(context, type_, type_, 80, 9000, 9, [0, 9])
+    assert context.last_kernel_name() == "grouped_stream"
+    run_columns(context, type_, type_, 256, 512, 400, [0, 30, 30, 400])
+    assert context.last_kernel_name() == "grouped_mfma"
+    run_columns(context, type_, type_, 40, 17, 3, [0, 3])
+    assert context.last_kernel_name() in ("generic", "grouped_mfma")
+    run_columns(context, type_, type_, 40, 2, 3, [0, 3])
+    assert context.last_kernel_name() == "generic"
+    run_depth(context, type_, type_, 256, 512, 400, [0, 30, 30, 400])
+    assert context.last_kernel_name() == "grouped_mfma"
+
+
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+@pytest.mark.parametrize("zeros", [False, True])
+def test_int4_where_something_does_not_fit_into_lds(context, type_, zeros):
+    # More scales than there is room for, with and without a whole last group.
+    for k in (70016, 131072 + 5):
+        run_int4(context, type_, S.F32, 20, k, 2, 32, zeros=zeros, scale_type=S.F32)
+        assert context.last_kernel_name() == "int4_stream"
+    # Tokens that do not lie side by side: some of them, or none, fit.
+    run_int4(context, type_, S.F32, 20, 9000, 12, 128, zeros=zeros, rhs_order=ROW)
+    assert context.last_kernel_name() == "int4_stream"
+    run_int4(context, type_, S.F32, 20, 70016, 2, 64, zeros=zeros, rhs_order=ROW)
+    assert context.last_kernel_name() == "generic"
+    # Slab by slab, with experts and a depth that ends inside a slab.
+    run_int4(context, type_, S.F32, 50, 4105, 90, 128, offsets=[0, 1, 1, 50, 90], zeros=zeros)
+    assert context.last_kernel_name() == "int4_stream"
