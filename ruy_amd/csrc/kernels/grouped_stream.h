@@ -16,11 +16,14 @@
 // make 2^e + q (half: 1024 + q, bfloat16: 16 + q), two at a time. Half: 1024 + zero is
 // then taken away, exactly and packed: 9 instructions to 8 weights. bfloat16 has no such
 // instruction: the product is formed with 16 + q, and (16 + zero) * sum(x), whose sums come from
-// the matrix cores as well (a product with ones), is taken away from every group's sum. fp32 tokens
-// are three bf16 rows each that add up to them (float_parts.h), so that every product is exact.
-// The scale multiplies a group's sum. Values that are not finite would make 16 + q and 16 + zero
-// meet as infinity - infinity; a wave that ends with one goes through its depth once more
-// with the exact q - zero.
+// the matrix cores as well (a product with ones), is taken away from every group's sum: the
+// sums' roundings are those of values up to 31 / 8 larger, far below a rounding to bfloat16. fp32 tokens
+// are three bf16 rows each that add up to them (float_parts.h), so that every product is exact;
+// they are multiplied by q - zero, formed in half and converted, 21 instructions to 8 weights, as
+// there is no later rounding that the sums' would be small beside. The scale multiplies a group's
+// sum. Values that are not finite would make 16 + q and 16 + zero, or a value's three parts, meet as
+// infinity - infinity; a wave that ends with one goes through its depth once more with the exact
+// q - zero and whole values.
 #ifndef RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 #define RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 
@@ -86,6 +89,8 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   constexpr int kStepsToScale = kInt4 ? T::kSteps / kScales : 1;
   constexpr bool kScalesInLds = kInt4 && kScaling != Scaling::kAny;
   constexpr bool kHalf = kType == RUYAMD_DTYPE_F16;
+  // Whether the products of 4-bit weights are formed with q - zero, not with 16 + q.
+  constexpr bool kDifference = kHalf || T::kParts;
   constexpr int kMmaType = kHalf ? RUYAMD_DTYPE_F16 : RUYAMD_DTYPE_BF16;  // of 4-bit weights
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const Call& c = args.c;
@@ -310,8 +315,8 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 
   // What the eight values of a word are taken apart with. (Held in registers: as constants
   // in the instructions they would each take one more.)
-  uint32_t low_mask = kHalf ? 0x000F000Fu : 0x00780078u, high_mask = 0x00F000F0u, sixteenth = 0x2C002C00u;
-  uint32_t exponent = kHalf ? 0x64006400u : 0x41804180u;
+  uint32_t low_mask = kDifference ? 0x000F000Fu : 0x00780078u, high_mask = 0x00F000F0u, sixteenth = 0x2C002C00u;
+  uint32_t exponent = kDifference ? 0x64006400u : 0x41804180u;
   asm("" : "+s"(low_mask));
   asm("" : "+s"(high_mask));
   asm("" : "+s"(sixteenth));
@@ -329,6 +334,16 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
                bits(__builtin_elementwise_fma(halves((x & high_mask) | exponent), halves(sixteenth), away_high)),
                bits(halves((y & low_mask) | exponent) - away_low),
                bits(__builtin_elementwise_fma(halves((y & high_mask) | exponent), halves(sixteenth), away_high))};
+  };
+  // The same as bfloat16, exact too (whole numbers of 4 bits and a sign).
+  const auto to_bf16 = [&](v4i x) __attribute__((always_inline)) -> v4i {
+    v4i y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const v2h pair = halves(x[e]);
+      y[e] = float_parts::RoundPair(static_cast<float>(pair[0]), static_cast<float>(pair[1]));
+    }
+    return y;
   };
   // bfloat16: 16 + q, in that order.
   const auto sixteen_and = [&](uint32_t x) __attribute__((always_inline)) -> v4i {
@@ -392,14 +407,17 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
           for (int t = 0; t < kCols; ++t) {
             x[t] = *reinterpret_cast<const v4i*>(at + lds_row[t] * args.pitch + unit_of(j) * 16);
-            if constexpr (!kHalf) {
+            if constexpr (!kDifference) {
               constexpr int kOnes = 0x3F803F80;
               Mma<kMmaType>(x[t], v4i{kOnes, kOnes, kOnes, kOnes}, ones[t]);
             }
           }
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
-            const v4i b = kHalf ? less_zero(words[r][j / 4][j % 4], zero[r][g]) : sixteen_and(words[r][j / 4][j % 4]);
+            const uint32_t word = words[r][j / 4][j % 4];
+            const v4i b = kHalf          ? less_zero(word, zero[r][g])
+                          : kDifference ? to_bf16(less_zero(word, zero[r][g]))
+                                        : sixteen_and(word);
 #pragma unroll
             for (int t = 0; t < kCols; ++t) Mma<kMmaType>(x[t], b, sum[r][t]);
           }
@@ -412,7 +430,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float v = sum[r][t][e];
-              if constexpr (!kHalf) v = __builtin_fmaf(away, ones[t][e], v);
+              if constexpr (!kDifference) v = __builtin_fmaf(away, ones[t][e], v);
               acc[r][t][e] = __builtin_fmaf(scale[r][g], v, acc[r][t][e]);
             }
         }
