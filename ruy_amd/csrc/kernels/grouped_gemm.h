@@ -442,59 +442,72 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
     // run, from the run's last 16 bytes (a run has as many); Put then moves it to its place and
     // zeroes what lies past the depth. (What lies past the tile's sides
     // ends up in rows of the tile that are not stored.)
+    // Where load n of a lane is in its run and how long the run is, in bytes; `row`, `k`: where the
+    // tile begins in the operand.
     struct Place {
-      const char* run;
-      int at, length;  // in bytes, of the run
+      int at, length;
     };
-    const auto place_of = [&](auto side, int n, const Side& from, Runs runs, bool dealt_rows, int first, int here, int s)
-                              __attribute__((always_inline)) -> Place {
+    const auto place_of = [&](auto side, int n, const Side& from, Runs runs, int row, int s) __attribute__((always_inline)) -> Place {
       using T = decltype(side);
-      const int run = T::RunOf(n, wave, lane), granule = T::GranuleOf(n, wave, lane), k0 = s * E::kDepth;
-      const int64_t row = first + (columns && dealt_rows ? range.begin : 0), k = columns ? 0 : range.begin;
+      const int granule = T::GranuleOf(n, wave, lane);
+      if (runs == Runs::kPlain) return {((columns ? 0 : range.begin) + s * E::kDepth + granule * E::kGranule) * E::kBytes, p.depth * E::kBytes};
+      return {(row + granule * E::kGranule) * E::kBytes, from.count * E::kBytes};
+    };
+    const int row_m = m0, row_n = n0 + (columns ? range.begin : 0);
+    // A lane's offsets, from an address that is the same for all: of the run (kPlain) or of the
+    // place in it, and of the other of the two, which ends at the operand's end and so goes by the step.
+    uint32_t off_m[M::kLoads], off_n[N::kLoads];
+    const auto offset_of = [&](auto side, int n, const Side& from, Runs runs, int row, int here) __attribute__((always_inline)) -> uint32_t {
+      using T = decltype(side);
+      if (runs == Runs::kPlain) return static_cast<uint32_t>(min(T::RunOf(n, wave, lane), here - 1) * from.pitch * E::kBytes);
+      const Place where = place_of(side, n, from, runs, row, 0);
+      return static_cast<uint32_t>(min(where.at, where.length - 16));
+    };
+#pragma unroll
+    for (int n = 0; n < M::kLoads; ++n) off_m[n] = offset_of(M(), n, p.m, kRunsM, row_m, here_m);
+#pragma unroll
+    for (int n = 0; n < N::kLoads; ++n) off_n[n] = offset_of(N(), n, p.n, kRunsN, row_n, here_n);
+    const auto load_side = [&](auto side, v4i* held, const uint32_t* off, const Side& from, Runs runs, bool dealt_rows, int row,
+                               int s) __attribute__((always_inline)) {
+      using T = decltype(side);
       const int64_t group = columns && !dealt_rows ? tile.group * from.group_stride : 0;
-      Place p2;
-      int64_t runs_from;
-      if (runs == Runs::kPlain) {
-        runs_from = row + min(run, here - 1);
-        p2.at = static_cast<int>(k) + k0 + granule * E::kGranule;
-        p2.length = p.depth;
-      } else {
-        runs_from = k + min(k0 + run, depth - 1);
-        p2.at = static_cast<int>(row) + granule * E::kGranule;
-        p2.length = from.count;
+      const int64_t k = (columns ? 0 : range.begin) + int64_t(s) * E::kDepth;
+      const char* const base = static_cast<const char*>(from.data) +
+                               (group + (runs == Runs::kPlain ? row : k) * from.pitch) * E::kBytes;
+      // (Steps have 64 runs at most.)
+      const uint32_t last_run = static_cast<uint32_t>(min(depth - 1 - s * E::kDepth, 64) * from.pitch * E::kBytes);
+#pragma unroll
+      for (int n = 0; n < T::kLoads; ++n) {
+        uint32_t other;
+        if (runs == Runs::kPlain) {
+          const Place where = place_of(side, n, from, runs, row, s);
+          other = min(where.at, where.length - 16);
+        } else {
+          other = min(static_cast<uint32_t>(T::RunOf(n, wave, lane) * from.pitch * E::kBytes), last_run);
+        }
+        held[n] = *reinterpret_cast<const granule::v4i_unaligned*>(base + (off[n] + other));
       }
-      p2.run = static_cast<const char*>(from.data) + (group + runs_from * from.pitch) * E::kBytes;
-      p2.at *= E::kBytes;
-      p2.length *= E::kBytes;
-      return p2;
     };
-    const auto load = [](const Place& from) __attribute__((always_inline)) -> v4i {
-      return *reinterpret_cast<const granule::v4i_unaligned*>(from.run + min(from.at, from.length - 16));
-    };
-    // Steps held in registers on their way: two of the small tile's.
-    constexpr int kSets = kBlocksM == 2 ? 2 : 1;
+    // Steps held in registers on their way.
+    constexpr int kSets = 2;
     struct Set {
       v4i m[M::kLoads], n[N::kLoads];
     };
     Set held[kSets];
     const auto fetch = [&](int s, Set& set) __attribute__((always_inline)) {
-#pragma unroll
-      for (int n = 0; n < M::kLoads; ++n) set.m[n] = load(place_of(M(), n, p.m, kRunsM, false, m0, here_m, s));
-#pragma unroll
-      for (int n = 0; n < N::kLoads; ++n) set.n[n] = load(place_of(N(), n, p.n, kRunsN, true, n0, here_n, s));
+      load_side(M(), set.m, off_m, p.m, kRunsM, false, row_m, s);
+      load_side(N(), set.n, off_n, p.n, kRunsN, true, row_n, s);
     };
-    const auto put_side = [&](auto side, v4i* held, const Side& from, Runs runs, bool dealt_rows, int first, int here, int s,
-                              char* to) __attribute__((always_inline)) {
+    const auto put_side = [&](auto side, v4i* held, const Side& from, Runs runs, int row, int s, char* to) __attribute__((always_inline)) {
       using T = decltype(side);
       const int k0 = s * E::kDepth;
       const bool depth_ends = k0 + E::kDepth > depth;
-      const int64_t row = first + (columns && dealt_rows ? range.begin : 0);
-      const bool run_ends = runs == Runs::kAcross && row + T::kRows > from.count;
+      const bool run_ends = runs == Runs::kAcross && int64_t(row) + T::kRows > from.count;
       // (Both the same for the whole workgroup.)
       if (depth_ends || run_ends) {
 #pragma unroll
         for (int n = 0; n < T::kLoads; ++n) {
-          const Place where = place_of(side, n, from, runs, dealt_rows, first, here, s);
+          const Place where = place_of(side, n, from, runs, row, s);
           v4i x = granule::PlaceGranule(held[n], where.at, where.length);
           const int run = T::RunOf(n, wave, lane), granule = T::GranuleOf(n, wave, lane);
           const int left = runs == Runs::kPlain ? depth - k0 - granule * E::kGranule : depth - k0 - run;  // values, or runs
@@ -509,8 +522,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
     };
     const auto put = [&](int s, int stage, Set& set) __attribute__((always_inline)) {
       char* to = lds + stage * kStage + (wave * 64 + lane) * 16;
-      put_side(M(), set.m, p.m, kRunsM, false, m0, here_m, s, to);
-      put_side(N(), set.n, p.n, kRunsN, true, n0, here_n, s, to + M::kBytes);
+      put_side(M(), set.m, p.m, kRunsM, row_m, s, to);
+      put_side(N(), set.n, p.n, kRunsN, row_n, s, to + M::kBytes);
     };
     // (Steps past the last are the last one again, to where nobody reads.)
     if (steps > 0) {

@@ -18,16 +18,17 @@ struct Grid {
 
 // A tile's sizes, the workgroups that a CU runs side by side, and how long one step
 // of all of them takes, with operands straight to LDS, through registers, and fp32 (0: there is no such
-// kernel). Measured, us: bfloat16, 8 x 4096 x 2048 x 8192 in 544 / 160 / 160 / 96 steps of every CU
-// 265 / 181 / 167 / 171, 16 x 1683 x 3968 x 6400 194 / 147 / 133 / 116.
+// kernel). Measured on each tile in that order, us: bfloat16, 8 x 4096 x 2048 x 8192
+// 265 / 181 / 167 / 171, 16 x 1683 x 3968 x 6400 194 / 147 / 133 / 116; through registers, 4 x 4095 x 2047 x 8191
+// 377 / 239 / 212, 16 x 1001 x 501 x 2001 11.9 / 18.2 / 21.0 (128x128 is nowhere the best there and left out).
 struct TileCost {
   Tile tile;
   int m, n, per_cu;
   float direct, through, f32;
 };
-constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 2, 0.48f, 0.6f, 1.05f},
+constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 2, 0.48f, 0.58f, 1.05f},
                                {Tile::k128x128, 128, 128, 2, 1.08f, 0, 3.9f},
-                               {Tile::k256x128, 256, 128, 1, 1.0f, 0, 0},
+                               {Tile::k256x128, 256, 128, 1, 1.0f, 1.6f, 0},
                                {Tile::k256x256, 256, 256, 1, 1.68f, 0, 0}};
 // What a workgroup does before its first step and after its last, in steps.
 constexpr float kFixedSteps = 6;
@@ -45,11 +46,12 @@ void LaunchKernel(hipStream_t stream, const GemmArgs& args, unsigned blocks) {
 // (Eight waves on the larger tiles, four on the others.)
 template <int kType, Runs kRunsM, Runs kRunsN, bool kDirect>
 void LaunchOne(hipStream_t stream, const GemmArgs& args, const Grid& grid) {
-  if constexpr (kDirect && kType != RUYAMD_DTYPE_F32) {
-    if (grid.tile == Tile::k256x256)
-      return LaunchKernel<kType, kRunsM, kRunsN, 2, 4, 8, 4, true, 2>(stream, args, grid.blocks);
+  if constexpr (kType != RUYAMD_DTYPE_F32) {
+    if constexpr (kDirect)
+      if (grid.tile == Tile::k256x256)
+        return LaunchKernel<kType, kRunsM, kRunsN, 2, 4, 8, 4, true, 2>(stream, args, grid.blocks);
     if (grid.tile == Tile::k256x128)
-      return LaunchKernel<kType, kRunsM, kRunsN, 4, 2, 4, 4, true, 3>(stream, args, grid.blocks);
+      return LaunchKernel<kType, kRunsM, kRunsN, 4, 2, 4, 4, kDirect, kDirect ? 3 : 2>(stream, args, grid.blocks);
   }
   if constexpr (kDirect)
     if (grid.tile == Tile::k128x128)
@@ -127,7 +129,14 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
   Grid grid;
   int64_t blocks = 0;
   float best = 0;
-  const auto step_of = [&](const TileCost& t) { return !direct ? t.through : call.type == RUYAMD_DTYPE_F32 ? t.f32 : t.direct; };
+  const auto step_of = [&](const TileCost& t) {
+    const bool f32 = call.type == RUYAMD_DTYPE_F32;
+    if (direct) return f32 ? t.f32 : t.direct;
+    if (t.tile == Tile::k64x64) return t.through;
+    // (Both operands across the depth: 4 x 4095 x 2047, depth 8191 358 us on 64x64, 261 on 256x128, 64 x 301 x 1501, depth
+    // 4001 46 and 53.)
+    return f32 ? 0.0f : t.through * (columns ? 1.0f : 1.25f);
+  };
   const auto forced = [&](const TileCost& t) { return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols; };
   const bool force = std::any_of(std::begin(kTiles), std::end(kTiles), [&](const TileCost& t) { return forced(t) && step_of(t) != 0; });
   for (const TileCost& t : kTiles) {
