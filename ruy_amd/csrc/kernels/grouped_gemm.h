@@ -386,7 +386,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
         for (int n = 0; n < M::kLoads; ++n) LoadToLds(to + n * kWaves * 1024, off_m[n], rsrc_m);
 #pragma unroll
         for (int n = 0; n < N::kLoads; ++n) LoadToLds(to + M::kBytes + n * kWaves * 1024, off_n[n], rsrc_n);
-      } else {  // the last, partial step: zeros past the depth
+      } else {  // the last, partial step, and those behind it: zeros past the depth
 #pragma unroll
         for (int n = 0; n < M::kLoads; ++n)
           LoadToLds(to + n * kWaves * 1024, depth_of(M(), n, kRunsM) < left ? off_m[n] : kNothing, rsrc_m);
@@ -395,8 +395,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
           LoadToLds(to + M::kBytes + n * kWaves * 1024, depth_of(N(), n, kRunsN) < left ? off_n[n] : kNothing, rsrc_n);
       }
     };
-    // Steps are on their way to LDS up to kStages ahead. (Past the last the last one again, to
-    // where nobody reads any more: the number of loads on their way is then always the same.)
+    // Steps are on their way to LDS up to kStages ahead. (Past the last
+    // zeros, to where nobody reads any more: the number of loads on their way is then always the same.)
     //
     // The two halves of a step's depth take turns: while the matrix cores have one, the fragments of the
     // other come out of LDS. In the middle of a step every wave has all of its fragments in registers
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
     // next step can be read, and this one's LDS be loaded into again.
     constexpr int kLoads = M::kLoads + N::kLoads;
     if (steps > 0) {
-      StaticFor<kStages>([&](auto d) __attribute__((always_inline)) { issue(min(int(d), steps - 1), d); });
+      StaticFor<kStages>([&](auto d) __attribute__((always_inline)) { issue(d, d); });
       WaitVmcnt<(kStages - 1) * kLoads>();
       Barrier();
       Fragments first, second;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
         interleave();
         WaitVmcnt<(kStages - 2) * kLoads>();
         Barrier();
-        issue(min(s + kStages, steps - 1), stage);
+        issue(s + kStages, stage);
         read((stage + 1) % kStages, 0, first);
         multiply(second);
         interleave();
@@ -489,11 +489,10 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
       }
     };
     // Steps held in registers on their way.
-    constexpr int kSets = 2;
     struct Set {
       v4i m[M::kLoads], n[N::kLoads];
     };
-    Set held[kSets];
+    Set held[2];
     const auto fetch = [&](int s, Set& set) __attribute__((always_inline)) {
       load_side(M(), set.m, off_m, p.m, kRunsM, false, row_m, s);
       load_side(N(), set.n, off_n, p.n, kRunsN, true, row_n, s);
@@ -525,29 +524,37 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
       put_side(M(), set.m, p.m, kRunsM, row_m, s, to);
       put_side(N(), set.n, p.n, kRunsN, row_n, s, to + M::kBytes);
     };
-    // (Steps past the last are the last one again, to where nobody reads.)
-    if (steps > 0) {
-      fetch(0, held[0]);
-      if constexpr (kSets == 2) fetch(min(1, steps - 1), held[1]);
-      put(0, 0, held[0]);
-      fetch(min(kSets, steps - 1), held[0]);
-    }
-    const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
+    const auto use = [&](int stage) __attribute__((always_inline)) {
       __syncthreads();
       Fragments first, second;
       read(stage, 0, first);
       read(stage, 1, second);
       multiply(first);
       multiply(second);
-      Set& next = held[(stage + 1) % kSets];
-      put(min(s + 1, steps - 1), 1 - stage, next);
-      fetch(min(s + 1 + kSets, steps - 1), next);
     };
-    for (int s = 0;;) {
-      if (s == steps) break;
-      step(s++, std::integral_constant<int, 0>());
-      if (s == steps) break;
-      step(s++, std::integral_constant<int, 1>());
+    if (steps == 1) {
+      fetch(0, held[0]);
+      put(0, 0, held[0]);
+      use(0);
+    } else if (steps > 1) {
+      // (Loads past the last step are the last one's again and go unused: the number of loads on
+      // their way is then always the same.)
+      fetch(0, held[0]);
+      fetch(1, held[1]);
+      put(0, 0, held[0]);
+      fetch(min(2, steps - 1), held[0]);
+      const auto next = [&](int s, auto stage) __attribute__((always_inline)) {
+        put(s, stage, held[stage]);
+        fetch(min(s + 2, steps - 1), held[stage]);
+      };
+      for (int s = 1;; ++s) {
+        use(0);
+        if (s == steps) break;
+        next(s, std::integral_constant<int, 1>());
+        use(1);
+        if (++s == steps) break;
+        next(s, std::integral_constant<int, 0>());
+      }
     }
   }
 

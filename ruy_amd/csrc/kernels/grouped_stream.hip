@@ -55,8 +55,8 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
 
   // Waves: 8 to a workgroup, along the depth as long as that makes no more than 16 to a CU
   // (of weights in 16 or 32 bits 64), along the rows otherwise; fewer rows where what goes with
-  // them into LDS is too much. (bfloat16, 64 x 4096x2048, one or two tokens each: 64 waves to a CU
-  // 40.6 us, 16 44.0. 4-bit, 64 x 1024x2048: 24.0 and 20.5; 16384 x 16384, one token: 32.2 and
+  // them into LDS is too much. (Half, 64 x 2048x2048, 32 tokens: 64 waves to a CU
+  // 40.6 us, 16 44.0. 4-bit, the same: 24.0 and 20.5; 16384 x 16384, one token: 32.2 and
   // 31.3, with 4 waves to a workgroup 40, with 2 59. Two blocks of 16 rows to a wave are no
   // faster anywhere, and slower where there are few rows.)
   int row_waves = RowWaves(plan.slabs, plan.cols), depth_waves = 8 / row_waves;
