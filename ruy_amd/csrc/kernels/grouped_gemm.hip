@@ -20,7 +20,7 @@ struct Grid {
 // of all of them takes, with operands straight to LDS, through registers, and fp32 (0: there is no such
 // kernel). Measured on each tile in that order, us: bfloat16, 8 x 4096 x 2048 x 8192
 // 265 / 181 / 167 / 171, 16 x 1683 x 3968 x 6400 194 / 147 / 133 / 116; through registers, 4 x 4095 x 2047 x 8191
-// 377 / 239 / 212, 16 x 1001 x 501 x 2001 11.9 / 18.2 / 21.0 (128x128 is nowhere the best there and left out).
+// 367 / 239 / 207, 16 x 1001 x 501 x 2001 10.8 / 18.2 / 19.2 (128x128 is nowhere the best there and left out).
 struct TileCost {
   Tile tile;
   int m, n, per_cu;
@@ -133,8 +133,8 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
     const bool f32 = call.type == RUYAMD_DTYPE_F32;
     if (direct) return f32 ? t.f32 : t.direct;
     if (t.tile == Tile::k64x64) return t.through;
-    // (Both operands across the depth: 4 x 4095 x 2047, depth 8191 358 us on 64x64, 261 on 256x128, 64 x 301 x 1501, depth
-    // 4001 46 and 53.)
+    // (Both operands across the depth: 4 x 4095 x 2047, depth 8191 352 us on 64x64, 264 on 256x128, 64 x 301 x 1501, depth
+    // 4001 31 and 37.)
     return f32 ? 0.0f : t.through * (columns ? 1.0f : 1.25f);
   };
   const auto forced = [&](const TileCost& t) { return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols; };

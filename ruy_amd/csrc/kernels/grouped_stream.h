@@ -24,6 +24,12 @@
 // sum. Values that are not finite would make 16 + q and 16 + zero, or a value's three parts, meet as
 // infinity - infinity; a wave that ends with one goes through its depth once more with the exact
 // q - zero and whole values.
+//
+// What bounds it is the rate of the weights' bytes out of HBM. Half, 64 matrices of
+// 2048x2048, 25 of them with one of 32 tokens or more: 210 MB in 40.6 us, 5.2 TB/s; 4-bit,
+// 16384x16384 with a scale to 128, one token: 138 MB in 31 us, 4.5 TB/s (6.5 TB/s is the
+// most that anything here reads at), 64 x 2048x2048 with a scale to 32: 59 MB in 20.5 us. Small ones are
+// one wave's way through its depth: 2048x2048 5.3 us of which 2.5 are the launch.
 #ifndef RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 #define RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 
