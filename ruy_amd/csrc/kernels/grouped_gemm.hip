@@ -108,6 +108,8 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
   a.dst_m_stride = swapped ? call.dst_cs : call.dst_rs;
   a.dst_n_stride = swapped ? call.dst_rs : call.dst_cs;
 
+  // (Sizes and depths are rounded up to tiles, and gone past by some steps, in 32 bits.)
+  if (max(call.m, max(call.n, call.k)) > 0x7fffffff - 2048) return false;
   // Offsets inside a tile are 31 bits.
   const int64_t longest = (int64_t(1) << 31) / (bytes * 128) - 128;
   if (a.m.pitch > longest || a.n.pitch > longest) return false;

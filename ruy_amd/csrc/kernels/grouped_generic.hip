@@ -17,7 +17,7 @@ __global__ __launch_bounds__(kTile* kTile) void GenericGroupedKernel(Call c, Int
   for (int g = blockIdx.z; g < c.groups; g += gridDim.z) {
     const bool by_columns = c.dealt == Dealt::kColumns;
     const Range range = RangeOf(c.offsets, g, by_columns ? c.n : c.k);
-    const int i = blockIdx.x * kTile + threadIdx.x;
+    const int64_t i = int64_t(blockIdx.x) * kTile + threadIdx.x;
     if (i >= c.m) return;
     const int columns = by_columns ? range.count : c.n;
     const int depth = by_columns ? c.k : range.count;

@@ -10,6 +10,8 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   if (!int4 && (call.dealt != Dealt::kColumns || call.lhs_cs != 1 || call.forced_tile_rows)) return false;
   // (A row has 16 bytes at least, and what a lane has of one ends before 2^31.)
   if (call.k < 32 || call.k > (1 << 28)) return false;
+  // (Sizes are rounded up to workgroups in 32 bits.)
+  if (max(call.m, call.n) > 0x7fffffff - 2048) return false;
   StreamArgs args;
   args.c = call;
   if (int4) args.w = *weights;
