@@ -88,7 +88,6 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   using T = Stream<kInt4, kType, kSlabs>;
   constexpr int kMostTokens = T::kTokens * kCols;
   constexpr int kRowWaves = RowWaves(kSlabs, kCols);
-  constexpr int kRows = 1;  // blocks of 16 rows to a wave
   // Scales to a chunk, steps to a scale.
   constexpr int kScales =
       T::kWeightLoads * (!kInt4 || kScaling == Scaling::kWide ? 1 : kScaling == Scaling::k64 ? 2 : 4);
@@ -105,7 +104,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int depth_waves = args.depth_waves, row_waves = kSlabs ? kRowWaves : args.row_waves;
   const int depth_wave = wave >> __builtin_ctz(row_waves), row_wave = wave & (row_waves - 1);
-  const int work_rows = 16 * kRows * row_waves;
+  const int work_rows = 16 * row_waves;
 
   TileOf tile;
   Range range;
@@ -125,25 +124,22 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 
   // Where this lane's rows of weights begin. (Rows past the last are the last one
   // again; their results are not stored.)
-  const uint8_t* row_data[kRows];
-  int64_t row_scales[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int64_t row = min(row0 + (row_wave * kRows + r) * 16 + l, c.m - 1);
-    if constexpr (kInt4) {
-      row_data[r] = w.data + tile.group * w.matrix_bytes + row * w.row_bytes;
-      row_scales[r] = tile.group * w.scales_matrix_stride + row * w.scale_stride;
-    } else {
-      row_data[r] = static_cast<const uint8_t*>(c.lhs) + (tile.group * c.matrix_stride + row * c.lhs_rs) * T::kBytes;
-    }
+  const uint8_t* row_data;
+  int64_t row_scales;
+  const int64_t my_row = min(row0 + row_wave * 16 + l, c.m - 1);
+  if constexpr (kInt4) {
+    row_data = w.data + tile.group * w.matrix_bytes + my_row * w.row_bytes;
+    row_scales = tile.group * w.scales_matrix_stride + my_row * w.scale_stride;
+  } else {
+    row_data = static_cast<const uint8_t*>(c.lhs) + (tile.group * c.matrix_stride + my_row * c.lhs_rs) * T::kBytes;
   }
   const int row_bytes = kInt4 ? (c.k + 1) / 2 : c.k * T::kBytes;
   const int row_scale_count = kInt4 ? (c.k + w.group_size - 1) / w.group_size : 0;
   const bool f32_scales = w.scale_type == RUYAMD_DTYPE_F32;
 
   struct Held {
-    v4i weights[kRows][T::kWeightLoads];
-    uint32_t scales[kScalesInLds ? 1 : kRows][kScales], zeros[kScalesInLds ? 1 : kRows][kScales];  // (Scaling::kAny)
+    v4i weights[T::kWeightLoads];
+    uint32_t scales[kScales], zeros[kScales];  // (Scaling::kAny)
   };
   // Loads never reach past the end of a row (which has 16 bytes at least): what would is
   // read from its last bytes, and moved to where it belongs by Place.
@@ -152,19 +148,15 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
       for (int g = 0; g < kScales; ++g) {
         const int at = min(chunk * T::kChunk + g * (T::kChunk / kScales), c.k - 1) / w.group_size;
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          h.scales[r][g] = f32_scales ? static_cast<const uint32_t*>(w.scales)[row_scales[r] + at]
-                                      : static_cast<const uint16_t*>(w.scales)[row_scales[r] + at];
-          h.zeros[r][g] = kZeroPoints ? w.zero_points[row_scales[r] + at] : 8;
-        }
+        h.scales[g] = f32_scales ? static_cast<const uint32_t*>(w.scales)[row_scales + at]
+                                 : static_cast<const uint16_t*>(w.scales)[row_scales + at];
+        h.zeros[g] = kZeroPoints ? w.zero_points[row_scales + at] : 8;
       }
     }
 #pragma unroll
     for (int i = 0; i < T::kWeightLoads; ++i) {
       const int at = min(chunk * (T::kWeightLoads * 64) + i * 64 + q * 16, row_bytes - 16);
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) h.weights[r][i] = *reinterpret_cast<const granule::v4i_unaligned*>(row_data[r] + at);
+      h.weights[i] = *reinterpret_cast<const granule::v4i_unaligned*>(row_data + at);
     }
   };
   const auto place = [&](int chunk, Held& h) __attribute__((always_inline)) {
@@ -172,8 +164,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
     for (int i = 0; i < T::kWeightLoads; ++i) {
       const int at = chunk * (T::kWeightLoads * 64) + i * 64 + q * 16;
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) h.weights[r][i] = granule::PlaceGranule(h.weights[r][i], at, row_bytes);
+      h.weights[i] = granule::PlaceGranule(h.weights[i], at, row_bytes);
     }
   };
   // A scale's bits, read as its type, as a number.
@@ -216,18 +207,15 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         }
     }
   };
-  const auto scales_of = [&](const Held& h, int chunk, float (&scale)[kRows][kScales], uint32_t (&zero)[kRows][kScales])
+  const auto scales_of = [&](const Held& h, int chunk, float (&scale)[kScales], uint32_t (&zero)[kScales])
                              __attribute__((always_inline)) {
+    const int row = row_wave * 16 + l;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int row = (row_wave * kRows + r) * 16 + l;
-#pragma unroll
-      for (int g = 0; g < kScales; ++g) {
-        scale[r][g] = kScalesInLds ? lds_scales[row * args.scale_pitch + chunk * kScales + g] : as_float(h.scales[r][g]);
-        zero[r][g] = 8;
-        if constexpr (kZeroPoints)
-          zero[r][g] = kScalesInLds ? lds_zeros[row * args.zero_pitch + chunk * kScales + g] : h.zeros[r][g];
-      }
+    for (int g = 0; g < kScales; ++g) {
+      scale[g] = kScalesInLds ? lds_scales[row * args.scale_pitch + chunk * kScales + g] : as_float(h.scales[g]);
+      zero[g] = 8;
+      if constexpr (kZeroPoints)
+        zero[g] = kScalesInLds ? lds_zeros[row * args.zero_pitch + chunk * kScales + g] : h.zeros[g];
     }
   };
 
@@ -317,7 +305,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
     lds_row[t] = (t * T::kTokens < tokens ? t * 16 : 0) + min(l, here - 1);
   }
 
-  v4f acc[kRows][kCols] = {};
+  v4f acc[kCols] = {};
 
   // What the eight values of a word are taken apart with. (Held in registers: as constants
   // in the instructions they would each take one more.)
@@ -390,21 +378,18 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
         for (int t = 0; t < kCols; ++t) {
           const v4i x = *reinterpret_cast<const v4i*>(at + lds_row[t] * args.pitch + unit_of(j) * 16);
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) Mma<kType>(x, h.weights[r][j], acc[r][t]);
+          Mma<kType>(x, h.weights[j], acc[t]);
         }
     } else {
-      v4i words[kRows][T::kWeightLoads];
-      float scale[kRows][kScales];
-      uint32_t zero[kRows][kScales];
+      v4i words[T::kWeightLoads];
+      float scale[kScales];
+      uint32_t zero[kScales];
       scales_of(h, chunk, scale, zero);
 #pragma unroll
-      for (int r = 0; r < kRows; ++r)
-#pragma unroll
-        for (int i = 0; i < T::kWeightLoads; ++i) words[r][i] = exchange(h.weights[r][i]);
+      for (int i = 0; i < T::kWeightLoads; ++i) words[i] = exchange(h.weights[i]);
 #pragma unroll
       for (int g = 0; g < kScales; ++g) {
-        v4f sum[kRows][kCols] = {};
+        v4f sum[kCols] = {};
         v4f ones[kCols] = {};
 #pragma unroll
         for (int f = 0; f < kStepsToScale; ++f) {
@@ -418,28 +403,22 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
               Mma<kMmaType>(x[t], v4i{kOnes, kOnes, kOnes, kOnes}, ones[t]);
             }
           }
+          const uint32_t word = words[j / 4][j % 4];
+          const v4i b = kHalf          ? less_zero(word, zero[g])
+                        : kDifference ? to_bf16(less_zero(word, zero[g]))
+                                      : sixteen_and(word);
 #pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            const uint32_t word = words[r][j / 4][j % 4];
-            const v4i b = kHalf          ? less_zero(word, zero[r][g])
-                          : kDifference ? to_bf16(less_zero(word, zero[r][g]))
-                                        : sixteen_and(word);
+          for (int t = 0; t < kCols; ++t) Mma<kMmaType>(x[t], b, sum[t]);
+        }
+        const float away = -16.0f - static_cast<float>(zero[g]);
 #pragma unroll
-            for (int t = 0; t < kCols; ++t) Mma<kMmaType>(x[t], b, sum[r][t]);
+        for (int t = 0; t < kCols; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = sum[t][e];
+            if constexpr (!kDifference) v = __builtin_fmaf(away, ones[t][e], v);
+            acc[t][e] = __builtin_fmaf(scale[g], v, acc[t][e]);
           }
-        }
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          const float away = -16.0f - static_cast<float>(zero[r][g]);
-#pragma unroll
-          for (int t = 0; t < kCols; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = sum[r][t][e];
-              if constexpr (!kDifference) v = __builtin_fmaf(away, ones[t][e], v);
-              acc[r][t][e] = __builtin_fmaf(scale[r][g], v, acc[r][t][e]);
-            }
-        }
       }
     }
   };
@@ -449,7 +428,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   // waves. What is left of the depth comes behind the loop.
   const int turns = kSlabs ? whole_chunks / depth_waves
                            : (whole_chunks - depth_wave + depth_waves - 1) / depth_waves;
-  // The depth begins at another place in every 16 * kRows rows and goes round: rows
+  // The depth begins at another place in every 16 rows and goes round: rows
   // often lie a power of two apart, and whoever goes through theirs side by side, from
   // the same place on, asks the same few memory channels. (Places by a multiplicative hash; one after
   // the other they meet again at some row lengths. 16384 rows of 8 KiB read alone, 4 waves
@@ -559,29 +538,23 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   if constexpr (kInt4 && !kHalf) {
     bool finite = true;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int t = 0; t < kCols; ++t)
 #pragma unroll
-      for (int t = 0; t < kCols; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) finite = finite && __builtin_isfinite(acc[r][t][e]);
+      for (int e = 0; e < 4; ++e) finite = finite && __builtin_isfinite(acc[t][e]);
     if (__any(!finite)) {
       // Once more, with q - zero itself: exact in bfloat16 and in fp32.
 #pragma unroll
-      for (int r = 0; r < kRows; ++r)
-#pragma unroll
-        for (int t = 0; t < kCols; ++t) acc[r][t] = v4f{0, 0, 0, 0};
+      for (int t = 0; t < kCols; ++t) acc[t] = v4f{0, 0, 0, 0};
 #pragma unroll 1
       for (int chunk = depth_wave; chunk < chunks; chunk += depth_waves) {
         Held h;
         load(chunk, h);
         place(chunk, h);
-        float scale[kRows][kScales];
-        uint32_t zero[kRows][kScales];
+        float scale[kScales];
+        uint32_t zero[kScales];
         scales_of(h, chunk, scale, zero);
 #pragma unroll
-        for (int r = 0; r < kRows; ++r)
-#pragma unroll
-          for (int i = 0; i < T::kWeightLoads; ++i) h.weights[r][i] = exchange(h.weights[r][i]);
+        for (int i = 0; i < T::kWeightLoads; ++i) h.weights[i] = exchange(h.weights[i]);
 #pragma unroll
         for (int g = 0; g < kScales; ++g) {
 #pragma unroll 1
@@ -592,33 +565,27 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
               // (fp32: the whole token in the place of its first part.)
               const int token = min(t * T::kTokens + (T::kParts ? l / 3 : l), tokens - 1);
               const Unit x = fetch(token, chunk * T::kChunkUnits + unit_of(j));
+              const uint32_t word = h.weights[g * kStepsToScale / 4][0];
+              float v[8];
 #pragma unroll
-              for (int r = 0; r < kRows; ++r) {
-                const uint32_t word = h.weights[r][g * kStepsToScale / 4][0];
-                float v[8];
+              for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>(word >> (4 * e) & 15) - static_cast<int>(zero[g]));
+              v4f sum = {0, 0, 0, 0};
+              if constexpr (T::kParts) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>(word >> (4 * e) & 15) - static_cast<int>(zero[r][g]));
-                v4f sum = {0, 0, 0, 0};
-                if constexpr (T::kParts) {
-#pragma unroll
-                  for (int e = 0; e < 8; ++e)
-                    sum = __builtin_amdgcn_mfma_f32_16x16x4f32(l % 3 == 0 ? __int_as_float(x.x[e / 4][e % 4]) : 0.0f, v[e],
-                                                               sum, 0, 0, 0);
-                } else {
-                  const v4i b = {float_parts::RoundPair(v[0], v[4]), float_parts::RoundPair(v[1], v[5]),
-                                 float_parts::RoundPair(v[2], v[6]), float_parts::RoundPair(v[3], v[7])};
-                  Mma<kMmaType>(in_word_order(x.x[0]), b, sum);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[r][t][e] = __builtin_fmaf(scale[r][g], sum[e], acc[r][t][e]);
+                for (int e = 0; e < 8; ++e)
+                  sum = __builtin_amdgcn_mfma_f32_16x16x4f32(l % 3 == 0 ? __int_as_float(x.x[e / 4][e % 4]) : 0.0f, v[e],
+                                                             sum, 0, 0, 0);
+              } else {
+                const v4i b = {float_parts::RoundPair(v[0], v[4]), float_parts::RoundPair(v[1], v[5]),
+                               float_parts::RoundPair(v[2], v[6]), float_parts::RoundPair(v[3], v[7])};
+                Mma<kMmaType>(in_word_order(x.x[0]), b, sum);
               }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[t][e] = __builtin_fmaf(scale[g], sum[e], acc[t][e]);
             }
             // (The next step's word in the place of this one's.)
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-              v4i& x = h.weights[r][g * kStepsToScale / 4];
-              x = v4i{x[1], x[2], x[3], 0};
-            }
+            v4i& x = h.weights[g * kStepsToScale / 4];
+            x = v4i{x[1], x[2], x[3], 0};
           }
         }
       }
@@ -632,9 +599,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
     if (t * T::kTokens >= tokens) break;  // (the same for all waves)
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) partial[((wave * kRows + r) * 4 + e) * 64 + lane] = acc[r][t][e];
+    for (int e = 0; e < 4; ++e) partial[(wave * 4 + e) * 64 + lane] = acc[t][e];
     __syncthreads();
     // Value number v: row v % 16 of a block of 16, token v / 16 % 16, block v / 256.
     for (int v = threadIdx.x; v < work_rows * T::kTokens; v += blockDim.x) {
@@ -646,7 +611,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
       for (int s = 0; s < (T::kParts ? 3 : 1); ++s) {
         const int at = T::kParts ? token * 3 + s : token;  // row of the accumulators' block
         const float* from = partial + (r * 4 + at % 4) * 64 + at / 4 * 16 + row;
-        for (int i = 0; i < depth_waves; ++i) sum += from[i * row_waves * kRows * 256];
+        for (int i = 0; i < depth_waves; ++i) sum += from[i * row_waves * 256];
       }
       if (c.bias) sum += c.bias[tile.group * c.bias_stride + m];
       StoreFloat(c.dst, c.dst_type, m * c.dst_rs + (int64_t(range.begin) + n) * c.dst_cs,
