@@ -1,5 +1,6 @@
 // Launches of the tiled kernel of grouped products.
 #include "grouped_gemm.h"
+#include "launch_geometry.h"
 
 #include <algorithm>
 #include <cmath>
@@ -110,7 +111,8 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
 
   // (Sizes and depths are rounded up to tiles, and gone past by some steps, in 32 bits.)
   if (max(call.m, max(call.n, call.k)) > 0x7fffffff - 2048) return false;
-  // Offsets inside a tile are 31 bits.
+  // Offsets inside a tile are 31 bits where it goes to LDS directly (fits, below, for each tile), and 32 otherwise:
+  // what this leaves fits 32 in any of them, and 31 in those of 128 rows and fewer.
   const int64_t longest = (int64_t(1) << 31) / (bytes * 128) - 128;
   if (a.m.pitch > longest || a.n.pitch > longest) return false;
   const auto aligned = [&](const Side& s, Runs runs, bool dealt_rows) {
@@ -131,8 +133,12 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
   Grid grid;
   int64_t blocks = 0;
   float best = 0;
+  const auto fits = [&](const Side& s, Runs runs, int rows) {
+    return runs == Runs::kAcross || TileOffsetsFit(rows, s.pitch * bytes, 128);
+  };
   const auto step_of = [&](const TileCost& t) {
     const bool f32 = call.type == RUYAMD_DTYPE_F32;
+    if (direct && !(fits(a.m, runs_m, t.m) && fits(a.n, runs_n, t.n))) return 0.0f;
     if (direct) return f32 ? t.f32 : t.direct;
     if (t.tile == Tile::k64x64) return t.through;
     // (Both operands across the depth: 4 x 4095 x 2047, depth 8191 352 us on 64x64, 264 on 256x128, 64 x 301 x 1501, depth

@@ -38,6 +38,13 @@ inline unsigned ElementwiseBlocks(int64_t n, int threads) {
   return static_cast<unsigned>(b < 1 ? 1 : (b > int64_t(kMaxGridX) ? int64_t(kMaxGridX) : b));
 }
 
+// Whether what a tile reads of `runs` runs, `pitch` bytes from one to the next and the first `length` bytes of each,
+// ends within the 2^31 bytes that a buffer resource of the tiled grouped kernel has. (What lies beyond
+// its end is read as zeros, with no error.)
+inline bool TileOffsetsFit(int64_t runs, int64_t pitch, int64_t length) {
+  return (runs - 1) * pitch + length <= int64_t(1) << 31;
+}
+
 }  // namespace ruyamd
 
 #endif  // RUY_AMD_CSRC_KERNELS_LAUNCH_GEOMETRY_H_

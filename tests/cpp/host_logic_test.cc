@@ -78,6 +78,16 @@ static void TestElementwiseBlocks() {
   EXPECT(ruyamd::ElementwiseBlocks(int64_t(1) << 40, 256) == ruyamd::kMaxGridX);
 }
 
+// 128 bytes of every row of a tile: the longest pitch that each tile's rows have.
+static void TestTileOffsetsFit() {
+  EXPECT(ruyamd::TileOffsetsFit(256, 2 * int64_t(4210752), 128));   // ends at 2^31
+  EXPECT(!ruyamd::TileOffsetsFit(256, 2 * int64_t(4210753), 128));
+  EXPECT(!ruyamd::TileOffsetsFit(256, 2 * int64_t(8388480), 128));
+  EXPECT(ruyamd::TileOffsetsFit(128, 2 * int64_t(8388480), 128));
+  EXPECT(ruyamd::TileOffsetsFit(128, 4 * int64_t(4194176), 128));
+  EXPECT(ruyamd::TileOffsetsFit(1, int64_t(1) << 62, 128));
+}
+
 namespace ds = ruyamd::depth_split;
 
 static void TestDepthPartsCoverEveryStepOnce() {
@@ -393,6 +403,7 @@ int main() {
   TestRowSumShares();
   TestGenericGrid();
   TestElementwiseBlocks();
+  TestTileOffsetsFit();
   TestDepthPartsCoverEveryStepOnce();
   TestDepthSplitArrivalProtocol();
   TestLargeTileSplitProtocol();
