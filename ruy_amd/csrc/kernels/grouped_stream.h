@@ -12,24 +12,24 @@
 // have through LDS. The tokens are put into LDS first, as the matrix instructions want
 // them: all of their depth where that fits, slab by slab otherwise (kSlabs).
 //
-// 4-bit weights. The four bits of q put into the mantissa of a 16-bit float of some exponent
-// make 2^e + q (half: 1024 + q, bfloat16: 16 + q), two at a time. Half: 1024 + zero is
-// then taken away, exactly and packed: 9 instructions to 8 weights. bfloat16 has no such
-// instruction: the product is formed with 16 + q, and (16 + zero) * sum(x), whose sums come from
-// the matrix cores as well (a product with ones), is taken away from every group's sum: the
-// sums' roundings are those of values up to 31 / 8 larger, far below a rounding to bfloat16. fp32 tokens
-// are three bf16 rows each that add up to them (float_parts.h), so that every product is exact;
-// they are multiplied by q - zero, formed in half and converted, 21 instructions to 8 weights, as
-// there is no later rounding that the sums' would be small beside. The scale multiplies a group's
-// sum. Values that are not finite would make 16 + q and 16 + zero, or a value's three parts, meet as
-// infinity - infinity; a wave that ends with one goes through its depth once more with the exact
-// q - zero and whole values.
+// 4-bit weights. What is multiplied is q - zero, exactly, whatever the tokens' type: any other
+// sum, from which the zero point's share is taken away later, is rounded by values that the
+// result does not have, without bound where a large token meets weights equal to their zero
+// point. The four bits of q put into the mantissa of 1024 as a half make 1024 + q, two at a
+// time. Half: 1024 + zero is then taken away, packed: 9 instructions to 8 weights. bfloat16 has
+// no such instruction: 1024 + zero is taken away in fp32, and the upper halves of the results,
+// which have all of them, are the bfloat16 values: 17 instructions (64 x 2048x2048 with a scale
+// to 32, below, 22.4 us; with products of 16 + q, two at a time, and their sums put right
+// afterwards 20.5). fp32 tokens are three bf16 rows each that add up to them (float_parts.h),
+// so that every product is exact, against the same weights. The scale multiplies a group's
+// sum. A value's three parts would meet as infinity - infinity where it is not finite; a wave
+// that ends with one goes through its depth once more with whole values.
 //
 // What bounds it is the rate of the weights' bytes out of HBM. Half, 64 matrices of
 // 2048x2048, 25 of them with one of 32 tokens or more: 210 MB in 40.6 us, 5.2 TB/s; 4-bit,
 // 16384x16384 with a scale to 128, one token: 138 MB in 31 us, 4.5 TB/s (6.5 TB/s is the
-// most that anything here reads at), 64 x 2048x2048 with a scale to 32: 59 MB in 20.5 us. Small ones are
-// one wave's way through its depth: 2048x2048 5.3 us of which 2.5 are the launch.
+// most that anything here reads at), 64 x 2048x2048 with a scale to 32: 59 MB in 22.4 us. Small ones are
+// one wave's way through its depth: 2048x2048 5.4 us of which 2.5 are the launch.
 #ifndef RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 #define RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 
@@ -94,8 +94,6 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   constexpr int kStepsToScale = kInt4 ? T::kSteps / kScales : 1;
   constexpr bool kScalesInLds = kInt4 && kScaling != Scaling::kAny;
   constexpr bool kHalf = kType == RUYAMD_DTYPE_F16;
-  // Whether the products of 4-bit weights are formed with q - zero, not with 16 + q.
-  constexpr bool kDifference = kHalf || T::kParts;
   constexpr int kMmaType = kHalf ? RUYAMD_DTYPE_F16 : RUYAMD_DTYPE_BF16;  // of 4-bit weights
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const Call& c = args.c;
@@ -309,8 +307,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 
   // What the eight values of a word are taken apart with. (Held in registers: as constants
   // in the instructions they would each take one more.)
-  uint32_t low_mask = kDifference ? 0x000F000Fu : 0x00780078u, high_mask = 0x00F000F0u, sixteenth = 0x2C002C00u;
-  uint32_t exponent = kDifference ? 0x64006400u : 0x41804180u;
+  uint32_t low_mask = 0x000F000Fu, high_mask = 0x00F000F0u, sixteenth = 0x2C002C00u, exponent = 0x64006400u;
   asm("" : "+s"(low_mask));
   asm("" : "+s"(high_mask));
   asm("" : "+s"(sixteenth));
@@ -329,20 +326,24 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
                bits(halves((y & low_mask) | exponent) - away_low),
                bits(__builtin_elementwise_fma(halves((y & high_mask) | exponent), halves(sixteenth), away_high))};
   };
-  // The same as bfloat16, exact too (whole numbers of 4 bits and a sign).
-  const auto to_bf16 = [&](v4i x) __attribute__((always_inline)) -> v4i {
-    v4i y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const v2h pair = halves(x[e]);
-      y[e] = float_parts::RoundPair(static_cast<float>(pair[0]), static_cast<float>(pair[1]));
-    }
-    return y;
-  };
-  // bfloat16: 16 + q, in that order.
-  const auto sixteen_and = [&](uint32_t x) __attribute__((always_inline)) -> v4i {
-    return v4i{static_cast<int>((x << 3 & low_mask) | exponent), static_cast<int>((x >> 1 & low_mask) | exponent),
-               static_cast<int>((x >> 5 & low_mask) | exponent), static_cast<int>((x >> 9 & low_mask) | exponent)};
+  // The same as bfloat16, exact too (whole numbers of 4 bits and a sign). The factors are variables: a product with a half
+  // and a sum are one instruction then, a conversion and a sum two.
+  float whole_factor = 1.0f, sixteenth_factor = 0.0625f;
+  asm("" : "+v"(whole_factor));
+  asm("" : "+v"(sixteenth_factor));
+  const auto less_zero_bf16 = [&](uint32_t x, uint32_t zero) __attribute__((always_inline)) -> v4i {
+    const float z = static_cast<float>(zero), away_low = -1024.0f - z, away_high = -64.0f - z;
+    const auto less = [&](uint32_t with_exponent, float factor, float away) __attribute__((always_inline)) -> int {
+      const v2h pair = halves(with_exponent);
+      const float first = __builtin_fmaf(static_cast<float>(pair[0]), factor, away);
+      const float second = __builtin_fmaf(static_cast<float>(pair[1]), factor, away);
+      return static_cast<int>(__builtin_amdgcn_perm(__float_as_uint(second), __float_as_uint(first), 0x07060302));
+    };
+    const uint32_t y = x >> 8;
+    return v4i{less((x & low_mask) | exponent, whole_factor, away_low),
+               less((x & high_mask) | exponent, sixteenth_factor, away_high),
+               less((y & low_mask) | exponent, whole_factor, away_low),
+               less((y & high_mask) | exponent, sixteenth_factor, away_high)};
   };
   // 16-byte pieces of four lanes to pieces of a 4-byte word each: word j of the
   // lane with q holds what bytes j * 16 + q * 4 .. of the row's 64 held. A step's 32 depth positions are
@@ -390,35 +391,22 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
 #pragma unroll
       for (int g = 0; g < kScales; ++g) {
         v4f sum[kCols] = {};
-        v4f ones[kCols] = {};
 #pragma unroll
         for (int f = 0; f < kStepsToScale; ++f) {
           const int j = g * kStepsToScale + f;
           v4i x[kCols];
 #pragma unroll
-          for (int t = 0; t < kCols; ++t) {
+          for (int t = 0; t < kCols; ++t)
             x[t] = *reinterpret_cast<const v4i*>(at + lds_row[t] * args.pitch + unit_of(j) * 16);
-            if constexpr (!kDifference) {
-              constexpr int kOnes = 0x3F803F80;
-              Mma<kMmaType>(x[t], v4i{kOnes, kOnes, kOnes, kOnes}, ones[t]);
-            }
-          }
           const uint32_t word = words[j / 4][j % 4];
-          const v4i b = kHalf          ? less_zero(word, zero[g])
-                        : kDifference ? to_bf16(less_zero(word, zero[g]))
-                                      : sixteen_and(word);
+          const v4i b = kHalf ? less_zero(word, zero[g]) : less_zero_bf16(word, zero[g]);
 #pragma unroll
           for (int t = 0; t < kCols; ++t) Mma<kMmaType>(x[t], b, sum[t]);
         }
-        const float away = -16.0f - static_cast<float>(zero[g]);
 #pragma unroll
         for (int t = 0; t < kCols; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = sum[t][e];
-            if constexpr (!kDifference) v = __builtin_fmaf(away, ones[t][e], v);
-            acc[t][e] = __builtin_fmaf(scale[g], v, acc[t][e]);
-          }
+          for (int e = 0; e < 4; ++e) acc[t][e] = __builtin_fmaf(scale[g], sum[t][e], acc[t][e]);
       }
     }
   };
@@ -535,14 +523,14 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
     }
   }
 
-  if constexpr (kInt4 && !kHalf) {
+  if constexpr (T::kParts) {
     bool finite = true;
 #pragma unroll
     for (int t = 0; t < kCols; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) finite = finite && __builtin_isfinite(acc[t][e]);
     if (__any(!finite)) {
-      // Once more, with q - zero itself: exact in bfloat16 and in fp32.
+      // Once more, with whole tokens on the fp32 instructions.
 #pragma unroll
       for (int t = 0; t < kCols; ++t) acc[t] = v4f{0, 0, 0, 0};
 #pragma unroll 1
@@ -562,24 +550,18 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
             const int j = g * kStepsToScale + f;
 #pragma unroll
             for (int t = 0; t < kCols; ++t) {
-              // (fp32: the whole token in the place of its first part.)
-              const int token = min(t * T::kTokens + (T::kParts ? l / 3 : l), tokens - 1);
+              // (The whole token in the place of its first part.)
+              const int token = min(t * T::kTokens + l / 3, tokens - 1);
               const Unit x = fetch(token, chunk * T::kChunkUnits + unit_of(j));
               const uint32_t word = h.weights[g * kStepsToScale / 4][0];
               float v[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>(word >> (4 * e) & 15) - static_cast<int>(zero[g]));
               v4f sum = {0, 0, 0, 0};
-              if constexpr (T::kParts) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  sum = __builtin_amdgcn_mfma_f32_16x16x4f32(l % 3 == 0 ? __int_as_float(x.x[e / 4][e % 4]) : 0.0f, v[e],
-                                                             sum, 0, 0, 0);
-              } else {
-                const v4i b = {float_parts::RoundPair(v[0], v[4]), float_parts::RoundPair(v[1], v[5]),
-                               float_parts::RoundPair(v[2], v[6]), float_parts::RoundPair(v[3], v[7])};
-                Mma<kMmaType>(in_word_order(x.x[0]), b, sum);
-              }
+              for (int e = 0; e < 8; ++e)
+                sum = __builtin_amdgcn_mfma_f32_16x16x4f32(l % 3 == 0 ? __int_as_float(x.x[e / 4][e % 4]) : 0.0f, v[e], sum,
+                                                           0, 0, 0);
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[t][e] = __builtin_fmaf(scale[g], sum[e], acc[t][e]);
             }

@@ -1,0 +1,96 @@
+"""4-bit products (ruyamd_mul_int4) where a sum of anything but (q - zero) * x, or a token taken apart, would lose what the
+definition keeps. Problems of whole numbers have to be exact; see test_gpu_grouped.py for all others."""
+import sys
+
+import pytest
+import torch
+
+import grouped_reference as R
+from grouped_reference import COL, ROW, Buffer
+from ruy_amd import _structs as S
+from ruy_amd import api
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [S.BF16, S.F16, S.F32]
+name_of = S.DTYPE_NAMES.get
+
+
+def announce(*what):
+    print("[case]", *what, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def context():
+    ctx = api.Context()
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield ctx
+    ctx.close()
+
+
+@pytest.fixture(params=["generic", "chosen"])
+def kernel(request, context):
+    context.force_generic_kernel(request.param == "generic")
+    yield request.param
+    context.force_generic_kernel(False)
+
+
+def generator(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+class Weights:
+    """rows x cols random 4-bit weights; `scales`: what becomes of random numbers between 0 and 1."""
+
+    def __init__(self, g, rows, cols, group_size, zeros, scale_type, scales):
+        groups = -(-cols // group_size)
+        self.q = torch.randint(16, (rows, cols + cols % 2), generator=g, device="cuda", dtype=torch.uint8)
+        self.scales = scales(torch.rand(rows, groups, generator=g, device="cuda")).to(R.TORCH[scale_type])
+        self.zeros = torch.randint(16, (rows, groups), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+        self.shape, self.group_size, self.scale_type = (rows, cols), group_size, scale_type
+
+    def set_to_zero_point(self, cols):
+        at = torch.tensor(cols, device="cuda")
+        self.q[:, at] = 8 if self.zeros is None else self.zeros[:, at // self.group_size]
+
+    def matrix(self):
+        self.data = self.q[:, 0::2] | self.q[:, 1::2] << 4
+        return api.Int4Matrix(*self.shape, self.group_size, self.data.contiguous(), self.scales, self.scale_type, self.zeros)
+
+    def values(self):
+        self.matrix()
+        return R.int4_values(self.data, self.scales, self.zeros, *self.shape, self.group_size)
+
+
+def product(context, weights, x, type_, dst_type, order=COL):
+    (m, k), n = weights.shape, x.shape[1]
+    rhs, dst = Buffer(type_, k, n, order).set(x), Buffer(dst_type, m, n, COL)
+    matrix = weights.matrix()
+    api.mul_int4(matrix, rhs.matrix(), api.MulParams(S.F32, dst_type), context, dst.matrix())
+    return dst.view(), rhs.view().double()
+
+
+def powers_of_two(random):
+    return torch.exp2(torch.floor(random * 5) - 2)
+
+
+# What weights equal to their zero point meet leaves no trace.
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group_size", [32, 64, 96, 128, 5000])
+def test_large_tokens_against_weights_of_zero(context, kernel, type_, zeros, group_size):
+    large = {S.BF16: 2.0 ** 100, S.F16: 2.0 ** 15, S.F32: 2.0 ** 100}[type_]
+    for m, k, n in [(48, 512, 1), (40, 1000, 5), (33, 2051, 20), (64, 700, 40)]:
+        announce("zeros", name_of(type_), m, k, n, group_size, zeros)
+        g = generator(k)
+        w = Weights(g, m, k, group_size, zeros, S.F32, powers_of_two)
+        places = [0, 77, k // 2, k - 1]
+        w.set_to_zero_point(places)
+        x = R.whole_numbers(g, (k, n), 3)
+        x[torch.tensor(places, device="cuda")] = large
+        for order in (COL, ROW):
+            got, x = product(context, w, x, type_, S.F32, order)
+            assert torch.equal(got.double(), w.values() @ x)
