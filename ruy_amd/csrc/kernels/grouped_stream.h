@@ -22,8 +22,9 @@
 // to 32, below, 22.4 us; with products of 16 + q, two at a time, and their sums put right
 // afterwards 20.5). fp32 tokens are three bf16 rows each that add up to them (float_parts.h),
 // so that every product is exact, against the same weights. The scale multiplies a group's
-// sum. A value's three parts would meet as infinity - infinity where it is not finite; a wave
-// that ends with one goes through its depth once more with whole values.
+// sum. Values that are not finite would meet as parts of infinity - infinity, and most below 2^-110 are
+// not the sum of their parts, whose remainders show it; a wave that ends with the former, and all waves of
+// a workgroup that meets one of the latter, go through their depth once more with whole values.
 //
 // What bounds it is the rate of the weights' bytes out of HBM. Half, 64 matrices of
 // 2048x2048, 25 of them with one of 32 tokens or more: 210 MB in 40.6 us, 5.2 TB/s; 4-bit,
@@ -51,6 +52,7 @@ struct StreamArgs {
   int scale_shift;   // Scaling::kWide: logarithm of the depth positions to a scale
   int scales_at, scale_pitch;  // scales of 4-bit weights in LDS: bytes, values from a row to the next
   int zeros_at, zero_pitch;    // and their zero points
+  int lost_at;  // a flag to each wave (fp32 tokens of 4-bit weights)
 };
 
 // LDS that a workgroup of these kernels may take.
@@ -268,6 +270,16 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
                static_cast<int>(__builtin_amdgcn_perm(x[3], x[1], 0x05040100)),
                static_cast<int>(__builtin_amdgcn_perm(x[3], x[1], 0x07060302))};
   };
+  // The remainders that the third parts of this lane's tokens were rounded from (float_parts::Lost), and whether a wave
+  // has had a token that is not its parts' sum: one for all waves, whichever has taken it apart.
+  int lost = 0;
+  int* const lds_lost = reinterpret_cast<int*>(lds + args.lost_at);
+  const auto put_lost = [&]() __attribute__((always_inline)) {
+    if constexpr (T::kParts) {
+      const bool any = __any(float_parts::Lost(lost)) != 0;
+      if (lane == 0) lds_lost[wave] = any;
+    }
+  };
   // `to`: the unit's place in its token's first row of LDS.
   const auto put = [&](const Unit& unit, char* to) __attribute__((always_inline)) {
     if constexpr (!kInt4) {
@@ -285,6 +297,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         middle[e] = float_parts::RoundPair(x, y);
         x -= float_parts::LowHalf(middle[e]);
         y -= float_parts::HighHalf(middle[e]);
+        lost |= __float_as_int(x) | __float_as_int(y);
         low[e] = float_parts::RoundPair(x, y);
       }
       *reinterpret_cast<v4i*>(to) = high;
@@ -488,6 +501,10 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         use(held[0], done + depth_wave, lds + depth_wave * kLdsChunk);
       }
     }
+    if constexpr (T::kParts) {
+      put_lost();
+      __syncthreads();
+    }
   } else {
     const int units = chunks * T::kChunkUnits;
     for (int n0 = threadIdx.x; n0 < tokens * units; n0 += 4 * blockDim.x) {
@@ -503,6 +520,7 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
         if (n < tokens * units) put(some[i], lds + row_in_lds(n / units) * args.pitch + n % units * 16);
       }
     }
+    put_lost();
     __syncthreads();
     if (turns > 0) {
       const auto turn = [&](int n, auto d) __attribute__((always_inline)) {
@@ -524,12 +542,13 @@ __global__ __launch_bounds__(512) void GroupedStreamKernel(StreamArgs args) {
   }
 
   if constexpr (T::kParts) {
-    bool finite = true;
+    bool again = false;
 #pragma unroll
     for (int t = 0; t < kCols; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) finite = finite && __builtin_isfinite(acc[t][e]);
-    if (__any(!finite)) {
+      for (int e = 0; e < 4; ++e) again = again || !__builtin_isfinite(acc[t][e]);
+    if (lane < depth_waves * row_waves) again = again || lds_lost[lane] != 0;
+    if (__any(again)) {
       // Once more, with whole tokens on the fp32 instructions.
 #pragma unroll
       for (int t = 0; t < kCols; ++t) acc[t] = v4f{0, 0, 0, 0};

@@ -75,6 +75,7 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   args.scale_pitch = padded_scales | 1;
   args.zero_pitch = ((padded_scales + 3) / 4 | 1) * 4;
   int64_t tokens_lds = 0, scales_lds = 0, zeros_lds = 0;
+  const int64_t lost_lds = parts ? 8 * sizeof(int) : 0;  // (for 8 waves, the most there are)
   int work_rows = 0;
   for (;;) {
     work_rows = 16 * row_waves;
@@ -91,7 +92,7 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
       scales_lds = int64_t(work_rows) * args.scale_pitch * 4;
       zeros_lds = weights->zero_points ? int64_t(work_rows) * args.zero_pitch : 0;
     }
-    if (tokens_lds + scales_lds + zeros_lds <= kStreamLds) break;
+    if (tokens_lds + scales_lds + zeros_lds + lost_lds <= kStreamLds) break;
     if (!plan.slabs && row_waves > 1) {
       row_waves /= 2;
       if (depth_waves * 2 <= chunks) depth_waves *= 2;
@@ -104,11 +105,12 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   }
   args.scales_at = static_cast<int>(tokens_lds);
   args.zeros_at = static_cast<int>(tokens_lds + scales_lds);
+  args.lost_at = static_cast<int>(tokens_lds + scales_lds + zeros_lds);
   plan.waves = depth_waves * row_waves;
   args.depth_waves = depth_waves;
   args.row_waves = row_waves;
   args.tiles_m = (call.m + work_rows - 1) / work_rows;
-  const int64_t lds = tokens_lds + scales_lds + zeros_lds, sums = int64_t(plan.waves) * 1024;
+  const int64_t lds = tokens_lds + scales_lds + zeros_lds + lost_lds, sums = int64_t(plan.waves) * 1024;
   plan.lds_bytes = static_cast<unsigned>(lds > sums ? lds : sums);
   const int64_t slots = call.offsets ? call.n / args.tokens + busy : (call.n + args.tokens - 1) / args.tokens;
   const int64_t blocks = (slots * args.tiles_m + 7) / 8 * 8;

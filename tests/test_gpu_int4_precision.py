@@ -94,3 +94,36 @@ def test_large_tokens_against_weights_of_zero(context, kernel, type_, zeros, gro
         for order in (COL, ROW):
             got, x = product(context, w, x, type_, S.F32, order)
             assert torch.equal(got.double(), w.values() @ x)
+
+
+# Tokens below the normal numbers, multiples of the smallest one. Scales bring the results back; sums of up to 2^24 smallest
+# parts are exact.
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group_size", [32, 64, 96, 128, 5000])
+def test_tokens_below_the_normal_numbers(context, kernel, type_, zeros, group_size):
+    smallest = {S.BF16: -133, S.F16: -24, S.F32: -149}[type_]
+    for m, k, n in [(48, 512, 1), (40, 300, 5), (33, 2051, 20), (64, 700, 40)]:
+        announce("small tokens", name_of(type_), m, k, n, group_size, zeros)
+        g = generator(k)
+        w = Weights(g, m, k, group_size, zeros, S.F32, lambda r: torch.exp2(torch.floor(r * 5) - smallest - 30))
+        x = R.whole_numbers(g, (k, n), min(2 ** 24 // (15 * 16 * k), 127)) * 2.0 ** smallest
+        # (Ordinary tokens beside them.)
+        x[:, 1::3] = R.whole_numbers(g, (k, len(range(1, n, 3))), 3) * 2.0 ** (smallest + 30)
+        for order in (COL, ROW):
+            got, x = product(context, w, x, type_, S.F32, order)
+            assert torch.equal(got.double(), w.values() @ x)
+
+
+# One value to a token, of 20 bits, from the smallest numbers up to where its parts hold all of them.
+@pytest.mark.parametrize("group_size", [32, 128])
+def test_tokens_around_the_smallest_that_parts_hold(context, kernel, group_size):
+    for m, k, n in [(40, 300, 12), (33, 2051, 12), (64, 520, 60)]:
+        announce("20 bits", m, k, n, group_size)
+        g = generator(n)
+        w = Weights(g, m, k, group_size, True, S.F32, lambda r: torch.exp2(torch.floor(r * 5) + 60))
+        x = torch.zeros(k, n, device="cuda", dtype=torch.double)
+        for j in range(n):
+            x[(37 * j + 5) % k, j] = (2 ** 19 + 2 * j + 1) * 2.0 ** (-149 + j * 36 // n)
+        got, x = product(context, w, x, S.F32, S.F32)
+        assert torch.equal(got.double(), w.values() @ x)
