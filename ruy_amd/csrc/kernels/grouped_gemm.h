@@ -280,7 +280,10 @@ __device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int
 // whole number of granules, so that tiles go to LDS without passing through
 // registers. Otherwise they are read 16 bytes a lane from wherever they begin, the
 // granule in which a run ends put in its place (granule.h), and written to LDS.
-template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages>
+// kFar (not kDirect): runs along the depth may have more than 2^31 bytes, as one row or column stored value behind value
+// may, such as the ones of a bias gradient.
+template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages,
+          bool kFar>
 // (At least two waves to a SIMD: with more registers than that leaves it the compiler puts the accumulators into the
 // second register file and moves them there and back on every step.)
 __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(GemmArgs p) {
@@ -451,13 +454,18 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
     // zeroes what lies past the depth. (What lies past the tile's sides
     // ends up in rows of the tile that are not stored.)
     // Where load n of a lane is in its run and how long the run is, in bytes; `row`, `k`: where the
-    // tile begins in the operand.
+    // tile begins in the operand. kFar: from step s on (256 bytes are as good as all that is left); addresses of runs along the
+    // depth then begin with the step, or, as the run may end less than 16 bytes behind that, 16 bytes in front of it. (Addresses
+    // that move with the step cost 2 to 3 % where products are large: 4 x 4095x2047 by 8191, transposed, 217 us and 224.)
     struct Place {
       int at, length;
     };
+    constexpr int kBefore = kFar ? 16 : 0;
     const auto place_of = [&](auto side, int n, const Side& from, Runs runs, int row, int s) __attribute__((always_inline)) -> Place {
       using T = decltype(side);
       const int granule = T::GranuleOf(n, wave, lane);
+      if (kFar && runs == Runs::kPlain)
+        return {granule * 16, min(p.depth - (columns ? 0 : range.begin) - s * E::kDepth, 256 / E::kBytes) * E::kBytes};
       if (runs == Runs::kPlain) return {((columns ? 0 : range.begin) + s * E::kDepth + granule * E::kGranule) * E::kBytes, p.depth * E::kBytes};
       return {(row + granule * E::kGranule) * E::kBytes, from.count * E::kBytes};
     };
@@ -481,7 +489,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
       const int64_t group = columns && !dealt_rows ? tile.group * from.group_stride : 0;
       const int64_t k = (columns ? 0 : range.begin) + int64_t(s) * E::kDepth;
       const char* const base = static_cast<const char*>(from.data) +
-                               (group + (runs == Runs::kPlain ? row : k) * from.pitch) * E::kBytes;
+                               (group + (runs == Runs::kPlain ? row : k) * from.pitch) * E::kBytes +
+                               (kFar && runs == Runs::kPlain ? k * E::kBytes - kBefore : 0);
       // (Steps have 64 runs at most.)
       const uint32_t last_run = static_cast<uint32_t>(min(depth - 1 - s * E::kDepth, 64) * from.pitch * E::kBytes);
 #pragma unroll
@@ -489,7 +498,7 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void GroupedGemmKernel(G
         uint32_t other;
         if (runs == Runs::kPlain) {
           const Place where = place_of(side, n, from, runs, row, s);
-          other = min(where.at, where.length - 16);
+          other = min(where.at + kBefore, where.length - 16 + kBefore);
         } else {
           other = min(static_cast<uint32_t>(T::RunOf(n, wave, lane) * from.pitch * E::kBytes), last_run);
         }

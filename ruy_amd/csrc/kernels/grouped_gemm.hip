@@ -15,6 +15,7 @@ enum class Tile { k64x64, k128x128, k256x128, k256x256 };
 struct Grid {
   unsigned blocks;
   Tile tile;
+  bool far;  // kFar of the kernel
 };
 
 // A tile's sizes, the workgroups that a CU runs side by side, and how long one step
@@ -34,10 +35,11 @@ constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 2, 0.48f, 0.58f, 1.05f},
 // What a workgroup does before its first step and after its last, in steps.
 constexpr float kFixedSteps = 6;
 
-template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages>
+template <int kType, Runs kRunsM, Runs kRunsN, int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages,
+          bool kFar = false>
 void LaunchKernel(hipStream_t stream, const GemmArgs& args, unsigned blocks) {
   constexpr int kLds = kStages * (kWavesM * kBlocksM + kWavesN * kBlocksN) * 16 * 128;
-  auto* const kernel = &GroupedGemmKernel<kType, kRunsM, kRunsN, kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect, kStages>;
+  auto* const kernel = &GroupedGemmKernel<kType, kRunsM, kRunsN, kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect, kStages, kFar>;
   static const hipError_t attribute = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   (void)attribute;  // (a launch that needs it fails)
@@ -57,6 +59,8 @@ void LaunchOne(hipStream_t stream, const GemmArgs& args, const Grid& grid) {
   if constexpr (kDirect)
     if (grid.tile == Tile::k128x128)
       return LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 4, 4, true, 2>(stream, args, grid.blocks);
+  if constexpr (!kDirect && (kRunsM == Runs::kPlain || kRunsN == Runs::kPlain))
+    if (grid.far) return LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 2, 2, false, 2, true>(stream, args, grid.blocks);
   LaunchKernel<kType, kRunsM, kRunsN, 2, 2, 2, 2, kDirect, kDirect ? 4 : 2>(stream, args, grid.blocks);
 }
 
@@ -125,12 +129,16 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
   // Runs that the registers' way reads have 16 bytes at least.
   const auto long_enough = [&](const Side& s, Runs runs) { return (runs == Runs::kPlain ? call.k : s.count) >= granule; };
   if (!direct && !(long_enough(a.m, runs_m) && long_enough(a.n, runs_n))) return false;
+  // Byte positions in a run along the depth that 32 bits do not hold, on 64x64 tiles. (Such a run is its side's only one:
+  // another's pitch would be too long.)
+  const bool far = !direct && (runs_m == Runs::kPlain || runs_n == Runs::kPlain) && int64_t(call.k) * bytes > 0x7fffffff - 512;
   // The tile that the CUs would be done with first. (How many tiles the groups' columns
   // make is known on the device only: here every group that can have a column ends with half a tile.)
   const int64_t busy = columns ? min(call.groups, a.n.count) : call.groups;
   const float group_depth = columns ? call.k : float(call.k) / call.groups;
   const float steps = group_depth * bytes / 128 + 0.5f + kFixedSteps;
   Grid grid;
+  grid.far = far;
   int64_t blocks = 0;
   float best = 0;
   const auto fits = [&](const Side& s, Runs runs, int rows) {
@@ -141,6 +149,7 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
     if (direct && !(fits(a.m, runs_m, t.m) && fits(a.n, runs_n, t.n))) return 0.0f;
     if (direct) return f32 ? t.f32 : t.direct;
     if (t.tile == Tile::k64x64) return t.through;
+    if (far) return 0.0f;
     // (Both operands across the depth: 4 x 4095 x 2047, depth 8191 352 us on 64x64, 264 on 256x128, 64 x 301 x 1501, depth
     // 4001 31 and 37.)
     return f32 ? 0.0f : t.through * (columns ? 1.0f : 1.25f);

@@ -100,3 +100,38 @@ def test_rows_of_a_tile_beyond_2_31_bytes_of_fp32(context, pitch):
             assert torch.equal(y.view().double(), far.double() @ x)
         finally:
             context.force_tile()
+
+
+@pytest.mark.parametrize("type_", [S.BF16, S.F16, S.F32], ids=name_of)
+def test_depth_positions_beyond_2_31_bytes(context, type_):
+    """The gradient of a bias, a product with a column of ones: one value behind the other over all of the depth. (Groups at
+    the end of it, of less than 16 bytes too: what is in front of them belongs to none.)"""
+    size = 4 if type_ == S.F32 else 2
+    m, depth = 16 // size, 2 ** 31 // size + 1000
+    needs(depth * (m + 1) * size >> 30)
+    lhs = torch.empty(depth, m, dtype=R.TORCH[type_], device="cuda")
+    ones = torch.empty(depth, dtype=R.TORCH[type_], device="cuda")
+    tail = 3000
+    first = depth - tail
+    lhs[first:] = R.whole_numbers(generator(5), (tail, m), 3).to(R.TORCH[type_])
+    # (No ones, for what a position read elsewhere would bring to differ.)
+    ones[first:] = R.whole_numbers(generator(6), (tail,), 3).to(R.TORCH[type_])
+    for bounds in ([0, 100, 100, 1990, tail], [5, 1999, 2001, 2005, 2900], [tail - 74, tail - 3, tail - 2, tail - 1, tail]):
+        announce("far depth", name_of(type_), depth, bounds)
+        dst = Buffer(S.F32, m, 1, ROW, count=4)
+        api.mul_grouped_depth(api.Matrix(type_, lhs, api.Layout(m, depth, m, COL)),
+                              api.Matrix(type_, ones, api.Layout(depth, 1, 1, ROW)), groups_of([first + b for b in bounds]),
+                              api.MulParams(S.F32, S.F32), context, dst.matrix())
+        assert context.last_kernel_name() == "grouped_mfma"
+        for i, (begin, end) in enumerate(zip(bounds, bounds[1:])):
+            want = (lhs[first + begin:first + end].double() * ones[first + begin:first + end, None].double()).sum(0)
+            assert torch.equal(dst.view(i)[:, 0].double(), want)
+        # The other way round: the ones as the only row of lhs, which then is the side along which dst is contiguous.
+        dst = Buffer(S.F32, 1, m, COL, count=4)
+        api.mul_grouped_depth(api.Matrix(type_, ones, api.Layout(1, depth, 1, COL)),
+                              api.Matrix(type_, lhs, api.Layout(depth, m, m, ROW)), groups_of([first + b for b in bounds]),
+                              api.MulParams(S.F32, S.F32), context, dst.matrix())
+        assert context.last_kernel_name() == "grouped_mfma"
+        for i, (begin, end) in enumerate(zip(bounds, bounds[1:])):
+            want = (lhs[first + begin:first + end].double() * ones[first + begin:first + end, None].double()).sum(0)
+            assert torch.equal(dst.view(i)[0].double(), want)
