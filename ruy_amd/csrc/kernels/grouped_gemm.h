@@ -232,6 +232,8 @@ __device__ __forceinline__ int InclusiveSum(int v) {
 // Workgroups go round the eight XCDs one by one; each XCD gets a contiguous
 // run of the tiles, so that what its L2 holds serves several of them. Tiles of a
 // group go in bands of kBand along the N side.
+// (Offsets that run backwards may have every other group take all columns. 64 groups have fewer than 2^31 tiles even so, as a
+// launch has fewer than 2^26 workgroups, and the search ends; their total may wrap round, and tiles are left out then.)
 constexpr int kBand = 8;
 __device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int columns, int tile_n, int tiles_m,
                                          TileOf* tile, Range* range) {

@@ -18,20 +18,20 @@ struct Grid {
   bool far;  // kFar of the kernel
 };
 
-// A tile's sizes, the workgroups that a CU runs side by side, and how long one step
+// A tile's sizes, the threads of its workgroup, the workgroups that a CU runs side by side, and how long one step
 // of all of them takes, with operands straight to LDS, through registers, and fp32 (0: there is no such
 // kernel). Measured on each tile in that order, us: bfloat16, 8 x 4096 x 2048 x 8192
 // 265 / 181 / 167 / 171, 16 x 1683 x 3968 x 6400 194 / 147 / 133 / 116; through registers, 4 x 4095 x 2047 x 8191
 // 367 / 239 / 207, 16 x 1001 x 501 x 2001 10.8 / 18.2 / 19.2 (128x128 is nowhere the best there and left out).
 struct TileCost {
   Tile tile;
-  int m, n, per_cu;
+  int m, n, threads, per_cu;
   float direct, through, f32;
 };
-constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 2, 0.48f, 0.58f, 1.05f},
-                               {Tile::k128x128, 128, 128, 2, 1.08f, 0, 3.9f},
-                               {Tile::k256x128, 256, 128, 1, 1.0f, 1.6f, 0},
-                               {Tile::k256x256, 256, 256, 1, 1.68f, 0, 0}};
+constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 256, 2, 0.48f, 0.58f, 1.05f},
+                               {Tile::k128x128, 128, 128, 256, 2, 1.08f, 0, 3.9f},
+                               {Tile::k256x128, 256, 128, 512, 1, 1.0f, 1.6f, 0},
+                               {Tile::k256x256, 256, 256, 512, 1, 1.68f, 0, 0}};
 // What a workgroup does before its first step and after its last, in steps.
 constexpr float kFixedSteps = 6;
 
@@ -154,23 +154,28 @@ bool LaunchTiles(hipStream_t stream, const Call& call, hipError_t* status) {
     // 4001 31 and 37.)
     return f32 ? 0.0f : t.through * (columns ? 1.0f : 1.25f);
   };
+  const auto most_along_n = [&](const TileCost& t) -> int64_t {
+    return columns ? a.n.count / t.n + busy : ((int64_t(a.n.count) + t.n - 1) / t.n) * busy;
+  };
+  const auto blocks_of = [&](const TileCost& t) {
+    return ((int64_t(a.m.count) + t.m - 1) / t.m * most_along_n(t) + 7) / 8 * 8;
+  };
+  const auto usable = [&](const TileCost& t) { return step_of(t) != 0 && LaunchFits(blocks_of(t), t.threads); };
   const auto forced = [&](const TileCost& t) { return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols; };
-  const bool force = std::any_of(std::begin(kTiles), std::end(kTiles), [&](const TileCost& t) { return forced(t) && step_of(t) != 0; });
+  const bool force = std::any_of(std::begin(kTiles), std::end(kTiles), [&](const TileCost& t) { return forced(t) && usable(t); });
   for (const TileCost& t : kTiles) {
-    const float step = step_of(t);
-    if (step == 0 || (force && !forced(t))) continue;
+    if (!usable(t) || (force && !forced(t))) continue;
     const int64_t tiles_m = (int64_t(a.m.count) + t.m - 1) / t.m;
-    const int64_t most_n = columns ? a.n.count / t.n + busy : ((int64_t(a.n.count) + t.n - 1) / t.n) * busy;
-    const float tiles_n = columns ? std::max(float(busy), float(a.n.count) / t.n + 0.5f * busy) : most_n;
+    const float tiles_n = columns ? std::max(float(busy), float(a.n.count) / t.n + 0.5f * busy) : most_along_n(t);
     const float rounds = std::ceil(tiles_m * tiles_n / (t.per_cu * call.compute_units) - 0.05f);
-    const float time = std::max(1.0f, rounds) * steps * step;
+    const float time = std::max(1.0f, rounds) * steps * step_of(t);
     if (blocks == 0 || time < best) {
       best = time;
       grid.tile = t.tile;
-      blocks = (tiles_m * most_n + 7) / 8 * 8;
+      blocks = blocks_of(t);
     }
   }
-  if (blocks > 0x7fffffff) return false;
+  if (blocks == 0) return false;
   grid.blocks = static_cast<unsigned>(blocks);
   if (direct)
     LaunchType<true>(stream, a, call.type, runs_m, runs_n, grid);

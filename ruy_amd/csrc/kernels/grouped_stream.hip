@@ -1,6 +1,7 @@
 // The streaming kernels of weights in the tokens' own type, and the choice of a
 // streaming kernel.
 #include "grouped_stream.h"
+#include "launch_geometry.h"
 
 namespace ruyamd {
 namespace grouped {
@@ -114,7 +115,7 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   plan.lds_bytes = static_cast<unsigned>(lds > sums ? lds : sums);
   const int64_t slots = call.offsets ? call.n / args.tokens + busy : (call.n + args.tokens - 1) / args.tokens;
   const int64_t blocks = (slots * args.tiles_m + 7) / 8 * 8;
-  if (blocks > 0x7fffffff) return false;
+  if (!LaunchFits(blocks, 64 * plan.waves)) return false;
   plan.blocks = static_cast<unsigned>(blocks);
 
   if (int4) {

@@ -8,9 +8,14 @@
 
 namespace ruyamd {
 
-// HIP limits: grid.x < 2^31, grid.y and grid.z <= 65535.
+// HIP limits: grid.x < 2^31, grid.y and grid.z <= 65535, fewer than 2^32 threads along a dimension.
 constexpr unsigned kMaxGridX = 0x7fffffffu;
 constexpr unsigned kMaxGridY = 65535u;
+
+// Whether `blocks` workgroups of `threads` can be launched along x.
+inline bool LaunchFits(int64_t blocks, int threads) {
+  return blocks <= int64_t(kMaxGridX) && blocks * threads <= int64_t(0xffffffff);
+}
 
 struct Grid2D {
   unsigned x = 1;

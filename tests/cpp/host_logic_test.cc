@@ -78,6 +78,17 @@ static void TestElementwiseBlocks() {
   EXPECT(ruyamd::ElementwiseBlocks(int64_t(1) << 40, 256) == ruyamd::kMaxGridX);
 }
 
+static void TestLaunchFits() {
+  EXPECT(ruyamd::LaunchFits(1, 1024));
+  EXPECT(ruyamd::LaunchFits((1 << 24) - 1, 256));
+  EXPECT(!ruyamd::LaunchFits(1 << 24, 256));  // 2^32 threads
+  EXPECT(ruyamd::LaunchFits((1 << 23) - 1, 512));
+  EXPECT(!ruyamd::LaunchFits(1 << 23, 512));
+  EXPECT(!ruyamd::LaunchFits(2048 * int64_t(6554), 512));  // 65536 rows by 65536 fp32 columns, 32 by 10 to a workgroup
+  EXPECT(ruyamd::LaunchFits(0x7fffffff, 1));
+  EXPECT(!ruyamd::LaunchFits(int64_t(1) << 31, 1));
+}
+
 // 128 bytes of every row of a tile: the longest pitch that each tile's rows have.
 static void TestTileOffsetsFit() {
   EXPECT(ruyamd::TileOffsetsFit(256, 2 * int64_t(4210752), 128));   // ends at 2^31
@@ -403,6 +414,7 @@ int main() {
   TestRowSumShares();
   TestGenericGrid();
   TestElementwiseBlocks();
+  TestLaunchFits();
   TestTileOffsetsFit();
   TestDepthPartsCoverEveryStepOnce();
   TestDepthSplitArrivalProtocol();

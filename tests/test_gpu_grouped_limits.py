@@ -135,3 +135,53 @@ def test_depth_positions_beyond_2_31_bytes(context, type_):
         for i, (begin, end) in enumerate(zip(bounds, bounds[1:])):
             want = (lhs[first + begin:first + end].double() * ones[first + begin:first + end, None].double()).sum(0)
             assert torch.equal(dst.view(i)[0].double(), want)
+
+
+# 2^20 rows by 1024 columns, a column to each group: more workgroups than 2^32 threads make, streaming and on 64x64 tiles. (One
+# group's weights begin a little behind another's: 1024 matrices of their own would be 64 GB.)
+MANY_ROWS, MANY_GROUPS = 1 << 20, 1024
+
+
+def check_columns(dst, values_of, x):
+    y = dst.view()
+    assert torch.isfinite(y).all()
+    for i in list(range(0, MANY_GROUPS, 61)) + [MANY_GROUPS - 1]:
+        assert torch.equal(y[:, i].double(), values_of(i) @ x[:, i])
+
+
+@pytest.mark.parametrize("tile", [(0, 0), (64, 64)], ids=str)
+def test_more_tiles_than_one_launch_takes(context, tile):
+    needs(8)
+    m, k, n, apart = MANY_ROWS, 32, MANY_GROUPS, 8
+    flat = R.whole_numbers(generator(7), (m * k + n * apart,), 3).to(torch.bfloat16)
+    x = R.whole_numbers(generator(8), (k, n), 2)  # (sums of up to 192: bfloat16 has them all)
+    rhs, dst = Buffer(S.BF16, k, n, COL).set(x), Buffer(S.BF16, m, n, COL)
+    context.force_tile(*tile)
+    try:
+        announce("more tiles than one launch takes", tile)
+        groups = groups_of(list(range(n + 1)))
+        groups.matrix_stride = apart
+        api.mul_grouped(api.Matrix(S.BF16, flat, api.Layout(m, k, k, ROW)), rhs.matrix(), groups,
+                        api.MulParams(S.F32, S.BF16), context, dst.matrix())
+        assert context.last_kernel_name() == "grouped_mfma"
+    finally:
+        context.force_tile()
+    check_columns(dst, lambda i: flat[i * apart:i * apart + m * k].view(m, k).double(), x)
+
+
+def test_more_4_bit_rows_than_one_launch_takes(context):
+    needs(8)
+    m, k, n = MANY_ROWS, 32, MANY_GROUPS
+    data = torch.randint(256, (m * k // 2 + n,), generator=generator(9), device="cuda", dtype=torch.uint8)
+    scales = torch.exp2(torch.randint(-2, 1, (m + n,), generator=generator(10), device="cuda").float())
+    x = R.whole_numbers(generator(11), (k, n), 1)
+    rhs, dst = Buffer(S.BF16, k, n, COL).set(x), Buffer(S.BF16, m, n, COL)
+    weights = api.Int4Matrix(m, k, 32, data, scales, S.F32, matrix_bytes=1, scales_matrix_stride=1)
+    announce("more 4-bit rows than one launch takes")
+    api.mul_int4(weights, rhs.matrix(), api.MulParams(S.F32, S.BF16), context, dst.matrix(), groups_of(list(range(n + 1))))
+    assert context.last_kernel_name() == "generic"
+
+    def values_of(i):
+        return R.int4_values(data[i:i + m * k // 2].view(m, k // 2), scales[i:i + m, None], None, m, k, 32)
+
+    check_columns(dst, values_of, x)  # (sums of up to 256 times the scale)
