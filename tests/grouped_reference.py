@@ -93,3 +93,14 @@ def random_offsets(rng, count, total, empty=0.3):
     if shares.sum() == 0:
         shares[rng.integers(count)] = 1.0
     return np.concatenate(([0], np.floor(np.cumsum(shares) / shares.sum() * total + 1e-9).astype(np.int64)))
+
+
+def relative_error(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+def relative_bound(terms, dst_dtype):
+    """The norm of an fp32 sum's error by that of many sums of `terms` terms without a common sign: a partial sum is
+    in the mean no larger than the whole, each addition is off by 2^-23 of it at most (instructions may cut off), and
+    what additions are off by has no common sign either. Then the rounding to the destination."""
+    return terms ** 0.5 * 2.0 ** -23 + (UNIT[dst_dtype] if dst_dtype != S.F32 else 0.0)

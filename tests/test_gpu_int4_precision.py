@@ -127,3 +127,39 @@ def test_tokens_around_the_smallest_that_parts_hold(context, kernel, group_size)
             x[(37 * j + 5) % k, j] = (2 ** 19 + 2 * j + 1) * 2.0 ** (-149 + j * 36 // n)
         got, x = product(context, w, x, S.F32, S.F32)
         assert torch.equal(got.double(), w.values() @ x)
+
+
+# Ordinary values by the norm of their error: tests/test_int4_tolerance.py shows which mistakes this finds.
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group_size", [32, 64, 96, 128, 10000])
+def test_norms_of_ordinary_values(context, kernel, type_, zeros, group_size):
+    for m, k, n in [(200, 2048, 1), (96, 2051, 3), (64, 8192, 40), (130, 300, 20), (256, 64, 7)]:
+        for dst_type in {S.F32, type_}:
+            for scale_type in {type_, S.F32}:
+                g = generator(k)
+                w = Weights(g, m, k, group_size, zeros, scale_type, lambda r: r + 0.5)
+                for order in (COL, ROW):
+                    got, x = product(context, w, torch.randn(k, n, generator=g, device="cuda").double(), type_, dst_type, order)
+                    far = R.relative_error(got, w.values() @ x)
+                    bound = R.relative_bound(k + len(w.scales[0]), dst_type)
+                    announce("norms", name_of(type_), name_of(dst_type), name_of(scale_type), m, k, n, group_size, zeros,
+                             "%.3g of %.3g" % (far, bound))
+                    assert far <= bound
+
+
+# The same beside tokens some thousand times larger that meet weights equal to their zero point.
+@pytest.mark.parametrize("type_", TYPES, ids=name_of)
+@pytest.mark.parametrize("group_size", [32, 128])
+def test_norms_beside_large_tokens(context, kernel, type_, group_size):
+    for m, k, n in [(200, 2048, 1), (64, 4100, 40)]:
+        g = generator(m)
+        w = Weights(g, m, k, group_size, True, S.F32, lambda r: r + 0.5)
+        places = [5, k // 3]
+        w.set_to_zero_point(places)
+        x = torch.randn(k, n, generator=g, device="cuda").double()
+        x[torch.tensor(places, device="cuda")] *= 4096
+        got, x = product(context, w, x, type_, S.F32)
+        far, bound = R.relative_error(got, w.values() @ x), R.relative_bound(k + len(w.scales[0]), S.F32)
+        announce("norms beside large tokens", name_of(type_), m, k, n, group_size, "%.3g of %.3g" % (far, bound))
+        assert far <= bound
