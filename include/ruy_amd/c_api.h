@@ -295,8 +295,10 @@ typedef struct ruyamd_int4_mat {
  * columns of a group (5 to 10 fp32 ones). With `groups` (not NULL) there is a weight matrix to each group, as
  * in ruyamd_mul_grouped (whose matrix_stride is not looked at here). rhs:
  * bfloat16, half or fp32, any order; dst its type or fp32; products with the
- * whole-numbered part of the weights are exact, sums are fp32, a group's scale is
- * applied to its sum. Parameters, memory and calls as in ruyamd_mul_grouped. */
+ * whole-numbered part of the weights, q - zero_point, are exact, sums are fp32, a group's scale is
+ * applied to its sum (which has to stay in the range of fp32). Parameters, memory and calls as in
+ * ruyamd_mul_grouped. Depths below 32 and tokens by rows of a depth above some
+ * 65000 (fp32: 21000) go to a kernel of one element to a lane, some hundred times slower. */
 RUYAMD_API int ruyamd_mul_int4(ruyamd_ctx* ctx, const ruyamd_int4_mat* lhs,
                                const ruyamd_mat* rhs,
                                const ruyamd_groups* groups,

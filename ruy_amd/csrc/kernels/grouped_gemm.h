@@ -8,10 +8,13 @@
 // operands of a weight gradient). Fragments of the latter come out of LDS through
 // the transposing reads of gfx950, so no operand is ever copied for its order.
 //
-// What bounds it is the rate at which steps reach LDS out of L2, 10 to 12 TB/s over the
-// card, whatever the tile: 256x256 needs a quarter of 64x64's bytes and is the best
-// tile wherever there are enough of them. bfloat16, 8 groups of 4096x2048 by 8192 columns: 161 us, 856 TFLOP/s (one
-// library product of that work 115 us, a floor of 95 at the rate of a large one). Where depths
+// What bounds it where there are many tiles: steps reach LDS out of L2 at 10 to 12 TB/s over the
+// card, of which 256x256 needs a quarter of 64x64's bytes and is the best tile wherever there are
+// enough of them; and the last round of tiles, of which a part of the CUs has none. bfloat16, 8 groups of 4096x2048
+// by 8192 columns: 162 us, 850 TFLOP/s (one library product of that work 115 us, a floor of 95 at the rate of a
+// large one), 576 tiles on 256 CUs; with groups of one size, 512 tiles, a tenth less. Where the depth is dealt, tiles go
+// to the XCDs by their number and not by their depth: 8 weight gradients of 2048x4096 over 8192 columns, fp32, 187 us with
+// groups of one size, 227, 263 and 361 where group i has a share of (i + 1) ^ -0.25, -0.5 and -1. Where depths
 // are short (half, 48 weight gradients of 515x771, depth 2500 in all, 40 us) it is the
 // latency of a tile's few steps and its write-back. fp32 runs on the matrix cores' own fp32
 // instructions: 4 groups of 1024x1024 by 1500 columns 36 us, 88 TFLOP/s of 143.

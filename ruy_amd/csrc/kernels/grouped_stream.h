@@ -28,9 +28,10 @@
 //
 // What bounds it is the rate of the weights' bytes out of HBM. Half, 64 matrices of
 // 2048x2048, 25 of them with one of 32 tokens or more: 210 MB in 40.6 us, 5.2 TB/s; 4-bit,
-// 16384x16384 with a scale to 128, one token: 138 MB in 31 us, 4.5 TB/s (6.5 TB/s is the
-// most that anything here reads at), 64 x 2048x2048 with a scale to 32: 59 MB in 22.4 us. Small ones are
-// one wave's way through its depth: 2048x2048 5.4 us of which 2.5 are the launch.
+// 16384x16384 with a scale to 128, one token: 138 MB in 30.7 us, 4.5 TB/s (6.5 TB/s is the
+// most that anything here reads at). The taking apart of 4-bit values is 0.6 of these and putting the scales into LDS
+// 1.9; with a scale to 32 and bfloat16, 64 x 2048x2048, 59 MB in 22.4 us, they are 4.9 and 3.1 (each left out alone, in
+// a copy). Small ones are one wave's way through its depth: 2048x2048 5.4 us of which 2.5 are the launch.
 #ifndef RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 #define RUY_AMD_CSRC_KERNELS_GROUPED_STREAM_H_
 

@@ -21,6 +21,11 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   const int block_tokens = parts ? 5 : 16, rows_to_token = parts ? 3 : 1;
   const int64_t busy = min(call.groups, call.n);
   const int64_t per_group = (call.n + busy - 1) / busy;
+  // (Weights in the tokens' type: up to 32 columns a group, in the mean over groups. Streaming and tiles, us, weights out of
+  // HBM: bfloat16 1 x 4096x4096, 16 columns 11.2 and 20.0, 32 17.4 and 20.7; 64 x 2048x2048, 1 a group 90 and 98, 8 102 and 101, 32
+  // 129 and 104; fp32 8 x 1024x1024, 16 16.3 and 21.1, 32 14.4 and 21.1; 64 x 512x1024, 16 54.7 and 37.9, 32 38.4 and 38.9.
+  // The line is right for few groups, about right for fp32, and late for 16 bits where the groups' weights make some hundred tiles: 8 x
+  // 4096x2048 1 31.3 and 31.2, 16 51.0 and 30.8, 32 35.5 and 30.9; 16 x 1024x1024 1 12.7 and 9.1, 32 13.0 and 9.6.)
   if (!int4 && per_group > 32) return false;
   StreamPlan plan;
 
@@ -59,8 +64,8 @@ bool LaunchStream(hipStream_t stream, const Call& call, const Int4* weights, hip
   // Waves: 8 to a workgroup, along the depth as long as that makes no more than 16 to a CU
   // (of weights in 16 or 32 bits 64), along the rows otherwise; fewer rows where what goes with
   // them into LDS is too much. (Half, 64 x 2048x2048, 32 tokens: 64 waves to a CU
-  // 40.6 us, 16 44.0. 4-bit, the same: 24.0 and 20.5; 16384 x 16384, one token: 32.2 and
-  // 31.3, with 4 waves to a workgroup 40, with 2 59. Two blocks of 16 rows to a wave are no
+  // 40.6 us, 16 44.0. 4-bit, the same: 24.9 and 22.5; 16384 x 16384, one token: 31.5 and
+  // 30.7, with 4 waves to a workgroup 40, with 2 59. Two blocks of 16 rows to a wave are no
   // faster anywhere, and slower where there are few rows.)
   int row_waves = RowWaves(plan.slabs, plan.cols), depth_waves = 8 / row_waves;
   if (!plan.slabs) {
