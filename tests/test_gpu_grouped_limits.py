@@ -185,3 +185,56 @@ def test_more_4_bit_rows_than_one_launch_takes(context):
         return R.int4_values(data[i:i + m * k // 2].view(m, k // 2), scales[i:i + m, None], None, m, k, 32)
 
     check_columns(dst, values_of, x)  # (sums of up to 256 times the scale)
+
+
+def test_as_many_groups_as_a_call_may_have(context):
+    """65536 groups, most of them empty, some with several columns or depth positions, in every kind of kernel."""
+    m, k, n, count, apart = 24, 64, 3000, 65536, 8
+    rng = torch.Generator().manual_seed(12)
+    ends = torch.sort(torch.randint(0, n + 1, (count - 1,), generator=rng)).values
+    ends = (ends // 40 * 40).tolist()  # (75 groups of 40, far apart)
+    bounds = [0] + ends + [n]
+    groups = groups_of(bounds)
+    full = [(i, b, e) for i, (b, e) in enumerate(zip(bounds, bounds[1:])) if b < e]
+    assert len(full) >= 70
+    x = R.whole_numbers(generator(13), (k, n), 3)
+    rhs = Buffer(S.BF16, k, n, COL).set(x)
+    groups.matrix_stride = apart
+    flat = R.whole_numbers(generator(14), (m * k + count * apart,), 3).to(torch.bfloat16)
+    dst = Buffer(S.F32, m, n, COL)
+    for tile in ((0, 0), (64, 64), (256, 256)):
+        context.force_tile(*tile)
+        try:
+            announce("many groups", tile)
+            api.mul_grouped(api.Matrix(S.BF16, flat, api.Layout(m, k, k, ROW)), rhs.matrix(), groups,
+                            api.MulParams(S.F32, S.F32), context, dst.matrix())
+            assert context.last_kernel_name() == ("grouped_mfma" if tile[0] else "grouped_stream")
+        finally:
+            context.force_tile()
+        for i, begin, end in full:
+            w = flat[i * apart:i * apart + m * k].view(m, k).double()
+            assert torch.equal(dst.view()[:, begin:end].double(), w @ x[:, begin:end])
+        dst.flat.fill_(float("nan"))
+    announce("many groups, 4 bits")
+    data = torch.randint(256, (m * k // 2 + count,), generator=generator(15), device="cuda", dtype=torch.uint8)
+    scales = torch.exp2(torch.randint(-2, 3, (m * 2 + count,), generator=generator(16), device="cuda").float())
+    weights = api.Int4Matrix(m, k, 32, data, scales, S.F32, matrix_bytes=1, scales_matrix_stride=1)
+    api.mul_int4(weights, rhs.matrix(), api.MulParams(S.F32, S.F32), context, dst.matrix(), groups)
+    assert context.last_kernel_name() == "int4_stream"
+    for i, begin, end in full:
+        w = R.int4_values(data[i:i + m * k // 2].view(m, k // 2), scales[i:i + 2 * m].view(m, 2), None, m, k, 32)
+        assert torch.equal(dst.view()[:, begin:end].double(), w @ x[:, begin:end])
+    announce("many groups, depth")
+    dy = R.whole_numbers(generator(17), (m, n), 3)
+    grad = Buffer(S.F32, m, 16, ROW, count=count)
+    by_rows = Buffer(S.BF16, n, 16, ROW).set(x[:16].t())
+    groups.matrix_stride = 0
+    api.mul_grouped_depth(Buffer(S.BF16, m, n, COL).set(dy).matrix(), by_rows.matrix(), groups,
+                          api.MulParams(S.F32, S.F32), context, grad.matrix())
+    assert context.last_kernel_name() == "grouped_mfma"
+    got = grad.flat[:count * m * 16].view(count, m, 16)
+    for i, begin, end in full:
+        assert torch.equal(got[i].double(), dy[:, begin:end].contiguous() @ x[:16, begin:end].t().contiguous())
+    empty = torch.ones(count, dtype=torch.bool, device="cuda")
+    empty[[i for i, _, _ in full]] = False
+    assert (got[empty] == 0).all()
