@@ -45,9 +45,11 @@ enum {
   RUYAMD_DTYPE_F32 = 5,
   RUYAMD_DTYPE_F64 = 6,
   /* 16-bit floating point: bfloat16 and IEEE half. Operands and destinations of
-   * ruyamd_mul_grouped, ruyamd_mul_grouped_depth and ruyamd_mul_int4 only. */
+   * the calls for layers of experts only (ruyamd_mul_grouped and those behind it). */
   RUYAMD_DTYPE_BF16 = 7,
   RUYAMD_DTYPE_F16 = 8,
+  /* 64-bit integers: expert numbers of ruyamd_sort_tokens only. */
+  RUYAMD_DTYPE_I64 = 9,
 };
 
 /* Values of ruy::CachePolicy (ruy/matrix.h:117-122). */
@@ -102,6 +104,11 @@ enum {
   RUYAMD_KERNEL_GROUPED_STREAM = 8, /* grouped products of a few columns a group:
                                        every weight read once, matrix cores */
   RUYAMD_KERNEL_INT4_STREAM = 9,    /* 4-bit weights, read once, matrix cores */
+  RUYAMD_KERNEL_TOKENS = 10,        /* tokens sorted, moved or added up, or to and
+                                       from 4 bits, 16 bytes to a lane */
+  RUYAMD_KERNEL_MXFP4_MFMA = 11,    /* 4-bit floats on tiles, matrix cores */
+  RUYAMD_KERNEL_MXFP4_STREAM = 12,  /* 4-bit floats by a few columns: every weight
+                                       read once, matrix cores */
 };
 
 /* Type-erased, non-owning matrix view: the fields of ruy::Matrix<T>
@@ -304,6 +311,127 @@ RUYAMD_API int ruyamd_mul_int4(ruyamd_ctx* ctx, const ruyamd_int4_mat* lhs,
                                const ruyamd_groups* groups,
                                const ruyamd_mul_params* params,
                                const ruyamd_mat* dst);
+
+/* ---- Tokens to their experts and back (no counterpart in the reference) ----
+ *
+ * Every token chooses `top` of `count` experts. ruyamd_sort_tokens gives each
+ * choice a place, so that the choices of one expert lie side by side, in the
+ * order of their tokens; with rows of matrices in these places the products
+ * above have their groups in `offsets`. */
+typedef struct ruyamd_routing {
+  int32_t* offsets; /* count + 1: places offsets[g] .. offsets[g + 1] - 1 are expert g's, as in
+                       ruyamd_groups */
+  int32_t* places;  /* tokens x top, a token's side by side: the place of each choice, or -1 */
+  int32_t* sources; /* tokens x top, or NULL: of each place its choice, token * top + number;
+                       -1 behind the last place */
+  int32_t tokens;
+  int32_t top;
+  int32_t count; /* 1 .. 65536 */
+  int32_t reserved;
+} ruyamd_routing;
+
+/* Sorts the choices: `experts` is a top x tokens matrix of RUYAMD_DTYPE_I32 or
+ * RUYAMD_DTYPE_I64, any order and stride; writes offsets, places and sources.
+ * A number outside 0 .. count - 1, such as the -1 of a token of padding, is no
+ * choice and has no place. The result depends on the numbers alone. tokens * top
+ * is below 2^31.
+ *
+ * This call and the ones below: every buffer is device memory, no memory is
+ * allocated, nothing is kept from one call to the next, a call may be recorded
+ * into a graph, and no destination may overlap another buffer of the call. They
+ * return when the destinations are complete, or once they are enqueued after
+ * ruyamd_ctx_set_synchronous(ctx, 0). Of the routing the others read `places`
+ * only, which may be a program's own: a place outside the matrix of rows is
+ * taken for none. */
+RUYAMD_API int ruyamd_sort_tokens(ruyamd_ctx* ctx, const ruyamd_mat* experts,
+                                  const ruyamd_routing* routing);
+
+/* dst[:, p] = src[:, t] for every place p of every token t; columns of dst that
+ * are no place are left as they are. src: a column to each token; dst: a column
+ * to each place, as many as there are or more, of src's type: fp32, bfloat16 or
+ * half, any order and stride. (The gradient of src is ruyamd_combine_tokens
+ * without weights.) */
+RUYAMD_API int ruyamd_dispatch_tokens(ruyamd_ctx* ctx, const ruyamd_mat* src,
+                                      const ruyamd_routing* routing,
+                                      const ruyamd_mat* dst);
+
+/* dst[:, t] = the sum over j of weights(j, t) * src[:, place j of token t]; zeros
+ * for a token without a place. weights: a top x tokens matrix of any of the three
+ * types and any order, or NULL for ones. dst: src's type or fp32. Sums are fp32, in the order of
+ * j, and rounded once; what lies in a column that is no place, or belongs to a choice without one (NaN,
+ * infinities, the weight of that choice), has no influence. */
+RUYAMD_API int ruyamd_combine_tokens(ruyamd_ctx* ctx, const ruyamd_mat* src,
+                                     const ruyamd_routing* routing,
+                                     const ruyamd_mat* weights,
+                                     const ruyamd_mat* dst);
+
+/* The gradients of ruyamd_combine_tokens from that of its dst, `grad` (grad_src's
+ * type or fp32, a column to each token), in one pass: of src,
+ *   grad_src[:, place j of t] = weights(j, t) * grad[:, t],
+ * other columns left as they are, and of weights,
+ *   grad_weights(j, t) = the sum over h of grad(h, t) * src(h, place j of t),
+ * 0 for a choice without a place. Either may be NULL; src is looked at for the
+ * second only and may be NULL without it. weights: as above. grad_src: src's type and
+ * size, any of the three types without src; grad_weights: any of the three types. Sums
+ * are fp32, in an order that depends on the sizes alone. */
+RUYAMD_API int ruyamd_combine_tokens_gradients(
+    ruyamd_ctx* ctx, const ruyamd_mat* grad, const ruyamd_mat* src,
+    const ruyamd_routing* routing, const ruyamd_mat* weights,
+    const ruyamd_mat* grad_src, const ruyamd_mat* grad_weights);
+
+/* ---- Microscaled 4-bit floating point (OCP MX, MXFP4; no counterpart in the
+ * reference) ----
+ *
+ * Values of 4 bits by rows, with a power of two to every 32 of a row (fewer
+ * where it ends): the value at (r, c) is
+ *   e2m1(q(r, c)) * 2^(s(r, c / 32) - 127)
+ * where q(r, c) is the low (c even) or high (c odd) half of byte
+ * data[r * row_bytes + c / 2]; e2m1 of 0 .. 7 is 0, 0.5, 1, 1.5, 2, 3, 4, 6, and of 8 .. 15 the
+ * same with a minus sign; s(r, i) is scales[r * scale_stride + i], and all
+ * values of a block whose s is 255 are NaN. */
+typedef struct ruyamd_mxfp4_mat {
+  void* data;
+  uint8_t* scales;
+  int32_t rows;
+  int32_t cols;
+  int32_t row_bytes;    /* from a row to the next; 0: (cols + 1) / 2 */
+  int32_t scale_stride; /* bytes from a row's scales to the next's; 0: (cols + 31) / 32 */
+  int64_t matrix_bytes;         /* from a group's data to the next one's and */
+  int64_t scales_matrix_stride; /* its scales; 0: one right behind the other */
+} ruyamd_mxfp4_mat;
+
+/* dst = src (rows x cols, fp32, bfloat16 or half, any order and stride) in 4
+ * bits. A block's power of two is that of its largest magnitude divided by 4, 2^-127
+ * at least (also for a block of zeros); values are divided by it and rounded to nearest, ties to
+ * even, those above 6 to 6; zeros keep their signs. A block that holds an infinity or
+ * a NaN gets s = 255 and q = 0. The unused half of an odd row's last byte is 0.
+ *
+ * With `routing` (not NULL) src has a row to each token, and dst gets a token's row
+ * in each of its places, as from ruyamd_dispatch_tokens; other rows are left as they are. */
+RUYAMD_API int ruyamd_quantize_mxfp4(ruyamd_ctx* ctx, const ruyamd_mat* src,
+                                     const ruyamd_routing* routing,
+                                     const ruyamd_mxfp4_mat* dst);
+
+/* dst (rows x cols, fp32, bfloat16 or half, any order and stride) = the values of
+ * src, rounded to dst's type: what a product's gradient takes for it, with
+ * ruyamd_mul_grouped and ruyamd_mul_grouped_depth. */
+RUYAMD_API int ruyamd_dequantize_mxfp4(ruyamd_ctx* ctx,
+                                       const ruyamd_mxfp4_mat* src,
+                                       const ruyamd_mat* dst);
+
+/* dst = clamp(lhs * transposed rhs + bias), dst M x N, lhs M x K, rhs N x K: rows
+ * of both run along the depth, and a row of rhs is a token. With `groups` (not
+ * NULL) the columns of dst, and with them the rows of rhs, are dealt to groups, each with
+ * an lhs of its own, as in ruyamd_mul_grouped (whose matrix_stride is not looked
+ * at here: lhs says where its matrices lie; rhs's are not looked at). dst: fp32, bfloat16 or half,
+ * any order. Sums are fp32, in which products of blocks below 2^-126 may be lost; the result is rounded once. Parameters, memory and
+ * calls as in ruyamd_mul_grouped. Depths below 32 go to a kernel of one element to
+ * a lane. */
+RUYAMD_API int ruyamd_mul_mxfp4(ruyamd_ctx* ctx, const ruyamd_mxfp4_mat* lhs,
+                                const ruyamd_mxfp4_mat* rhs,
+                                const ruyamd_groups* groups,
+                                const ruyamd_mul_params* params,
+                                const ruyamd_mat* dst);
 
 /* Stream control. By default a context owns a stream and every ruyamd_mul
  * synchronises it before returning, which is ruy::Mul's contract

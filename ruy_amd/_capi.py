@@ -33,6 +33,8 @@ _ctx = C.c_void_p
 _matp = C.POINTER(S.Mat)
 _parp = C.POINTER(S.MulParamsStruct)
 _grpp = C.POINTER(S.Groups)
+_roup = C.POINTER(S.Routing)
+_mx4p = C.POINTER(S.MxFp4Mat)
 
 PROTOTYPES = {
     "ruyamd_ctx_create": (C.c_int, [C.POINTER(C.c_void_p)]),
@@ -43,6 +45,13 @@ PROTOTYPES = {
     "ruyamd_mul_grouped": (C.c_int, [_ctx, _matp, _matp, _grpp, _parp, _matp]),
     "ruyamd_mul_grouped_depth": (C.c_int, [_ctx, _matp, _matp, _grpp, _parp, _matp]),
     "ruyamd_mul_int4": (C.c_int, [_ctx, C.POINTER(S.Int4Mat), _matp, _grpp, _parp, _matp]),
+    "ruyamd_sort_tokens": (C.c_int, [_ctx, _matp, _roup]),
+    "ruyamd_dispatch_tokens": (C.c_int, [_ctx, _matp, _roup, _matp]),
+    "ruyamd_combine_tokens": (C.c_int, [_ctx, _matp, _roup, _matp, _matp]),
+    "ruyamd_combine_tokens_gradients": (C.c_int, [_ctx, _matp, _matp, _roup, _matp, _matp, _matp]),
+    "ruyamd_quantize_mxfp4": (C.c_int, [_ctx, _matp, _roup, _mx4p]),
+    "ruyamd_dequantize_mxfp4": (C.c_int, [_ctx, _mx4p, _matp]),
+    "ruyamd_mul_mxfp4": (C.c_int, [_ctx, _mx4p, _mx4p, _grpp, _parp, _matp]),
     "ruyamd_ctx_set_stream": (C.c_int, [_ctx, C.c_void_p]),
     "ruyamd_ctx_set_synchronous": (C.c_int, [_ctx, C.c_int]),
     "ruyamd_ctx_synchronize": (C.c_int, [_ctx]),

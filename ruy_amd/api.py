@@ -264,6 +264,44 @@ class Int4Matrix:
         return m
 
 
+class Routing:
+    """ruyamd_routing: each of `tokens` tokens chooses `top` of `count` experts.
+    Device memory, int32: `offsets` (count + 1 values), `places` (tokens x top,
+    a token's side by side) and, where it is wanted, `sources` (tokens x top)."""
+
+    def __init__(self, tokens, top, count, offsets, places, sources=None):
+        self.tokens, self.top, self.count = tokens, top, count
+        self.offsets, self.places, self.sources = offsets, places, sources
+
+    def groups(self, matrix_stride=0, bias_stride=0):
+        """The places of each expert as the groups of a product."""
+        return Groups(self.offsets, self.count, matrix_stride, bias_stride)
+
+    def to_struct(self):
+        r = S.Routing()
+        r.offsets, r.places, r.sources = _address(self.offsets), _address(self.places), _address(self.sources)
+        r.tokens, r.top, r.count = self.tokens, self.top, self.count
+        return r
+
+
+class MxFp4Matrix:
+    """ruyamd_mxfp4_mat: 4-bit floating-point values by rows, two to a byte, with
+    a power of two (a byte: its exponent + 127) to every 32 of a row."""
+
+    def __init__(self, rows, cols, data, scales, row_bytes=0, scale_stride=0, matrix_bytes=0, scales_matrix_stride=0):
+        self.rows, self.cols, self.data, self.scales = rows, cols, data, scales
+        self.row_bytes, self.scale_stride = row_bytes, scale_stride
+        self.matrix_bytes, self.scales_matrix_stride = matrix_bytes, scales_matrix_stride
+
+    def to_struct(self):
+        m = S.MxFp4Mat()
+        m.data, m.scales = _address(self.data), _address(self.scales)
+        m.rows, m.cols = self.rows, self.cols
+        m.row_bytes, m.scale_stride = self.row_bytes, self.scale_stride
+        m.matrix_bytes, m.scales_matrix_stride = self.matrix_bytes, self.scales_matrix_stride
+        return m
+
+
 class RuyAmdError(RuntimeError):
     def __init__(self, code, message):
         super().__init__("ruy_amd error %d: %s" % (code, message))
@@ -465,6 +503,64 @@ def mul_int4(lhs, rhs, mul_params, context, dst, groups=None):
     _call_with_groups(2, lhs, rhs, groups, mul_params, context, dst)
 
 
+def _call(which, context, *objects):
+    """Function number `which` of _CALLS with the objects' structs (None: a null pointer)."""
+    rc = native.call(which, context._address, *objects) if native else None
+    if rc is None:  # As in mul: what the native path does not take.
+        structs = [None if o is None else C.byref(o.to_struct()) for o in objects]
+        rc = _CALLS[which](context._h, *structs)
+    if rc:
+        context._check(rc)
+
+
+_CALLS = (lib.ruyamd_sort_tokens, lib.ruyamd_dispatch_tokens, lib.ruyamd_combine_tokens,
+          lib.ruyamd_combine_tokens_gradients, lib.ruyamd_quantize_mxfp4, lib.ruyamd_dequantize_mxfp4,
+          lib.ruyamd_mul_mxfp4)
+
+
+def sort_tokens(experts, routing, context):
+    """Gives every choice of `experts` (top x tokens, I32 or I64) its place in
+    `routing` (ruyamd_sort_tokens)."""
+    _call(0, context, experts, routing)
+
+
+def dispatch_tokens(src, routing, context, dst):
+    """dst[:, p] = src[:, t] for every place p of token t (ruyamd_dispatch_tokens)."""
+    _call(1, context, src, routing, dst)
+
+
+def combine_tokens(src, routing, weights, context, dst):
+    """dst[:, t] = the sum over token t's places of weight * src[:, place];
+    weights: top x tokens, or None for ones (ruyamd_combine_tokens)."""
+    _call(2, context, src, routing, weights, dst)
+
+
+def combine_tokens_gradients(grad, src, routing, weights, context, grad_src, grad_weights):
+    """The gradients of combine_tokens; src, weights, grad_src and grad_weights
+    may be None (ruyamd_combine_tokens_gradients)."""
+    _call(3, context, grad, src, routing, weights, grad_src, grad_weights)
+
+
+def quantize_mxfp4(src, context, dst, routing=None):
+    """dst (an MxFp4Matrix) = the rows of src in 4 bits, each in its token's
+    places where there is a routing (ruyamd_quantize_mxfp4)."""
+    _call(4, context, src, routing, dst)
+
+
+def dequantize_mxfp4(src, context, dst):
+    """dst = what the MxFp4Matrix src stands for (ruyamd_dequantize_mxfp4)."""
+    _call(5, context, src, dst)
+
+
+def mul_mxfp4(lhs, rhs, mul_params, context, dst, groups=None):
+    """dst = clamp(lhs * transposed rhs + bias) of two MxFp4Matrix, an lhs to each
+    of `groups` where there are any (ruyamd_mul_mxfp4)."""
+    if mul_params.dst_dtype != dst.dtype:
+        raise ValueError("MulParams DstScalar does not match the destination matrix")
+    _call(6, context, lhs, rhs, groups, mul_params, dst)
+
+
 if native:
+    native.bind_calls([C.cast(f, C.c_void_p).value for f in _CALLS], Routing, MxFp4Matrix)
     native.bind_with_groups([C.cast(f, C.c_void_p).value for f in _WITH_GROUPS], Groups, Int4Matrix)
     native.bind(C.cast(lib.ruyamd_mul, C.c_void_p).value, Matrix, Layout, MulParams)

@@ -1,8 +1,8 @@
 // ruyamd_mul_grouped, ruyamd_mul_grouped_depth and ruyamd_mul_int4: the checks
 // of a call, the choice of its kernel, and its launch on the context's stream.
-#include <cmath>
 #include <string>
 
+#include "checks.h"
 #include "context.h"
 #include "internal.h"
 #include "kernels/grouped.h"
@@ -12,65 +12,9 @@ namespace {
 
 using grouped::Dealt;
 
-constexpr int kMostGroups = 65536;
-
-int Fail(ruyamd_ctx* ctx, int code, const std::string& msg) {
-  ctx->last_error = msg;
-  return code;
-}
-
-bool IsOperandType(int dtype) {
-  return dtype == RUYAMD_DTYPE_F32 || dtype == RUYAMD_DTYPE_BF16 || dtype == RUYAMD_DTYPE_F16;
-}
-
 int64_t Extent(const ruyamd_mat& m) {
   const int64_t outer = m.order == RUYAMD_ORDER_COL_MAJOR ? m.cols : m.rows;
   return outer * m.stride;
-}
-
-int CheckMatrix(ruyamd_ctx* ctx, const ruyamd_mat& m, const std::string& name) {
-  if (m.rows < 0 || m.cols < 0) return Fail(ctx, RUYAMD_E_INVALID, name + ": negative size");
-  if (m.order != RUYAMD_ORDER_COL_MAJOR && m.order != RUYAMD_ORDER_ROW_MAJOR)
-    return Fail(ctx, RUYAMD_E_INVALID, name + ": bad order");
-  if (m.stride < (m.order == RUYAMD_ORDER_COL_MAJOR ? m.rows : m.cols))
-    return Fail(ctx, RUYAMD_E_INVALID, name + ": stride smaller than the contiguous dimension");
-  if (!IsOperandType(m.dtype)) return Fail(ctx, RUYAMD_E_UNSUPPORTED, name + ": the type must be fp32, bfloat16 or half");
-  if (m.zero_point) return Fail(ctx, RUYAMD_E_INVALID, name + ": floating-point matrices need zero_point == 0");
-  if (m.rows > 0 && m.cols > 0) {
-    if (!m.data) return Fail(ctx, RUYAMD_E_INVALID, name + ": null data");
-    const uintptr_t size = m.dtype == RUYAMD_DTYPE_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(m.data) % size)
-      return Fail(ctx, RUYAMD_E_INVALID, name + ": data not aligned to its type");
-    if (MemoryOf(m.data) != Memory::kDevice) return Fail(ctx, RUYAMD_E_UNSUPPORTED, name + ": not device memory");
-  }
-  return RUYAMD_OK;
-}
-
-int CheckDeviceBuffer(ruyamd_ctx* ctx, const void* p, uintptr_t alignment, const char* name) {
-  if (!p) return Fail(ctx, RUYAMD_E_INVALID, std::string(name) + ": null");
-  if (reinterpret_cast<uintptr_t>(p) % alignment)
-    return Fail(ctx, RUYAMD_E_INVALID, std::string(name) + ": not aligned to its type");
-  if (MemoryOf(p) != Memory::kDevice) return Fail(ctx, RUYAMD_E_UNSUPPORTED, std::string(name) + ": not device memory");
-  return RUYAMD_OK;
-}
-
-int CheckGroups(ruyamd_ctx* ctx, const ruyamd_groups& g) {
-  if (g.count < 1 || g.count > kMostGroups) return Fail(ctx, RUYAMD_E_INVALID, "groups: count must be 1 .. 65536");
-  if (g.matrix_stride < 0 || g.bias_stride < 0) return Fail(ctx, RUYAMD_E_INVALID, "groups: negative stride");
-  return CheckDeviceBuffer(ctx, g.offsets, 4, "groups: offsets");
-}
-
-int CheckParams(ruyamd_ctx* ctx, const ruyamd_mul_params& p, bool may_have_bias) {
-  if (p.accum_dtype != RUYAMD_DTYPE_F32) return Fail(ctx, RUYAMD_E_UNSUPPORTED, "the accumulator must be fp32");
-  if (p.multiplier_fixedpoint_perchannel || p.multiplier_exponent_perchannel || p.multiplier_fixedpoint ||
-      p.multiplier_exponent)
-    return Fail(ctx, RUYAMD_E_INVALID, "multiplier set on a floating-point product");
-  if (std::isnan(p.clamp_min) || std::isnan(p.clamp_max)) return Fail(ctx, RUYAMD_E_INVALID, "clamp bounds are not numbers");
-  if (p.channel_dimension > RUYAMD_CHANNEL_COL) return Fail(ctx, RUYAMD_E_INVALID, "bad channel dimension");
-  if (!p.bias) return RUYAMD_OK;
-  if (!may_have_bias) return Fail(ctx, RUYAMD_E_UNSUPPORTED, "ruyamd_mul_grouped_depth takes no bias");
-  if (p.channel_dimension != RUYAMD_CHANNEL_ROW) return Fail(ctx, RUYAMD_E_UNSUPPORTED, "the bias must be one to each row");
-  return CheckDeviceBuffer(ctx, p.bias, 4, "bias");
 }
 
 // Both sides, dst and what they have to agree in. `lhs_rows` x `depth` is the left-hand operand.
@@ -108,48 +52,23 @@ void SetMatrices(const ruyamd_mat& rhs, const ruyamd_mat& dst, const ruyamd_mul_
   call->bias_stride = groups->bias_stride ? groups->bias_stride : dst.rows;
 }
 
-// Launches a checked call on the context's stream and, unless the context is
-// asynchronous or its stream records a graph, waits for it.
+// Launches a checked call.
 int Run(ruyamd_ctx* ctx, grouped::Call* call, const grouped::Int4* weights) {
-  const int enabled = ruyamd_ctx_get_runtime_enabled_paths(ctx);
-  if (!(enabled & RUYAMD_PATH_GFX950)) {
-    ctx->last_used_path = RUYAMD_PATH_NONE;
-    return Fail(ctx, RUYAMD_E_NO_PATH, "runtime-enabled paths exclude gfx950 and this library has no CPU path");
-  }
-  ctx->last_used_path = RUYAMD_PATH_GFX950;
-  ctx->last_kernel = RUYAMD_KERNEL_NONE;
-  int current_device = -1;
-  if (hipGetDevice(&current_device) != hipSuccess || current_device != ctx->device) {
-    if (hipSetDevice(ctx->device) != hipSuccess) return Fail(ctx, RUYAMD_E_HIP, "hipSetDevice failed");
-  }
-  if (call->m == 0 || call->n == 0) return RUYAMD_OK;
   call->compute_units = ctx->multiprocessor_count;
   call->forced_tile_rows = ctx->forced_tile_rows;
   call->forced_tile_cols = ctx->forced_tile_cols;
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {
-    (void)hipGetLastError();
-    status = hipStreamCaptureStatusNone;
-  }
-  ctx->capturing = status == hipStreamCaptureStatusActive;
-  const bool timed = ctx->TimingBegin();
-  hipError_t launched = hipSuccess;
-  if (!ctx->force_generic && grouped::LaunchStream(ctx->stream, *call, weights, &launched)) {
-    ctx->last_kernel = weights ? RUYAMD_KERNEL_INT4_STREAM : RUYAMD_KERNEL_GROUPED_STREAM;
-  } else if (!ctx->force_generic && !weights && grouped::LaunchTiles(ctx->stream, *call, &launched)) {
-    ctx->last_kernel = RUYAMD_KERNEL_GROUPED_MFMA;
-  } else {
-    launched = grouped::LaunchGeneric(ctx->stream, *call, weights);
-    ctx->last_kernel = RUYAMD_KERNEL_GENERIC;
-  }
-  if (timed) ctx->TimingEnd();
-  const bool wait = ctx->synchronous && !ctx->capturing;
-  ctx->capturing = false;
-  if (launched != hipSuccess)
-    return Fail(ctx, RUYAMD_E_HIP, std::string("kernel launch failed: ") + hipGetErrorString(launched));
-  if (wait && hipStreamSynchronize(ctx->stream) != hipSuccess)
-    return Fail(ctx, RUYAMD_E_HIP, std::string("kernel execution failed: ") + hipGetErrorString(hipGetLastError()));
-  return RUYAMD_OK;
+  return LaunchChecked(ctx, call->m == 0 || call->n == 0, [&]() -> hipError_t {
+    hipError_t launched = hipSuccess;
+    if (!ctx->force_generic && grouped::LaunchStream(ctx->stream, *call, weights, &launched)) {
+      ctx->last_kernel = weights ? RUYAMD_KERNEL_INT4_STREAM : RUYAMD_KERNEL_GROUPED_STREAM;
+    } else if (!ctx->force_generic && !weights && grouped::LaunchTiles(ctx->stream, *call, &launched)) {
+      ctx->last_kernel = RUYAMD_KERNEL_GROUPED_MFMA;
+    } else {
+      launched = grouped::LaunchGeneric(ctx->stream, *call, weights);
+      ctx->last_kernel = RUYAMD_KERNEL_GENERIC;
+    }
+    return launched;
+  });
 }
 
 int MulGrouped(ruyamd_ctx* ctx, Dealt dealt, const ruyamd_mat* lhs, const ruyamd_mat* rhs, const ruyamd_groups* groups,

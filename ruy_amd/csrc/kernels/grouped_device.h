@@ -26,6 +26,20 @@ __device__ __forceinline__ void StoreFloat(void* p, int type, int64_t i, float v
     static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
 }
 
+// Two values rounded to a 16-bit type, in one register.
+template <int kType>
+__device__ __forceinline__ int RoundPair(float x, float y) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const v2f both = {x, y};
+  if constexpr (kType == RUYAMD_DTYPE_BF16) {
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, __builtin_convertvector(both, v2bf));
+  } else {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, __builtin_convertvector(both, v2h));
+  }
+}
+
 // min first, then max, as ruy does it (ruy/reference_mul.h:47-48); a NaN stays one.
 __device__ __forceinline__ float Clamp(float v, float low, float high) {
   v = high < v ? high : v;

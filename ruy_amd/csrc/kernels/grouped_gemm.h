@@ -195,20 +195,6 @@ struct TileSide {
   }
 };
 
-// Two values rounded to a 16-bit type, in one register.
-template <int kType>
-__device__ __forceinline__ int RoundPair(float x, float y) {
-  typedef float v2f __attribute__((ext_vector_type(2)));
-  const v2f both = {x, y};
-  if constexpr (kType == RUYAMD_DTYPE_BF16) {
-    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(int, __builtin_convertvector(both, v2bf));
-  } else {
-    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(int, __builtin_convertvector(both, v2h));
-  }
-}
-
 // The range of a group that is the same for the whole wave, in scalar registers.
 __device__ __forceinline__ Range UniformRangeOf(const int32_t* offsets, int group, int total) {
   const Range r = RangeOf(offsets, group, total);

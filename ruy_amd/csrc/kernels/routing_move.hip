@@ -1,0 +1,401 @@
+// Tokens copied to their places, the rows in these places added up, and the
+// gradients of that (ruyamd_dispatch_tokens, ruyamd_combine_tokens,
+// ruyamd_combine_tokens_gradients).
+//
+// All of these go token by token: what belongs to a token once (its values, its sum, its gradient) is
+// read or written once, and its rows, wherever they are, as whole lines. A lane has units of 16
+// bytes (8 values of 16 bits, 4 of 32); the last unit of a row that is no whole number of them
+// ends where the row ends, and overlaps the one before.
+#include <algorithm>
+
+#include "granule.h"
+#include "grouped_device.h"
+#include "launch_geometry.h"
+#include "routing.h"
+
+namespace ruyamd {
+namespace routing {
+namespace {
+
+using granule::v4i;
+using granule::v4i_unaligned;
+using grouped::LoadFloat;
+using grouped::RoundPair;
+using grouped::StoreFloat;
+
+constexpr int Bytes(int type) { return type == RUYAMD_DTYPE_F32 ? 4 : 2; }
+
+// kValues values from number `at` on.
+template <int kType, int kValues>
+__device__ __forceinline__ void Load(const void* data, int64_t at, v4i (&raw)[kValues * Bytes(kType) / 16]) {
+  const v4i_unaligned* const p =
+      reinterpret_cast<const v4i_unaligned*>(static_cast<const char*>(data) + at * Bytes(kType));
+#pragma unroll
+  for (int i = 0; i < kValues * Bytes(kType) / 16; ++i) raw[i] = p[i];
+}
+template <int kType, int kValues>
+__device__ __forceinline__ float Value(const v4i (&raw)[kValues * Bytes(kType) / 16], int e) {
+  if constexpr (kType == RUYAMD_DTYPE_F32) {
+    return __int_as_float(raw[e / 4][e % 4]);
+  } else {
+    const uint32_t word = static_cast<uint32_t>(raw[0][e / 2]);
+    if constexpr (kType == RUYAMD_DTYPE_BF16) return __uint_as_float(e % 2 ? word & 0xffff0000u : word << 16);
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(e % 2 ? word >> 16 : word)));
+  }
+}
+template <int kType, int kValues>
+__device__ __forceinline__ void Store(void* data, int64_t at, const float (&v)[kValues]) {
+  v4i_unaligned* const p = reinterpret_cast<v4i_unaligned*>(static_cast<char*>(data) + at * Bytes(kType));
+#pragma unroll
+  for (int i = 0; i < kValues * Bytes(kType) / 16; ++i) {
+    v4i raw;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (kType == RUYAMD_DTYPE_F32)
+        raw[e] = __float_as_int(v[i * 4 + e]);
+      else
+        raw[e] = RoundPair<kType>(v[2 * e], v[2 * e + 1]);
+    }
+    p[i] = raw;
+  }
+}
+
+// A token and which of its segments of 64 * kUnits units this wave has. (Whole waves: scalars.)
+struct Piece {
+  int token, segment;
+};
+__device__ __forceinline__ int64_t FirstPiece() {
+  return int64_t(blockIdx.x) * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+}
+__device__ __forceinline__ int64_t PieceStride() { return int64_t(gridDim.x) * (blockDim.x >> 6); }
+__device__ __forceinline__ Piece PieceOf(int64_t i, int segments) {
+  const int token = static_cast<int>(i / segments);
+  return {token, static_cast<int>(i - int64_t(token) * segments)};
+}
+
+// The place of choice j of a token, or -1.
+__device__ __forceinline__ int PlaceOf(const Call& c, int token, int j) {
+  const int p = c.places[int64_t(token) * c.top + j];
+  return p >= 0 && p < c.columns ? p : -1;
+}
+__device__ __forceinline__ float WeightOf(const Call& c, int token, int j) {
+  return c.weights.data ? LoadFloat(c.weights.data, c.weights.type, j * c.weights.rs + token * c.weights.cs) : 1.0f;
+}
+
+constexpr int kAtOnce = 4;  // choices of a token whose rows are on their way together
+
+// ---- Tokens to their places ----
+
+template <int kBytes, int kUnits>
+__global__ __launch_bounds__(256) void DispatchKernel(Call c, int segments) {
+  const int lane = threadIdx.x & 63;
+  const int64_t bytes = int64_t(c.width) * kBytes, pieces = int64_t(c.tokens) * segments;
+  for (int64_t i = FirstPiece(); i < pieces; i += PieceStride()) {
+    const Piece piece = PieceOf(i, segments);
+    const char* const from = static_cast<const char*>(c.token_side.data) + piece.token * c.token_side.cs * kBytes;
+    const int64_t first = int64_t(piece.segment) * (1024 * kUnits);
+    v4i held[kUnits];
+    int64_t at[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      at[u] = min(first + u * 1024 + lane * 16, bytes - 16);
+      if (first + u * 1024 < bytes) held[u] = *reinterpret_cast<const v4i_unaligned*>(from + at[u]);
+    }
+    for (int j = 0; j < c.top; ++j) {
+      const int place = PlaceOf(c, piece.token, j);
+      if (place < 0) continue;
+      char* const to = static_cast<char*>(c.place_side.data) + place * c.place_side.cs * kBytes;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u)
+        if (first + u * 1024 < bytes) *reinterpret_cast<v4i_unaligned*>(to + at[u]) = held[u];
+    }
+  }
+}
+
+// ---- The sum of a token's rows ----
+
+template <int kType, int kDstType, int kUnits>
+__global__ __launch_bounds__(256) void CombineKernel(Call c, int segments) {
+  constexpr int kValues = 16 / Bytes(kType);
+  const int lane = threadIdx.x & 63;
+  const int64_t pieces = int64_t(c.tokens) * segments;
+  for (int64_t i = FirstPiece(); i < pieces; i += PieceStride()) {
+    const Piece piece = PieceOf(i, segments);
+    const int64_t first = int64_t(piece.segment) * (64 * kValues * kUnits);
+    int64_t at[kUnits];
+    float sum[kUnits][kValues] = {};
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) at[u] = min(first + (u * 64 + lane) * kValues, int64_t(c.width) - kValues);
+    for (int j0 = 0; j0 < c.top; j0 += kAtOnce) {
+      v4i held[kAtOnce][kUnits][1];
+      int place[kAtOnce];
+      float weight[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        place[j] = j0 + j < c.top ? PlaceOf(c, piece.token, j0 + j) : -1;
+        if (place[j] < 0) continue;
+        weight[j] = WeightOf(c, piece.token, j0 + j);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+          if (first + u * 64 * kValues < c.width) Load<kType, kValues>(c.place_side.data, place[j] * c.place_side.cs + at[u], held[j][u]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (place[j] < 0) continue;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+          for (int e = 0; e < kValues; ++e) sum[u][e] += weight[j] * Value<kType, kValues>(held[j][u], e);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+      if (first + u * 64 * kValues < c.width)
+        Store<kDstType, kValues>(c.token_side.data, piece.token * c.token_side.cs + at[u], sum[u]);
+  }
+}
+
+// ---- The gradients of that sum ----
+
+__device__ __forceinline__ float WaveSum(float v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+  return v;
+}
+
+constexpr int kMostWaves = 8;
+constexpr int kDots = 8;  // choices of a token at a time
+
+// A workgroup to a token; its waves take units of 64 lanes in turn.
+template <int kType, int kGradType>
+__global__ __launch_bounds__(64 * kMostWaves) void GradientsKernel(Call c) {
+  constexpr int kValues = 16 / Bytes(kType);
+  __shared__ float dots[kMostWaves][kDots];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const bool rows = c.grad_src.data, weights = c.grad_weights.data;
+  for (int token = blockIdx.x; token < c.tokens; token += gridDim.x) {
+    for (int j0 = 0; j0 < c.top; j0 += kDots) {
+      int place[kDots];
+      float weight[kDots], dot[kDots] = {};
+#pragma unroll
+      for (int j = 0; j < kDots; ++j) {
+        place[j] = j0 + j < c.top ? PlaceOf(c, token, j0 + j) : -1;
+        weight[j] = place[j] >= 0 && rows ? WeightOf(c, token, j0 + j) : 0.0f;
+      }
+      for (int64_t first = int64_t(wave) * (64 * kValues); first < c.width; first += int64_t(waves) * (64 * kValues)) {
+        const int64_t wanted = first + lane * kValues, at = min(wanted, int64_t(c.width) - kValues);
+        const int again = static_cast<int>(min(wanted - at, int64_t(kValues)));  // values that the lane before has
+        v4i grad[kValues * Bytes(kGradType) / 16], held[kDots][1];
+        Load<kGradType, kValues>(c.token_side.data, token * c.token_side.cs + at, grad);
+        if (weights) {
+#pragma unroll
+          for (int j = 0; j < kDots; ++j)
+            if (place[j] >= 0) Load<kType, kValues>(c.place_side.data, place[j] * c.place_side.cs + at, held[j]);
+        }
+        if (rows) {
+#pragma unroll
+          for (int j = 0; j < kDots; ++j) {
+            if (place[j] < 0) continue;
+            float v[kValues];
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) v[e] = weight[j] * Value<kGradType, kValues>(grad, e);
+            Store<kType, kValues>(c.grad_src.data, place[j] * c.grad_src.cs + at, v);
+          }
+        }
+        if (weights) {
+#pragma unroll
+          for (int j = 0; j < kDots; ++j) {
+            if (place[j] < 0) continue;
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) {
+              const float product = Value<kGradType, kValues>(grad, e) * Value<kType, kValues>(held[j], e);
+              dot[j] += e >= again ? product : 0.0f;
+            }
+          }
+        }
+      }
+      if (!weights) continue;
+#pragma unroll
+      for (int j = 0; j < kDots; ++j) {
+        const float sum = WaveSum(dot[j]);
+        if (lane == 0) dots[wave][j] = sum;
+      }
+      __syncthreads();
+      if (threadIdx.x < kDots && j0 + int(threadIdx.x) < c.top) {
+        float sum = 0;
+        for (int w = 0; w < waves; ++w) sum += dots[w][threadIdx.x];
+        const int j = j0 + threadIdx.x;
+        StoreFloat(c.grad_weights.data, c.grad_weights.type, j * c.grad_weights.rs + token * c.grad_weights.cs, sum);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---- One value to a lane ----
+
+constexpr unsigned kMostBlocks = 1u << 20;
+unsigned BlocksFor(int64_t work, int threads) {
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((work + threads - 1) / threads, kMostBlocks)));
+}
+// A value of a token and the token; the former is the fast one where values lie side by side.
+__device__ __forceinline__ void TokenAndValue(const Call& c, bool by_values, int64_t i, int* token, int* value) {
+  const int fast = by_values ? c.width : c.tokens;
+  const int slow = static_cast<int>(i / fast), rest = static_cast<int>(i - int64_t(slow) * fast);
+  *token = by_values ? slow : rest;
+  *value = by_values ? rest : slow;
+}
+
+__global__ __launch_bounds__(256) void GenericDispatchKernel(Call c) {
+  const int64_t all = int64_t(c.tokens) * c.width;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+    int token, h;
+    TokenAndValue(c, c.token_side.rs == 1, i, &token, &h);
+    const int64_t from = h * c.token_side.rs + token * c.token_side.cs;
+    for (int j = 0; j < c.top; ++j) {
+      const int place = PlaceOf(c, token, j);
+      if (place < 0) continue;
+      const int64_t to = h * c.place_side.rs + place * c.place_side.cs;
+      if (c.token_side.type == RUYAMD_DTYPE_F32)
+        static_cast<uint32_t*>(c.place_side.data)[to] = static_cast<const uint32_t*>(c.token_side.data)[from];
+      else
+        static_cast<uint16_t*>(c.place_side.data)[to] = static_cast<const uint16_t*>(c.token_side.data)[from];
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void GenericCombineKernel(Call c) {
+  const int64_t all = int64_t(c.tokens) * c.width;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+    int token, h;
+    TokenAndValue(c, c.token_side.rs == 1, i, &token, &h);
+    float sum = 0;
+    for (int j = 0; j < c.top; ++j) {
+      const int place = PlaceOf(c, token, j);
+      if (place >= 0)
+        sum += WeightOf(c, token, j) * LoadFloat(c.place_side.data, c.place_side.type, h * c.place_side.rs + place * c.place_side.cs);
+    }
+    StoreFloat(c.token_side.data, c.token_side.type, h * c.token_side.rs + token * c.token_side.cs, sum);
+  }
+}
+
+__global__ __launch_bounds__(256) void GenericRowGradientsKernel(Call c) {
+  const int64_t all = int64_t(c.tokens) * c.width;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+    int token, h;
+    TokenAndValue(c, c.token_side.rs == 1, i, &token, &h);
+    const float grad = LoadFloat(c.token_side.data, c.token_side.type, h * c.token_side.rs + token * c.token_side.cs);
+    for (int j = 0; j < c.top; ++j) {
+      const int place = PlaceOf(c, token, j);
+      if (place >= 0)
+        StoreFloat(c.grad_src.data, c.grad_src.type, h * c.grad_src.rs + place * c.grad_src.cs, WeightOf(c, token, j) * grad);
+    }
+  }
+}
+
+// A wave to a choice.
+__global__ __launch_bounds__(256) void GenericWeightGradientsKernel(Call c) {
+  const int lane = threadIdx.x & 63;
+  const int64_t choices = int64_t(c.tokens) * c.top;
+  for (int64_t i = FirstPiece(); i < choices; i += PieceStride()) {
+    const Piece choice = PieceOf(i, c.top);
+    const int place = PlaceOf(c, choice.token, choice.segment);
+    float sum = 0;
+    if (place >= 0)
+      for (int64_t h = lane; h < c.width; h += 64)
+        sum += LoadFloat(c.token_side.data, c.token_side.type, h * c.token_side.rs + choice.token * c.token_side.cs) *
+               LoadFloat(c.place_side.data, c.place_side.type, h * c.place_side.rs + place * c.place_side.cs);
+    sum = WaveSum(sum);
+    if (lane == 0)
+      StoreFloat(c.grad_weights.data, c.grad_weights.type, choice.segment * c.grad_weights.rs + choice.token * c.grad_weights.cs, sum);
+  }
+}
+
+// Whether a view's values of a token lie side by side (one value alone does).
+bool SideBySide(const Call& c, const View& v) { return !v.data || v.rs == 1 || c.width == 1; }
+
+// Segments of 64 * units units of 16 bytes, and how many units: as many as leave every CU some waves. f(units as a
+// constant, segments, blocks).
+template <class F>
+void WithUnits(const Call& c, int type, int compute_units, F&& f) {
+  const int64_t unit = 64 * (16 / Bytes(type));
+  const auto segments = [&](int units) { return (c.width + unit * units - 1) / (unit * units); };
+  const auto blocks = [&](int64_t s) { return BlocksFor(c.tokens * s, 4); };
+  const int64_t enough = int64_t(16) * compute_units;
+  if (c.tokens * segments(4) >= enough) return f(std::integral_constant<int, 4>(), int(segments(4)), blocks(segments(4)));
+  if (c.tokens * segments(2) >= enough) return f(std::integral_constant<int, 2>(), int(segments(2)), blocks(segments(2)));
+  f(std::integral_constant<int, 1>(), int(segments(1)), blocks(segments(1)));
+}
+
+// f(type of the rows, other type): the other is the rows' or fp32.
+template <class F>
+void WithTypes(int type, int other, F&& f) {
+  using BF16 = std::integral_constant<int, RUYAMD_DTYPE_BF16>;
+  using F16 = std::integral_constant<int, RUYAMD_DTYPE_F16>;
+  using F32 = std::integral_constant<int, RUYAMD_DTYPE_F32>;
+  if (type == RUYAMD_DTYPE_F32) return f(F32(), F32());
+  if (type == RUYAMD_DTYPE_BF16) return other == type ? f(BF16(), BF16()) : f(BF16(), F32());
+  return other == type ? f(F16(), F16()) : f(F16(), F32());
+}
+
+}  // namespace
+
+bool LaunchDispatch(hipStream_t stream, const Call& c, int compute_units, hipError_t* status) {
+  const int type = c.token_side.type;
+  if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side)) return false;
+  WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
+    constexpr int kUnits = decltype(units)::value;
+    if (type == RUYAMD_DTYPE_F32)
+      hipLaunchKernelGGL((DispatchKernel<4, kUnits>), dim3(blocks), dim3(256), 0, stream, c, segments);
+    else
+      hipLaunchKernelGGL((DispatchKernel<2, kUnits>), dim3(blocks), dim3(256), 0, stream, c, segments);
+  });
+  *status = hipGetLastError();
+  return true;
+}
+
+bool LaunchCombine(hipStream_t stream, const Call& c, int compute_units, hipError_t* status) {
+  const int type = c.place_side.type;
+  if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side)) return false;
+  WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
+    WithTypes(type, c.token_side.type, [&](auto t, auto dst) {
+      hipLaunchKernelGGL((CombineKernel<decltype(t)::value, decltype(dst)::value, decltype(units)::value>), dim3(blocks), dim3(256),
+                         0, stream, c, segments);
+    });
+  });
+  *status = hipGetLastError();
+  return true;
+}
+
+bool LaunchGradients(hipStream_t stream, const Call& c, int compute_units, hipError_t* status) {
+  const int type = c.place_side.type;
+  if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side) || !SideBySide(c, c.grad_src))
+    return false;
+  const int64_t units = (c.width + 64 * (16 / Bytes(type)) - 1) / (64 * (16 / Bytes(type)));
+  const int waves = static_cast<int>(std::min<int64_t>(units, kMostWaves));
+  WithTypes(type, c.token_side.type, [&](auto t, auto grad) {
+    hipLaunchKernelGGL((GradientsKernel<decltype(t)::value, decltype(grad)::value>), dim3(BlocksFor(c.tokens, 1)), dim3(64 * waves),
+                       0, stream, c);
+  });
+  *status = hipGetLastError();
+  return true;
+}
+
+hipError_t LaunchGenericDispatch(hipStream_t stream, const Call& c) {
+  hipLaunchKernelGGL(GenericDispatchKernel, dim3(BlocksFor(int64_t(c.tokens) * c.width, 256)), dim3(256), 0, stream, c);
+  return hipGetLastError();
+}
+hipError_t LaunchGenericCombine(hipStream_t stream, const Call& c) {
+  hipLaunchKernelGGL(GenericCombineKernel, dim3(BlocksFor(int64_t(c.tokens) * c.width, 256)), dim3(256), 0, stream, c);
+  return hipGetLastError();
+}
+hipError_t LaunchGenericGradients(hipStream_t stream, const Call& c) {
+  if (c.grad_src.data && c.width)
+    hipLaunchKernelGGL(GenericRowGradientsKernel, dim3(BlocksFor(int64_t(c.tokens) * c.width, 256)), dim3(256), 0, stream, c);
+  if (c.grad_weights.data)
+    hipLaunchKernelGGL(GenericWeightGradientsKernel, dim3(BlocksFor(int64_t(c.tokens) * c.top, 4)), dim3(256), 0, stream, c);
+  return hipGetLastError();
+}
+
+}  // namespace routing
+}  // namespace ruyamd

@@ -1,4 +1,5 @@
-// The Python mirror's call path in native code: ruy_amd.api.mul hands its
+// The Python mirror's call path in native code: ruy_amd.api.mul (and the calls
+// for layers of experts) hands its
 // objects over here, where their fields are gathered into the plain structs of
 // c_api.h and ruyamd_mul is called. Filling four ctypes structures field by
 // field and calling through ctypes took 2.4 us of a call whose launch takes
@@ -32,12 +33,22 @@ uintptr_t grouped_functions[3] = {};  // ruyamd_mul_grouped, ruyamd_mul_grouped_
 PyTypeObject* groups_type = nullptr;
 PyTypeObject* int4_type = nullptr;
 
+// The calls around and beside those products, in the order of api._CALLS, and
+// what each takes: a matrix (m, or null: M), a routing (r, or null: R), 4-bit
+// values (x), groups or null (G), parameters (p).
+constexpr int kCalls = 7;
+constexpr int kMostArguments = 6;
+const char* const call_arguments[kCalls] = {"mr", "mrm", "mrMm", "mMrMMM", "mRx", "xm", "xxGpm"};
+uintptr_t call_functions[kCalls] = {};
+PyTypeObject* routing_type = nullptr;
+PyTypeObject* mxfp4_type = nullptr;
+
 #define RUYAMD_NAMES(X)                                                                                        \
   X(dtype) X(data) X(layout) X(zero_point) X(cache_policy) X(rows) X(cols) X(stride) X(order) X(data_ptr)      \
   X(ctypes) X(bias) X(_perchannel) X(_mf) X(_me) X(_mf_pc) X(_me_pc) X(clamp_min) X(clamp_max) X(accum_dtype) \
   X(dst_dtype) X(channel_dimension) X(_rounding_log2) X(offsets) X(count) X(matrix_stride) X(bias_stride)      \
   X(group_size) X(scales) X(scale_dtype) X(zero_points) X(row_bytes) X(scale_stride) X(matrix_bytes)          \
-  X(scales_matrix_stride)
+  X(scales_matrix_stride) X(tokens) X(top) X(places) X(sources)
 #define RUYAMD_DECLARE(name) PyObject* name_##name;
 RUYAMD_NAMES(RUYAMD_DECLARE)
 
@@ -287,6 +298,158 @@ PyObject* MulWithGroups(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return PyLong_FromLong(rc);
 }
 
+Outcome Routing(PyObject* object, ruyamd_routing* r) {
+  if (Py_TYPE(object) != routing_type) return kNotHandled;
+  const Ref dict = DictOf(object);
+  const Ref offsets = Field(dict, name_offsets);
+  const Ref places = Field(dict, name_places);
+  const Ref sources = Field(dict, name_sources);
+  uint64_t tokens, top, count;
+  if (!offsets || !places || !sources || !Integer(dict, name_tokens, &tokens) || !Integer(dict, name_top, &top) ||
+      !Integer(dict, name_count, &count))
+    return kNotHandled;
+  r->tokens = static_cast<int32_t>(tokens);
+  r->top = static_cast<int32_t>(top);
+  r->count = static_cast<int32_t>(count);
+  r->reserved = 0;
+  void* address = nullptr;
+  if (Outcome o = Address(offsets, &address)) return o;
+  r->offsets = static_cast<int32_t*>(address);
+  if (Outcome o = Address(places, &address)) return o;
+  r->places = static_cast<int32_t*>(address);
+  if (Outcome o = Address(sources, &address)) return o;
+  r->sources = static_cast<int32_t*>(address);
+  return kDone;
+}
+
+Outcome MxFp4(PyObject* object, ruyamd_mxfp4_mat* m) {
+  if (Py_TYPE(object) != mxfp4_type) return kNotHandled;
+  const Ref dict = DictOf(object);
+  const Ref data = Field(dict, name_data);
+  const Ref scales = Field(dict, name_scales);
+  uint64_t rows, cols, row_bytes, scale_stride, matrix_bytes, scales_matrix_stride;
+  if (!data || !scales || !Integer(dict, name_rows, &rows) || !Integer(dict, name_cols, &cols) ||
+      !Integer(dict, name_row_bytes, &row_bytes) || !Integer(dict, name_scale_stride, &scale_stride) ||
+      !Integer(dict, name_matrix_bytes, &matrix_bytes) ||
+      !Integer(dict, name_scales_matrix_stride, &scales_matrix_stride))
+    return kNotHandled;
+  m->rows = static_cast<int32_t>(rows);
+  m->cols = static_cast<int32_t>(cols);
+  m->row_bytes = static_cast<int32_t>(row_bytes);
+  m->scale_stride = static_cast<int32_t>(scale_stride);
+  m->matrix_bytes = static_cast<int64_t>(matrix_bytes);
+  m->scales_matrix_stride = static_cast<int64_t>(scales_matrix_stride);
+  void* address = nullptr;
+  if (Outcome o = Address(data, &address)) return o;
+  m->data = address;
+  if (Outcome o = Address(scales, &address)) return o;
+  m->scales = static_cast<uint8_t*>(address);
+  return kDone;
+}
+
+// Room for any of the structs.
+union Struct {
+  ruyamd_mat matrix;
+  ruyamd_routing routing;
+  ruyamd_mxfp4_mat mxfp4;
+  ruyamd_groups groups;
+  ruyamd_mul_params params;
+};
+
+int CallNumber(long which, ruyamd_ctx* ctx, const Struct* const* a) {
+  const auto m = [&](int i) { return a[i] ? &a[i]->matrix : nullptr; };
+  const auto r = [&](int i) { return a[i] ? &a[i]->routing : nullptr; };
+  const auto x = [&](int i) { return &a[i]->mxfp4; };
+  const uintptr_t f = call_functions[which];
+  switch (which) {
+    case 0:
+      return reinterpret_cast<decltype(&ruyamd_sort_tokens)>(f)(ctx, m(0), r(1));
+    case 1:
+      return reinterpret_cast<decltype(&ruyamd_dispatch_tokens)>(f)(ctx, m(0), r(1), m(2));
+    case 2:
+      return reinterpret_cast<decltype(&ruyamd_combine_tokens)>(f)(ctx, m(0), r(1), m(2), m(3));
+    case 3:
+      return reinterpret_cast<decltype(&ruyamd_combine_tokens_gradients)>(f)(ctx, m(0), m(1), r(2), m(3), m(4), m(5));
+    case 4:
+      return reinterpret_cast<decltype(&ruyamd_quantize_mxfp4)>(f)(ctx, m(0), r(1), x(2));
+    case 5:
+      return reinterpret_cast<decltype(&ruyamd_dequantize_mxfp4)>(f)(ctx, x(0), m(1));
+    default:
+      return reinterpret_cast<decltype(&ruyamd_mul_mxfp4)>(f)(ctx, x(0), x(1), a[2] ? &a[2]->groups : nullptr,
+                                                              &a[3]->params, m(4));
+  }
+}
+
+// call(which, context address, objects...): as Mul, of the function number `which`.
+PyObject* Call(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  const long which = count >= 2 && PyLong_Check(args[0]) ? PyLong_AsLong(args[0]) : -1;
+  if (which < 0 || which >= kCalls || !call_functions[which] ||
+      count != 2 + static_cast<Py_ssize_t>(std::strlen(call_arguments[which]))) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "call(which, context address, objects...)");
+    return nullptr;
+  }
+  Struct structs[kMostArguments];
+  const Struct* pointers[kMostArguments] = {};
+  Outcome o = PyLong_Check(args[1]) ? kDone : kNotHandled;
+  for (int i = 0; o == kDone && call_arguments[which][i]; ++i) {
+    PyObject* const object = args[2 + i];
+    const char kind = call_arguments[which][i];
+    if (object == Py_None && (kind == 'M' || kind == 'R' || kind == 'G')) continue;
+    Struct& s = structs[i];
+    uint64_t dst_dtype;
+    switch (kind) {
+      case 'm':
+      case 'M':
+        o = Matrix(object, &s.matrix);
+        break;
+      case 'r':
+      case 'R':
+        o = Routing(object, &s.routing);
+        break;
+      case 'x':
+        o = MxFp4(object, &s.mxfp4);
+        break;
+      case 'G':
+        o = Groups(object, &s.groups);
+        break;
+      default:
+        o = Params(object, &s.params, &dst_dtype);
+    }
+    pointers[i] = &s;
+  }
+  if (o == kError) return nullptr;
+  if (o == kNotHandled) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  ruyamd_ctx* ctx = reinterpret_cast<ruyamd_ctx*>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLongMask(args[1])));
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = CallNumber(which, ctx, pointers);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// bind_calls([addresses in the order of api._CALLS], Routing, MxFp4Matrix)
+PyObject* BindCalls(PyObject*, PyObject* args) {
+  PyObject *addresses, *routing, *mxfp4;
+  if (!PyArg_ParseTuple(args, "O!O!O!", &PyList_Type, &addresses, &PyType_Type, &routing, &PyType_Type, &mxfp4))
+    return nullptr;
+  if (PyList_GET_SIZE(addresses) != kCalls) {
+    PyErr_SetString(PyExc_ValueError, "an address to each call");
+    return nullptr;
+  }
+  for (int i = 0; i < kCalls; ++i) {
+    const unsigned long long address = PyLong_AsUnsignedLongLong(PyList_GET_ITEM(addresses, i));
+    if (PyErr_Occurred()) return nullptr;
+    call_functions[i] = static_cast<uintptr_t>(address);
+  }
+  for (PyObject* t : {routing, mxfp4}) Py_INCREF(t);
+  routing_type = reinterpret_cast<PyTypeObject*>(routing);
+  mxfp4_type = reinterpret_cast<PyTypeObject*>(mxfp4);
+  Py_RETURN_NONE;
+}
+
 // bind_with_groups([addresses of the three functions], Groups, Int4Matrix)
 PyObject* BindWithGroups(PyObject*, PyObject* args) {
   PyObject *addresses, *groups, *int4;
@@ -327,6 +490,8 @@ PyMethodDef methods[] = {
     {"mul_with_groups", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(MulWithGroups)), METH_FASTCALL,
      nullptr},
     {"bind_with_groups", BindWithGroups, METH_VARARGS, nullptr},
+    {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Call)), METH_FASTCALL, nullptr},
+    {"bind_calls", BindCalls, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
