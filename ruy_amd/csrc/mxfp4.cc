@@ -132,6 +132,9 @@ extern "C" int ruyamd_mul_mxfp4(ruyamd_ctx* ctx, const ruyamd_mxfp4_mat* lhs, co
   call.forced_tile_rows = ctx->forced_tile_rows;
   call.forced_tile_cols = ctx->forced_tile_cols;
   return LaunchChecked(ctx, call.m == 0 || call.n == 0, [&]() -> hipError_t {
+    hipError_t launched = hipSuccess;
+    ctx->last_kernel = RUYAMD_KERNEL_MXFP4_STREAM;
+    if (!ctx->force_generic && mxfp4::LaunchStream(ctx->stream, call, &launched)) return launched;
     ctx->last_kernel = RUYAMD_KERNEL_GENERIC;
     return mxfp4::LaunchGeneric(ctx->stream, call);
   });
