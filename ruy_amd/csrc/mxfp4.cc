@@ -135,6 +135,8 @@ extern "C" int ruyamd_mul_mxfp4(ruyamd_ctx* ctx, const ruyamd_mxfp4_mat* lhs, co
     hipError_t launched = hipSuccess;
     ctx->last_kernel = RUYAMD_KERNEL_MXFP4_STREAM;
     if (!ctx->force_generic && mxfp4::LaunchStream(ctx->stream, call, &launched)) return launched;
+    ctx->last_kernel = RUYAMD_KERNEL_MXFP4_MFMA;
+    if (!ctx->force_generic && mxfp4::LaunchTiles(ctx->stream, call, &launched)) return launched;
     ctx->last_kernel = RUYAMD_KERNEL_GENERIC;
     return mxfp4::LaunchGeneric(ctx->stream, call);
   });
