@@ -7,6 +7,7 @@
 #include "grouped_gemm.h"
 #include "launch_geometry.h"
 #include "mxfp4_device.h"
+#include "mxfp4_large.h"
 
 #include <algorithm>
 #include <cmath>
@@ -36,7 +37,7 @@ constexpr int kStep = 8 * kBlock;  // depth positions to a step: 128 bytes
 // kDirect: rows of both sides begin at multiples of 16 bytes and are whole blocks, so that tiles go to LDS without passing
 // through registers. Otherwise rows are read 16 bytes a lane from wherever they begin.
 template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect>
-__global__ __launch_bounds__(64 * kWavesM * kWavesN, kBlocksM* kBlocksN > 32 ? 1 : 2) void MxFp4GemmKernel(MulCall c) {
+__global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(MulCall c) {
   constexpr int kWaves = kWavesM * kWavesN;
   constexpr int kTileM = kWavesM * kBlocksM * 16, kTileN = kWavesN * kBlocksN * 16;
   // (How rows lie in LDS, which is a matter of bytes alone.)
@@ -289,7 +290,7 @@ struct TileCost {
 };
 constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 256, 2, 0.48f, 0.58f},
                                {Tile::k128x128, 128, 128, 256, 2, 1.08f, 1.5f},
-                               {Tile::k256x256, 256, 256, 512, 1, 1.68f, 0}};
+                               {Tile::k256x256, 256, 256, 256, 1, 1.2f, 0}};
 // What a workgroup does before its first step and after its last, in steps.
 constexpr float kFixedSteps = 6;
 
@@ -307,8 +308,7 @@ hipError_t LaunchKernel(hipStream_t stream, const MulCall& call, unsigned blocks
 
 template <bool kDirect>
 hipError_t LaunchTile(hipStream_t stream, const MulCall& call, Tile tile, unsigned blocks) {
-  if constexpr (kDirect)
-    if (tile == Tile::k256x256) return LaunchKernel<2, 4, 8, 4, true>(stream, call, blocks);
+  if (tile == Tile::k256x256) return LaunchLarge(stream, call, blocks);
   if (tile == Tile::k128x128) return LaunchKernel<2, 2, 4, 4, kDirect>(stream, call, blocks);
   return LaunchKernel<2, 2, 2, 2, kDirect>(stream, call, blocks);
 }
@@ -327,7 +327,16 @@ bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status) {
   // make is known on the device only: here every group that can have a column ends with half a tile.)
   const int64_t busy = std::min(call.groups, call.n);
   const float steps = float(call.k) / kStep + 0.5f + kFixedSteps;
+  const auto scales_aligned = [&](const Matrix& m) {
+    return reinterpret_cast<uintptr_t>(m.scales) % 4 == 0 && m.scale_stride % 4 == 0;
+  };
+  const bool large = direct && call.k % 128 == 0 && call.k >= 512 && scales_aligned(call.lhs) && scales_aligned(call.rhs) &&
+                     call.lhs.scales_matrix_stride % 4 == 0 && TileOffsetsFit(256, call.lhs.row_bytes, call.lhs.row_bytes) &&
+                     TileOffsetsFit(256, call.rhs.row_bytes, call.rhs.row_bytes) &&
+                     TileOffsetsFit(256, call.lhs.scale_stride, call.lhs.scale_stride) &&
+                     TileOffsetsFit(256, call.rhs.scale_stride, call.rhs.scale_stride);
   const auto step_of = [&](const TileCost& t) {
+    if (t.tile == Tile::k256x256) return large ? t.direct : 0.0f;
     if (direct && TileOffsetsFit(t.m, call.lhs.row_bytes, 128) && TileOffsetsFit(t.n, call.rhs.row_bytes, 128)) return t.direct;
     return direct ? 0.0f : t.through;
   };

@@ -315,6 +315,18 @@ def test_every_tile_at_every_end_of_the_depth(context, tile, k):
         context.force_tile(0, 0)
 
 
+@pytest.mark.parametrize("k", [512, 640, 768, 896, 1024, 1152, 1280, 1408, 1536, 2048, 2176, 2688, 4096, 4224, 7168])
+def test_the_largest_tile(context, k):
+    """Odd and even numbers of steps and of pairs of steps, whole and cut short by one to three quarters of 512."""
+    context.force_tile(256, 256)
+    try:
+        run_mul(context, S.BF16, 512, 256, k)
+        run_mul(context, S.F32, 700, 300, k, None, (16, 4 - k // 32 % 4, 32, 4), 0, 0, COL, 1, True, seed=1)
+        run_mul(context, S.F16, 260, 700, k, np.array([0, 5, 5, 300, 650]), (0, 0, 16, 16 - k // 32 % 16), 0, 32, ROW, 0, True, 0.0, seed=2)
+    finally:
+        context.force_tile(0, 0)
+
+
 @pytest.mark.parametrize("m,n,k", [(100, 3, 4096), (64, 20, 1000), (130, 140, 2048), (300, 300, 8000), (16, 1, 40000)])
 def test_products_of_scales_of_any_size(context, kernel, m, n, k):
     run_mul(context, S.F32, m, n, k, scales=(110, 140))
