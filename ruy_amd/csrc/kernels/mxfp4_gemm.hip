@@ -8,6 +8,7 @@
 #include "launch_geometry.h"
 #include "mxfp4_device.h"
 #include "mxfp4_large.h"
+#include "mxfp4_write_back.h"
 
 #include <algorithm>
 #include <cmath>
@@ -18,16 +19,13 @@ namespace mxfp4 {
 namespace {
 
 using grouped::Barrier;
-using grouped::Clamp;
 using grouped::FindTile;
 using grouped::kNothing;
 using grouped::LoadToLds;
 using grouped::Range;
 using grouped::Resource;
-using grouped::RoundPair;
 using grouped::Runs;
 using grouped::StaticFor;
-using grouped::StoreFloat;
 using grouped::TileOf;
 using grouped::TileSide;
 using grouped::WaitVmcnt;
@@ -46,6 +44,8 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
   constexpr int kStage = M::kBytes + N::kBytes, kStages = 2;
   constexpr int kRows = kTileM + kTileN, kScalesAt = kStages * kStage;
   static_assert(kRows <= 64 * kWaves, "a row's scales to a thread");
+  using Out = WriteBack<kBlocksM, kBlocksN>;
+  static_assert(kWaves * Out::kLds <= kScalesAt, "");
   extern __shared__ __attribute__((aligned(16))) char lds[];
 
   const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
@@ -179,7 +179,6 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
       step(s, std::integral_constant<int, 1>());
       if (++s == steps) break;
     }
-    // (LDS may be another workgroup's once this one has ended.)
     WaitVmcnt<0>();
   } else {
     // A granule is read where it lies, or, where it would reach past the end of its row, from the row's last 16 bytes, and
@@ -239,44 +238,11 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
     }
   }
 
-  // Write-back, as in grouped_gemm.h: lane l holds column l % 16 of each block of the N side and, of each pair of blocks of the M
-  // side, 8 rows one after the other.
-  const float* const bias = c.bias ? c.bias + tile.group * c.bias_stride + m0 : nullptr;
-  typedef __attribute__((aligned(2))) v4i v4i_of_2;
-  typedef __attribute__((aligned(4))) v4f v4f_of_4;
-#pragma unroll
-  for (int i = 0; i < kBlocksM; i += 2) {
-    const int m = wave_m * M::kWaveRows + M::RowOf(i, q * 4);
-    float add[8] = {};
-    if (bias)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) add[e] = m + e < here_m ? bias[m + e] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < kBlocksN; ++j) {
-      const int n = wave_n * N::kWaveRows + j * 16 + l;
-      if (n >= here_n) continue;
-      const int64_t to = (int64_t(range.begin) + n0 + n) * c.dst_cs + (m0 + m) * c.dst_rs;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = Clamp(acc[i + e / 4][j][e % 4] + add[e], c.clamp_min, c.clamp_max);
-      if (c.dst_rs != 1 || m + 8 > here_m) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (m + e < here_m) StoreFloat(c.dst, c.dst_type, to + e * c.dst_rs, v[e]);
-      } else if (c.dst_type == RUYAMD_DTYPE_F32) {
-        v4f_of_4* const p = reinterpret_cast<v4f_of_4*>(static_cast<float*>(c.dst) + to);
-        p[0] = v4f{v[0], v[1], v[2], v[3]};
-        p[1] = v4f{v[4], v[5], v[6], v[7]};
-      } else {
-        v4i packed;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          packed[e] = c.dst_type == RUYAMD_DTYPE_BF16 ? RoundPair<RUYAMD_DTYPE_BF16>(v[2 * e], v[2 * e + 1])
-                                                      : RoundPair<RUYAMD_DTYPE_F16>(v[2 * e], v[2 * e + 1]);
-        *reinterpret_cast<v4i_of_2*>(static_cast<uint16_t*>(c.dst) + to) = packed;
-      }
-    }
-  }
+  // (LDS is the write-back's now.)
+  __syncthreads();
+  const int row0 = wave_m * M::kWaveRows, column0 = wave_n * N::kWaveRows;
+  Out{c, acc, lds + wave * Out::kLds, c.bias ? c.bias + tile.group * c.bias_stride + m0 + row0 : nullptr, m0 + row0,
+      int64_t(range.begin) + n0 + column0, here_m - row0, here_n - column0}();
 }
 
 enum class Tile { k64x64, k128x128, k256x256 };

@@ -18,20 +18,18 @@
 #include "grouped_gemm.h"
 #include "mxfp4_device.h"
 #include "mxfp4_large.h"
+#include "mxfp4_write_back.h"
 #include "paired_schedule.h"
 
 namespace ruyamd {
 namespace mxfp4 {
 namespace {
 
-using grouped::Clamp;
 using grouped::FindTile;
 using grouped::kNothing;
 using grouped::Range;
 using grouped::Resource;
-using grouped::RoundPair;
 using grouped::StaticFor;
-using grouped::StoreFloat;
 using grouped::TileOf;
 using grouped::WaitVmcnt;
 namespace ps = paired_schedule;
@@ -39,6 +37,7 @@ namespace ps = paired_schedule;
 constexpr int kTile = 256, kStepBytes = 128, kStep = 8 * kBlock;
 constexpr int kSide = kTile * kStepBytes, kStage = 2 * kSide;  // bytes in LDS: of a side's step, of a step
 constexpr int kRaw = 2 * kStage, kScales = kRaw + 2 * kTile * 16, kLds = kScales + 2 * kTile * 16;
+static_assert(4 * WriteBack<ps::kBlocks, ps::kBlocks>::kLds <= kLds, "");
 static_assert(ps::kBlocks == 8 && ps::kWaves == 4 && ps::kLoads * ps::kRowsPerLoad * ps::kWaves == kTile, "");
 
 // The instruction with byte kByte of either side's scales. (The compiler's hazard checks do not look inside: an
@@ -264,46 +263,13 @@ __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
   }
   if (s < steps) step(s, Odd(), No(), No());
   Drain();
-  // (LDS may be another workgroup's once this one has ended.)
   WaitVmcnt<0>();
 
-  // Write-back: lane l has column l % 16 of each block and, of each pair of block rows, 8 rows one after the other.
-  const float* const bias = c.bias ? c.bias + tile.group * c.bias_stride + m0 : nullptr;
-  typedef __attribute__((aligned(2))) v4i v4i_of_2;
-  typedef __attribute__((aligned(4))) v4f v4f_of_4;
-#pragma unroll
-  for (int i = 0; i < ps::kBlocks; i += 2) {
-    const int m = wave_m * 128 + i * 16 + q * 8;
-    float add[8] = {};
-    if (bias)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) add[e] = m + e < here_m ? bias[m + e] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < ps::kBlocks; ++j) {
-      const int n = wave_n * 128 + j * 16 + l;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = Clamp(acc[i + e / 4][j][e % 4] + add[e], c.clamp_min, c.clamp_max);
-      if (n >= here_n) continue;
-      const int64_t to = (int64_t(range.begin) + n0 + n) * c.dst_cs + (m0 + m) * c.dst_rs;
-      if (c.dst_rs != 1 || m + 8 > here_m) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (m + e < here_m) StoreFloat(c.dst, c.dst_type, to + e * c.dst_rs, v[e]);
-      } else if (c.dst_type == RUYAMD_DTYPE_F32) {
-        v4f_of_4* const p = reinterpret_cast<v4f_of_4*>(static_cast<float*>(c.dst) + to);
-        p[0] = v4f{v[0], v[1], v[2], v[3]};
-        p[1] = v4f{v[4], v[5], v[6], v[7]};
-      } else {
-        v4i packed;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          packed[e] = c.dst_type == RUYAMD_DTYPE_BF16 ? RoundPair<RUYAMD_DTYPE_BF16>(v[2 * e], v[2 * e + 1])
-                                                      : RoundPair<RUYAMD_DTYPE_F16>(v[2 * e], v[2 * e + 1]);
-        *reinterpret_cast<v4i_of_2*>(static_cast<uint16_t*>(c.dst) + to) = packed;
-      }
-    }
-  }
+  // (LDS is the write-back's now.)
+  __syncthreads();
+  using Out = WriteBack<ps::kBlocks, ps::kBlocks>;
+  Out{c, acc, lds + wave * Out::kLds, c.bias ? c.bias + tile.group * c.bias_stride + m0 + wave_m * 128 : nullptr,
+      m0 + wave_m * 128, int64_t(range.begin) + n0 + wave_n * 128, here_m - wave_m * 128, here_n - wave_n * 128}();
 }
 
 }  // namespace
