@@ -34,7 +34,7 @@ struct StreamArgs {
 
 // LDS that a workgroup may take.
 constexpr int kMostLds = 156 << 10;
-constexpr int kMostWaves = 8;
+constexpr int kMostWaves = 16;
 
 template <int kCols>
 __global__ __launch_bounds__(64 * kMostWaves) void MxFp4StreamKernel(StreamArgs args) {
@@ -66,8 +66,16 @@ __global__ __launch_bounds__(64 * kMostWaves) void MxFp4StreamKernel(StreamArgs 
       h.weights[i] = granule::LoadGranule<false>(weights, chunk * (kChunk / 2) + i * 64 + q * 16, row_bytes);
     h.scales = LoadScales(scales, chunk * 16, row_scales);
   };
+  // This wave's chunks are depth_wave + i * depth_waves, `mine` of them. It starts with another one for each block of rows and
+  // goes round: rows lie a power of two apart as often as not, and all waves at one depth would be at few of the memory's channels.
+  const int mine = (chunks - depth_wave + args.depth_waves - 1) / args.depth_waves;
+  const int start = static_cast<int>(uint32_t(tile.m * args.row_waves + row_wave) % uint32_t(mine));
+  const auto chunk_of = [&](int i) __attribute__((always_inline)) {
+    const int at = i + start;
+    return depth_wave + (at < mine ? at : at - mine) * args.depth_waves;
+  };
   Held first, second;
-  if (depth_wave < chunks) load(depth_wave, first);
+  load(chunk_of(0), first);
 
   // The tokens, and their scales.
   const uint8_t* const token_data = c.rhs.data + (int64_t(range.begin) + token0) * c.rhs.row_bytes;
@@ -116,13 +124,13 @@ __global__ __launch_bounds__(64 * kMostWaves) void MxFp4StreamKernel(StreamArgs 
     }
   };
   // Two chunks of the weights are on their way.
-  if (depth_wave + args.depth_waves < chunks) load(depth_wave + args.depth_waves, second);
-  for (int chunk = depth_wave; chunk < chunks; chunk += 2 * args.depth_waves) {
-    use(chunk, first);
-    if (chunk + 2 * args.depth_waves < chunks) load(chunk + 2 * args.depth_waves, first);
-    if (chunk + args.depth_waves >= chunks) break;
-    use(chunk + args.depth_waves, second);
-    if (chunk + 3 * args.depth_waves < chunks) load(chunk + 3 * args.depth_waves, second);
+  if (mine > 1) load(chunk_of(1), second);
+  for (int i = 0; i < mine; i += 2) {
+    use(chunk_of(i), first);
+    if (i + 2 < mine) load(chunk_of(i + 2), first);
+    if (i + 1 >= mine) break;
+    use(chunk_of(i + 1), second);
+    if (i + 3 < mine) load(chunk_of(i + 3), second);
   }
 
   // The waves' sums, added up in the order of the depth, and the write-back. Lane l holds rows
@@ -173,11 +181,21 @@ bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
   if (fit < 1) return false;
   const int cols = call.n > 16 * busy && fit > 16 ? 2 : 1;
   args.tokens = static_cast<int>(std::min<int64_t>({16 * cols, fit, call.n}));
-  int depth_waves = kMostWaves;
+  // Waves along the depth: neighbours of a workgroup are at neighbouring chunks, 2 KB of a row with eight. Fewer where they would have less
+  // than four chunks each and there are rows for 16 waves to a CU without. (us, one token, eight and four of them: 16384 x 16384
+  // 28.0 and 28.3, with two 38; 28672 x 8192 30.1 and 24.8; 2048 x 8192 6.6 and 7.1; 64 experts of 2048 x 2048, 32 tokens, four and
+  // one 18.6 and 15.4.) Along the rows as many as make all workgroups fit the CUs, whose LDS the tokens fill, at once, in exchange for
+  // waves along the depth where need be. (16 tokens, 16384 x 16384: 8 x 1 65, 8 x 2 39, 4 x 4 35; 32, 8192 x 8192: 8 x 1 29, 8 x 2 16;
+  // one, 2048 x 2048: 4 x 1 4.6, 4 x 2 6.0.)
   const int64_t units = (int64_t(call.m) + 15) / 16 * busy;
-  while (depth_waves > 1 && units * depth_waves > int64_t(16) * call.compute_units) depth_waves /= 2;
-  int row_waves = kMostWaves / depth_waves;
+  int depth_waves = 8, row_waves = 1;
+  while (depth_waves > 1 && chunks < 4 * depth_waves && units * depth_waves > int64_t(16) * call.compute_units) depth_waves /= 2;
   while (depth_waves > 1 && chunks < depth_waves) depth_waves /= 2;
+  const int64_t tokens_lds = args.tokens * (pitch + scale_pitch), at_once = kMostLds / tokens_lds * call.compute_units;
+  while (row_waves < kMostWaves && units > at_once * row_waves) {
+    row_waves *= 2;
+    if (depth_waves * row_waves > kMostWaves) depth_waves /= 2;
+  }
   args.depth_waves = depth_waves;
   args.row_waves = row_waves;
   const int work_rows = 16 * row_waves, waves = depth_waves * row_waves;
@@ -185,7 +203,7 @@ bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
   args.pitch = static_cast<int>(pitch);
   args.scale_pitch = static_cast<int>(scale_pitch);
   args.scales_at = static_cast<int>(args.tokens * pitch);
-  const int64_t lds = std::max(args.tokens * (pitch + scale_pitch), int64_t(waves) * 1024);
+  const int64_t lds = std::max(tokens_lds, int64_t(waves) * 1024);
   const int64_t slots = call.n / args.tokens + busy;
   const int64_t blocks = (slots * args.tiles_m + 7) / 8 * 8;
   if (!LaunchFits(blocks, 64 * waves)) return false;
