@@ -34,14 +34,18 @@ constexpr int kStep = 8 * kBlock;  // depth positions to a step: 128 bytes
 
 // kDirect: rows of both sides begin at multiples of 16 bytes and are whole blocks, so that tiles go to LDS without passing
 // through registers. Otherwise rows are read 16 bytes a lane from wherever they begin.
-template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect>
+// kStages: steps on their way to LDS (kDirect). More than two: the scales of the whole depth are put into LDS first, for whose
+// loads the waves would otherwise wait, and for those of all steps with them, in every other step.
+template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages>
 __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(MulCall c) {
   constexpr int kWaves = kWavesM * kWavesN;
   constexpr int kTileM = kWavesM * kBlocksM * 16, kTileN = kWavesN * kBlocksN * 16;
   // (How rows lie in LDS, which is a matter of bytes alone.)
   using M = TileSide<RUYAMD_DTYPE_BF16, Runs::kPlain, kTileM, kBlocksM, true, kWaves>;
   using N = TileSide<RUYAMD_DTYPE_BF16, Runs::kPlain, kTileN, kBlocksN, false, kWaves>;
-  constexpr int kStage = M::kBytes + N::kBytes, kStages = 2;
+  constexpr int kStage = M::kBytes + N::kBytes;
+  constexpr bool kAllScales = kStages > 2;
+  static_assert(kDirect || kStages == 2, "");
   constexpr int kRows = kTileM + kTileN, kScalesAt = kStages * kStage;
   static_assert(kRows <= 64 * kWaves, "a row's scales to a thread");
   using Out = WriteBack<kBlocksM, kBlocksN>;
@@ -93,17 +97,19 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
       for (int j = 0; j < kBlocksN; ++j) Mma<byte>(f.m[i], f.n[j], s.m[i], s.n[j], acc[i][j]);
   };
 
-  // A thread's row, whose scales it brings. (Those of rows past the tile's sides are the last row's.)
-  const int row = threadIdx.x;
-  const uint8_t* scale_row = c.lhs.scales;
-  if (row < kTileM)
-    scale_row += tile.group * c.lhs.scales_matrix_stride + int64_t(m0 + min(row, here_m - 1)) * c.lhs.scale_stride;
-  else
-    scale_row = c.rhs.scales + (int64_t(range.begin) + n0 + min(row - kTileM, here_n - 1)) * c.rhs.scale_stride;
+  // The scales of a row of either side. (Those of rows past the tile's sides are the last row's.)
+  const auto scales_of_row = [&](int row) __attribute__((always_inline)) {
+    return row < kTileM ? c.lhs.scales + tile.group * c.lhs.scales_matrix_stride + int64_t(m0 + min(row, here_m - 1)) * c.lhs.scale_stride
+                        : c.rhs.scales + (int64_t(range.begin) + n0 + min(row - kTileM, here_n - 1)) * c.rhs.scale_stride;
+  };
+  const auto put_scales_of_row = [&](const v4i& x, int row, int pair, int buffer) __attribute__((always_inline)) {
+    *reinterpret_cast<v4i*>(lds + kScalesAt + buffer * (kRows * 16) + row * 16) = Transposed(PlaceScales(x, pair * 16, row_scales));
+  };
+  // A thread brings those of one row, pair by pair.
+  const uint8_t* const scale_row = scales_of_row(threadIdx.x);
   const auto fetch_scales = [&](int pair) __attribute__((always_inline)) { return LoadScales(scale_row, pair * 16, row_scales); };
   const auto put_scales = [&](const v4i& x, int pair, int buffer) __attribute__((always_inline)) {
-    if (row < kRows)
-      *reinterpret_cast<v4i*>(lds + kScalesAt + buffer * (kRows * 16) + row * 16) = Transposed(PlaceScales(x, pair * 16, row_scales));
+    if (int(threadIdx.x) < kRows) put_scales_of_row(x, threadIdx.x, pair, buffer);
   };
 
   if constexpr (kDirect) {
@@ -143,32 +149,52 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
         __builtin_amdgcn_sched_group_barrier(0x008, kProducts / kReads > 0 ? kProducts / kReads : 1, 0);
       });
     };
-    // As in grouped_gemm.h: steps are on their way to LDS two ahead, and the two halves of a step's depth take turns: while the
+    // As in grouped_gemm.h: steps are on their way to LDS kStages ahead, and the two halves of a step's depth take turns: while the
     // matrix cores have one, the fragments of the other come out of LDS. In the middle of a step all waves wait for the loads
-    // of the next one and for each other; in every other step the scales of the next pair, which have come with these
-    // loads, go into LDS before that, and out of it after.
-    v4i next_scales = fetch_scales(0);
-    issue(0, 0);
-    issue(1, 1);
-    put_scales(next_scales, 0, 0);
-    WaitVmcnt<0>();
+    // of the next one and for each other. With two stages, in every other step the scales of the next pair, which have come with
+    // these loads, go into LDS before that, and out of it after.
+    constexpr int kLoads = M::kLoads + N::kLoads;
+    v4i next_scales = {};
+    if constexpr (!kAllScales) next_scales = fetch_scales(0);
+    StaticFor<kStages>([&](auto d) __attribute__((always_inline)) { issue(d, d); });
+    if constexpr (kAllScales) {
+      constexpr int kAtOnce = 4, kThreads = 64 * kWaves;
+      const int all = (steps + 1) / 2 * kRows;
+      for (int i0 = threadIdx.x; i0 < all; i0 += kAtOnce * kThreads) {
+        v4i x[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int i = min(i0 + u * kThreads, all - 1);
+          x[u] = LoadScales(scales_of_row(i % kRows), i / kRows * 16, row_scales);
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int i = i0 + u * kThreads;
+          if (i < all) put_scales_of_row(x[u], i % kRows, i / kRows, i / kRows);
+        }
+      }
+    } else {
+      put_scales(next_scales, 0, 0);
+    }
+    WaitVmcnt<(kStages - 1) * kLoads>();
     Barrier();
     Fragments first, second;
     Scales scales, later;
     read(0, 0, first);
     read_scales(0, scales);
-    const auto step = [&](int s, auto odd) __attribute__((always_inline)) {
-      constexpr int kOdd = decltype(odd)::value;
-      read(kOdd, 1, second);
+    const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
+      constexpr int kAt = decltype(stage)::value, kOdd = kAt % 2;
+      read(kAt, 1, second);
       multiply(first, scales, std::integral_constant<int, 2 * kOdd>());
       interleave();
-      WaitVmcnt<0>();
-      if constexpr (kOdd) put_scales(next_scales, (s + 1) / 2, 0);
+      WaitVmcnt<(kStages - 2) * kLoads>();
+      if constexpr (kOdd && !kAllScales) put_scales(next_scales, (s + 1) / 2, 0);
       Barrier();
-      if constexpr (!kOdd) next_scales = fetch_scales(s / 2 + 1);
-      issue(s + 2, kOdd);
-      read(1 - kOdd, 0, first);
-      if constexpr (kOdd) read_scales(0, later);
+      if constexpr (!kOdd && !kAllScales) next_scales = fetch_scales(s / 2 + 1);
+      issue(s + kStages, kAt);
+      read((kAt + 1) % kStages, 0, first);
+      // (Past the last pair: the last one again, of which nothing is used.)
+      if constexpr (kOdd) read_scales(kAllScales ? min((s + 1) / 2, (steps - 1) / 2) : 0, later);
       multiply(second, scales, std::integral_constant<int, 2 * kOdd + 1>());
       interleave();
       if constexpr (kOdd) scales = later;
@@ -178,6 +204,12 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
       if (++s == steps) break;
       step(s, std::integral_constant<int, 1>());
       if (++s == steps) break;
+      if constexpr (kStages > 2) {
+        step(s, std::integral_constant<int, 2>());
+        if (++s == steps) break;
+        step(s, std::integral_constant<int, 3>());
+        if (++s == steps) break;
+      }
     }
     WaitVmcnt<0>();
   } else {
@@ -245,36 +277,49 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
       int64_t(range.begin) + n0 + column0, here_m - row0, here_n - column0}();
 }
 
-enum class Tile { k64x64, k128x128, k256x256 };
+// The kernels: 64x64 with two and with four stages and 128x128 (above), and 256x256 (mxfp4_large.h).
+enum class Tile { k64x64, k64x64Deep, k128x128, k256x256 };
 
-// A tile's sizes, the threads of its workgroup, the workgroups that a CU runs side by side, and how long one step of all of them
-// takes, us, with operands straight to LDS and through registers (0: there is no such kernel).
+// How long a kernel takes, us: with its tiles dealt to `per_cu` workgroups of every CU in rounds, the last of which costs at least
+// `last` of a full one, fixed + rounds * (steps + more) * step, a step being 256 positions of depth. Fitted to 290 shapes of 256 to
+// 16384 rows, 48 to 8192 columns and depths of 512 to 16384, bfloat16 destinations, to 5 to 11 % root mean square. Choosing by it
+// costs 1.3 % over the fastest kernel at each of these shapes (20 % at the worst, 256 x 48, depth 512: 5.6 us for 4.6).
+struct Timing {
+  int per_cu;
+  float fixed, step, more, last;
+};
 struct TileCost {
   Tile tile;
-  int m, n, threads, per_cu;
-  float direct, through;
+  int m, n;
+  Timing direct, through;  // operands straight to LDS, and through registers (step 0: there is no such kernel)
 };
-constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, 256, 2, 0.48f, 0.58f},
-                               {Tile::k128x128, 128, 128, 256, 2, 1.08f, 1.5f},
-                               {Tile::k256x256, 256, 256, 256, 1, 1.2f, 0}};
-// What a workgroup does before its first step and after its last, in steps.
-constexpr float kFixedSteps = 6;
+constexpr int kThreads = 256;
+constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, {4, 2.8f, 0.96f, 2.7f, 0.33f}, {2, 2.5f, 0.715f, 1.2f, 0.71f}},
+                               {Tile::k64x64Deep, 64, 64, {1, 3.2f, 0.315f, 3.6f, 0.88f}, {1, 0, 0, 0, 0}},
+                               {Tile::k128x128, 128, 128, {2, 2.3f, 1.34f, 3.1f, 0.51f}, {1, 3.8f, 1.24f, 0.5f, 0.90f}},
+                               {Tile::k256x256, 256, 256, {1, 2.75f, 1.64f, 5.6f, 0.63f}, {1, 0, 0, 0, 0}}};
 
-template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect>
+// LDS that a workgroup may take, and what 64x64 tiles of four stages do.
+constexpr int kMostLds = 156 << 10;
+int64_t DeepLds(int64_t k) { return 4 * 128 * 128 + (k + kChunk - 1) / kChunk * (128 * 16); }
+
+template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages = 2>
 hipError_t LaunchKernel(hipStream_t stream, const MulCall& call, unsigned blocks) {
   constexpr int kRows = (kWavesM * kBlocksM + kWavesN * kBlocksN) * 16;
-  constexpr int kLds = 2 * kRows * 128 + (kDirect ? 1 : 2) * kRows * 16;
-  auto* const kernel = &MxFp4GemmKernel<kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect>;
+  const int lds = kStages > 2 ? static_cast<int>(DeepLds(call.k)) : 2 * kRows * 128 + (kDirect ? 1 : 2) * kRows * 16;
+  auto* const kernel = &MxFp4GemmKernel<kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect, kStages>;
   static const hipError_t attribute =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
   if (attribute != hipSuccess) return attribute;
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWavesM * kWavesN), kLds, stream, call);
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kWavesM * kWavesN), lds, stream, call);
   return hipGetLastError();
 }
 
 template <bool kDirect>
 hipError_t LaunchTile(hipStream_t stream, const MulCall& call, Tile tile, unsigned blocks) {
   if (tile == Tile::k256x256) return LaunchLarge(stream, call, blocks);
+  if constexpr (kDirect)
+    if (tile == Tile::k64x64Deep) return LaunchKernel<2, 2, 2, 2, true, 4>(stream, call, blocks);
   if (tile == Tile::k128x128) return LaunchKernel<2, 2, 4, 4, kDirect>(stream, call, blocks);
   return LaunchKernel<2, 2, 2, 2, kDirect>(stream, call, blocks);
 }
@@ -289,10 +334,6 @@ bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status) {
     return reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && m.row_bytes % 16 == 0;
   };
   const bool direct = call.k % kBlock == 0 && aligned(call.lhs) && aligned(call.rhs) && call.lhs.matrix_bytes % 16 == 0;
-  // The tile that the CUs would be done with first. (How many tiles the groups' columns
-  // make is known on the device only: here every group that can have a column ends with half a tile.)
-  const int64_t busy = std::min(call.groups, call.n);
-  const float steps = float(call.k) / kStep + 0.5f + kFixedSteps;
   const auto scales_aligned = [&](const Matrix& m) {
     return reinterpret_cast<uintptr_t>(m.scales) % 4 == 0 && m.scale_stride % 4 == 0;
   };
@@ -301,26 +342,37 @@ bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status) {
                      TileOffsetsFit(256, call.rhs.row_bytes, call.rhs.row_bytes) &&
                      TileOffsetsFit(256, call.lhs.scale_stride, call.lhs.scale_stride) &&
                      TileOffsetsFit(256, call.rhs.scale_stride, call.rhs.scale_stride);
-  const auto step_of = [&](const TileCost& t) {
-    if (t.tile == Tile::k256x256) return large ? t.direct : 0.0f;
-    if (direct && TileOffsetsFit(t.m, call.lhs.row_bytes, 128) && TileOffsetsFit(t.n, call.rhs.row_bytes, 128)) return t.direct;
-    return direct ? 0.0f : t.through;
+  const auto fits = [&](const TileCost& t) {
+    return TileOffsetsFit(t.m, call.lhs.row_bytes, 128) && TileOffsetsFit(t.n, call.rhs.row_bytes, 128);
   };
+  const auto timing_of = [&](const TileCost& t) {
+    const Timing none = {1, 0, 0, 0, 0};
+    if (t.tile == Tile::k256x256) return large ? t.direct : none;
+    if (t.tile == Tile::k64x64Deep && DeepLds(call.k) > kMostLds) return none;
+    return !direct ? t.through : fits(t) ? t.direct : none;
+  };
+  const int64_t busy = std::min(call.groups, call.n);
   const auto blocks_of = [&](const TileCost& t) {
     return ((int64_t(call.m) + t.m - 1) / t.m * (call.n / t.n + busy) + 7) / 8 * 8;
   };
-  const auto usable = [&](const TileCost& t) { return step_of(t) != 0 && LaunchFits(blocks_of(t), t.threads); };
-  const auto forced = [&](const TileCost& t) { return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols; };
+  const auto usable = [&](const TileCost& t) { return timing_of(t).step != 0 && LaunchFits(blocks_of(t), kThreads); };
+  const auto forced = [&](const TileCost& t) {
+    return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols && (t.tile == Tile::k64x64Deep) == call.forced_deep;
+  };
   const bool force = std::any_of(std::begin(kTiles), std::end(kTiles), [&](const TileCost& t) { return forced(t) && usable(t); });
+  // The kernel that would be done first. (How many tiles the groups' columns make is known on the device only: here every group that can
+  // have a column ends with half a tile.)
   Tile tile = Tile::k64x64;
   int64_t blocks = 0;
   float best = 0;
   for (const TileCost& t : kTiles) {
     if (!usable(t) || (force && !forced(t))) continue;
+    const Timing timing = timing_of(t);
     const int64_t tiles_m = (int64_t(call.m) + t.m - 1) / t.m;
-    const float tiles_n = std::max(float(busy), float(call.n) / t.n + 0.5f * busy);
-    const float rounds = std::ceil(tiles_m * tiles_n / (t.per_cu * call.compute_units) - 0.05f);
-    const float time = std::max(1.0f, rounds) * steps * step_of(t);
+    const float tiles_n = busy == 1 ? std::ceil(float(call.n) / t.n) : std::max(float(busy), float(call.n) / t.n + 0.5f * busy);
+    const float all = tiles_m * tiles_n / (timing.per_cu * call.compute_units), full = std::floor(all);
+    const float rounds = std::max(timing.last, full + (all > full ? timing.last + (1 - timing.last) * (all - full) : 0.0f));
+    const float time = timing.fixed + rounds * (float(call.k) / kStep + timing.more) * timing.step;
     if (blocks == 0 || time < best) {
       best = time;
       tile = t.tile;

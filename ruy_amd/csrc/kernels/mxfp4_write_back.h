@@ -48,26 +48,42 @@ struct WriteBack {
       if constexpr (!kPlain) v[e] = __builtin_elementwise_maximum(__builtin_elementwise_minimum(v[e] + add[e], c.clamp_max), c.clamp_min);
     }
   }
+  // The bias of a lane's rows, all of it on its way at once.
+  struct Added {
+    float of[kBlocksM / 2][8];
+  };
   template <bool kPlain>
-  __device__ __forceinline__ void Bias(int i, float (&add)[8]) const {
-    if constexpr (!kPlain) {
-      const int m = i * 32 + q * 8;
+  __device__ __forceinline__ Added Bias() const {
+    Added add = {};
+    if (!kPlain && bias) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) add[e] = bias && m + e < rows ? bias[m + e] : 0.0f;
+      for (int i = 0; i < kBlocksM / 2; ++i) {
+        const int m = i * 32 + q * 8;
+        if (m + 8 <= rows) {
+          const v4f low = *reinterpret_cast<const v4f_of_4*>(bias + m), high = *reinterpret_cast<const v4f_of_4*>(bias + m + 4);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) add.of[i][e] = e < 4 ? low[e & 3] : high[e & 3];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (m + e < rows) add.of[i][e] = bias[m + e];
+        }
+      }
     }
+    return add;
   }
 
   // 16-bit values by columns: rounded where they are, and through LDS, so that whole lines of dst are stored.
   template <bool kPlain>
   __device__ __forceinline__ void Half() const {
     const bool bf16 = c.dst_type == RUYAMD_DTYPE_BF16;
+    const Added add = Bias<kPlain>();
 #pragma unroll
     for (int i = 0; i < kBlocksM / 2; ++i) {
-      float add[8], v[8];
-      Bias<kPlain>(i, add);
+      float v[8];
 #pragma unroll
       for (int j = 0; j < kBlocksN; ++j) {
-        Values<kPlain>(i, j, add, v);
+        Values<kPlain>(i, j, add.of[i], v);
         v4i packed;
         if (bf16) {
 #pragma unroll
@@ -107,13 +123,13 @@ struct WriteBack {
   // fp32 by columns, all rows: four lanes' 32 bytes are a whole line.
   template <bool kPlain>
   __device__ __forceinline__ void Full() const {
+    const Added add = Bias<kPlain>();
 #pragma unroll
     for (int i = 0; i < kBlocksM / 2; ++i) {
-      float add[8], v[8];
-      Bias<kPlain>(i, add);
+      float v[8];
 #pragma unroll
       for (int j = 0; j < kBlocksN; ++j) {
-        Values<kPlain>(i, j, add, v);
+        Values<kPlain>(i, j, add.of[i], v);
         if (j * 16 + l >= columns) continue;
         v4f_of_4* const p = reinterpret_cast<v4f_of_4*>(static_cast<float*>(c.dst) + (n0 + j * 16 + l) * c.dst_cs + m0 + i * 32 + q * 8);
         p[0] = v4f{v[0], v[1], v[2], v[3]};

@@ -131,6 +131,7 @@ extern "C" int ruyamd_mul_mxfp4(ruyamd_ctx* ctx, const ruyamd_mxfp4_mat* lhs, co
   call.compute_units = ctx->multiprocessor_count;
   call.forced_tile_rows = ctx->forced_tile_rows;
   call.forced_tile_cols = ctx->forced_tile_cols;
+  call.forced_deep = ctx->forced_depth_parts != 0;
   return LaunchChecked(ctx, call.m == 0 || call.n == 0, [&]() -> hipError_t {
     hipError_t launched = hipSuccess;
     ctx->last_kernel = RUYAMD_KERNEL_MXFP4_STREAM;

@@ -315,6 +315,21 @@ def test_every_tile_at_every_end_of_the_depth(context, tile, k):
         context.force_tile(0, 0)
 
 
+@pytest.mark.parametrize("k", [32, 64, 256, 480, 512, 544, 768, 1024, 1280, 1504, 2048, 2080, 4096, 7168, 22528])
+def test_tiles_of_four_stages(context, k):
+    """Fewer steps than stages, as many, more, pairs cut short anywhere; the deepest that LDS has scales for, and (on
+    another tile) deeper."""
+    context.force_tile(64, 64, 1)
+    try:
+        run_mul(context, S.BF16, 200, 130, k)
+        assert context.last_kernel_name() == "mxfp4_mfma"
+        run_mul(context, S.F32, 97, 300, k, np.array([0, 33, 33, 250, 300]), (16 - (k // 2) % 16, 3, 0, 2), 0, 16, COL, 1, True, 0.0, seed=1)
+        run_mul(context, S.F16, 70, 65, k, None, (16 - (k // 2) % 16, 4, 16 - (k // 2) % 16, 1), 0, 0, ROW, 0, True, seed=2)
+        run_mul(context, S.F32, 70, 65, k + 1600, scales=(120, 133), seed=3)
+    finally:
+        context.force_tile(0, 0)
+
+
 @pytest.mark.parametrize("k", [512, 640, 768, 896, 1024, 1152, 1280, 1408, 1536, 2048, 2176, 2688, 4096, 4224, 7168])
 def test_the_largest_tile(context, k):
     """Odd and even numbers of steps and of pairs of steps, whole and cut short by one to three quarters of 512."""
