@@ -59,6 +59,8 @@ struct MulCall {
 // As in grouped.h.
 hipError_t LaunchGeneric(hipStream_t stream, const MulCall& call);
 bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status);
+float TilesMicroseconds(const MulCall& call);  // how long that takes, about; negative: not a call for them
+// (Also where tiles would take less time.)
 bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status);
 
 }  // namespace mxfp4

@@ -324,12 +324,19 @@ hipError_t LaunchTile(hipStream_t stream, const MulCall& call, Tile tile, unsign
   return LaunchKernel<2, 2, 2, 2, kDirect>(stream, call, blocks);
 }
 
-}  // namespace
+// The tiles of a call, how many at most, and how long they take (blocks 0: none are its).
+struct Choice {
+  Tile tile = Tile::k64x64;
+  bool direct = false;
+  int64_t blocks = 0;
+  float time = 0;
+};
 
-bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status) {
-  if (call.k < kBlock) return false;  // (a row has 16 bytes at least)
+Choice Choose(const MulCall& call) {
+  Choice choice;
+  if (call.k < kBlock) return choice;  // (a row has 16 bytes at least)
   // (Sizes and depths are rounded up to tiles, and gone past by some steps, in 32 bits.)
-  if (std::max(call.m, std::max(call.n, call.k)) > 0x7fffffff - 2048) return false;
+  if (std::max(call.m, std::max(call.n, call.k)) > 0x7fffffff - 2048) return choice;
   const auto aligned = [&](const Matrix& m) {
     return reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && m.row_bytes % 16 == 0;
   };
@@ -362,9 +369,7 @@ bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status) {
   const bool force = std::any_of(std::begin(kTiles), std::end(kTiles), [&](const TileCost& t) { return forced(t) && usable(t); });
   // The kernel that would be done first. (How many tiles the groups' columns make is known on the device only: here every group that can
   // have a column ends with half a tile.)
-  Tile tile = Tile::k64x64;
-  int64_t blocks = 0;
-  float best = 0;
+  choice.direct = direct;
   for (const TileCost& t : kTiles) {
     if (!usable(t) || (force && !forced(t))) continue;
     const Timing timing = timing_of(t);
@@ -373,15 +378,30 @@ bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status) {
     const float all = tiles_m * tiles_n / (timing.per_cu * call.compute_units), full = std::floor(all);
     const float rounds = std::max(timing.last, full + (all > full ? timing.last + (1 - timing.last) * (all - full) : 0.0f));
     const float time = timing.fixed + rounds * (float(call.k) / kStep + timing.more) * timing.step;
-    if (blocks == 0 || time < best) {
-      best = time;
-      tile = t.tile;
-      blocks = blocks_of(t);
+    if (choice.blocks == 0 || time < choice.time) {
+      choice.time = time;
+      choice.tile = t.tile;
+      choice.blocks = blocks_of(t);
     }
   }
-  if (blocks == 0) return false;
-  *status = direct ? LaunchTile<true>(stream, call, tile, static_cast<unsigned>(blocks))
-                   : LaunchTile<false>(stream, call, tile, static_cast<unsigned>(blocks));
+  // Weights out of HBM, one matrix and one to each group.
+  const double bytes = double(busy) * call.m * (call.lhs.row_bytes + call.lhs.scale_stride);
+  choice.time = std::max(choice.time, 3.0f + static_cast<float>(bytes / (busy == 1 ? 3.9e6 : 4.5e6)));
+  return choice;
+}
+
+}  // namespace
+
+float TilesMicroseconds(const MulCall& call) {
+  const Choice choice = Choose(call);
+  return choice.blocks ? choice.time : -1;
+}
+
+bool LaunchTiles(hipStream_t stream, const MulCall& call, hipError_t* status) {
+  const Choice choice = Choose(call);
+  if (choice.blocks == 0) return false;
+  const unsigned blocks = static_cast<unsigned>(choice.blocks);
+  *status = choice.direct ? LaunchTile<true>(stream, call, choice.tile, blocks) : LaunchTile<false>(stream, call, choice.tile, blocks);
   return true;
 }
 

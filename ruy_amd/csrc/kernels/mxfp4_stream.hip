@@ -168,9 +168,11 @@ hipError_t Launch(hipStream_t stream, const StreamArgs& args, unsigned blocks, i
 }  // namespace
 
 bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
-  if (call.k < kBlock) return false;  // (a row has 16 bytes at least)
+  if (call.k < kBlock || call.forced_tile_rows) return false;  // (a row has 16 bytes at least)
   const int64_t busy = std::min(call.groups, call.n);
-  if (call.n > 32 * busy) return false;
+  // (More than a workgroup has tokens, or, as groups are mostly of many sizes, more than the largest of these would have: 64 experts
+  // of 2048 x 2048, us here and on tiles: 8 tokens to each in the mean 36.3 and 36.3, 16 42.4 and 39.1, 32 53 and 41.)
+  if (call.n > (busy > 1 ? 8 : 32) * busy) return false;
   if (call.k > 0x7fffffff - 2 * kChunk || call.m > 0x7fffffff - 128) return false;
   StreamArgs args;
   args.c = call;
@@ -196,6 +198,17 @@ bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
     row_waves *= 2;
     if (depth_waves * row_waves > kMostWaves) depth_waves /= 2;
   }
+  // About how long this takes, us: a launch, the weights at the rate of a stream, once to each lot of tokens, and a CU's workgroups putting
+  // their tokens into LDS. Tiles of many columns read the weights more slowly and go through no more of them for more tokens.
+  // (us, this and the fastest tiles: 2048 x 2048, 16 tokens 5.6 and 6.1; 32 7.5 and 6.1; 16384 x 4096, 4 tokens 12.1 and 10.4;
+  // 28672 x 8192, 4 tokens 28.3 and 35.1, 16 36.7 and 35.2; 8 experts of 4096 x 4096, 32 tokens 17.2 and 17.9.)
+  const int64_t lots = (call.n + busy * args.tokens - 1) / (busy * args.tokens);
+  const double weights = double(busy) * lots * call.m * (call.lhs.row_bytes + call.lhs.scale_stride);
+  const int64_t mean_tokens = std::min<int64_t>(args.tokens, (call.n + busy - 1) / busy);
+  const int64_t each_cu = (units * lots + int64_t(row_waves) * call.compute_units - 1) / (int64_t(row_waves) * call.compute_units);
+  const float time = 4.5f + static_cast<float>(weights / 5.2e6) + 2.65e-5f * float(each_cu * mean_tokens * (pitch + scale_pitch));
+  const float tiles = TilesMicroseconds(call);
+  if (tiles >= 0 && tiles < time) return false;
   args.depth_waves = depth_waves;
   args.row_waves = row_waves;
   const int work_rows = 16 * row_waves, waves = depth_waves * row_waves;
