@@ -168,11 +168,13 @@ hipError_t Launch(hipStream_t stream, const StreamArgs& args, unsigned blocks, i
 }  // namespace
 
 bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
-  if (call.k < kBlock || call.forced_tile_rows) return false;  // (a row has 16 bytes at least)
+  if (call.k < kBlock) return false;  // (a row has 16 bytes at least)
+  const bool forced = call.forced_tile_rows == 16 && call.forced_tile_cols == 16;
+  if (call.forced_tile_rows && !forced) return false;
   const int64_t busy = std::min(call.groups, call.n);
   // (More than a workgroup has tokens, or, as groups are mostly of many sizes, more than the largest of these would have: 64 experts
   // of 2048 x 2048, us here and on tiles: 8 tokens to each in the mean 36.3 and 36.3, 16 42.4 and 39.1, 32 53 and 41.)
-  if (call.n > (busy > 1 ? 8 : 32) * busy) return false;
+  if (!forced && call.n > (busy > 1 ? 8 : 32) * busy) return false;
   if (call.k > 0x7fffffff - 2 * kChunk || call.m > 0x7fffffff - 128) return false;
   StreamArgs args;
   args.c = call;
@@ -208,7 +210,7 @@ bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
   const int64_t each_cu = (units * lots + int64_t(row_waves) * call.compute_units - 1) / (int64_t(row_waves) * call.compute_units);
   const float time = 4.5f + static_cast<float>(weights / 5.2e6) + 2.65e-5f * float(each_cu * mean_tokens * (pitch + scale_pitch));
   const float tiles = TilesMicroseconds(call);
-  if (tiles >= 0 && tiles < time) return false;
+  if (!forced && tiles >= 0 && tiles < time) return false;
   args.depth_waves = depth_waves;
   args.row_waves = row_waves;
   const int work_rows = 16 * row_waves, waves = depth_waves * row_waves;

@@ -250,10 +250,10 @@ def run_mul(context, dst_type, m, n, k, offsets=None, pads=(0, 0, 0, 0), shift=0
         part = x[begin:end].t().contiguous()
         want = w @ part
         bound = None
-        if not exact:
-            bound = R.error_bound(w.abs() @ part.abs() + (b[i, :m, None].abs() if bias else 0), k, want, dst_type)
         if bias:
             want = want + b[i, :m, None].double()
+        if not exact:  # (what is rounded to dst's type has the bias in it: half a step of the whole)
+            bound = R.error_bound(w.abs() @ part.abs() + (b[i, :m, None].abs() if bias else 0), k, want, dst_type)
         if low is not None or high is not None:
             want = R.clamp(want, -np.inf if low is None else low, np.inf if high is None else high)
         got = dst.view()[:, begin:end]
@@ -311,6 +311,20 @@ def test_every_tile_at_every_end_of_the_depth(context, tile, k):
         run_mul(context, S.F32, 270, 300, k, np.array([0, 33, 33, 200, 300]), (16 - (k + 1) // 2 % 16, 3, 16 - (k + 1) // 2 % 16, 1), 0, 16,
                 COL, 0, True, 0.0, seed=1)
         run_mul(context, S.F16, 257, 513, k, None, (1, 0, 3, 0), 1, seed=2)
+    finally:
+        context.force_tile(0, 0)
+
+
+@pytest.mark.parametrize("k", [32, 33, 95, 480, 511, 512, 513, 1000, 2048, 3333, 4096, 4111, 16384, 40000])
+def test_streams(context, k):
+    """Fewer chunks than waves and more, cut short anywhere; one lot of tokens and several, as many as LDS has room for."""
+    context.force_tile(16, 16)
+    try:
+        for m, n in ((200, 1), (33, 20), (130, 70)):
+            run_mul(context, S.BF16, m, n, k, scales=(126, 128) if k <= 7281 else (120, 133), seed=n)
+            assert context.last_kernel_name() == "mxfp4_stream"
+        run_mul(context, S.F32, 97, 90, k, np.array([0, 33, 33, 40, 90]), (3, 1, 1, 2), 1, 5, COL, 1, True, 0.0, seed=1, scales=(120, 133))
+        run_mul(context, S.F16, 70, 40, k, None, (16, 4, 0, 1), 0, 0, ROW, 0, True, seed=2, scales=(124, 129))
     finally:
         context.force_tile(0, 0)
 
