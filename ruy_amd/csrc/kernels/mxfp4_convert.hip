@@ -106,9 +106,15 @@ __global__ __launch_bounds__(256) void QuantizeKernel(ConvertCall c, int segment
       for (int e = 0; e < 8; ++e) v[u][e] *= inverse;
       packed[u] = scale[u] == kNaNScale ? 0 : Round8(v[u]);
     }
+    // Lane 4 b + u stores the scale of unit u's block b.
+    int my_scale = scale[0];
+#pragma unroll
+    for (int u = 1; u < kUnits; ++u) my_scale = (lane & 3) == u ? scale[u] : my_scale;
+    const int64_t my_block = int64_t(piece.segment) * (16 * kUnits) + (lane & 3) * 16 + (lane >> 2);
     ForEachPlace(c, piece.row, [&](int row) __attribute__((always_inline)) {
       uint8_t* const data = c.matrix.data + row * c.matrix.row_bytes;
       uint8_t* const scales = c.matrix.scales + row * c.matrix.scale_stride;
+      if ((lane & 3) < kUnits && my_block * kBlock < cols) scales[my_block] = static_cast<uint8_t>(my_scale);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int64_t first = (unit0 + u * 64) * 8;
@@ -117,7 +123,6 @@ __global__ __launch_bounds__(256) void QuantizeKernel(ConvertCall c, int segment
         } else if (first < cols) {
           for (int b = 0; b < (cols - first + 1) / 2; ++b) data[first / 2 + b] = static_cast<uint8_t>(packed[u] >> (8 * b));
         }
-        if ((lane & 3) == 0 && first < cols) scales[first / kBlock] = static_cast<uint8_t>(scale[u]);
       }
     });
   }

@@ -157,77 +157,119 @@ __global__ __launch_bounds__(256) void CombineKernel(Call c, int segments) {
 
 // ---- The gradients of that sum ----
 
+// The lanes' values added up, in every lane, always in the same order: over 2, 4, 8 and 16 neighbours, then over the four rows of 16.
+template <int kExchange>
+__device__ __forceinline__ float Exchanged(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kExchange, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float WaveSum(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  return v;
+  v += Exchanged<0xb1>(v);   // lanes 1 0 3 2
+  v += Exchanged<0x4e>(v);   // lanes 2 3 0 1
+  v += Exchanged<0x141>(v);  // eight lanes backwards
+  v += Exchanged<0x140>(v);  // sixteen lanes backwards
+  const int w = __float_as_int(v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  v = __int_as_float(rows[0]) + __int_as_float(rows[1]);
+  const int x = __float_as_int(v);
+  const auto halves = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __int_as_float(halves[0]) + __int_as_float(halves[1]);
 }
 
 constexpr int kMostWaves = 8;
-constexpr int kDots = 8;  // choices of a token at a time
 
-// A workgroup to a token; its waves take units of 64 lanes in turn.
-template <int kType, int kGradType>
-__global__ __launch_bounds__(64 * kMostWaves) void GradientsKernel(Call c) {
-  constexpr int kValues = 16 / Bytes(kType);
+// `waves` waves to a token, whole tokens to a workgroup; the waves of a token take 64 * kUnits units in turn. kDots: choices at a time.
+template <int kType, int kGradType, int kDots, int kUnits>
+__global__ __launch_bounds__(64 * kMostWaves) void GradientsKernel(Call c, int waves) {
+  constexpr int kValues = 16 / Bytes(kType), kUnit = 64 * kValues;
   __shared__ float dots[kMostWaves][kDots];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, my_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tokens_here = (blockDim.x >> 6) / waves, wave = my_wave % waves;
   const bool rows = c.grad_src.data, weights = c.grad_weights.data;
-  for (int token = blockIdx.x; token < c.tokens; token += gridDim.x) {
+  for (int64_t token0 = int64_t(blockIdx.x) * tokens_here; token0 < c.tokens; token0 += int64_t(gridDim.x) * tokens_here) {
+    const int token = static_cast<int>(token0) + my_wave / waves;
+    const bool there = token < c.tokens;  // (all waves go through the barriers)
     for (int j0 = 0; j0 < c.top; j0 += kDots) {
       int place[kDots];
       float weight[kDots], dot[kDots] = {};
 #pragma unroll
       for (int j = 0; j < kDots; ++j) {
-        place[j] = j0 + j < c.top ? PlaceOf(c, token, j0 + j) : -1;
+        place[j] = there && j0 + j < c.top ? PlaceOf(c, token, j0 + j) : -1;
         weight[j] = place[j] >= 0 && rows ? WeightOf(c, token, j0 + j) : 0.0f;
       }
-      for (int64_t first = int64_t(wave) * (64 * kValues); first < c.width; first += int64_t(waves) * (64 * kValues)) {
-        const int64_t wanted = first + lane * kValues, at = min(wanted, int64_t(c.width) - kValues);
-        const int again = static_cast<int>(min(wanted - at, int64_t(kValues)));  // values that the lane before has
-        v4i grad[kValues * Bytes(kGradType) / 16], held[kDots][1];
-        Load<kGradType, kValues>(c.token_side.data, token * c.token_side.cs + at, grad);
+      for (int64_t first = int64_t(wave) * (kUnit * kUnits); there && first < c.width; first += int64_t(waves) * (kUnit * kUnits)) {
+        int64_t at[kUnits];
+        v4i grad[kUnits][kValues * Bytes(kGradType) / 16], held[kDots][kUnits][1];
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          at[u] = min(first + u * kUnit + lane * kValues, int64_t(c.width) - kValues);
+          if (first + u * kUnit < c.width) Load<kGradType, kValues>(c.token_side.data, token * c.token_side.cs + at[u], grad[u]);
+        }
         if (weights) {
 #pragma unroll
           for (int j = 0; j < kDots; ++j)
-            if (place[j] >= 0) Load<kType, kValues>(c.place_side.data, place[j] * c.place_side.cs + at, held[j]);
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u)
+              if (place[j] >= 0 && first + u * kUnit < c.width)
+                Load<kType, kValues>(c.place_side.data, place[j] * c.place_side.cs + at[u], held[j][u]);
         }
         if (rows) {
 #pragma unroll
           for (int j = 0; j < kDots; ++j) {
             if (place[j] < 0) continue;
-            float v[kValues];
 #pragma unroll
-            for (int e = 0; e < kValues; ++e) v[e] = weight[j] * Value<kGradType, kValues>(grad, e);
-            Store<kType, kValues>(c.grad_src.data, place[j] * c.grad_src.cs + at, v);
+            for (int u = 0; u < kUnits; ++u) {
+              if (first + u * kUnit >= c.width) continue;
+              float v[kValues];
+#pragma unroll
+              for (int e = 0; e < kValues; ++e) v[e] = weight[j] * Value<kGradType, kValues>(grad[u], e);
+              Store<kType, kValues>(c.grad_src.data, place[j] * c.grad_src.cs + at[u], v);
+            }
           }
         }
         if (weights) {
 #pragma unroll
-          for (int j = 0; j < kDots; ++j) {
-            if (place[j] < 0) continue;
+          for (int u = 0; u < kUnits; ++u) {
+            if (first + u * kUnit >= c.width) continue;
+            // (Values that the lane before has too.)
+            const int again = static_cast<int>(min(first + u * kUnit + lane * kValues - at[u], int64_t(kValues)));
+            float g[kValues];
 #pragma unroll
-            for (int e = 0; e < kValues; ++e) {
-              const float product = Value<kGradType, kValues>(grad, e) * Value<kType, kValues>(held[j], e);
-              dot[j] += e >= again ? product : 0.0f;
+            for (int e = 0; e < kValues; ++e) g[e] = Value<kGradType, kValues>(grad[u], e);
+#pragma unroll
+            for (int j = 0; j < kDots; ++j) {
+              if (place[j] < 0) continue;
+              if (first + (u + 1) * kUnit <= c.width) {  // (none)
+#pragma unroll
+                for (int e = 0; e < kValues; ++e) dot[j] += g[e] * Value<kType, kValues>(held[j][u], e);
+              } else {
+#pragma unroll
+                for (int e = 0; e < kValues; ++e) {
+                  const float product = g[e] * Value<kType, kValues>(held[j][u], e);
+                  dot[j] += e >= again ? product : 0.0f;
+                }
+              }
             }
           }
         }
       }
       if (!weights) continue;
+      float mine = 0;  // lane j's: choice j
 #pragma unroll
       for (int j = 0; j < kDots; ++j) {
+        if (j0 + j >= c.top) break;
         const float sum = WaveSum(dot[j]);
-        if (lane == 0) dots[wave][j] = sum;
+        mine = lane == j ? sum : mine;
       }
-      __syncthreads();
-      if (threadIdx.x < kDots && j0 + int(threadIdx.x) < c.top) {
-        float sum = 0;
-        for (int w = 0; w < waves; ++w) sum += dots[w][threadIdx.x];
-        const int j = j0 + threadIdx.x;
-        StoreFloat(c.grad_weights.data, c.grad_weights.type, j * c.grad_weights.rs + token * c.grad_weights.cs, sum);
+      if (waves > 1) {
+        if (lane < kDots) dots[my_wave][lane] = mine;
+        __syncthreads();
+        mine = 0;
+        if (wave == 0 && lane < kDots)
+          for (int w = 0; w < waves; ++w) mine += dots[my_wave + w][lane];
+        __syncthreads();
       }
-      __syncthreads();
+      if (there && wave == 0 && lane < kDots && j0 + lane < c.top)
+        StoreFloat(c.grad_weights.data, c.grad_weights.type, (j0 + lane) * c.grad_weights.rs + token * c.grad_weights.cs, mine);
     }
   }
 }
@@ -371,11 +413,20 @@ bool LaunchGradients(hipStream_t stream, const Call& c, int compute_units, hipEr
   const int type = c.place_side.type;
   if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side) || !SideBySide(c, c.grad_src))
     return false;
+  // Waves to a token: as few as leave every CU 16, each with a unit at least.
   const int64_t units = (c.width + 64 * (16 / Bytes(type)) - 1) / (64 * (16 / Bytes(type)));
-  const int waves = static_cast<int>(std::min<int64_t>(units, kMostWaves));
+  int waves = 1;
+  while (waves < kMostWaves && waves < units && int64_t(c.tokens) * waves < int64_t(16) * compute_units) waves *= 2;
+  const int block = std::max(waves, 4);
+  const dim3 grid(BlocksFor(int64_t(c.tokens) * waves, block)), threads(64 * block);
   WithTypes(type, c.token_side.type, [&](auto t, auto grad) {
-    hipLaunchKernelGGL((GradientsKernel<decltype(t)::value, decltype(grad)::value>), dim3(BlocksFor(c.tokens, 1)), dim3(64 * waves),
-                       0, stream, c);
+    constexpr int kType = decltype(t)::value, kGrad = decltype(grad)::value;
+    if (c.top <= 2)
+      hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 2, 2>), grid, threads, 0, stream, c, waves);
+    else if (c.top <= 4)
+      hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 4, 2>), grid, threads, 0, stream, c, waves);
+    else
+      hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 8, 1>), grid, threads, 0, stream, c, waves);
   });
   *status = hipGetLastError();
   return true;
