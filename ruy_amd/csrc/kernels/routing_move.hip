@@ -43,7 +43,15 @@ __device__ __forceinline__ float Value(const v4i (&raw)[kValues * Bytes(kType) /
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(e % 2 ? word >> 16 : word)));
   }
 }
-template <int kType, int kValues>
+// kStreamed: past the caches, for what is more than they hold anyway (kStreamFrom).
+template <bool kStreamed>
+__device__ __forceinline__ void StoreGranule(v4i_unaligned* p, const v4i& x) {
+  if constexpr (kStreamed)
+    __builtin_nontemporal_store(x, p);
+  else
+    *p = x;
+}
+template <int kType, int kValues, bool kStreamed = false>
 __device__ __forceinline__ void Store(void* data, int64_t at, const float (&v)[kValues]) {
   v4i_unaligned* const p = reinterpret_cast<v4i_unaligned*>(static_cast<char*>(data) + at * Bytes(kType));
 #pragma unroll
@@ -56,7 +64,7 @@ __device__ __forceinline__ void Store(void* data, int64_t at, const float (&v)[k
       else
         raw[e] = RoundPair<kType>(v[2 * e], v[2 * e + 1]);
     }
-    p[i] = raw;
+    StoreGranule<kStreamed>(p + i, raw);
   }
 }
 
@@ -86,7 +94,7 @@ constexpr int kAtOnce = 4;  // choices of a token whose rows are on their way to
 
 // ---- Tokens to their places ----
 
-template <int kBytes, int kUnits>
+template <int kBytes, int kUnits, bool kStreamed>
 __global__ __launch_bounds__(256) void DispatchKernel(Call c, int segments) {
   const int lane = threadIdx.x & 63;
   const int64_t bytes = int64_t(c.width) * kBytes, pieces = int64_t(c.tokens) * segments;
@@ -107,14 +115,14 @@ __global__ __launch_bounds__(256) void DispatchKernel(Call c, int segments) {
       char* const to = static_cast<char*>(c.place_side.data) + place * c.place_side.cs * kBytes;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u)
-        if (first + u * 1024 < bytes) *reinterpret_cast<v4i_unaligned*>(to + at[u]) = held[u];
+        if (first + u * 1024 < bytes) StoreGranule<kStreamed>(reinterpret_cast<v4i_unaligned*>(to + at[u]), held[u]);
     }
   }
 }
 
 // ---- The sum of a token's rows ----
 
-template <int kType, int kDstType, int kUnits>
+template <int kType, int kDstType, int kUnits, bool kStreamed>
 __global__ __launch_bounds__(256) void CombineKernel(Call c, int segments) {
   constexpr int kValues = 16 / Bytes(kType);
   const int lane = threadIdx.x & 63;
@@ -151,7 +159,7 @@ __global__ __launch_bounds__(256) void CombineKernel(Call c, int segments) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
       if (first + u * 64 * kValues < c.width)
-        Store<kDstType, kValues>(c.token_side.data, piece.token * c.token_side.cs + at[u], sum[u]);
+        Store<kDstType, kValues, kStreamed>(c.token_side.data, piece.token * c.token_side.cs + at[u], sum[u]);
   }
 }
 
@@ -369,6 +377,16 @@ void WithUnits(const Call& c, int type, int compute_units, F&& f) {
   f(std::integral_constant<int, 1>(), int(segments(1)), blocks(segments(1)));
 }
 
+// Bytes written from which on they go past the caches: 32 MiB, which is what all L2s hold. (us, tokens of 4096 values in bfloat16 and two
+// places each, 17, 34, 67 and 134 MB dispatched: 6.7 10.1 24.3 41.8, past them 5.5 9.0 16.7 32.7; combined, 8, 17, 34 and 67 MB: 6.4 9.6 22.8
+// 41.5, past them 5.9 9.6 17.3 37.9; combined and dispatched again, 2048 tokens 18.8 and 21.0, 4096 44.7 and 40.0.)
+constexpr int64_t kStreamFrom = int64_t(1) << 25;
+template <class F>
+void WithStores(int64_t bytes, F&& f) {
+  if (bytes >= kStreamFrom) return f(std::true_type());
+  f(std::false_type());
+}
+
 // f(type of the rows, other type): the other is the rows' or fp32.
 template <class F>
 void WithTypes(int type, int other, F&& f) {
@@ -387,10 +405,13 @@ bool LaunchDispatch(hipStream_t stream, const Call& c, int compute_units, hipErr
   if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side)) return false;
   WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
     constexpr int kUnits = decltype(units)::value;
-    if (type == RUYAMD_DTYPE_F32)
-      hipLaunchKernelGGL((DispatchKernel<4, kUnits>), dim3(blocks), dim3(256), 0, stream, c, segments);
-    else
-      hipLaunchKernelGGL((DispatchKernel<2, kUnits>), dim3(blocks), dim3(256), 0, stream, c, segments);
+    WithStores(int64_t(c.tokens) * c.top * c.width * Bytes(type), [&](auto streamed) {
+      constexpr bool kStreamed = decltype(streamed)::value;
+      if (type == RUYAMD_DTYPE_F32)
+        hipLaunchKernelGGL((DispatchKernel<4, kUnits, kStreamed>), dim3(blocks), dim3(256), 0, stream, c, segments);
+      else
+        hipLaunchKernelGGL((DispatchKernel<2, kUnits, kStreamed>), dim3(blocks), dim3(256), 0, stream, c, segments);
+    });
   });
   *status = hipGetLastError();
   return true;
@@ -401,8 +422,10 @@ bool LaunchCombine(hipStream_t stream, const Call& c, int compute_units, hipErro
   if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side)) return false;
   WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
     WithTypes(type, c.token_side.type, [&](auto t, auto dst) {
-      hipLaunchKernelGGL((CombineKernel<decltype(t)::value, decltype(dst)::value, decltype(units)::value>), dim3(blocks), dim3(256),
-                         0, stream, c, segments);
+      constexpr int kType = decltype(t)::value, kDst = decltype(dst)::value, kUnits = decltype(units)::value;
+      WithStores(int64_t(c.tokens) * c.width * Bytes(kDst), [&](auto streamed) {
+        hipLaunchKernelGGL((CombineKernel<kType, kDst, kUnits, decltype(streamed)::value>), dim3(blocks), dim3(256), 0, stream, c, segments);
+      });
     });
   });
   *status = hipGetLastError();

@@ -12,6 +12,7 @@
 // where its places will be (a part has as many choices as there are experts, or more): no other memory is needed.
 #include <algorithm>
 
+#include "grouped_gemm.h"
 #include "launch_geometry.h"
 #include "routing.h"
 
@@ -19,20 +20,39 @@ namespace ruyamd {
 namespace routing {
 namespace {
 
-// The expert of choice i, or -1.
+// What stands for the expert of a choice that has none, and for that of a choice behind the last.
+constexpr uint32_t kNone = 0xffffffffu, kPast = 0xfffffffeu;
+
+// The expert of choice i, or kNone.
 template <bool kWide, bool kPlain>
-__device__ __forceinline__ int NumberOf(const SortCall& c, int i) {
+__device__ __forceinline__ uint32_t NumberOf(const SortCall& c, int64_t i) {
   int64_t at = i;
   if constexpr (!kPlain) {
     const int t = static_cast<int>(uint32_t(i) / uint32_t(c.top));
-    at = t * c.cs + (i - t * c.top) * c.rs;
+    at = t * c.cs + (i - int64_t(t) * c.top) * c.rs;
   }
   if constexpr (kWide) {
-    const int64_t v = static_cast<const int64_t*>(c.experts)[at];
-    return v >= 0 && v < c.count ? static_cast<int>(v) : -1;
+    const uint2 v = static_cast<const uint2*>(c.experts)[at];
+    return v.y == 0 && v.x < uint32_t(c.count) ? v.x : kNone;
   } else {
-    const int v = static_cast<const int32_t*>(c.experts)[at];
-    return v >= 0 && v < c.count ? v : -1;
+    const uint32_t v = static_cast<const uint32_t*>(c.experts)[at];
+    return v < uint32_t(c.count) ? v : kNone;
+  }
+}
+// Those of the lane in kAtOnce rows of 64 from `at` on, of choices in front of `end`.
+constexpr int kAtOnce = 8;
+template <bool kWide, bool kPlain>
+__device__ __forceinline__ void NumbersOf(const SortCall& c, int64_t at, int64_t end, int lane, uint32_t (&v)[kAtOnce]) {
+  if (at + 64 * kAtOnce <= end) {
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) v[u] = NumberOf<kWide, kPlain>(c, at + lane + u * 64);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int64_t mine = at + lane + u * 64;
+      v[u] = NumberOf<kWide, kPlain>(c, min(mine, end - 1));
+      if (mine >= end) v[u] = kPast;
+    }
   }
 }
 
@@ -47,7 +67,7 @@ __device__ __forceinline__ int WaveSum(int v) {
 }
 
 constexpr int kMostWaves = 16;
-constexpr int kAtOnce = 8;  // loads of a lane on their way together
+constexpr int kHeld = 32 * 64;  // choices that a wave looks at before it counts on, a bit of each lane to each 64
 
 // Expert blockIdx.x; every wave has a contiguous part of the choices.
 template <bool kWide, bool kPlain>
@@ -58,25 +78,29 @@ __global__ __launch_bounds__(64 * kMostWaves) void SortByExpertKernel(SortCall c
   const int n = c.tokens * c.top, expert = blockIdx.x;
   const int64_t part = (int64_t(n) + 64 * waves - 1) / (64 * waves) * 64;
   const int64_t begin = wave * part, end = min(int64_t(n), begin + part);
-  // Which of the lane's first 32 choices are the expert's: a part of no more is read once.
-  uint32_t held = 0;
+  // Which of the lane's 32 choices of kHeld from `at` on are the expert's. first: the first time that they are looked at.
   int lower_here = 0, own_here = 0;
-  for (int64_t at = begin, i = 0; at < end; at += 64 * kAtOnce, i += kAtOnce) {
-    int v[kAtOnce];
+  const auto look = [&](int64_t at, bool first) __attribute__((always_inline)) -> uint32_t {
+    uint32_t held = 0;
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int64_t mine = at + u * 64 + lane;
-      v[u] = NumberOf<kWide, kPlain>(c, static_cast<int>(min(mine, end - 1)));
-      if (mine >= end) v[u] = 0x7fffffff;
-    }
+    for (int b = 0; b < 32 / kAtOnce; ++b) {
+      const int64_t from = at + b * (64 * kAtOnce);
+      if (from >= end) break;
+      uint32_t v[kAtOnce];
+      NumbersOf<kWide, kPlain>(c, from, end, lane, v);
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      lower_here += uint32_t(v[u]) < uint32_t(expert);
-      own_here += v[u] == expert;
-      if (i + u < 32) held |= uint32_t(v[u] == expert) << (i + u);
-      if (expert == 0 && v[u] < 0) c.places[at + u * 64 + lane] = -1;
+      for (int u = 0; u < kAtOnce; ++u) {
+        held |= uint32_t(v[u] == uint32_t(expert)) << (b * kAtOnce + u);
+        if (!first) continue;
+        lower_here += v[u] < uint32_t(expert);
+        if (expert == 0 && v[u] == kNone) c.places[from + u * 64 + lane] = -1;
+      }
     }
-  }
+    if (first) own_here += __builtin_popcount(held);
+    return held;
+  };
+  const uint32_t first_held = look(begin, true);
+  for (int64_t at = begin + kHeld; at < end; at += kHeld) look(at, true);
   lower_here = WaveSum(lower_here);
   own_here = WaveSum(own_here);
   if (lane == 0) {
@@ -96,17 +120,36 @@ __global__ __launch_bounds__(64 * kMostWaves) void SortByExpertKernel(SortCall c
   }
   if (expert == c.count - 1 && c.sources)
     for (int64_t p = int64_t(first) + total + threadIdx.x; p < n; p += blockDim.x) c.sources[p] = -1;
-  next += first;
-  for (int64_t at = begin, i = 0; at < end; at += 64, ++i) {
-    const int64_t mine = at + lane;
-    const bool is = i < 32 ? held >> i & 1 : mine < end && NumberOf<kWide, kPlain>(c, static_cast<int>(mine)) == expert;
-    const uint64_t all = __ballot(is);
-    if (is) {
-      const int place = next + BelowMe(all);
-      c.places[mine] = place;
-      if (c.sources) c.sources[place] = static_cast<int>(mine);
+  next = __builtin_amdgcn_readfirstlane(next + first);
+  for (int64_t at = begin; at < end; at += kHeld) {
+    uint32_t held = at == begin ? first_held : look(at, false);
+    // Lane i has, of the 64 choices number i, which are the expert's and how many places are taken before them. A
+    // lane then goes through its own choices only: few, where there are many experts.
+    uint32_t low = 0, high = 0;
+#pragma unroll
+    for (int b = 0; b < 32 / kAtOnce; ++b) {
+      if (at + b * (64 * kAtOnce) >= end) break;
+#pragma unroll
+      for (int i = b * kAtOnce; i < (b + 1) * kAtOnce; ++i) {
+        const uint64_t all = __ballot(held >> i & 1);
+        low = lane == i ? static_cast<uint32_t>(all) : low;
+        high = lane == i ? static_cast<uint32_t>(all >> 32) : high;
+      }
     }
-    next += __builtin_popcountll(all);
+    const int here = __builtin_popcount(low) + __builtin_popcount(high), upto = grouped::InclusiveSum(here);
+    const int before = next + upto - here;
+    next += __builtin_amdgcn_readlane(upto, 63);
+    while (__any(held != 0)) {
+      const int i = held ? __builtin_ctz(held) : 0;
+      const uint32_t l = __shfl(low, i), h = __shfl(high, i);
+      const int place = __builtin_amdgcn_mbcnt_hi(h, __builtin_amdgcn_mbcnt_lo(l, __shfl(before, i)));
+      if (held) {
+        const int64_t mine = at + i * 64 + lane;
+        c.places[mine] = place;
+        if (c.sources) c.sources[place] = static_cast<int>(mine);
+      }
+      held &= held - 1;
+    }
   }
 }
 
@@ -123,16 +166,11 @@ __global__ __launch_bounds__(64) void CountKernel(SortCall c, Parts parts) {
   for (int e = lane; e < c.count; e += 64) counts[e] = 0;
   __syncthreads();
   for (int64_t at = begin; at < end; at += 64 * kAtOnce) {
-    int v[kAtOnce];
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int64_t mine = at + u * 64 + lane;
-      v[u] = NumberOf<kWide, kPlain>(c, static_cast<int>(min(mine, int64_t(end) - 1)));
-      if (mine >= end) v[u] = -1;
-    }
+    uint32_t v[kAtOnce];
+    NumbersOf<kWide, kPlain>(c, at, end, lane, v);
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u)
-      if (v[u] >= 0) atomicAdd(&counts[v[u]], 1);  // (a sum of ones: any order)
+      if (v[u] < kPast) atomicAdd(&counts[v[u]], 1);  // (a sum of ones: any order)
   }
   __syncthreads();
   for (int e = lane; e < c.count; e += 64) c.places[begin + e] = counts[e];
@@ -202,15 +240,15 @@ __global__ __launch_bounds__(64) void PlaceKernel(SortCall c, Parts parts, int b
   const int used = c.offsets[c.count];
   for (int64_t at = begin; at < end; at += 64) {
     const int64_t mine = at + lane;
-    const int v = mine < end ? NumberOf<kWide, kPlain>(c, static_cast<int>(mine)) : -1;
-    uint64_t same = __ballot(v >= 0);
+    const uint32_t v = mine < end ? NumberOf<kWide, kPlain>(c, mine) : kPast;
+    uint64_t same = __ballot(v < kPast);
     for (int bit = 0; bit < bits; ++bit) {
       const bool set = v >> bit & 1;
       const uint64_t with = __ballot(set);
       same &= set ? with : ~with;
     }
     int place = -1;
-    if (v >= 0) {
+    if (v < kPast) {
       const int rank = BelowMe(same);
       place = next[v] + rank;
       __builtin_amdgcn_wave_barrier();
