@@ -48,15 +48,17 @@ __device__ __forceinline__ void ForEachPlace(const ConvertCall& c, int row, F&& 
   }
 }
 
-// Unit u's 8 values of a row; those behind the row's end are 0.
+// 8 values as they lie, and as numbers.
 template <int kType>
-__device__ __forceinline__ void LoadUnit(const char* row, int64_t first, int cols, float (&v)[8]) {
-  constexpr int kGranules = 8 * Bytes(kType) / 16;
-  if (first + 8 <= cols) {
-    v4i raw[kGranules];
+struct Unit {
+  static constexpr int kGranules = 8 * Bytes(kType) / 16;
+  v4i raw[kGranules];
+
+  __device__ __forceinline__ void Load(const char* row, int64_t first) {
 #pragma unroll
-    for (int i = 0; i < kGranules; ++i)
-      raw[i] = reinterpret_cast<const v4i_unaligned*>(row + first * Bytes(kType))[i];
+    for (int i = 0; i < kGranules; ++i) raw[i] = reinterpret_cast<const v4i_unaligned*>(row + first * Bytes(kType))[i];
+  }
+  __device__ __forceinline__ void Values(float (&v)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (kType == RUYAMD_DTYPE_F32) {
@@ -69,11 +71,21 @@ __device__ __forceinline__ void LoadUnit(const char* row, int64_t first, int col
           v[e] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(e % 2 ? word >> 16 : word)));
       }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = first + e < cols ? LoadFloat(row, kType, first + e) : 0.0f;
   }
-}
+  __device__ __forceinline__ void Store(char* row, int64_t first, const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < kGranules; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (kType == RUYAMD_DTYPE_F32)
+          raw[i][e] = __float_as_int(v[i * 4 + e]);
+        else
+          raw[i][e] = RoundPair<kType>(v[2 * e], v[2 * e + 1]);
+      }
+      reinterpret_cast<v4i_unaligned*>(row + first * Bytes(kType))[i] = raw[i];
+    }
+  }
+};
 
 // The largest over each four neighbouring lanes.
 __device__ __forceinline__ uint32_t LargestOfFour(uint32_t v) {
@@ -90,11 +102,37 @@ __global__ __launch_bounds__(256) void QuantizeKernel(ConvertCall c, int segment
     const Piece piece = PieceOf(i, segments);
     const char* const from = static_cast<const char*>(c.data) + piece.row * c.rs * Bytes(kType);
     const int64_t unit0 = int64_t(piece.segment) * (64 * kUnits) + lane;
+    // (All of the segment inside the row, the same for all lanes: its loads go out together.)
+    const bool whole = (int64_t(piece.segment) + 1) * (512 * kUnits) <= cols;
     float v[kUnits][8];
     uint32_t packed[kUnits];
     int scale[kUnits];
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) LoadUnit<kType>(from, (unit0 + u * 64) * 8, cols, v[u]);
+    for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[u][e] = 0;
+    }
+    if (whole) {
+      Unit<kType> held[kUnits];
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) held[u].Load(from, (unit0 + u * 64) * 8);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) held[u].Values(v[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int64_t first = (unit0 + u * 64) * 8;
+        if (first + 8 <= cols) {
+          Unit<kType> held;
+          held.Load(from, first);
+          held.Values(v[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (first + e < cols) v[u][e] = LoadFloat(from, kType, first + e);
+        }
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       uint32_t largest = 0;
@@ -118,7 +156,7 @@ __global__ __launch_bounds__(256) void QuantizeKernel(ConvertCall c, int segment
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int64_t first = (unit0 + u * 64) * 8;
-        if (first + 8 <= cols) {
+        if (whole || first + 8 <= cols) {
           *reinterpret_cast<u32_unaligned*>(data + first / 2) = packed[u];
         } else if (first < cols) {
           for (int b = 0; b < (cols - first + 1) / 2; ++b) data[first / 2 + b] = static_cast<uint8_t>(packed[u] >> (8 * b));
@@ -138,18 +176,28 @@ __global__ __launch_bounds__(256) void DequantizeKernel(ConvertCall c, int segme
     const uint8_t* const scales = c.matrix.scales + piece.row * c.matrix.scale_stride;
     char* const to = static_cast<char*>(c.data) + piece.row * c.rs * Bytes(kType);
     const int64_t unit0 = int64_t(piece.segment) * (64 * kUnits) + lane;
+    const bool whole = (int64_t(piece.segment) + 1) * (512 * kUnits) <= cols;
     uint32_t packed[kUnits];
     int scale[kUnits];
+    if (whole) {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int64_t first = (unit0 + u * 64) * 8;
-      packed[u] = 0;
-      scale[u] = first < cols ? scales[first / kBlock] : 0;
-      if (first + 8 <= cols)
+      for (int u = 0; u < kUnits; ++u) {
+        const int64_t first = (unit0 + u * 64) * 8;
+        scale[u] = scales[first / kBlock];
         packed[u] = *reinterpret_cast<const u32_unaligned*>(data + first / 2);
-      else
-        for (int b = 0; b < 4; ++b)
-          if (first + 2 * b < cols) packed[u] |= uint32_t(data[first / 2 + b]) << (8 * b);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int64_t first = (unit0 + u * 64) * 8;
+        packed[u] = 0;
+        scale[u] = first < cols ? scales[first / kBlock] : 0;
+        if (first + 8 <= cols)
+          packed[u] = *reinterpret_cast<const u32_unaligned*>(data + first / 2);
+        else
+          for (int b = 0; b < 4; ++b)
+            if (first + 2 * b < cols) packed[u] |= uint32_t(data[first / 2 + b]) << (8 * b);
+      }
     }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
@@ -158,20 +206,9 @@ __global__ __launch_bounds__(256) void DequantizeKernel(ConvertCall c, int segme
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = ValueOf(packed[u] >> (4 * e) & 15) * power;
-      if (first + 8 <= cols) {
-        v4i_unaligned* const p = reinterpret_cast<v4i_unaligned*>(to + first * Bytes(kType));
-#pragma unroll
-        for (int i = 0; i < 8 * Bytes(kType) / 16; ++i) {
-          v4i raw;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (kType == RUYAMD_DTYPE_F32)
-              raw[e] = __float_as_int(v[i * 4 + e]);
-            else
-              raw[e] = RoundPair<kType>(v[2 * e], v[2 * e + 1]);
-          }
-          p[i] = raw;
-        }
+      if (whole || first + 8 <= cols) {
+        Unit<kType> held;
+        held.Store(to, first, v);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)

@@ -90,7 +90,6 @@ __device__ __forceinline__ float WeightOf(const Call& c, int token, int j) {
   return c.weights.data ? LoadFloat(c.weights.data, c.weights.type, j * c.weights.rs + token * c.weights.cs) : 1.0f;
 }
 
-constexpr int kAtOnce = 4;  // choices of a token whose rows are on their way together
 
 // ---- Tokens to their places ----
 
@@ -125,6 +124,7 @@ __global__ __launch_bounds__(256) void DispatchKernel(Call c, int segments) {
 template <int kType, int kDstType, int kUnits, bool kStreamed>
 __global__ __launch_bounds__(256) void CombineKernel(Call c, int segments) {
   constexpr int kValues = 16 / Bytes(kType);
+  constexpr int kAtOnce = 4;  // choices of a token whose rows are on their way together
   const int lane = threadIdx.x & 63;
   const int64_t pieces = int64_t(c.tokens) * segments;
   for (int64_t i = FirstPiece(); i < pieces; i += PieceStride()) {
@@ -186,7 +186,7 @@ __device__ __forceinline__ float WaveSum(float v) {
 constexpr int kMostWaves = 8;
 
 // `waves` waves to a token, whole tokens to a workgroup; the waves of a token take 64 * kUnits units in turn. kDots: choices at a time.
-template <int kType, int kGradType, int kDots, int kUnits>
+template <int kType, int kGradType, int kDots, int kUnits, bool kStreamed>
 __global__ __launch_bounds__(64 * kMostWaves) void GradientsKernel(Call c, int waves) {
   constexpr int kValues = 16 / Bytes(kType), kUnit = 64 * kValues;
   __shared__ float dots[kMostWaves][kDots];
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void GradientsKernel(Call c, int w
               float v[kValues];
 #pragma unroll
               for (int e = 0; e < kValues; ++e) v[e] = weight[j] * Value<kGradType, kValues>(grad[u], e);
-              Store<kType, kValues>(c.grad_src.data, place[j] * c.grad_src.cs + at[u], v);
+              Store<kType, kValues, kStreamed>(c.grad_src.data, place[j] * c.grad_src.cs + at[u], v);
             }
           }
         }
@@ -444,12 +444,15 @@ bool LaunchGradients(hipStream_t stream, const Call& c, int compute_units, hipEr
   const dim3 grid(BlocksFor(int64_t(c.tokens) * waves, block)), threads(64 * block);
   WithTypes(type, c.token_side.type, [&](auto t, auto grad) {
     constexpr int kType = decltype(t)::value, kGrad = decltype(grad)::value;
-    if (c.top <= 2)
-      hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 2, 2>), grid, threads, 0, stream, c, waves);
-    else if (c.top <= 4)
-      hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 4, 2>), grid, threads, 0, stream, c, waves);
-    else
-      hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 8, 1>), grid, threads, 0, stream, c, waves);
+    WithStores(c.grad_src.data ? int64_t(c.tokens) * c.top * c.width * Bytes(kType) : 0, [&](auto streamed) {
+      constexpr bool kStreamed = decltype(streamed)::value;
+      if (c.top <= 2)
+        hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 2, 2, kStreamed>), grid, threads, 0, stream, c, waves);
+      else if (c.top <= 4)
+        hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 4, 2, kStreamed>), grid, threads, 0, stream, c, waves);
+      else
+        hipLaunchKernelGGL((GradientsKernel<kType, kGrad, 8, 1, kStreamed>), grid, threads, 0, stream, c, waves);
+    });
   });
   *status = hipGetLastError();
   return true;
