@@ -4,12 +4,15 @@ Every token goes to `top` of the experts, y = sum over them of gate * W2 relu(W1
 
   python examples/expert_layer.py [--experts 16] [--width 512] [--hidden 1024] [--tokens 2048]
 
-Training: the tokens are put in the order of their experts once a step; W1, W2 and both
-gradients of either are then one product each (ruyamd_mul_grouped with the weights
-as they lie, and transposed; ruyamd_mul_grouped_depth), whatever the experts' shares are.
-The offsets stay on the device: nothing in a step waits for it. Serving: the weights
-in 4 bits, a scale and a zero point to every 64 of a row (ruyamd_mul_int4), a few
-tokens at a time.
+Training: the router's choices are sorted by expert (ruyamd_sort_tokens) and the tokens put
+in their places (ruyamd_dispatch_tokens); W1, W2 and both gradients of either are then
+one product each (ruyamd_mul_grouped with the weights as they lie, and transposed;
+ruyamd_mul_grouped_depth), whatever the experts' shares are; the answers are weighted and
+added up (ruyamd_combine_tokens), and so are gradients on their way back
+(ruyamd_combine_tokens_gradients). The offsets stay on the device: nothing in a step waits for
+it. Serving: the weights in 4 bits, a scale and a zero point to every 64 of a row
+(ruyamd_mul_int4), a few tokens at a time; or weights and tokens both in 4-bit floats
+(ruyamd_quantize_mxfp4, ruyamd_mul_mxfp4), any number at a time.
 """
 import argparse
 import os
@@ -21,7 +24,7 @@ sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."
 from ruy_amd import _structs as S  # noqa: E402
 from ruy_amd import api  # noqa: E402
 
-DTYPES = {torch.bfloat16: S.BF16, torch.float16: S.F16, torch.float32: S.F32}
+DTYPES = {torch.bfloat16: S.BF16, torch.float16: S.F16, torch.float32: S.F32, torch.int64: S.I64}
 
 
 def by_columns(t):
@@ -41,23 +44,67 @@ def params(dtype, bias=None, relu=False):
     return p
 
 
+_contexts = {}
+
+
+def shared_context():
+    """The context of calls that belong to no layer: on torch's current stream, without waiting."""
+    stream = torch.cuda.current_stream().cuda_stream
+    if stream not in _contexts:
+        _contexts[stream] = api.Context()
+        _contexts[stream].set_stream(stream)
+        _contexts[stream].set_synchronous(False)
+    return _contexts[stream]
+
+
 class Routing:
-    """Which expert each of a batch's tokens goes to, in the order of the experts."""
+    """Which experts each of a batch's tokens goes to, and its places in their order."""
 
     def __init__(self, scores, top):
-        gate, expert = torch.topk(torch.softmax(scores.float(), dim=1), top, dim=1)
-        experts = scores.shape[1]
-        order = torch.argsort(expert.flatten(), stable=True)
-        self.token = order // top
-        self.gate = gate.flatten()[order]
-        edges = torch.arange(experts + 1, device=scores.device)
-        self.offsets = torch.searchsorted(expert.flatten()[order].contiguous(), edges).int()
-        self.groups = api.Groups(self.offsets, experts)
+        self.gates, choices = torch.topk(torch.softmax(scores.float(), dim=1), top, dim=1)
+        self.gates, choices = self.gates.contiguous(), choices.contiguous()
+        tokens, experts = scores.shape
+        ints = dict(dtype=torch.int32, device=scores.device)
+        self.offsets = torch.empty(experts + 1, **ints)
+        self.places, self.sources = torch.empty(tokens, top, **ints), torch.empty(tokens * top, **ints)
+        self.routing = api.Routing(tokens, top, experts, self.offsets, self.places, self.sources)
+        api.sort_tokens(by_columns(choices), self.routing, shared_context())
+        self.groups = self.routing.groups()
+
+    @property
+    def token(self):
+        """The token of each place."""
+        return self.sources.long() // self.routing.top
+
+    @property
+    def gate(self):
+        """The weight of each place."""
+        return self.gates.flatten()[self.sources.long()]
+
+    def dispatch(self, x):
+        """The tokens in their places."""
+        chosen = torch.empty(self.sources.numel(), x.shape[1], dtype=x.dtype, device=x.device)
+        api.dispatch_tokens(by_columns(x), self.routing, shared_context(), by_columns(chosen))
+        return chosen
 
     def join(self, y, count):
         """The experts' answers to each of `count` tokens, weighted and added up."""
-        out = torch.zeros(count, y.shape[1], dtype=torch.float32, device=y.device)
-        return out.index_add_(0, self.token, y.float() * self.gate[:, None])
+        out = torch.empty(count, y.shape[1], dtype=torch.float32, device=y.device)
+        api.combine_tokens(by_columns(y), self.routing, by_columns(self.gates), shared_context(), by_columns(out))
+        return out
+
+    def join_gradients(self, grad, y):
+        """From the gradient of join's result those of y and of the gates."""
+        grad_y, grad_gates = torch.empty_like(y), torch.empty_like(self.gates)
+        api.combine_tokens_gradients(by_columns(grad), by_columns(y), self.routing, by_columns(self.gates), shared_context(),
+                                     by_columns(grad_y), by_columns(grad_gates))
+        return grad_y, grad_gates
+
+    def dispatch_gradient(self, grad_chosen):
+        """From the gradient of dispatch's result that of the tokens."""
+        grad_x = torch.empty(self.routing.tokens, grad_chosen.shape[1], dtype=torch.float32, device=grad_chosen.device)
+        api.combine_tokens(by_columns(grad_chosen), self.routing, None, shared_context(), by_columns(grad_x))
+        return grad_x
 
 
 class Experts:
@@ -78,7 +125,7 @@ class Experts:
     def forward(self, x, routing):
         """The experts' answers, one row to each token and expert it goes to."""
         w1, w2 = self.w1.to(self.dtype), self.w2.to(self.dtype)
-        chosen = x.to(self.dtype)[routing.token]
+        chosen = routing.dispatch(x.to(self.dtype))
         n = chosen.shape[0]
         h = torch.empty(n, w1.shape[1], dtype=self.dtype, device="cuda")
         y = torch.empty(n, w2.shape[1], dtype=self.dtype, device="cuda")
@@ -113,7 +160,7 @@ class Experts:
         """One step of gradient descent on the mean squared error; the loss before it."""
         y, kept = self.forward(x, routing)
         error = routing.join(y, x.shape[0]) - target
-        grad_y = (error * (2.0 / error.numel()))[routing.token] * routing.gate[:, None]
+        grad_y, _ = routing.join_gradients(error * (2.0 / error.numel()), y)
         _, grad_w1, grad_b1, grad_w2 = self.backward(grad_y, kept, routing)
         self.w1 -= rate * grad_w1
         self.b1 -= rate * grad_b1
@@ -146,13 +193,54 @@ class Server:
         self.w2, self.w2_values = quantize(trained.w2, group_size)
 
     def answer(self, x, routing):
-        chosen = x.to(self.dtype)[routing.token]
+        chosen = routing.dispatch(x.to(self.dtype))
         n = chosen.shape[0]
         h = torch.empty(n, self.w1.rows, dtype=self.dtype, device="cuda")
         y = torch.empty(n, self.w2.rows, dtype=self.dtype, device="cuda")
         api.mul_int4(self.w1, by_columns(chosen), params(self.dtype, self.b1, relu=True), self.context, by_columns(h),
                      routing.groups)
         api.mul_int4(self.w2, by_columns(h), params(self.dtype), self.context, by_columns(y), routing.groups)
+        return routing.join(y, x.shape[0])
+
+
+class FloatServer:
+    """The trained experts in 4-bit floats with a power of two to every 32, and tokens in the same."""
+
+    def __init__(self, trained):
+        self.dtype, self.context, self.b1 = trained.dtype, trained.context, trained.b1
+        self.experts = trained.w1.shape[0]
+        self.w1, self.w2 = self.quantize_weights(trained.w1), self.quantize_weights(trained.w2)
+
+    def empty(self, rows, cols):
+        return (torch.empty(rows, (cols + 1) // 2, dtype=torch.uint8, device="cuda"),
+                torch.empty(rows, (cols + 31) // 32, dtype=torch.uint8, device="cuda"))
+
+    def quantize_weights(self, w):
+        experts, rows, cols = w.shape
+        data, scales = self.empty(experts * rows, cols)
+        flat = w.reshape(experts * rows, cols).contiguous()
+        api.quantize_mxfp4(by_rows(flat), self.context, api.MxFp4Matrix(experts * rows, cols, data, scales))
+        return api.MxFp4Matrix(rows, cols, data, scales)  # the first expert's; the others lie behind it
+
+    def values(self, w):
+        """What quantised weights stand for."""
+        out = torch.empty(self.experts * w.rows, w.cols, device="cuda")
+        api.dequantize_mxfp4(api.MxFp4Matrix(self.experts * w.rows, w.cols, w.data, w.scales), self.context, by_rows(out))
+        return out.view(self.experts, w.rows, w.cols)
+
+    def tokens(self, x, routing=None):
+        """x in 4 bits, in the tokens' places where there is a routing."""
+        n = routing.sources.numel() if routing else x.shape[0]
+        held = api.MxFp4Matrix(n, x.shape[1], *self.empty(n, x.shape[1]))
+        api.quantize_mxfp4(by_rows(x), self.context, held, routing.routing if routing else None)
+        return held
+
+    def answer(self, x, routing):
+        chosen = self.tokens(x.to(self.dtype).contiguous(), routing)
+        h = torch.empty(chosen.rows, self.w1.rows, dtype=self.dtype, device="cuda")
+        y = torch.empty(chosen.rows, self.w2.rows, dtype=self.dtype, device="cuda")
+        api.mul_mxfp4(self.w1, chosen, params(self.dtype, self.b1, relu=True), self.context, by_columns(h), routing.groups)
+        api.mul_mxfp4(self.w2, self.tokens(h), params(self.dtype), self.context, by_columns(y), routing.groups)
         return routing.join(y, x.shape[0])
 
 
@@ -182,6 +270,8 @@ def main():
     routing = Routing(few @ router, args.top)
     y, wanted = server.answer(few, routing), routing.join(layer.forward(few, routing)[0], 3)
     print("4 bits, 3 tokens: %.3f of the answers' norm away from those of 16 bits" % ((y - wanted).norm() / wanted.norm()))
+    y = FloatServer(layer).answer(few, routing)
+    print("4-bit floats, 3 tokens: %.3f of it" % ((y - wanted).norm() / wanted.norm()))
     layer.close()
     teacher.close()
 

@@ -175,7 +175,7 @@ bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
   // (More than a workgroup has tokens, or, as groups are mostly of many sizes, more than the largest of these would have: 64 experts
   // of 2048 x 2048, us here and on tiles: 8 tokens to each in the mean 36.3 and 36.3, 16 42.4 and 39.1, 32 53 and 41.)
   if (!forced && call.n > (busy > 1 ? 8 : 32) * busy) return false;
-  if (call.k > 0x7fffffff - 2 * kChunk || call.m > 0x7fffffff - 128) return false;
+  if (call.k > 0x7fffffff - 2 * kChunk || call.m > 0x7fffffff - 512) return false;
   StreamArgs args;
   args.c = call;
   const int64_t chunks = (int64_t(call.k) + kChunk - 1) / kChunk;
