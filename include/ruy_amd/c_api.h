@@ -342,7 +342,8 @@ typedef struct ruyamd_routing {
  * return when the destinations are complete, or once they are enqueued after
  * ruyamd_ctx_set_synchronous(ctx, 0). Of the routing the others read `places`
  * only, which may be a program's own: a place outside the matrix of rows is
- * taken for none. */
+ * taken for none, and no two choices may have one place where rows are written
+ * (what is written there is then of either). */
 RUYAMD_API int ruyamd_sort_tokens(ruyamd_ctx* ctx, const ruyamd_mat* experts,
                                   const ruyamd_routing* routing);
 
@@ -424,9 +425,11 @@ RUYAMD_API int ruyamd_dequantize_mxfp4(ruyamd_ctx* ctx,
  * NULL) the columns of dst, and with them the rows of rhs, are dealt to groups, each with
  * an lhs of its own, as in ruyamd_mul_grouped (whose matrix_stride is not looked
  * at here: lhs says where its matrices lie; rhs's are not looked at). dst: fp32, bfloat16 or half,
- * any order. Sums are fp32, in which products of blocks below 2^-126 may be lost; the result is rounded once. Parameters, memory and
- * calls as in ruyamd_mul_grouped. Depths below 32 go to a kernel of one element to
- * a lane. */
+ * any order. A block's sum of products is exact; sums of blocks are fp32, in
+ * which those below 2^-126 may be lost; the result is rounded once. Parameters,
+ * memory and calls as in ruyamd_mul_grouped. Depths below 32 go to a kernel of one element to
+ * a lane; rows that do not begin at multiples of 16 bytes, or are no whole number of blocks, cost
+ * about half as much again where columns are many. */
 RUYAMD_API int ruyamd_mul_mxfp4(ruyamd_ctx* ctx, const ruyamd_mxfp4_mat* lhs,
                                 const ruyamd_mxfp4_mat* rhs,
                                 const ruyamd_groups* groups,
@@ -510,7 +513,9 @@ RUYAMD_API void ruyamd_ctx_force_generic_kernel(ruyamd_ctx* ctx, int force);
  * picks, where the kernel has that tile, also for products that would run on the
  * kernel for small ones instead; 0, 0 restores the model's choice. (Grouped
  * products: 256x256, 256x128, 128x128 or 64x64, rows along dst's contiguous dimension,
- * and no streaming kernel for matrices of bfloat16, half or fp32.)
+ * and no streaming kernel for matrices of bfloat16, half or fp32. Products of 4-bit floats: 64x64, 128x128 or
+ * 256x256, rows those of dst, 64x64 with depth_parts not 0 the one whose steps are four ahead, 16x16 the
+ * streaming kernel.)
  * depth_parts, looked at with the 256x256 tile forced on int8 data: not 0 =
  * split the depth over that many workgroups per tile (2, 4 or 8; 1: over none;
  * rounded down to what leaves no part without a depth step) instead of what
