@@ -428,8 +428,8 @@ RUYAMD_API int ruyamd_dequantize_mxfp4(ruyamd_ctx* ctx,
  * any order. A block's sum of products is exact; sums of blocks are fp32, in
  * which those below 2^-126 may be lost; the result is rounded once. Parameters,
  * memory and calls as in ruyamd_mul_grouped. Depths below 32 go to a kernel of one element to
- * a lane; rows that do not begin at multiples of 16 bytes, or are no whole number of blocks, cost
- * about half as much again where columns are many. */
+ * a lane; rows that do not begin at multiples of 4 bytes, or are no whole number of blocks, cost
+ * up to twice as much where columns are many. */
 RUYAMD_API int ruyamd_mul_mxfp4(ruyamd_ctx* ctx, const ruyamd_mxfp4_mat* lhs,
                                 const ruyamd_mxfp4_mat* rhs,
                                 const ruyamd_groups* groups,

@@ -32,8 +32,11 @@ using grouped::WaitVmcnt;
 
 constexpr int kStep = 8 * kBlock;  // depth positions to a step: 128 bytes
 
-// kDirect: rows of both sides begin at multiples of 16 bytes and are whole blocks, so that tiles go to LDS without passing
-// through registers. Otherwise rows are read 16 bytes a lane from wherever they begin.
+// kDirect: rows of both sides begin at multiples of 4 bytes, which is what a load to LDS asks of an address, and are whole blocks, so
+// that tiles go to LDS without passing through registers. (8192 x 8192 x 8192, rows 4100 bytes apart: 263 us, through registers
+// 406; 4096 and 4112 apart 245 and 260.) Otherwise rows are read 16 bytes a lane from wherever they begin: 8192 x 8192 x
+// 8192, rows 4097 bytes apart 496 us. (Reading the five words that hold 16 bytes and shifting them takes 503, and 8 % longer at
+// 4096 x 4096 x 4096.)
 // kStages: steps on their way to LDS (kDirect). More than two: the scales of the whole depth are put into LDS first, for whose
 // loads the waves would otherwise wait, and for those of all steps with them, in every other step.
 template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages>
@@ -338,9 +341,9 @@ Choice Choose(const MulCall& call) {
   // (Sizes and depths are rounded up to tiles, and gone past by some steps, in 32 bits.)
   if (std::max(call.m, std::max(call.n, call.k)) > 0x7fffffff - 2048) return choice;
   const auto aligned = [&](const Matrix& m) {
-    return reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && m.row_bytes % 16 == 0;
+    return reinterpret_cast<uintptr_t>(m.data) % 4 == 0 && m.row_bytes % 4 == 0;
   };
-  const bool direct = call.k % kBlock == 0 && aligned(call.lhs) && aligned(call.rhs) && call.lhs.matrix_bytes % 16 == 0;
+  const bool direct = call.k % kBlock == 0 && aligned(call.lhs) && aligned(call.rhs) && call.lhs.matrix_bytes % 4 == 0;
   const auto scales_aligned = [&](const Matrix& m) {
     return reinterpret_cast<uintptr_t>(m.scales) % 4 == 0 && m.scale_stride % 4 == 0;
   };

@@ -315,6 +315,20 @@ def test_every_tile_at_every_end_of_the_depth(context, tile, k):
         context.force_tile(0, 0)
 
 
+@pytest.mark.parametrize("tile", [(64, 64, 0), (64, 64, 1), (128, 128, 0), (256, 256, 0)])
+@pytest.mark.parametrize("pad", [1, 2, 3, 4, 8, 12, 20])
+def test_every_tile_at_every_alignment(context, tile, pad):
+    """Rows at multiples of 4 bytes and at any; the matrices of groups apart by multiples of what rows are and not."""
+    context.force_tile(*tile)
+    try:
+        for k in (32, 352, 640, 1024, 1025, 1027):
+            run_mul(context, S.F32, 140, 70, k, None, (pad, 0, 0, 4))
+            run_mul(context, S.BF16, 70, 140, k, np.array([0, 33, 33, 100, 140]), (pad, 4, 12, 0), 4, 4 * (pad % 3), COL, 1, True, seed=1)
+            run_mul(context, S.F16, 65, 66, k, np.array([0, 66]), (0, 0, pad, 1), pad % 4, 0, ROW, 0, True, seed=2)
+    finally:
+        context.force_tile(0, 0)
+
+
 @pytest.mark.parametrize("k", [32, 33, 95, 480, 511, 512, 513, 1000, 2048, 3333, 4096, 4111, 16384, 40000])
 def test_streams(context, k):
     """Fewer chunks than waves and more, cut short anywhere; one lot of tokens and several, as many as LDS has room for."""
