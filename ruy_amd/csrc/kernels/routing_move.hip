@@ -82,11 +82,11 @@ __device__ __forceinline__ Piece PieceOf(int64_t i, int segments) {
 }
 
 // The place of choice j of a token, or -1.
-__device__ __forceinline__ int PlaceOf(const Call& c, int token, int j) {
-  const int p = c.places[int64_t(token) * c.top + j];
+__device__ __forceinline__ int PlaceOf(const Call& c, int64_t token, int j) {
+  const int p = c.places[token * c.top + j];
   return p >= 0 && p < c.columns ? p : -1;
 }
-__device__ __forceinline__ float WeightOf(const Call& c, int token, int j) {
+__device__ __forceinline__ float WeightOf(const Call& c, int64_t token, int j) {
   return c.weights.data ? LoadFloat(c.weights.data, c.weights.type, j * c.weights.rs + token * c.weights.cs) : 1.0f;
 }
 
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void GradientsKernel(Call c, int w
   const int tokens_here = (blockDim.x >> 6) / waves, wave = my_wave % waves;
   const bool rows = c.grad_src.data, weights = c.grad_weights.data;
   for (int64_t token0 = int64_t(blockIdx.x) * tokens_here; token0 < c.tokens; token0 += int64_t(gridDim.x) * tokens_here) {
-    const int token = static_cast<int>(token0) + my_wave / waves;
+    const int64_t token = token0 + my_wave / waves;
     const bool there = token < c.tokens;  // (all waves go through the barriers)
     for (int j0 = 0; j0 < c.top; j0 += kDots) {
       int place[kDots];

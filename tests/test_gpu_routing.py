@@ -396,9 +396,61 @@ def test_long_rows_and_far_columns(context):
     api.combine_tokens(far, routing_of(places), None, context, api.Matrix(S.F32, y, api.Layout(width, 3, width, COL)))
     assert torch.equal(y, 2 * x.float())
     dw = torch.zeros(3, 2, device="cuda")
-    api.combine_tokens_gradients(near, far, routing_of(places), None, context, far, api.Matrix(S.F32, dw, api.Layout(2, 3, 2, COL)))
+    api.combine_tokens_gradients(near, far, routing_of(places), None, context, None, api.Matrix(S.F32, dw, api.Layout(2, 3, 2, COL)))
     want = (x.double() ** 2).sum(1, keepdim=True).expand(3, 2)
     assert ((dw.double() - want).abs() <= R.error_bound(want, width, want, S.F32)).all()
+    rows.fill_(0)
+    api.combine_tokens_gradients(near, None, routing_of(places), None, context, far, None)
+    for t in range(3):
+        for p in places[t]:
+            assert torch.equal(rows[p], x[t])
+
+
+def test_the_most_tokens(context):
+    """2^31 - 1 choices, one of each token: the last workgroup's waves have tokens up to the last number there is, and none behind."""
+    tokens, width, columns, piece = 2 ** 31 - 1, 8, 5, 1 << 26
+    announce("most tokens")
+    places = torch.full((tokens,), -1, dtype=torch.int32, device="cuda")
+    where = torch.tensor([0, 1 << 30, tokens - 2, tokens - 1], device="cuda")
+    places[where] = torch.tensor([3, 0, 4, 1], dtype=torch.int32, device="cuda")
+    routing = api.Routing(tokens, 1, 1, None, places)
+    g = generator(5)
+    src = torch.randint(-4, 5, (columns, width), generator=g, device="cuda").to(torch.bfloat16)
+    grad = torch.ones(tokens, width, dtype=torch.bfloat16, device="cuda")
+    grad[where] = torch.randint(-4, 5, (4, width), generator=g, device="cuda").to(torch.bfloat16)
+    grad_src = torch.full((columns, width), -77.0, dtype=torch.bfloat16, device="cuda")
+    grad_weights = torch.full((tokens,), -77.0, dtype=torch.bfloat16, device="cuda")
+    api.combine_tokens_gradients(api.Matrix(S.BF16, grad, api.Layout(width, tokens, width, COL)),
+                                 api.Matrix(S.BF16, src, api.Layout(width, columns, width, COL)), routing, None, context,
+                                 api.Matrix(S.BF16, grad_src, api.Layout(width, columns, width, COL)),
+                                 api.Matrix(S.BF16, grad_weights, api.Layout(1, tokens, 1, COL)))
+    taken = places[where].long()
+    assert torch.equal(grad_src[taken], grad[where]) and bool((grad_src[2] == -77).all())
+    assert torch.equal(grad_weights[where], (grad[where].float() * src[taken].float()).sum(1).to(torch.bfloat16))
+    grad_weights[where] = 0
+    for at in range(0, tokens, piece):
+        assert not grad_weights[at:at + piece].any().item()
+
+    # grad's memory as the sums'.
+    api.combine_tokens(api.Matrix(S.BF16, src, api.Layout(width, columns, width, COL)), routing, None, context,
+                       api.Matrix(S.BF16, grad, api.Layout(width, tokens, width, COL)))
+    assert torch.equal(grad[where], src[taken])
+    grad[where] = 0
+    for at in range(0, tokens, piece):
+        assert not grad[at:at + piece].any().item()
+
+    # And their places: token t chooses expert t % 64.
+    del grad, grad_weights
+    experts = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    experts &= 63
+    offsets = torch.zeros(65, dtype=torch.int32, device="cuda")
+    api.sort_tokens(api.Matrix(S.I32, experts, api.Layout(1, tokens, 1, COL)), api.Routing(tokens, 1, 64, offsets, places), context)
+    begins = torch.arange(65, dtype=torch.int64) * (1 << 25)
+    begins[64] = tokens  # (the last expert has one less)
+    assert torch.equal(offsets.cpu().long(), begins)
+    for at in range(0, tokens, piece):
+        t = torch.arange(at, min(at + piece, tokens), dtype=torch.int64, device="cuda")
+        assert torch.equal(places[at:at + piece].long(), (t & 63) * (1 << 25) + (t >> 6))
 
 
 def test_results_do_not_change_from_call_to_call(context):
