@@ -428,6 +428,47 @@ def test_empty_calls(context, kernel):
     api.dequantize_mxfp4(api.MxFp4Matrix(5, 0, None, None), context, api.Matrix(S.F32, None, api.Layout(5, 0, 0, ROW)))
 
 
+@pytest.mark.parametrize("stride", [1 << 23, (1 << 23) + 4, 1 << 25])
+def test_rows_far_from_each_other(context, stride):
+    """Rows of values, scales and results that lie up to 2^32 bytes and more behind the first one's, and just inside what the offsets of a
+    tile of 256 rows reach."""
+    m, n, k = 300, 270, 640
+    rng = np.random.default_rng(0)
+    flat = [torch.empty((rows - 1) * stride + k // 2, dtype=torch.uint8, device="cuda") for rows in (m, m, n, n)]
+    values = []
+    for rows, data, scales in ((m, *flat[:2]), (n, *flat[2:])):
+        numbers, s = rng.integers(0, 16, (rows, k), dtype=np.uint8), rng.integers(126, 129, (rows, k // 32)).astype(np.uint8)
+        torch.as_strided(data, (rows, k // 2), (stride, 1)).copy_(torch.from_numpy(Q.pack(numbers)))
+        torch.as_strided(scales, (rows, k // 32), (stride, 1)).copy_(torch.from_numpy(s))
+        values.append(torch.from_numpy(Q.values(numbers, s)).cuda())
+    want = values[1] @ values[0].t().contiguous()
+    apart = 1 << 22  # (of columns of dst, in values)
+    y = torch.empty((n - 1) * apart + k, dtype=torch.float32, device="cuda")
+    results = torch.as_strided(y, (n, m), (apart, 1))
+    matrices = [api.MxFp4Matrix(m, k, *flat[:2], stride, stride), api.MxFp4Matrix(n, k, *flat[2:], stride, stride)]
+    try:
+        for tile in ((16, 16), (64, 64), (64, 64, 1), (128, 128), (256, 256), None):
+            announce("far rows", stride, tile)
+            context.force_tile(*(tile or (0, 0)))
+            context.force_generic_kernel(tile is None)
+            results.fill_(-77)
+            api.mul_mxfp4(*matrices, params_of(S.F32), context, api.Matrix(S.F32, y, api.Layout(m, n, apart, COL)))
+            assert torch.equal(results.double(), want)
+    finally:
+        context.force_tile(0, 0)
+        context.force_generic_kernel(False)
+    # Quantised there from columns far from each other, and back.
+    x = torch.as_strided(y, (n, k), (apart, 1))
+    x.copy_(values[1])
+    for t, width in zip(flat[2:], (k // 2, k // 32)):
+        torch.as_strided(t, (n, width), (stride, 1)).zero_()
+    api.quantize_mxfp4(api.Matrix(S.F32, y, api.Layout(n, k, apart, ROW)), context, matrices[1])
+    x.zero_()
+    api.dequantize_mxfp4(matrices[1], context, api.Matrix(S.F32, y, api.Layout(n, k, apart, ROW)))
+    numbers, scales = Q.quantize(values[1].cpu().numpy())
+    assert torch.equal(x.double().cpu(), torch.from_numpy(Q.values(numbers, scales)))
+
+
 def test_gradients_of_a_product_on_its_values(context):
     """What straight-through training does: forward in 4 bits, the gradient of tokens on dequantised
     weights. With whole numbers, <dy, difference of y> is <dx, step> exactly."""
