@@ -15,29 +15,21 @@
 //   odd step 2 S + 1, in front of barrier 1: and writes them, transposed (kScales: pair S has been read by all waves
 //     in front of barrier 2 of the even step). The words of pair S + 1 are read behind barrier 2 of this step, and in front of
 //     barrier 2 of the next.
-#include "grouped_gemm.h"
-#include "mxfp4_device.h"
 #include "mxfp4_large.h"
-#include "mxfp4_write_back.h"
+#include "mxfp4_tile.h"
 #include "paired_schedule.h"
 
 namespace ruyamd {
 namespace mxfp4 {
 namespace {
 
-using grouped::FindTile;
-using grouped::kNothing;
-using grouped::Range;
-using grouped::Resource;
-using grouped::StaticFor;
-using grouped::TileOf;
-using grouped::WaitVmcnt;
 namespace ps = paired_schedule;
 
-constexpr int kTile = 256, kStepBytes = 128, kStep = 8 * kBlock;
+constexpr int kTile = 256, kStepBytes = 128;
 constexpr int kSide = kTile * kStepBytes, kStage = 2 * kSide;  // bytes in LDS: of a side's step, of a step
 constexpr int kRaw = 2 * kStage, kScales = kRaw + 2 * kTile * 16, kLds = kScales + 2 * kTile * 16;
 static_assert(4 * WriteBack<ps::kBlocks, ps::kBlocks>::kLds <= kLds, "");
+static_assert(4 * (256 * kStepBytes) + 3 * (256 * 16) <= kLds, "a quarter's four stages, its scales and two pairs of them as they lie");
 static_assert(ps::kBlocks == 8 && ps::kWaves == 4 && ps::kLoads * ps::kRowsPerLoad * ps::kWaves == kTile, "");
 
 // The instruction with byte kByte of either side's scales. (The compiler's hazard checks do not look inside: an
@@ -94,7 +86,14 @@ __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
   const int tiles_m = (c.m + kTile - 1) / kTile;
   TileOf tile;
   Range range;
-  if (!FindTile(c.offsets, c.groups, c.n, kTile, tiles_m, &tile, &range)) return;
+  int quarter;
+  if (!FindTile(c.offsets, c.groups, c.n, kTile, tiles_m, &tile, &range, c.compute_units / 8, &quarter)) return;
+  if (quarter >= 0) {
+    tile.m = 2 * tile.m + (quarter & 1);
+    tile.n = 2 * tile.n + (quarter >> 1);
+    if (tile.m * 128 >= c.m || tile.n * 128 >= range.count) return;
+    return MultiplyTile<2, 2, 4, 4, true, 4, ScaleLoads::kAhead>(c, tile, range, lds);
+  }
   const int m0 = tile.m * kTile, n0 = tile.n * kTile;
   const int here_m = min(kTile, c.m - m0), here_n = min(kTile, range.count - n0);
   const int steps = (c.k + kStep - 1) / kStep, row_scales = c.k / kBlock;

@@ -1,0 +1,351 @@
+// A tile of a product of 4-bit values on the matrix cores.
+#ifndef RUY_AMD_CSRC_KERNELS_MXFP4_TILE_H_
+#define RUY_AMD_CSRC_KERNELS_MXFP4_TILE_H_
+
+#include "grouped_gemm.h"
+#include "mxfp4_device.h"
+#include "mxfp4_write_back.h"
+
+#include <type_traits>
+
+namespace ruyamd {
+namespace mxfp4 {
+
+using grouped::Barrier;
+using grouped::FindTile;
+using grouped::kNothing;
+using grouped::Range;
+using grouped::Resource;
+using grouped::Runs;
+using grouped::StaticFor;
+using grouped::TileOf;
+using grouped::TileSide;
+using grouped::WaitVmcnt;
+
+// 16 bytes a lane to LDS, from `soffset` bytes behind its offset.
+__device__ __forceinline__ void LoadToLds(uint32_t lds, uint32_t voffset, v4i rsrc, uint32_t soffset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(lds), "v"(voffset), "s"(rsrc), "s"(soffset)
+      : "memory");
+}
+
+constexpr int kStep = 8 * kBlock;  // depth positions to a step: 128 bytes
+
+// kDirect: rows of both sides begin at multiples of 4 bytes, which is what a load to LDS asks of an address, and are whole blocks, so
+// that tiles go to LDS without passing through registers. (8192 x 8192 x 8192, rows 4100 bytes apart: 263 us, through registers
+// 406; 4096 and 4112 apart 245 and 260.) Otherwise rows are read 16 bytes a lane from wherever they begin: 8192 x 8192 x
+// 8192, rows 4097 bytes apart 496 us. (Reading the five words that hold 16 bytes and shifting them takes 503, and 8 % longer at
+// 4096 x 4096 x 4096.)
+// kStages: steps on their way to LDS (kDirect), two or four.
+// How scales come to LDS. Through registers, a pair of steps ahead: the waves wait for these loads, and for those of all steps with
+// them, in every other step, which with more than two stages would be all that the other stages are for. All of the depth's first. Or, where
+// their rows begin at multiples of 4 bytes and have 16, as they lie, two pairs ahead: then each thread takes its own row's
+// out of LDS, and puts them back transposed.
+enum class ScaleLoads { kThroughRegisters, kAllFirst, kAhead };
+template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages, ScaleLoads kScaleLoads>
+__device__ __forceinline__ void MultiplyTile(const MulCall& c, const TileOf& tile, const Range& range, char* lds) {
+  constexpr int kWaves = kWavesM * kWavesN;
+  constexpr int kTileM = kWavesM * kBlocksM * 16, kTileN = kWavesN * kBlocksN * 16;
+  // (How rows lie in LDS, which is a matter of bytes alone.)
+  using M = TileSide<RUYAMD_DTYPE_BF16, Runs::kPlain, kTileM, kBlocksM, true, kWaves>;
+  using N = TileSide<RUYAMD_DTYPE_BF16, Runs::kPlain, kTileN, kBlocksN, false, kWaves>;
+  constexpr int kStage = M::kBytes + N::kBytes;
+  constexpr bool kAllScales = kScaleLoads == ScaleLoads::kAllFirst, kAhead = kScaleLoads == ScaleLoads::kAhead;
+  constexpr bool kThrough = kScaleLoads == ScaleLoads::kThroughRegisters;
+  static_assert(kDirect || (kStages == 2 && kThrough), "");
+  constexpr int kRows = kTileM + kTileN, kScalesAt = kStages * kStage, kRawAt = kScalesAt + kRows * 16;
+  static_assert(!kAhead || (kRows == 64 * kWaves && kTileM % 64 == 0), "a wave's rows are of one side");
+  static_assert(kRows <= 64 * kWaves, "a row's scales to a thread");
+  using Out = WriteBack<kBlocksM, kBlocksN>;
+  static_assert(kWaves * Out::kLds <= kScalesAt, "");
+
+  const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_m = wave % kWavesM, wave_n = wave / kWavesM;
+  const int m0 = tile.m * kTileM, n0 = tile.n * kTileN;
+  const int here_m = min(kTileM, c.m - m0), here_n = min(kTileN, range.count - n0);
+  const int steps = (c.k + kStep - 1) / kStep;
+  const int row_bytes = (c.k + 1) / 2, row_scales = (c.k + kBlock - 1) / kBlock;
+  const uint8_t* const base_m = c.lhs.data + tile.group * c.lhs.matrix_bytes + m0 * c.lhs.row_bytes;
+  const uint8_t* const base_n = c.rhs.data + (int64_t(range.begin) + n0) * c.rhs.row_bytes;
+
+  v4f acc[kBlocksM][kBlocksN] = {};
+  struct Fragments {
+    v4i m[kBlocksM], n[kBlocksN];
+  };
+  struct Scales {
+    int m[kBlocksM], n[kBlocksN];
+  };
+  const auto read = [&](int stage, int kk, Fragments& f) __attribute__((always_inline)) {
+    const char* const side_m = lds + stage * kStage;
+#pragma unroll
+    for (int j = 0; j < kBlocksN; ++j) f.n[j] = N::Fragment(side_m + M::kBytes, wave_n, j, kk, lane);
+#pragma unroll
+    for (int i = 0; i < kBlocksM; ++i) f.m[i] = M::Fragment(side_m, wave_m, i, kk, lane);
+  };
+  // The bytes of a pair of steps: one to each half of either step.
+  const auto read_scales = [&](int buffer, Scales& s) __attribute__((always_inline)) {
+    const char* const at = lds + kScalesAt + buffer * (kRows * 16) + q * 4;
+#pragma unroll
+    for (int j = 0; j < kBlocksN; ++j)
+      s.n[j] = *reinterpret_cast<const int*>(at + (kTileM + wave_n * N::kWaveRows + N::RowOf(j, l)) * 16);
+#pragma unroll
+    for (int i = 0; i < kBlocksM; ++i)
+      s.m[i] = *reinterpret_cast<const int*>(at + (wave_m * M::kWaveRows + M::RowOf(i, l)) * 16);
+  };
+  const auto multiply = [&](const Fragments& f, const Scales& s, auto byte) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kBlocksM; ++i)
+#pragma unroll
+      for (int j = 0; j < kBlocksN; ++j) Mma<byte>(f.m[i], f.n[j], s.m[i], s.n[j], acc[i][j]);
+  };
+
+  // The scales of a row of either side. (Those of rows past the tile's sides are the last row's.)
+  const auto scales_of_row = [&](int row) __attribute__((always_inline)) {
+    return row < kTileM ? c.lhs.scales + tile.group * c.lhs.scales_matrix_stride + int64_t(m0 + min(row, here_m - 1)) * c.lhs.scale_stride
+                        : c.rhs.scales + (int64_t(range.begin) + n0 + min(row - kTileM, here_n - 1)) * c.rhs.scale_stride;
+  };
+  const auto put_scales_of_row = [&](const v4i& x, int row, int pair, int buffer) __attribute__((always_inline)) {
+    *reinterpret_cast<v4i*>(lds + kScalesAt + buffer * (kRows * 16) + row * 16) =
+        Transposed(kAhead ? granule::PlaceGranule(x, pair * 16, row_scales) : PlaceScales(x, pair * 16, row_scales));
+  };
+  // A thread brings those of one row, pair by pair.
+  const uint8_t* const scale_row = scales_of_row(threadIdx.x);
+  const auto fetch_scales = [&](int pair) __attribute__((always_inline)) { return LoadScales(scale_row, pair * 16, row_scales); };
+  const auto put_scales = [&](const v4i& x, int pair, int buffer) __attribute__((always_inline)) {
+    if (kRows == 64 * kWaves || int(threadIdx.x) < kRows) put_scales_of_row(x, threadIdx.x, pair, buffer);
+  };
+
+  if constexpr (kDirect) {
+    const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    uint32_t off_m[M::kLoads], off_n[N::kLoads];
+    // (What lies beyond the tile's side is read from its last row: it ends up in rows of the tile that are not stored.)
+#pragma unroll
+    for (int n = 0; n < M::kLoads; ++n)
+      off_m[n] = static_cast<uint32_t>(min(M::RunOf(n, wave, lane), here_m - 1) * c.lhs.row_bytes) + M::GranuleOf(n, wave, lane) * 16;
+#pragma unroll
+    for (int n = 0; n < N::kLoads; ++n)
+      off_n[n] = static_cast<uint32_t>(min(N::RunOf(n, wave, lane), here_n - 1) * c.rhs.row_bytes) + N::GranuleOf(n, wave, lane) * 16;
+    const v4i rsrc_m = Resource(reinterpret_cast<const char*>(base_m)), rsrc_n = Resource(reinterpret_cast<const char*>(base_n));
+    constexpr int kLoads = M::kLoads + N::kLoads;
+    // What a step that reaches past the depth takes from there are zeros, and all steps behind it.
+    const auto end_at = [&](int s) __attribute__((always_inline)) {
+      const int left = (c.k - s * kStep) / kBlock;  // granules
+      if (left >= 8) return;
+#pragma unroll
+      for (int n = 0; n < M::kLoads; ++n)
+        if (M::GranuleOf(n, wave, lane) >= left) off_m[n] = kNothing;
+#pragma unroll
+      for (int n = 0; n < N::kLoads; ++n)
+        if (N::GranuleOf(n, wave, lane) >= left) off_n[n] = kNothing;
+    };
+    const auto load = [&](auto number, int s, int stage) __attribute__((always_inline)) {
+      constexpr int n = decltype(number)::value;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds_base + stage * kStage + wave * 1024);
+      const uint32_t from = __builtin_amdgcn_readfirstlane(s * 128);
+      if constexpr (n < M::kLoads)
+        LoadToLds(to + n * kWaves * 1024, off_m[n], rsrc_m, from);
+      else
+        LoadToLds(to + M::kBytes + (n - M::kLoads) * kWaves * 1024, off_n[n - M::kLoads], rsrc_n, from);
+    };
+    constexpr int kReads = kBlocksM + kBlocksN, kProducts = kBlocksM * kBlocksN;
+    const auto read_one = [&](auto number, int stage, int kk, Fragments& f) __attribute__((always_inline)) {
+      constexpr int n = decltype(number)::value;
+      const char* const side_m = lds + stage * kStage;
+      if constexpr (n < kBlocksN)
+        f.n[n] = N::Fragment(side_m + M::kBytes, wave_n, n, kk, lane);
+      else
+        f.m[n - kBlocksN] = M::Fragment(side_m, wave_m, n - kBlocksN, kk, lane);
+    };
+    const auto read_scales_one = [&](auto number, int buffer, Scales& s) __attribute__((always_inline)) {
+      constexpr int n = decltype(number)::value;
+      const char* const at = lds + kScalesAt + buffer * (kRows * 16) + q * 4;
+      if constexpr (n < kBlocksN)
+        s.n[n] = *reinterpret_cast<const int*>(at + (kTileM + wave_n * N::kWaveRows + N::RowOf(n, l)) * 16);
+      else
+        s.m[n - kBlocksN] = *reinterpret_cast<const int*>(at + (wave_m * M::kWaveRows + M::RowOf(n - kBlocksN, l)) * 16);
+    };
+    const auto product = [&](auto number, const Fragments& f, const Scales& s, auto byte) __attribute__((always_inline)) {
+      constexpr int i = decltype(number)::value / kBlocksN, j = decltype(number)::value % kBlocksN;
+      Mma<decltype(byte)::value>(f.m[i], f.n[j], s.m[i], s.n[j], acc[i][j]);
+    };
+    // f(i) for those of kAll that come behind product number `at`.
+    const auto share = [&](auto at, auto all, auto&& f) __attribute__((always_inline)) {
+      constexpr int kFrom = decltype(at)::value * decltype(all)::value / kProducts;
+      constexpr int kTo = (decltype(at)::value + 1) * decltype(all)::value / kProducts;
+      StaticFor<kTo - kFrom>([&](auto i) __attribute__((always_inline)) { f(std::integral_constant<int, kFrom + decltype(i)::value>()); });
+    };
+    using Reads = std::integral_constant<int, kReads>;
+    using Loads = std::integral_constant<int, kLoads>;
+    // As in grouped_gemm.h: steps are on their way to LDS kStages ahead, and the two halves of a step's depth take turns: while the
+    // matrix cores have one, the fragments of the other come out of LDS. In the middle of a step all waves wait for the loads
+    // of the next one and for each other. With two stages, in every other step the scales of the next pair, which have come with
+    // these loads, go into LDS before that, and out of it after.
+    v4i next_scales = {};
+    if constexpr (kThrough) next_scales = fetch_scales(0);
+    // (kAhead: two buffers, of pairs in turn.)
+    const int my_row = threadIdx.x & ~63;  // the wave's first one
+    const uint32_t scales_off =
+        my_row < kTileM ? static_cast<uint32_t>(min(my_row + lane, here_m - 1) * c.lhs.scale_stride)
+                        : static_cast<uint32_t>(min(my_row - kTileM + lane, here_n - 1) * c.rhs.scale_stride);
+    const char* const scales_base =
+        reinterpret_cast<const char*>(my_row < kTileM ? c.lhs.scales + tile.group * c.lhs.scales_matrix_stride + m0 * c.lhs.scale_stride
+                                                      : c.rhs.scales + (int64_t(range.begin) + n0) * c.rhs.scale_stride);
+    const v4i scales_rsrc = Resource(scales_base);
+    const auto load_raw = [&](int pair) __attribute__((always_inline)) {
+      LoadToLds(__builtin_amdgcn_readfirstlane(lds_base + kRawAt + (pair & 1) * (kRows * 16) + wave * 1024), scales_off,
+                scales_rsrc, __builtin_amdgcn_readfirstlane(min(pair * 16, row_scales - 16)));
+    };
+    const auto read_raw = [&](int pair) __attribute__((always_inline)) {
+      return *reinterpret_cast<const v4i*>(lds + kRawAt + (pair & 1) * (kRows * 16) + threadIdx.x * 16);
+    };
+    if constexpr (kAhead) {
+      load_raw(0);
+      load_raw(1);
+    }
+    StaticFor<kStages>([&](auto d) __attribute__((always_inline)) {
+      end_at(d);
+      StaticFor<kLoads>([&](auto n) __attribute__((always_inline)) { load(n, d, d); });
+    });
+    if constexpr (kAllScales) {
+      constexpr int kAtOnce = 4, kThreads = 64 * kWaves;
+      const int all = (steps + 1) / 2 * kRows;
+      for (int i0 = threadIdx.x; i0 < all; i0 += kAtOnce * kThreads) {
+        v4i x[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int i = min(i0 + u * kThreads, all - 1);
+          x[u] = LoadScales(scales_of_row(i % kRows), i / kRows * 16, row_scales);
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int i = i0 + u * kThreads;
+          if (i < all) put_scales_of_row(x[u], i % kRows, i / kRows, i / kRows);
+        }
+      }
+    } else if constexpr (kThrough) {
+      put_scales(next_scales, 0, 0);
+    }
+    WaitVmcnt<(kStages - 1) * kLoads>();
+    if constexpr (kAhead) put_scales(read_raw(0), 0, 0);
+    Barrier();
+    Fragments first, second;
+    Scales scales, later;
+    read(0, 0, first);
+    read_scales(0, scales);
+    const auto step = [&](int s, auto stage) __attribute__((always_inline)) {
+      constexpr int kAt = decltype(stage)::value, kOdd = kAt % 2, kNext = (kAt + 1) % kStages;
+      end_at(s + kStages);
+      StaticFor<kProducts>([&](auto p) __attribute__((always_inline)) {
+        product(p, first, scales, std::integral_constant<int, 2 * kOdd>());
+        share(p, Reads(), [&](auto r) __attribute__((always_inline)) { read_one(r, kAt, 1, second); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      // (kAhead: in odd steps with the load of scales that went out in the last one; in even ones what they hold has come.)
+      WaitVmcnt<(kStages - 2) * kLoads + (kAhead && kOdd ? 1 : 0)>();
+      if constexpr (kOdd && !kAllScales) put_scales(next_scales, (s + 1) / 2, 0);
+      Barrier();
+      if constexpr (!kOdd && kThrough) next_scales = fetch_scales(s / 2 + 1);
+      if constexpr (!kOdd && kAhead) {
+        next_scales = read_raw(s / 2 + 1);
+        load_raw(s / 2 + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      StaticFor<kProducts>([&](auto p) __attribute__((always_inline)) {
+        product(p, second, scales, std::integral_constant<int, 2 * kOdd + 1>());
+        share(p, Reads(), [&](auto r) __attribute__((always_inline)) {
+          read_one(r, kNext, 0, first);
+          // (Past the last pair: the last one again, of which nothing is used.)
+          if constexpr (kOdd) read_scales_one(r, kAllScales ? min((s + 1) / 2, (steps - 1) / 2) : 0, later);
+        });
+        share(p, Loads(), [&](auto n) __attribute__((always_inline)) { load(n, s + kStages, kAt); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (kOdd) scales = later;
+    };
+    for (int s = 0;;) {
+      step(s, std::integral_constant<int, 0>());
+      if (++s == steps) break;
+      step(s, std::integral_constant<int, 1>());
+      if (++s == steps) break;
+      if constexpr (kStages > 2) {
+        step(s, std::integral_constant<int, 2>());
+        if (++s == steps) break;
+        step(s, std::integral_constant<int, 3>());
+        if (++s == steps) break;
+      }
+    }
+    WaitVmcnt<0>();
+  } else {
+    // A granule is read where it lies, or, where it would reach past the end of its row, from the row's last 16 bytes, and
+    // put in its place then.
+    struct Set {
+      v4i m[M::kLoads], n[N::kLoads], scales;
+    };
+    Set held;
+    const auto fetch = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < M::kLoads; ++n)
+        held.m[n] = granule::LoadGranule<false>(base_m + min(M::RunOf(n, wave, lane), here_m - 1) * c.lhs.row_bytes,
+                                                s * 128 + M::GranuleOf(n, wave, lane) * 16, row_bytes);
+#pragma unroll
+      for (int n = 0; n < N::kLoads; ++n)
+        held.n[n] = granule::LoadGranule<false>(base_n + min(N::RunOf(n, wave, lane), here_n - 1) * c.rhs.row_bytes,
+                                                s * 128 + N::GranuleOf(n, wave, lane) * 16, row_bytes);
+      if (s % 2 == 0) held.scales = fetch_scales(s / 2);
+    };
+    const auto put = [&](int s, int stage) __attribute__((always_inline)) {
+      if ((s + 1) * 128 >= row_bytes) {
+#pragma unroll
+        for (int n = 0; n < M::kLoads; ++n) {
+          const int at = s * 128 + M::GranuleOf(n, wave, lane) * 16;
+          held.m[n] = WithoutOddHalf(granule::PlaceGranule(held.m[n], at, row_bytes), int64_t(at) * 2, c.k);
+        }
+#pragma unroll
+        for (int n = 0; n < N::kLoads; ++n)
+          held.n[n] = granule::PlaceGranule(held.n[n], s * 128 + N::GranuleOf(n, wave, lane) * 16, row_bytes);
+      }
+      char* const to = lds + stage * kStage + (wave * 64 + lane) * 16;
+#pragma unroll
+      for (int n = 0; n < M::kLoads; ++n) *reinterpret_cast<v4i*>(to + n * kWaves * 1024) = held.m[n];
+#pragma unroll
+      for (int n = 0; n < N::kLoads; ++n) *reinterpret_cast<v4i*>(to + M::kBytes + n * kWaves * 1024) = held.n[n];
+      if (s % 2 == 0) put_scales(held.scales, s / 2, s / 2 % 2);
+    };
+    fetch(0);
+    Scales scales;
+    const auto step = [&](int s, auto odd) __attribute__((always_inline)) {
+      constexpr int kOdd = decltype(odd)::value;
+      put(s, kOdd);
+      __syncthreads();
+      if (s + 1 < steps) fetch(s + 1);
+      Fragments first, second;
+      if constexpr (!kOdd) read_scales(s / 2 % 2, scales);
+      read(kOdd, 0, first);
+      read(kOdd, 1, second);
+      multiply(first, scales, std::integral_constant<int, 2 * kOdd>());
+      multiply(second, scales, std::integral_constant<int, 2 * kOdd + 1>());
+    };
+    for (int s = 0;;) {
+      step(s, std::integral_constant<int, 0>());
+      if (++s == steps) break;
+      step(s, std::integral_constant<int, 1>());
+      if (++s == steps) break;
+    }
+  }
+
+  // (LDS is the write-back's now.)
+  __syncthreads();
+  const int row0 = wave_m * M::kWaveRows, column0 = wave_n * N::kWaveRows;
+  Out{c, acc, lds + wave * Out::kLds, c.bias ? c.bias + tile.group * c.bias_stride + m0 + row0 : nullptr, m0 + row0,
+      int64_t(range.begin) + n0 + column0, here_m - row0, here_n - column0}();
+}
+
+}  // namespace mxfp4
+}  // namespace ruyamd
+
+#endif  // RUY_AMD_CSRC_KERNELS_MXFP4_TILE_H_

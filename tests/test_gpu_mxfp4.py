@@ -370,6 +370,20 @@ def test_the_largest_tile(context, k):
         context.force_tile(0, 0)
 
 
+@pytest.mark.parametrize("m,n,k,offsets", [
+    (4200, 4352, 512, None), (4352, 4096, 640, None), (5120, 3700, 1152, None), (16384, 1100, 512, None),
+    (2048, 9000, 512, [0, 1874, 3199, 4281, 5218, 6056, 6821, 7530, 9000]), (4096, 4480, 768, [0, 0, 4400, 4401, 4480]),
+    (512, 33300, 512, list(range(0, 33301, 333)))])
+def test_tiles_left_after_full_rounds(context, m, n, k, offsets):
+    """More tiles of 256 x 256 than there are CUs: few ones more, half a round of them, and more than that."""
+    context.force_tile(256, 256)
+    try:
+        run_mul(context, S.BF16, m, n, k, offsets and np.array(offsets), bias=True, low=0.0)
+        run_mul(context, S.F32, m, n, k, offsets and np.array(offsets), (12, 4, 4, 8), 0, 16, COL, 3, seed=1)
+    finally:
+        context.force_tile(0, 0)
+
+
 @pytest.mark.parametrize("m,n,k", [(100, 3, 4096), (64, 20, 1000), (130, 140, 2048), (300, 300, 8000), (16, 1, 40000)])
 def test_products_of_scales_of_any_size(context, kernel, m, n, k):
     run_mul(context, S.F32, m, n, k, scales=(110, 140))
