@@ -26,13 +26,15 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
   MultiplyTile<kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect, kStages, kScaleLoads>(c, tile, range, lds);
 }
 
-// The kernels: 64x64 with two and with four stages and 128x128 (above), and 256x256 (mxfp4_large.h).
+// The kernels: 64x64 and 128x128 with two and with four stages (mxfp4_tile.h), and 256x256 (mxfp4_large.h).
 enum class Tile { k64x64, k64x64Deep, k128x128, k128x128Deep, k256x256 };
+bool IsDeep(Tile t) { return t == Tile::k64x64Deep || t == Tile::k128x128Deep; }
 
 // How long a kernel takes, us: with its tiles dealt to `per_cu` workgroups of every CU in rounds, the last of which costs at least
-// `last` of a full one, fixed + rounds * (steps + more) * step, a step being 256 positions of depth. Fitted to 290 shapes of 256 to
+// `last` of a full one, fixed + rounds * (steps + more) * step, a step being 256 positions of depth; a quarter of a round or less
+// of 256x256 tiles behind full ones, which is made in quarters, (steps + kQuarters.more) * kQuarters.step. Fitted to 530 shapes of 256 to
 // 16384 rows, 48 to 8192 columns and depths of 512 to 16384, bfloat16 destinations, to 5 to 11 % root mean square. Choosing by it
-// costs 1.3 % over the fastest kernel at each of these shapes (20 % at the worst, 256 x 48, depth 512: 5.6 us for 4.6).
+// costs 0.6 % over the fastest kernel at each of these shapes (17 % at the worst, 3500 x 512, depth 4096: 12.8 us for 11.0).
 struct Timing {
   int per_cu;
   float fixed, step, more, last;
@@ -43,11 +45,14 @@ struct TileCost {
   Timing direct, through;  // operands straight to LDS, and through registers (step 0: there is no such kernel)
 };
 constexpr int kThreads = 256;
-constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, {4, 2.8f, 0.96f, 2.7f, 0.33f}, {2, 2.5f, 0.715f, 1.2f, 0.71f}},
-                               {Tile::k64x64Deep, 64, 64, {1, 3.2f, 0.315f, 3.6f, 0.88f}, {1, 0, 0, 0, 0}},
-                               {Tile::k128x128, 128, 128, {2, 2.3f, 1.34f, 3.1f, 0.51f}, {1, 3.8f, 1.24f, 0.5f, 0.90f}},
-                               {Tile::k128x128Deep, 128, 128, {1, 2.3f, 0.68f, 3.1f, 1.0f}, {1, 0, 0, 0, 0}},
-                               {Tile::k256x256, 256, 256, {1, 2.75f, 1.64f, 5.6f, 0.63f}, {1, 0, 0, 0, 0}}};
+constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, {4, 2.85f, 0.95f, 2.6f, 0.34f}, {2, 2.65f, 0.707f, 1.2f, 0.70f}},
+                               {Tile::k64x64Deep, 64, 64, {1, 3.2f, 0.268f, 4.5f, 0.82f}, {1, 0, 0, 0, 0}},
+                               {Tile::k128x128, 128, 128, {2, 2.84f, 1.18f, 3.7f, 0.43f}, {1, 4.1f, 1.24f, 0.45f, 0.89f}},
+                               {Tile::k128x128Deep, 128, 128, {1, 2.3f, 0.617f, 6.5f, 0.75f}, {1, 0, 0, 0, 0}},
+                               {Tile::k256x256, 256, 256, {1, 3.0f, 1.57f, 5.8f, 0.66f}, {1, 0, 0, 0, 0}}};
+constexpr struct {
+  float step, more;
+} kQuarters = {0.605f, 6.0f};
 
 // LDS that a workgroup may take, and what 64x64 tiles of four stages do.
 constexpr int kMostLds = 156 << 10;
@@ -115,12 +120,16 @@ Choice Choose(const MulCall& call) {
   };
   const int64_t busy = std::min(call.groups, call.n);
   const auto blocks_of = [&](const TileCost& t) {
-    const int64_t blocks = ((int64_t(call.m) + t.m - 1) / t.m * (call.n / t.n + busy) + 7) / 8 * 8;
-    return t.tile == Tile::k256x256 && blocks > call.compute_units ? blocks + call.compute_units / 32 * 24 : blocks;
+    const int64_t tiles_m = (int64_t(call.m) + t.m - 1) / t.m;
+    const int64_t tiles = call.offsets ? tiles_m * (call.n / t.n + busy) : tiles_m * ((int64_t(call.n) + t.n - 1) / t.n);
+    // (Of the largest tiles three more workgroups for each that may go to quarters.)
+    const int64_t at_once = call.compute_units / 8, each_xcd = (tiles + 7) / 8, rest = each_xcd % at_once;
+    if (t.tile != Tile::k256x256 || each_xcd < at_once) return each_xcd * 8;
+    return (each_xcd + (call.offsets ? at_once / 4 * 3 : rest * 4 <= at_once ? rest * 3 : 0)) * 8;
   };
   const auto usable = [&](const TileCost& t) { return timing_of(t).step != 0 && LaunchFits(blocks_of(t), kThreads); };
   const auto forced = [&](const TileCost& t) {
-    return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols && (t.tile == Tile::k64x64Deep || t.tile == Tile::k128x128Deep) == call.forced_deep;
+    return t.m == call.forced_tile_rows && t.n == call.forced_tile_cols && IsDeep(t.tile) == call.forced_deep;
   };
   const bool force = std::any_of(std::begin(kTiles), std::end(kTiles), [&](const TileCost& t) { return forced(t) && usable(t); });
   // The kernel that would be done first. (How many tiles the groups' columns make is known on the device only: here every group that can
@@ -132,8 +141,12 @@ Choice Choose(const MulCall& call) {
     const int64_t tiles_m = (int64_t(call.m) + t.m - 1) / t.m;
     const float tiles_n = busy == 1 ? std::ceil(float(call.n) / t.n) : std::max(float(busy), float(call.n) / t.n + 0.5f * busy);
     const float all = tiles_m * tiles_n / (timing.per_cu * call.compute_units), full = std::floor(all);
-    const float rounds = std::max(timing.last, full + (all > full ? timing.last + (1 - timing.last) * (all - full) : 0.0f));
-    const float time = timing.fixed + rounds * (float(call.k) / kStep + timing.more) * timing.step;
+    const float steps = float(call.k) / kStep;
+    const bool quarters = t.tile == Tile::k256x256 && full >= 1 && all > full && all - full <= 0.25f;
+    const float rounds =
+        quarters ? full : std::max(timing.last, full + (all > full ? timing.last + (1 - timing.last) * (all - full) : 0.0f));
+    const float time = timing.fixed + rounds * (steps + timing.more) * timing.step +
+                       (quarters ? (steps + kQuarters.more) * kQuarters.step : 0.0f);
     if (choice.blocks == 0 || time < choice.time) {
       choice.time = time;
       choice.tile = t.tile;
