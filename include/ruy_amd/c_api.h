@@ -334,7 +334,8 @@ typedef struct ruyamd_routing {
  * RUYAMD_DTYPE_I64, any order and stride; writes offsets, places and sources.
  * A number outside 0 .. count - 1, such as the -1 of a token of padding, is no
  * choice and has no place. The result depends on the numbers alone. tokens * top
- * is below 2^31.
+ * is below 2^31. (With more than 16384 experts every expert looks at every choice, and
+ * the time goes by the product of both numbers.)
  *
  * This call and the ones below: every buffer is device memory, no memory is
  * allocated, nothing is kept from one call to the next, a call may be recorded
