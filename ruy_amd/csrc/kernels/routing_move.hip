@@ -6,6 +6,11 @@
 // read or written once, and its rows, wherever they are, as whole lines. A lane has units of 16
 // bytes (8 values of 16 bits, 4 of 32); the last unit of a row that is no whole number of them
 // ends where the row ends, and overlaps the one before.
+//
+// All are copies with a little arithmetic, bound by HBM, and by the launch where there is little to copy. What is left to choose is how much a lane
+// has on its way at once (WithUnits, and four choices of a token together) and which writes go past the caches (kStreamFrom).
+// Moved, 8192 tokens of 4096 values in bfloat16 and two places each, 201 MB: to their places 33 us, 6.1 TB/s; added up, 37 us, 5.4;
+// gradients, 336 MB, 70 us, 4.8, of which the rows alone would be 35. Sixteen tokens of 2048 values: 2.8 us and 3.3.
 #include <algorithm>
 
 #include "granule.h"

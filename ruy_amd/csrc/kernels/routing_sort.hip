@@ -10,6 +10,10 @@
 // has in it; one workgroup adds these up, over parts and experts; a wave to a part hands out places, 64 choices at a time, those of
 // one expert among them found by comparing the numbers bit by bit over the wave. The counts of a part lie meanwhile
 // where its places will be (a part has as many choices as there are experts, or more): no other memory is needed.
+//
+// What bounds both is latency, not the 8 to 20 bytes of a choice: a launch, a read of the choices, a sum over the workgroup and the
+// writes of the places. Among 64 experts, 64-bit numbers: 32 choices 3.3 us; 32768 10.2 in one launch, whose workgroups have 2048 choices to
+// a wave and read all 256 KB out of L2 (half of the time; with all 32 loads of a lane on their way at once no less); 131072 14.4 in three.
 #include <algorithm>
 
 #include "grouped_gemm.h"
@@ -270,8 +274,10 @@ hipError_t Launch(hipStream_t stream, const SortCall& c, bool one_launch) {
   const int64_t n = int64_t(c.tokens) * c.top;
   // Parts: as long as there are experts at least, some thousand at most.
   const int64_t part = std::max<int64_t>({(c.count + 63) / 64 * 64, 512, (n + 1023) / 1024 / 64 * 64});
-  // (One launch reads all choices once to each expert.)
-  if (one_launch || c.count > 16384 || n < 2 * part || n * c.count <= int64_t(4) << 20) {
+  // One launch reads all choices once to each expert, and a wave keeps in registers what it has seen of 2048 of them. (us, one and
+  // three, int64: 32768 choices, 16 experts 10.3 and 12.9, 256 10.0 and 15.9, 512 17.2 and 20.1; 40000, 16 experts 13.3 and 13.7, 256 12.0 and
+  // 17.6; 65536, 16 experts 21.4 and 13.6, 64 18.9 and 12.9, 256 18.4 and 18.4, 512 32.0 and 24.8.)
+  if (one_launch || c.count > 16384 || n < 2 * part || (n <= 49152 && n * c.count <= int64_t(1) << 25)) {
     const int waves = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostWaves, (n + 255) / 256)));
     hipLaunchKernelGGL((SortByExpertKernel<kWide, kPlain>), dim3(c.count), dim3(64 * waves), 0, stream, c);
     return hipGetLastError();
