@@ -126,7 +126,7 @@ class MulParams:
 
     def __init__(self, accum_dtype, dst_dtype):
         self.accum_dtype, self.dst_dtype = accum_dtype, dst_dtype
-        # (bfloat16 and half: destinations of mul_grouped, mul_grouped_depth, mul_int4.)
+        # (bfloat16 and half: destinations of the products for layers of experts.)
         fp_dst = dst_dtype in (S.F32, S.F64, S.BF16, S.F16)
         if fp_dst != (accum_dtype in (S.F32, S.F64)):
             raise ValueError("floating-point Dst requires floating-point Accum and vice versa")

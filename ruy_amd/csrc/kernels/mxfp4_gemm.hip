@@ -4,6 +4,12 @@
 // 128 bytes of a row (256 values) through LDS, as those of grouped_gemm.h do; a fragment of 16
 // bytes to a lane is 128 values of depth here. Scales go with them in pairs of steps, 16 bytes of a row at a time,
 // transposed on their way into LDS (mxfp4_device.h), so that a fragment's scales of two steps are one word.
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 cycles with 4-bit values on both sides, so a wave's step of 64x64 is 512 cycles of products, of 16 KB
+// out of LDS (a CU's four waves 512 cycles) and of 8 KB into it; a tile waits for what is not done beside its products. Few
+// tiles: four stages, and one workgroup to a CU (2048 x 2048 x 8192: 128x128 25.5 us, 2.7 PFLOP/s; with two stages 29.8). Many:
+// two workgroups of 128x128 to a CU, one of which multiplies while the other waits (2048 x 4096 x 4096 25.7 us, with
+// four stages 30.3), or 256x256, which read half as much for a product (4096 x 4096 x 4096 38.4 us, 128x128 50).
 #include "launch_geometry.h"
 #include "mxfp4_large.h"
 #include "mxfp4_tile.h"

@@ -15,6 +15,16 @@
 //   odd step 2 S + 1, in front of barrier 1: and writes them, transposed (kScales: pair S has been read by all waves
 //     in front of barrier 2 of the even step). The words of pair S + 1 are read behind barrier 2 of this step, and in front of
 //     barrier 2 of the next.
+//
+// Tiles left after full rounds of all CUs, a quarter of a round or less, are made as quarters of 128x128 by four workgroups each
+// (mxfp4_tile.h, four stages): 4352 x 4096 x 2048, 272 tiles, 38.3 -> 33 us; 5120 x 4096 x 8192, 320 tiles, 104 -> 87. Of half a round two rounds of
+// quarters take longer than one of whole tiles (6144 x 4096 x 2048 44.5 us and 38.9).
+//
+// 8192 x 8192 x 8192: 240 to 252 us (from card to card), 4.4 to 4.6 PFLOP/s; a loop of these instructions alone, on random
+// values in registers, makes 7.1 and on zeros 9.7. What bounds it is the power that the card may take: over a deep
+// product (4096 x 4096 x 32768, 5.0 PFLOP/s) it runs at 1.68 of its 2.4 GHz, the matrix cores are busy in 68 % of the cycles, and
+// LDS has bank conflicts in 17 % of its own. A tile's first loads and its write-back take as long as 5.8 steps of 256 (kTiles in mxfp4_gemm.hip), which is
+// what bounds shallow products: 8 experts of 4096 x 2048 and 8192 tokens, 8 steps to a tile, 56 us, 2.5 PFLOP/s.
 #include "mxfp4_large.h"
 #include "mxfp4_tile.h"
 #include "paired_schedule.h"

@@ -6,6 +6,10 @@
 // have through LDS. The tokens are put into LDS first, with zeros behind the depth, so that
 // what is read of the weights there does not matter, and their scales transposed
 // (mxfp4_device.h); those of the weights are read where they lie, 16 bytes of a row to a chunk.
+//
+// HBM bounds it: 16384 x 16384 and one token, 143 MB in 27 us, 5.2 TB/s (a launch and the tokens' way into LDS some 3 us of it; a plain read
+// reaches 6.5); 64 experts of 2048 x 2048 and 32 tokens, of which 25 experts have some, 56 MB in 13.6. Loads that go past the caches, or three
+// and four chunks on their way and not two, gained nothing. Small ones are a launch and one wave's way through its depth: 2048 x 2048, 5.0 us.
 #include "grouped_gemm.h"
 #include "launch_geometry.h"
 #include "mxfp4_device.h"

@@ -1,4 +1,10 @@
-// A tile of a product of 4-bit values on the matrix cores.
+// A tile of a product of 4-bit values on the matrix cores: the steps of the kernels in mxfp4_gemm.hip, and of the largest tile's
+// quarters.
+//
+// Products, LDS reads and loads stand in the order in which they are issued: behind each product what there is of the
+// others, so that neither the matrix core nor the address unit waits for the end of a run of the other's. (Left to the compiler, products
+// sank behind the barrier: 2048 x 2048 x 8192 on 128x128, four stages 29.0 -> 25.2 us, two 34.9 -> 29.8.) A step of four stages still
+// takes 0.65 us at 2.2 GHz, in which the matrix cores are busy for a third; loads spread over both halves of a step gained nothing.
 #ifndef RUY_AMD_CSRC_KERNELS_MXFP4_TILE_H_
 #define RUY_AMD_CSRC_KERNELS_MXFP4_TILE_H_
 

@@ -1,7 +1,6 @@
-// The Python mirror's call path in native code: ruy_amd.api.mul (and the calls
-// for layers of experts) hands its
-// objects over here, where their fields are gathered into the plain structs of
-// c_api.h and ruyamd_mul is called. Filling four ctypes structures field by
+// The Python mirror's call path in native code: ruy_amd.api.mul, and the calls
+// for layers of experts, hand their objects over here, where their fields are
+// gathered into the plain structs of c_api.h and the C function is called. Filling four ctypes structures field by
 // field and calling through ctypes took 2.4 us of a call whose launch takes
 // 2.4 and whose kernel, for the smallest products, takes no more than both.
 //
