@@ -9,7 +9,8 @@
 // out of LDS (a CU's four waves 512 cycles) and of 8 KB into it; a tile waits for what is not done beside its products. Few
 // tiles: four stages, and one workgroup to a CU (2048 x 2048 x 8192: 128x128 25.5 us, 2.7 PFLOP/s; with two stages 29.8). Many:
 // two workgroups of 128x128 to a CU, one of which multiplies while the other waits (2048 x 4096 x 4096 25.7 us, with
-// four stages 30.3), or 256x256, which read half as much for a product (4096 x 4096 x 4096 38.4 us, 128x128 50).
+// four stages 30.3), of 256x128 (mxfp4_wide.hip; 16384 x 3300 x 512 35.0 us, 128x128 49.5), or 256x256, which read half as much for a
+// product (4096 x 4096 x 4096 38.4 us, 128x128 50).
 #include "launch_geometry.h"
 #include "mxfp4_large.h"
 #include "mxfp4_tile.h"
@@ -32,15 +33,15 @@ __global__ __launch_bounds__(64 * kWavesM * kWavesN, 2) void MxFp4GemmKernel(Mul
   MultiplyTile<kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect, kStages, kScaleLoads>(c, tile, range, lds);
 }
 
-// The kernels: 64x64 and 128x128 with two and with four stages (mxfp4_tile.h), and 256x256 (mxfp4_large.h).
-enum class Tile { k64x64, k64x64Deep, k128x128, k128x128Deep, k256x256 };
+// The kernels: 64x64 and 128x128 with two and with four stages (mxfp4_tile.h), 256x128 and 256x256 (mxfp4_large.h).
+enum class Tile { k64x64, k64x64Deep, k128x128, k128x128Deep, k256x128, k256x256 };
 bool IsDeep(Tile t) { return t == Tile::k64x64Deep || t == Tile::k128x128Deep; }
 
 // How long a kernel takes, us: with its tiles dealt to `per_cu` workgroups of every CU in rounds, the last of which costs at least
 // `last` of a full one, fixed + rounds * (steps + more) * step, a step being 256 positions of depth; a quarter of a round or less
-// of 256x256 tiles behind full ones, which is made in quarters, (steps + kQuarters.more) * kQuarters.step. Fitted to 530 shapes of 256 to
-// 16384 rows, 48 to 8192 columns and depths of 512 to 16384, bfloat16 destinations, to 5 to 11 % root mean square. Choosing by it
-// costs 0.6 % over the fastest kernel at each of these shapes (17 % at the worst, 3500 x 512, depth 4096: 12.8 us for 11.0).
+// of 256x256 tiles behind full ones, which is made in quarters, (steps + kQuarters.more) * kQuarters.step. Fitted to 551 shapes of 256 to
+// 16384 rows, 48 to 8192 columns and depths of 512 to 8192, bfloat16 destinations, to 5 to 10 % root mean square. Choosing by it
+// costs 0.9 % over the fastest kernel at each of these shapes (16 % at the worst, 256 x 6000, depth 4096: 12.0 us for 10.4).
 struct Timing {
   int per_cu;
   float fixed, step, more, last;
@@ -51,14 +52,15 @@ struct TileCost {
   Timing direct, through;  // operands straight to LDS, and through registers (step 0: there is no such kernel)
 };
 constexpr int kThreads = 256;
-constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, {4, 2.85f, 0.95f, 2.6f, 0.34f}, {2, 2.65f, 0.707f, 1.2f, 0.70f}},
-                               {Tile::k64x64Deep, 64, 64, {1, 3.2f, 0.268f, 4.5f, 0.82f}, {1, 0, 0, 0, 0}},
-                               {Tile::k128x128, 128, 128, {2, 2.84f, 1.18f, 3.7f, 0.43f}, {1, 4.1f, 1.24f, 0.45f, 0.89f}},
-                               {Tile::k128x128Deep, 128, 128, {1, 2.3f, 0.617f, 6.5f, 0.75f}, {1, 0, 0, 0, 0}},
-                               {Tile::k256x256, 256, 256, {1, 3.0f, 1.57f, 5.8f, 0.66f}, {1, 0, 0, 0, 0}}};
+constexpr TileCost kTiles[] = {{Tile::k64x64, 64, 64, {4, 3.0f, 0.943f, 2.6f, 0.31f}, {2, 2.7f, 0.702f, 1.2f, 0.67f}},
+                               {Tile::k64x64Deep, 64, 64, {1, 3.2f, 0.236f, 5.8f, 0.87f}, {1, 0, 0, 0, 0}},
+                               {Tile::k128x128, 128, 128, {2, 3.2f, 1.21f, 3.35f, 0.39f}, {1, 4.1f, 1.22f, 0.38f, 0.90f}},
+                               {Tile::k128x128Deep, 128, 128, {1, 2.45f, 0.628f, 6.4f, 0.72f}, {1, 0, 0, 0, 0}},
+                               {Tile::k256x128, 256, 128, {1, 4.0f, 1.26f, 1.5f, 0.72f}, {1, 0, 0, 0, 0}},
+                               {Tile::k256x256, 256, 256, {1, 3.6f, 1.66f, 5.15f, 0.63f}, {1, 0, 0, 0, 0}}};
 constexpr struct {
   float step, more;
-} kQuarters = {0.605f, 6.0f};
+} kQuarters = {0.58f, 6.4f};
 
 // LDS that a workgroup may take, and what 64x64 tiles of four stages do.
 constexpr int kMostLds = 156 << 10;
@@ -82,6 +84,7 @@ hipError_t LaunchKernel(hipStream_t stream, const MulCall& call, unsigned blocks
 template <bool kDirect>
 hipError_t LaunchTile(hipStream_t stream, const MulCall& call, Tile tile, unsigned blocks) {
   if (tile == Tile::k256x256) return LaunchLarge(stream, call, blocks);
+  if (tile == Tile::k256x128) return LaunchWide(stream, call, blocks);
   if constexpr (kDirect)
     if (tile == Tile::k64x64Deep) return LaunchKernel<2, 2, 2, 2, true, 4, ScaleLoads::kAllFirst>(stream, call, blocks);
   if constexpr (kDirect)
@@ -120,7 +123,7 @@ Choice Choose(const MulCall& call) {
   };
   const auto timing_of = [&](const TileCost& t) {
     const Timing none = {1, 0, 0, 0, 0};
-    if (t.tile == Tile::k256x256 || t.tile == Tile::k128x128Deep) return large ? t.direct : none;
+    if (t.tile == Tile::k256x256 || t.tile == Tile::k256x128 || t.tile == Tile::k128x128Deep) return large ? t.direct : none;
     if (t.tile == Tile::k64x64Deep && DeepLds(call.k) > kMostLds) return none;
     return !direct ? t.through : fits(t) ? t.direct : none;
   };

@@ -7,9 +7,10 @@
 namespace ruyamd {
 namespace mxfp4 {
 
-// Operands straight to LDS: rows of data and of scales begin at multiples of 4 bytes, the depth is a multiple of
+// The largest tiles. Operands straight to LDS: rows of data and of scales begin at multiples of 4 bytes, the depth is a multiple of
 // 128 (16 bytes of scales then end at a multiple of 4) and 512 at least (a row has 16).
-hipError_t LaunchLarge(hipStream_t stream, const MulCall& call, unsigned blocks);
+hipError_t LaunchLarge(hipStream_t stream, const MulCall& call, unsigned blocks);  // 256x256
+hipError_t LaunchWide(hipStream_t stream, const MulCall& call, unsigned blocks);   // 256x128
 
 }  // namespace mxfp4
 }  // namespace ruyamd

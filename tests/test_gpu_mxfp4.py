@@ -315,7 +315,7 @@ def test_every_tile_at_every_end_of_the_depth(context, tile, k):
         context.force_tile(0, 0)
 
 
-@pytest.mark.parametrize("tile", [(64, 64, 0), (64, 64, 1), (128, 128, 0), (256, 256, 0)])
+@pytest.mark.parametrize("tile", [(64, 64, 0), (64, 64, 1), (128, 128, 0), (128, 128, 1), (256, 128, 0), (256, 256, 0)])
 @pytest.mark.parametrize("pad", [1, 2, 3, 4, 8, 12, 20])
 def test_every_tile_at_every_alignment(context, tile, pad):
     """Rows at multiples of 4 bytes and at any; the matrices of groups apart by multiples of what rows are and not."""
@@ -354,6 +354,20 @@ def test_tiles_of_four_stages(context, k):
         run_mul(context, S.F32, 97, 300, k, np.array([0, 33, 33, 250, 300]), (16 - (k // 2) % 16, 3, 0, 2), 0, 16, COL, 1, True, 0.0, seed=1)
         run_mul(context, S.F16, 70, 65, k, None, (16 - (k // 2) % 16, 4, 16 - (k // 2) % 16, 1), 0, 0, ROW, 0, True, seed=2)
         run_mul(context, S.F32, 70, 65, k + 1600, scales=(120, 133), seed=3)
+    finally:
+        context.force_tile(0, 0)
+
+
+@pytest.mark.parametrize("k", [512, 640, 768, 896, 1024, 1152, 1664, 2048, 4096])
+def test_tiles_of_steps_of_128(context, k):
+    """Every number of steps to a last lot of scales; one tile and several, cut short on either side."""
+    context.force_tile(256, 128)
+    try:
+        run_mul(context, S.BF16, 256, 128, k)
+        assert context.last_kernel_name() == "mxfp4_mfma"
+        run_mul(context, S.F32, 300, 290, k, np.array([0, 33, 33, 200, 290]), (4, 4, 12, 8), 4, 16, COL, 1, True, 0.0, seed=1)
+        run_mul(context, S.F16, 257, 513, k, None, (16, 4, 0, 0), 0, 0, ROW, 0, True, seed=2)
+        run_mul(context, S.BF16, 1000, 700, k, seed=3, scales=(120, 133))
     finally:
         context.force_tile(0, 0)
 
@@ -461,7 +475,7 @@ def test_rows_far_from_each_other(context, stride):
     results = torch.as_strided(y, (n, m), (apart, 1))
     matrices = [api.MxFp4Matrix(m, k, *flat[:2], stride, stride), api.MxFp4Matrix(n, k, *flat[2:], stride, stride)]
     try:
-        for tile in ((16, 16), (64, 64), (64, 64, 1), (128, 128), (256, 256), None):
+        for tile in ((16, 16), (64, 64), (64, 64, 1), (128, 128), (128, 128, 1), (256, 128), (256, 256), None):
             announce("far rows", stride, tile)
             context.force_tile(*(tile or (0, 0)))
             context.force_generic_kernel(tile is None)
