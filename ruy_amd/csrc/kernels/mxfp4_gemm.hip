@@ -164,7 +164,7 @@ Choice Choose(const MulCall& call) {
   }
   // Weights out of HBM, one matrix and one to each group.
   const double bytes = double(busy) * call.m * (call.lhs.row_bytes + call.lhs.scale_stride);
-  choice.time = std::max(choice.time, 3.0f + static_cast<float>(bytes / (busy == 1 ? 3.9e6 : 4.5e6)));
+  choice.time = std::max(choice.time, 2.6f + static_cast<float>(bytes / (busy == 1 ? 4.6e6 : 5.0e6)));
   return choice;
 }
 

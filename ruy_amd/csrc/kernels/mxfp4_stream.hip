@@ -176,9 +176,10 @@ bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
   const bool forced = call.forced_tile_rows == 16 && call.forced_tile_cols == 16;
   if (call.forced_tile_rows && !forced) return false;
   const int64_t busy = std::min(call.groups, call.n);
-  // (More than a workgroup has tokens, or, as groups are mostly of many sizes, more than the largest of these would have: 64 experts
-  // of 2048 x 2048, us here and on tiles: 8 tokens to each in the mean 36.3 and 36.3, 16 42.4 and 39.1, 32 53 and 41.)
-  if (!forced && call.n > (busy > 1 ? 8 : 32) * busy) return false;
+  // (More than a workgroup has tokens, or, as groups are mostly of many sizes, more than the largest of these would have, who then read
+  // their weights again: 64 experts of 2048 x 2048, us here and on tiles: 32 tokens 14.9 and 14.7, 256 35.5 and 32.0; of 4096 x 4096, 16
+  // 25.5 and 22.9, 256 134 and 107.)
+  if (!forced && call.n > (busy > 1 ? 2 : 32) * busy) return false;
   if (call.k > 0x7fffffff - 2 * kChunk || call.m > 0x7fffffff - 512) return false;
   StreamArgs args;
   args.c = call;
@@ -205,14 +206,15 @@ bool LaunchStream(hipStream_t stream, const MulCall& call, hipError_t* status) {
     if (depth_waves * row_waves > kMostWaves) depth_waves /= 2;
   }
   // About how long this takes, us: a launch, the weights at the rate of a stream, once to each lot of tokens, and a CU's workgroups putting
-  // their tokens into LDS. Tiles of many columns read the weights more slowly and go through no more of them for more tokens.
-  // (us, this and the fastest tiles: 2048 x 2048, 16 tokens 5.6 and 6.1; 32 7.5 and 6.1; 16384 x 4096, 4 tokens 12.1 and 10.4;
-  // 28672 x 8192, 4 tokens 28.3 and 35.1, 16 36.7 and 35.2; 8 experts of 4096 x 4096, 32 tokens 17.2 and 17.9.)
+  // their tokens into LDS. Tiles of many columns read the weights more slowly and go through no more of them for more tokens. Choosing
+  // by both costs 1.4 % over the faster one, in the mean over 432 calls of 1 to 256 tokens and weights of 1 to 570 MB. (us, this and the
+  // fastest tiles: 16384 x 8192, one token 14.7 and 15.6, 8 18.8 and 15.6, 32 21.7 and 16.0; 2048 x 2048, 16 5.6 and 6.1, 32 7.5 and 6.1;
+  // 8 experts of 2048 x 8192, 4 tokens 9.4 and 12.0.)
   const int64_t lots = (call.n + busy * args.tokens - 1) / (busy * args.tokens);
   const double weights = double(busy) * lots * call.m * (call.lhs.row_bytes + call.lhs.scale_stride);
   const int64_t mean_tokens = std::min<int64_t>(args.tokens, (call.n + busy - 1) / busy);
   const int64_t each_cu = (units * lots + int64_t(row_waves) * call.compute_units - 1) / (int64_t(row_waves) * call.compute_units);
-  const float time = 4.5f + static_cast<float>(weights / 5.2e6) + 2.65e-5f * float(each_cu * mean_tokens * (pitch + scale_pitch));
+  const float time = 4.5f + static_cast<float>(weights / (busy == 1 ? 7.0e6 : 6.0e6)) + 4.5e-5f * float(each_cu * mean_tokens * (pitch + scale_pitch));
   const float tiles = TilesMicroseconds(call);
   if (!forced && tiles >= 0 && tiles < time) return false;
   args.depth_waves = depth_waves;
