@@ -514,9 +514,9 @@ RUYAMD_API void ruyamd_ctx_force_generic_kernel(ruyamd_ctx* ctx, int force);
  * picks, where the kernel has that tile, also for products that would run on the
  * kernel for small ones instead; 0, 0 restores the model's choice. (Grouped
  * products: 256x256, 256x128, 128x128 or 64x64, rows along dst's contiguous dimension,
- * and no streaming kernel for matrices of bfloat16, half or fp32. Products of 4-bit floats: 64x64, 128x128 or
- * 256x256, rows those of dst, 64x64 with depth_parts not 0 the one whose steps are four ahead, 16x16 the
- * streaming kernel.)
+ * and no streaming kernel for matrices of bfloat16, half or fp32. Products of 4-bit floats: 64x64, 128x128,
+ * 256x128 or 256x256, rows those of dst, the first two with depth_parts not 0 those whose steps are four
+ * ahead, 16x16 the streaming kernel.)
  * depth_parts, looked at with the 256x256 tile forced on int8 data: not 0 =
  * split the depth over that many workgroups per tile (2, 4 or 8; 1: over none;
  * rounded down to what leaves no part without a depth step) instead of what
