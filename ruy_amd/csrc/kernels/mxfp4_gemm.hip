@@ -70,9 +70,10 @@ template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, in
           ScaleLoads kScaleLoads = ScaleLoads::kThroughRegisters>
 hipError_t LaunchKernel(hipStream_t stream, const MulCall& call, unsigned blocks) {
   constexpr int kRows = (kWavesM * kBlocksM + kWavesN * kBlocksN) * 16;
-  const int lds = kScaleLoads == ScaleLoads::kAllFirst ? static_cast<int>(DeepLds(call.k))
-                  : kScaleLoads == ScaleLoads::kAhead  ? kStages * kRows * 128 + 3 * kRows * 16
-                                                       : kStages * kRows * 128 + (kDirect ? 1 : 2) * kRows * 16;
+  const int lds = kScaleLoads == ScaleLoads::kAllFirst     ? static_cast<int>(DeepLds(call.k))
+                  : kScaleLoads == ScaleLoads::kAhead      ? kStages * kRows * 128 + 3 * kRows * 16
+                  : kScaleLoads == ScaleLoads::kAheadWords ? kStages * kRows * 128 + kRows * 16 + 2 * kRows * 20
+                                                           : kStages * kRows * 128 + (kDirect ? 1 : 2) * kRows * 16;
   auto* const kernel = &MxFp4GemmKernel<kWavesM, kWavesN, kBlocksM, kBlocksN, kDirect, kStages, kScaleLoads>;
   static const hipError_t attribute =
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
@@ -88,7 +89,9 @@ hipError_t LaunchTile(hipStream_t stream, const MulCall& call, Tile tile, unsign
   if constexpr (kDirect)
     if (tile == Tile::k64x64Deep) return LaunchKernel<2, 2, 2, 2, true, 4, ScaleLoads::kAllFirst>(stream, call, blocks);
   if constexpr (kDirect)
-    if (tile == Tile::k128x128Deep) return LaunchKernel<2, 2, 4, 4, true, 4, ScaleLoads::kAhead>(stream, call, blocks);
+    if (tile == Tile::k128x128Deep)
+      return ScalesNeedWords(call) ? LaunchKernel<2, 2, 4, 4, true, 4, ScaleLoads::kAheadWords>(stream, call, blocks)
+                                   : LaunchKernel<2, 2, 4, 4, true, 4, ScaleLoads::kAhead>(stream, call, blocks);
   if (tile == Tile::k128x128) return LaunchKernel<2, 2, 4, 4, kDirect>(stream, call, blocks);
   return LaunchKernel<2, 2, 2, 2, kDirect>(stream, call, blocks);
 }
@@ -110,14 +113,10 @@ Choice Choose(const MulCall& call) {
     return reinterpret_cast<uintptr_t>(m.data) % 4 == 0 && m.row_bytes % 4 == 0;
   };
   const bool direct = call.k % kBlock == 0 && aligned(call.lhs) && aligned(call.rhs) && call.lhs.matrix_bytes % 4 == 0;
-  const auto scales_aligned = [&](const Matrix& m) {
-    return reinterpret_cast<uintptr_t>(m.scales) % 4 == 0 && m.scale_stride % 4 == 0;
-  };
-  const bool large = direct && call.k % 128 == 0 && call.k >= 512 && scales_aligned(call.lhs) && scales_aligned(call.rhs) &&
-                     call.lhs.scales_matrix_stride % 4 == 0 && TileOffsetsFit(256, call.lhs.row_bytes, call.lhs.row_bytes) &&
+  const bool large = direct && call.k >= 512 && TileOffsetsFit(256, call.lhs.row_bytes, call.lhs.row_bytes) &&
                      TileOffsetsFit(256, call.rhs.row_bytes, call.rhs.row_bytes) &&
-                     TileOffsetsFit(256, call.lhs.scale_stride, call.lhs.scale_stride) &&
-                     TileOffsetsFit(256, call.rhs.scale_stride, call.rhs.scale_stride);
+                     TileOffsetsFit(256, call.lhs.scale_stride, call.lhs.scale_stride + 4) &&
+                     TileOffsetsFit(256, call.rhs.scale_stride, call.rhs.scale_stride + 4);
   const auto fits = [&](const TileCost& t) {
     return TileOffsetsFit(t.m, call.lhs.row_bytes, call.lhs.row_bytes) && TileOffsetsFit(t.n, call.rhs.row_bytes, call.rhs.row_bytes);
   };

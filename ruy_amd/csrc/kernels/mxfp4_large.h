@@ -7,8 +7,13 @@
 namespace ruyamd {
 namespace mxfp4 {
 
-// The largest tiles. Operands straight to LDS: rows of data and of scales begin at multiples of 4 bytes, the depth is a multiple of
-// 128 (16 bytes of scales then end at a multiple of 4) and 512 at least (a row has 16).
+// The largest tiles. Operands straight to LDS: rows of data begin at multiples of 4 bytes, the depth is a whole number of blocks, and
+// 512 at least (a row has 16 scales).
+// Of scales see ScaleRows (mxfp4_tile.h).
+inline bool ScalesNeedWords(const MulCall& call) {
+  const auto aligned = [](const Matrix& m) { return reinterpret_cast<uintptr_t>(m.scales) % 4 == 0 && m.scale_stride % 4 == 0; };
+  return call.k % 128 != 0 || !aligned(call.lhs) || !aligned(call.rhs) || call.lhs.scales_matrix_stride % 4 != 0;
+}
 hipError_t LaunchLarge(hipStream_t stream, const MulCall& call, unsigned blocks);  // 256x256
 hipError_t LaunchWide(hipStream_t stream, const MulCall& call, unsigned blocks);   // 256x128
 

@@ -37,9 +37,10 @@ namespace ps = paired_schedule;
 
 constexpr int kTile = 256, kStepBytes = 128;
 constexpr int kSide = kTile * kStepBytes, kStage = 2 * kSide;  // bytes in LDS: of a side's step, of a step
-constexpr int kRaw = 2 * kStage, kScales = kRaw + 2 * kTile * 16, kLds = kScales + 2 * kTile * 16;
+constexpr int kRaw = 2 * kStage, kScales = kRaw + 2 * kTile * 16, kFifths = kScales + 2 * kTile * 16;
+constexpr int kLds = kFifths + 2 * kTile * 4;
 static_assert(4 * WriteBack<ps::kBlocks, ps::kBlocks>::kLds <= kLds, "");
-static_assert(4 * (256 * kStepBytes) + 3 * (256 * 16) <= kLds, "a quarter's four stages, its scales and two pairs of them as they lie");
+static_assert(4 * (256 * kStepBytes) + 256 * 16 + 2 * (256 * 20) <= kLds && kLds <= 160 << 10, "a quarter's four stages, its scales and two pairs of them as they lie");
 static_assert(ps::kBlocks == 8 && ps::kWaves == 4 && ps::kLoads * ps::kRowsPerLoad * ps::kWaves == kTile, "");
 
 // The instruction with byte kByte of either side's scales. (The compiler's hazard checks do not look inside: an
@@ -89,7 +90,9 @@ __device__ __forceinline__ constexpr int RowOfBlock(int b) {
   return kM ? (b >> 1) * 32 + (b & 1) * 4 : b * 16;
 }
 
+template <bool kWords>
 __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
+  using Scaling = ScaleRows<kWords>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_m = wave >> 1, wave_n = wave & 1;
@@ -102,7 +105,7 @@ __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
     tile.m = 2 * tile.m + (quarter & 1);
     tile.n = 2 * tile.n + (quarter >> 1);
     if (tile.m * 128 >= c.m || tile.n * 128 >= range.count) return;
-    return MultiplyTile<2, 2, 4, 4, true, 4, ScaleLoads::kAhead>(c, tile, range, lds);
+    return MultiplyTile<2, 2, 4, 4, true, 4, kWords ? ScaleLoads::kAheadWords : ScaleLoads::kAhead>(c, tile, range, lds);
   }
   const int m0 = tile.m * kTile, n0 = tile.n * kTile;
   const int here_m = min(kTile, c.m - m0), here_n = min(kTile, range.count - n0);
@@ -126,28 +129,31 @@ __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
   }
   // Of the scales: waves 0 and 1 have those of the M side, 2 and 3 those of the N side, 64 rows to a load.
   const bool of_m = wave < 2;
-  const char* const scales_base =
-      of_m ? reinterpret_cast<const char*>(c.lhs.scales) + tile.group * c.lhs.scales_matrix_stride + m0 * c.lhs.scale_stride
-           : reinterpret_cast<const char*>(c.rhs.scales) + (int64_t(range.begin) + n0) * c.rhs.scale_stride;
-  const v4i scales_rsrc = Resource(scales_base);
-  uint32_t scales_off[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  const uint8_t* const scales_base = of_m ? c.lhs.scales + tile.group * c.lhs.scales_matrix_stride + m0 * c.lhs.scale_stride
+                                          : c.rhs.scales + (int64_t(range.begin) + n0) * c.rhs.scale_stride;
+  const auto rows_of = [&](int i) __attribute__((always_inline)) {
     const int r = (wave & 1) * 128 + i * 64 + lane;
-    scales_off[i] = static_cast<uint32_t>(of_m ? min(r, here_m - 1) * c.lhs.scale_stride : min(r, here_n - 1) * c.rhs.scale_stride);
-  }
+    return Scaling(scales_base, of_m ? min(r, here_m - 1) * c.lhs.scale_stride : min(r, here_n - 1) * c.rhs.scale_stride);
+  };
+  const Scaling scale_rows[2] = {rows_of(0), rows_of(1)};
   const uint32_t raw_target = __builtin_amdgcn_readfirstlane(lds_base + kRaw + wave * 2048);
+  const uint32_t words_target = __builtin_amdgcn_readfirstlane(lds_base + kFifths + wave * 512);
   const auto load_scales = [&](int pair, int i) __attribute__((always_inline)) {
-    SetTarget(raw_target + i * 1024);
-    asm volatile("s_nop 0");
-    // (The last 16 of a row, where there are no 16 more.)
-    LoadToTarget(scales_off[i], static_cast<uint32_t>(min(pair * 16, row_scales - 16)), scales_rsrc);
+    scale_rows[i].Load(raw_target + i * 1024, words_target + i * 256, pair * 16, row_scales);
   };
   char* const mine = lds + kRaw + wave * 2048 + lane * 16;  // (and 1024 bytes behind that)
-  const auto read_raw = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<const v4i*>(mine + i * 1024); };
-  const auto put_scales = [&](v4i x, int pair, int i) __attribute__((always_inline)) {
-    if (pair * 16 + 16 > row_scales) x = granule::PlaceGranule(x, pair * 16, row_scales);
-    *reinterpret_cast<v4i*>(mine + (kScales - kRaw) + i * 1024) = Transposed(x);
+  struct Raw {
+    v4i x;
+    int fifth;
+  };
+  const auto read_raw = [&](int i) __attribute__((always_inline)) {
+    Raw raw = {*reinterpret_cast<const v4i*>(mine + i * 1024), 0};
+    if constexpr (kWords) raw.fifth = *reinterpret_cast<const int*>(lds + kFifths + wave * 512 + i * 256 + lane * 4);
+    return raw;
+  };
+  const auto put_scales = [&](const Raw& raw, int pair, int i) __attribute__((always_inline)) {
+    *reinterpret_cast<v4i*>(mine + (kScales - kRaw) + i * 1024) =
+        Transposed(Scaling::Place(raw.x, raw.fifth, scale_rows[i].at, pair * 16, row_scales));
   };
 
   // The fragments and their scales: of the M side's rows and the N side's columns, both depth halves of a step.
@@ -193,13 +199,13 @@ __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
     for (int i = 0; i < ps::kLoads; ++i) issue(s, IsM(), i);
   }
   WaitVmcnt<4 * ps::kLoads>();
-  v4i raw[2] = {read_raw(0), read_raw(1)};
+  Raw raw[2] = {read_raw(0), read_raw(1)};
   put_scales(raw[0], 0, 0);
   put_scales(raw[1], 0, 1);
   // (What has been read of kRaw is in registers: put_scales has used it.)
   load_scales(1, 0);
   load_scales(1, 1);
-  WaitVmcnt<2 * ps::kLoads + 2>();
+  WaitVmcnt<2 * ps::kLoads + 2 * Scaling::kLoads>();
   __syncthreads();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -281,14 +287,19 @@ __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
       m0 + wave_m * 128, int64_t(range.begin) + n0 + wave_n * 128, here_m - wave_m * 128, here_n - wave_n * 128}();
 }
 
+template <bool kWords>
+hipError_t Launch(hipStream_t stream, const MulCall& call, unsigned blocks) {
+  static const hipError_t attribute =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&MxFp4LargeKernel<kWords>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (attribute != hipSuccess) return attribute;
+  hipLaunchKernelGGL(MxFp4LargeKernel<kWords>, dim3(blocks), dim3(256), kLds, stream, call);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t LaunchLarge(hipStream_t stream, const MulCall& call, unsigned blocks) {
-  static const hipError_t attribute =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(MxFp4LargeKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  if (attribute != hipSuccess) return attribute;
-  hipLaunchKernelGGL(MxFp4LargeKernel, dim3(blocks), dim3(256), kLds, stream, call);
-  return hipGetLastError();
+  return ScalesNeedWords(call) ? Launch<true>(stream, call, blocks) : Launch<false>(stream, call, blocks);
 }
 
 }  // namespace mxfp4

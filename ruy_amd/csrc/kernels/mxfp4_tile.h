@@ -39,6 +39,53 @@ __device__ __forceinline__ void LoadToLds(uint32_t lds, uint32_t voffset, v4i rs
       : "memory");
 }
 
+// 4 bytes a lane.
+__device__ __forceinline__ void LoadWordToLds(uint32_t lds, uint32_t voffset, v4i rsrc) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(voffset), "s"(rsrc)
+      : "memory");
+}
+
+// Scales straight to LDS, 16 bytes of a row at a time, of which it has as many at least; where there are no 16 from `first` on the last
+// 16 are read, and put in place when they are read there. A load to LDS begins at a multiple of 4 bytes. kWords: rows that begin anywhere,
+// or whose number of scales is no multiple of 4: 16 bytes come as the five words that hold them (no byte outside these is read), four to
+// a lane and one to a lane, and are shifted. (Where rows are aligned it costs 4 % of 256x256 tiles' time and 10 of the
+// others'. 4096 x 4096 x 4064, whose rows have 127 scales: 41.4 us, on 128x128 with scales through registers 57.)
+template <bool kWords>
+struct ScaleRows {
+  static constexpr int kLoads = kWords ? 2 : 1;
+  static constexpr int kBytes = kWords ? 20 : 16;  // in LDS
+  v4i rsrc;
+  uint32_t at;  // the lane's row, in bytes from the resource's base (a multiple of 4)
+
+  __device__ __forceinline__ ScaleRows(const uint8_t* base, int64_t row_offset)
+      : rsrc(Resource(reinterpret_cast<const char*>(base) - (reinterpret_cast<uintptr_t>(base) & 3))),
+        at(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base) & 3) + static_cast<uint32_t>(row_offset)) {}
+  static __device__ __forceinline__ uint32_t From(int first, int count) { return static_cast<uint32_t>(min(first, count - 16)); }
+  __device__ __forceinline__ void Load(uint32_t lds, uint32_t lds_words, int first, int count) const {
+    if constexpr (kWords) {
+      const uint32_t from = at + From(first, count), whole = from & ~3u;
+      LoadToLds(lds, whole, rsrc, 0);
+      LoadWordToLds(lds_words, whole + (from & 3 ? 16 : 12), rsrc);
+    } else {
+      LoadToLds(lds, at, rsrc, __builtin_amdgcn_readfirstlane(From(first, count)));
+    }
+  }
+  // `x` and `fifth` (in LDS) are what Load brought.
+  static __device__ __forceinline__ v4i Place(v4i x, int fifth, uint32_t row_at, int first, int count) {
+    if constexpr (kWords) {
+      const uint32_t low = (row_at + From(first, count)) & 3;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<int>(__builtin_amdgcn_alignbyte(e < 3 ? x[e + 1] : fifth, x[e], low));
+    }
+    return granule::PlaceGranule(x, first, count);
+  }
+};
+
 constexpr int kStep = 8 * kBlock;  // depth positions to a step: 128 bytes
 
 // kDirect: rows of both sides begin at multiples of 4 bytes, which is what a load to LDS asks of an address, and are whole blocks, so
@@ -49,9 +96,9 @@ constexpr int kStep = 8 * kBlock;  // depth positions to a step: 128 bytes
 // kStages: steps on their way to LDS (kDirect), two or four.
 // How scales come to LDS. Through registers, a pair of steps ahead: the waves wait for these loads, and for those of all steps with
 // them, in every other step, which with more than two stages would be all that the other stages are for. All of the depth's first. Or, where
-// their rows begin at multiples of 4 bytes and have 16, as they lie, two pairs ahead: then each thread takes its own row's
-// out of LDS, and puts them back transposed.
-enum class ScaleLoads { kThroughRegisters, kAllFirst, kAhead };
+// a row has 16 of them, as they lie (ScaleRows, with kWords or without), two pairs ahead: then each thread takes its own row's out of
+// LDS, and puts them back transposed.
+enum class ScaleLoads { kThroughRegisters, kAllFirst, kAhead, kAheadWords };
 template <int kWavesM, int kWavesN, int kBlocksM, int kBlocksN, bool kDirect, int kStages, ScaleLoads kScaleLoads>
 __device__ __forceinline__ void MultiplyTile(const MulCall& c, const TileOf& tile, const Range& range, char* lds) {
   constexpr int kWaves = kWavesM * kWavesN;
@@ -60,7 +107,9 @@ __device__ __forceinline__ void MultiplyTile(const MulCall& c, const TileOf& til
   using M = TileSide<RUYAMD_DTYPE_BF16, Runs::kPlain, kTileM, kBlocksM, true, kWaves>;
   using N = TileSide<RUYAMD_DTYPE_BF16, Runs::kPlain, kTileN, kBlocksN, false, kWaves>;
   constexpr int kStage = M::kBytes + N::kBytes;
-  constexpr bool kAllScales = kScaleLoads == ScaleLoads::kAllFirst, kAhead = kScaleLoads == ScaleLoads::kAhead;
+  constexpr bool kAllScales = kScaleLoads == ScaleLoads::kAllFirst;
+  constexpr bool kAhead = kScaleLoads == ScaleLoads::kAhead || kScaleLoads == ScaleLoads::kAheadWords;
+  using Scaling = ScaleRows<kScaleLoads == ScaleLoads::kAheadWords>;
   constexpr bool kThrough = kScaleLoads == ScaleLoads::kThroughRegisters;
   static_assert(kDirect || (kStages == 2 && kThrough), "");
   constexpr int kRows = kTileM + kTileN, kScalesAt = kStages * kStage, kRawAt = kScalesAt + kRows * 16;
@@ -117,7 +166,7 @@ __device__ __forceinline__ void MultiplyTile(const MulCall& c, const TileOf& til
   };
   const auto put_scales_of_row = [&](const v4i& x, int row, int pair, int buffer) __attribute__((always_inline)) {
     *reinterpret_cast<v4i*>(lds + kScalesAt + buffer * (kRows * 16) + row * 16) =
-        Transposed(kAhead ? granule::PlaceGranule(x, pair * 16, row_scales) : PlaceScales(x, pair * 16, row_scales));
+        Transposed(kAhead ? x : PlaceScales(x, pair * 16, row_scales));
   };
   // A thread brings those of one row, pair by pair.
   const uint8_t* const scale_row = scales_of_row(threadIdx.x);
@@ -195,19 +244,21 @@ __device__ __forceinline__ void MultiplyTile(const MulCall& c, const TileOf& til
     if constexpr (kThrough) next_scales = fetch_scales(0);
     // (kAhead: two buffers, of pairs in turn.)
     const int my_row = threadIdx.x & ~63;  // the wave's first one
-    const uint32_t scales_off =
-        my_row < kTileM ? static_cast<uint32_t>(min(my_row + lane, here_m - 1) * c.lhs.scale_stride)
-                        : static_cast<uint32_t>(min(my_row - kTileM + lane, here_n - 1) * c.rhs.scale_stride);
-    const char* const scales_base =
-        reinterpret_cast<const char*>(my_row < kTileM ? c.lhs.scales + tile.group * c.lhs.scales_matrix_stride + m0 * c.lhs.scale_stride
-                                                      : c.rhs.scales + (int64_t(range.begin) + n0) * c.rhs.scale_stride);
-    const v4i scales_rsrc = Resource(scales_base);
+    const Scaling rows(my_row < kTileM ? c.lhs.scales + tile.group * c.lhs.scales_matrix_stride + m0 * c.lhs.scale_stride
+                                       : c.rhs.scales + (int64_t(range.begin) + n0) * c.rhs.scale_stride,
+                       my_row < kTileM ? min(my_row + lane, here_m - 1) * c.lhs.scale_stride
+                                       : min(my_row - kTileM + lane, here_n - 1) * c.rhs.scale_stride);
+    constexpr int kRawBytes = kRows * Scaling::kBytes;  // of a buffer: 16 bytes of all rows, and 4 bytes of all rows
     const auto load_raw = [&](int pair) __attribute__((always_inline)) {
-      LoadToLds(__builtin_amdgcn_readfirstlane(lds_base + kRawAt + (pair & 1) * (kRows * 16) + wave * 1024), scales_off,
-                scales_rsrc, __builtin_amdgcn_readfirstlane(min(pair * 16, row_scales - 16)));
+      const uint32_t to = lds_base + kRawAt + (pair & 1) * kRawBytes;
+      rows.Load(__builtin_amdgcn_readfirstlane(to + wave * 1024), __builtin_amdgcn_readfirstlane(to + kRows * 16 + wave * 256), pair * 16,
+                row_scales);
     };
     const auto read_raw = [&](int pair) __attribute__((always_inline)) {
-      return *reinterpret_cast<const v4i*>(lds + kRawAt + (pair & 1) * (kRows * 16) + threadIdx.x * 16);
+      const char* const from = lds + kRawAt + (pair & 1) * kRawBytes;
+      int fifth = 0;
+      if constexpr (Scaling::kLoads > 1) fifth = *reinterpret_cast<const int*>(from + kRows * 16 + threadIdx.x * 4);
+      return Scaling::Place(*reinterpret_cast<const v4i*>(from + threadIdx.x * 16), fifth, rows.at, pair * 16, row_scales);
     };
     if constexpr (kAhead) {
       load_raw(0);
@@ -252,8 +303,8 @@ __device__ __forceinline__ void MultiplyTile(const MulCall& c, const TileOf& til
         share(p, Reads(), [&](auto r) __attribute__((always_inline)) { read_one(r, kAt, 1, second); });
         __builtin_amdgcn_sched_barrier(0);
       });
-      // (kAhead: in odd steps with the load of scales that went out in the last one; in even ones what they hold has come.)
-      WaitVmcnt<(kStages - 2) * kLoads + (kAhead && kOdd ? 1 : 0)>();
+      // (kAhead: in odd steps with the loads of scales that went out in the last one; in even ones what they hold has come.)
+      WaitVmcnt<(kStages - 2) * kLoads + (kAhead && kOdd ? Scaling::kLoads : 0)>();
       if constexpr (kOdd && !kAllScales) put_scales(next_scales, (s + 1) / 2, 0);
       Barrier();
       if constexpr (!kOdd && kThrough) next_scales = fetch_scales(s / 2 + 1);

@@ -20,7 +20,7 @@ namespace {
 constexpr int kTileM = 256, kTileN = 128, kRows = kTileM + kTileN, kWaves = 4;
 constexpr int kBlocksM = 8, kBlocksN = 4;
 constexpr int kRowBytes = 64, kStages = 3, kStage = kRows * kRowBytes;
-constexpr int kScales = kStages * kStage, kLds = kScales + kRows * 16;
+constexpr int kScales = kStages * kStage, kFifths = kScales + kRows * 16, kLds = kFifths + kRows * 4;
 constexpr int kLoadsM = kTileM * kRowBytes / 1024 / kWaves, kLoadsN = kTileN * kRowBytes / 1024 / kWaves, kLoads = kLoadsM + kLoadsN;
 using Out = WriteBack<kBlocksM, kBlocksN>;
 static_assert(kWaves * Out::kLds <= kLds, "");
@@ -33,7 +33,9 @@ __device__ __forceinline__ int Key(int r) {
   return kM ? (r >> 3) & 3 : (r >> 2) & 3;
 }
 
+template <bool kWords>
 __global__ __launch_bounds__(64 * kWaves, 2) void MxFp4WideKernel(MulCall c) {
+  using Scaling = ScaleRows<kWords>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_m = wave & 1, wave_n = wave >> 1;
@@ -42,20 +44,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void MxFp4WideKernel(MulCall c) {
   if (!FindTile(c.offsets, c.groups, c.n, kTileN, (c.m + kTileM - 1) / kTileM, &tile, &range)) return;
   const int m0 = tile.m * kTileM, n0 = tile.n * kTileN;
   const int here_m = min(kTileM, c.m - m0), here_n = min(kTileN, range.count - n0);
-  const int steps = c.k / 128, row_scales = c.k / kBlock;
+  const int steps = (c.k + 127) / 128, row_scales = c.k / kBlock;
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
   // The loads: 16 rows each. (Rows past the tile's sides are the last one: they end up in rows of the tile that are not stored.)
   const v4i rsrc_m = Resource(reinterpret_cast<const char*>(c.lhs.data) + tile.group * c.lhs.matrix_bytes + m0 * c.lhs.row_bytes);
   const v4i rsrc_n = Resource(reinterpret_cast<const char*>(c.rhs.data) + (int64_t(range.begin) + n0) * c.rhs.row_bytes);
   uint32_t off[kLoads];
+  const auto row_of = [&](int n, int of_lane) __attribute__((always_inline)) {
+    return ((n < kLoadsM ? n : n - kLoadsM) * kWaves + wave) * 16 + (of_lane >> 2);
+  };
+  const auto granule_of = [&](int n, int of_lane) __attribute__((always_inline)) {
+    return (of_lane & 3) ^ (n < kLoadsM ? Key<true>(row_of(n, of_lane)) : Key<false>(row_of(n, of_lane)));
+  };
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const bool is_m = i < kLoadsM;
-    const int r = ((is_m ? i : i - kLoadsM) * kWaves + wave) * 16 + (lane >> 2);
-    off[i] = is_m ? static_cast<uint32_t>(min(r, here_m - 1) * c.lhs.row_bytes) + ((lane & 3) ^ Key<true>(r)) * 16
-                  : static_cast<uint32_t>(min(r, here_n - 1) * c.rhs.row_bytes) + ((lane & 3) ^ Key<false>(r)) * 16;
-  }
+  for (int n = 0; n < kLoads; ++n)
+    off[n] = static_cast<uint32_t>(n < kLoadsM ? min(row_of(n, lane), here_m - 1) * c.lhs.row_bytes : min(row_of(n, lane), here_n - 1) * c.rhs.row_bytes) +
+             granule_of(n, lane) * 16;
   const auto load = [&](auto number, int s, uint32_t stage_at) __attribute__((always_inline)) {
     constexpr int n = decltype(number)::value;
     constexpr int kTo = n < kLoadsM ? n * kWaves * 1024 : kTileM * kRowBytes + (n - kLoadsM) * kWaves * 1024;
@@ -63,15 +68,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void MxFp4WideKernel(MulCall c) {
               __builtin_amdgcn_readfirstlane(s * kRowBytes));
   };
   // Those of scales: 64 rows of the M side to a wave, and 64 of the N side to two waves, and to the other two again.
-  const v4i scales_m = Resource(reinterpret_cast<const char*>(c.lhs.scales) + tile.group * c.lhs.scales_matrix_stride + m0 * c.lhs.scale_stride);
-  const v4i scales_n = Resource(reinterpret_cast<const char*>(c.rhs.scales) + (int64_t(range.begin) + n0) * c.rhs.scale_stride);
-  const uint32_t scales_off_m = static_cast<uint32_t>(min(wave * 64 + lane, here_m - 1) * c.lhs.scale_stride);
-  const uint32_t scales_off_n = static_cast<uint32_t>(min((wave & 1) * 64 + lane, here_n - 1) * c.rhs.scale_stride);
+  const uint8_t* const scales_m = c.lhs.scales + tile.group * c.lhs.scales_matrix_stride + m0 * c.lhs.scale_stride;
+  const uint8_t* const scales_n = c.rhs.scales + (int64_t(range.begin) + n0) * c.rhs.scale_stride;
+  const Scaling rows_m(scales_m, min(wave * 64 + lane, here_m - 1) * c.lhs.scale_stride);
+  const Scaling rows_n(scales_n, min((wave & 1) * 64 + lane, here_n - 1) * c.rhs.scale_stride);
   const auto load_scales = [&](int chunk) __attribute__((always_inline)) {
-    // (The last 16 of a row, where there are no 16 more.)
-    const uint32_t from = __builtin_amdgcn_readfirstlane(min(chunk * 16, row_scales - 16));
-    LoadToLds(__builtin_amdgcn_readfirstlane(lds_base + kScales + wave * 1024), scales_off_m, scales_m, from);
-    LoadToLds(__builtin_amdgcn_readfirstlane(lds_base + kScales + (kTileM / 64 + (wave & 1)) * 1024), scales_off_n, scales_n, from);
+    const int n = kTileM / 64 + (wave & 1);
+    rows_m.Load(__builtin_amdgcn_readfirstlane(lds_base + kScales + wave * 1024), __builtin_amdgcn_readfirstlane(lds_base + kFifths + wave * 256),
+                chunk * 16, row_scales);
+    rows_n.Load(__builtin_amdgcn_readfirstlane(lds_base + kScales + n * 1024), __builtin_amdgcn_readfirstlane(lds_base + kFifths + n * 256),
+                chunk * 16, row_scales);
   };
 
   const int a_row = wave_m * 128 + (l >> 2) * 8 + (l & 3), b_row = wave_n * 64 + l;
@@ -79,22 +85,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void MxFp4WideKernel(MulCall c) {
   const char* const a_at = lds + a_row * kRowBytes + slot;
   const char* const b_at = lds + (kTileM + b_row) * kRowBytes + slot;
   const auto offset_of_a = [](int i) { return (i >> 1) * 32 + (i & 1) * 4; };  // rows
-  const uint32_t selector = ColumnSelector(q);
   int sa[kBlocksM], sb[kBlocksN];
+  // What is needed once to four steps, or at the end, is made of the lane's number then: registers are few.
+  const auto lane_again = [&]() __attribute__((always_inline)) {
+    int v = threadIdx.x;
+    asm volatile("" : "+v"(v));
+    return v & 63;
+  };
   const auto read_scales = [&](int chunk) __attribute__((always_inline)) {
-    v4i raw[kBlocksM + kBlocksN];
+    const int lane2 = lane_again(), l2 = lane2 & 15;
+    const int a_row2 = wave_m * 128 + (l2 >> 2) * 8 + (l2 & 3), b_row2 = wave_n * 64 + l2;
+    const uint32_t selector = ColumnSelector(lane2 >> 4);
+    // (A lane's rows of a side are multiples of 4 apart: what is left of their addresses by 4 is the same.)
+    const uint32_t a_low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(scales_m)) + static_cast<uint32_t>(a_row2) * static_cast<uint32_t>(c.lhs.scale_stride);
+    const uint32_t b_low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(scales_n)) + static_cast<uint32_t>(b_row2) * static_cast<uint32_t>(c.rhs.scale_stride);
+    const auto column = [&](int row, uint32_t low) __attribute__((always_inline)) {
+      int fifth = 0;
+      if constexpr (kWords) fifth = *reinterpret_cast<const int*>(lds + kFifths + row * 4);
+      const v4i x = *reinterpret_cast<const v4i*>(lds + kScales + row * 16);
+      return ColumnOf(Scaling::Place(x, fifth, low, chunk * 16, row_scales), selector);
+    };
 #pragma unroll
-    for (int j = 0; j < kBlocksN; ++j) raw[j] = *reinterpret_cast<const v4i*>(lds + kScales + (kTileM + b_row + j * 16) * 16);
+    for (int j = 0; j < kBlocksN; ++j) sb[j] = column(kTileM + b_row2 + j * 16, b_low);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kBlocksM; ++i) raw[kBlocksN + i] = *reinterpret_cast<const v4i*>(lds + kScales + (a_row + offset_of_a(i)) * 16);
-    if (chunk * 16 + 16 > row_scales) {
-#pragma unroll
-      for (int i = 0; i < kBlocksM + kBlocksN; ++i) raw[i] = granule::PlaceGranule(raw[i], chunk * 16, row_scales);
+    for (int i = 0; i < kBlocksM; ++i) {
+      sa[i] = column(a_row2 + offset_of_a(i), a_low);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int j = 0; j < kBlocksN; ++j) sb[j] = ColumnOf(raw[j], selector);
-#pragma unroll
-    for (int i = 0; i < kBlocksM; ++i) sa[i] = ColumnOf(raw[kBlocksN + i], selector);
   };
 
   v4f acc[kBlocksM][kBlocksN] = {};
@@ -107,13 +125,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void MxFp4WideKernel(MulCall c) {
   // out with them, are all that is left.
   const auto step = [&](int s, auto part) __attribute__((always_inline)) {
     constexpr int kPart = decltype(part)::value;
-    WaitVmcnt<kLoads + (kPart == 2 ? 2 : 0)>();
+    WaitVmcnt<kLoads + (kPart == 2 ? 2 * Scaling::kLoads : 0)>();
     Barrier();
     if constexpr (kPart == 0) read_scales(s / 4);
     if constexpr (kPart == 1) load_scales(s / 4 + 1);  // (all waves have read the ones before)
-    if (s + 2 == steps) {
+    const int left = row_scales - (s + 2) * 4;  // granules of the step that is loaded
+    if (left < 4) {
+      const int of_lane = lane_again();
 #pragma unroll
-      for (int n = 0; n < kLoads; ++n) off[n] = kNothing;  // (from here on zeros, to where nobody reads)
+      for (int n = 0; n < kLoads; ++n)
+        if (granule_of(n, of_lane) >= left) off[n] = kNothing;  // (zeros past the depth, from here on)
     }
     v4i a[kBlocksM], b[kBlocksN];
 #pragma unroll
@@ -149,14 +170,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void MxFp4WideKernel(MulCall c) {
       int64_t(range.begin) + n0 + column0, here_m - row0, here_n - column0}();
 }
 
+template <bool kWords>
+hipError_t Launch(hipStream_t stream, const MulCall& call, unsigned blocks) {
+  static const hipError_t attribute =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&MxFp4WideKernel<kWords>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (attribute != hipSuccess) return attribute;
+  hipLaunchKernelGGL(MxFp4WideKernel<kWords>, dim3(blocks), dim3(64 * kWaves), kLds, stream, call);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t LaunchWide(hipStream_t stream, const MulCall& call, unsigned blocks) {
-  static const hipError_t attribute =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(MxFp4WideKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  if (attribute != hipSuccess) return attribute;
-  hipLaunchKernelGGL(MxFp4WideKernel, dim3(blocks), dim3(64 * kWaves), kLds, stream, call);
-  return hipGetLastError();
+  return ScalesNeedWords(call) ? Launch<true>(stream, call, blocks) : Launch<false>(stream, call, blocks);
 }
 
 }  // namespace mxfp4

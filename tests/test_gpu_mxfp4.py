@@ -372,6 +372,32 @@ def test_tiles_of_steps_of_128(context, k):
         context.force_tile(0, 0)
 
 
+@pytest.mark.parametrize("tile", [(128, 128, 1), (256, 128, 0), (256, 256, 0)])
+@pytest.mark.parametrize("k", [512, 544, 576, 608, 640, 992, 1056, 1120, 1184, 2080, 4064])
+def test_scales_at_any_address(context, tile, k):
+    """Rows of scales of any number and any distance, beginning anywhere, where they go to LDS as they lie; the last ones end with their
+    memory."""
+    context.force_tile(*tile)
+    try:
+        for pad, shift in ((0, 0), (1, 4), (2, 12), (3, 4)):
+            run_mul(context, S.BF16, 300, 140, k, None, (0, pad, 16, 0), shift, seed=pad)
+            run_mul(context, S.F32, 70, 300, k, np.array([0, 33, 33, 200, 300]), (4, 0, 0, pad), shift, 4 * pad + 4, COL, 1, True, 0.0, seed=pad)
+        rng = np.random.default_rng(k)
+        m, n = 129, 131
+        held = []
+        for rows in (m, n):
+            numbers, scales = rng.integers(0, 16, (rows, k), dtype=np.uint8), rng.integers(126, 129, (rows, k // 32)).astype(np.uint8)
+            odd = torch.zeros(rows * (k // 32) + 1, dtype=torch.uint8, device="cuda")
+            odd[1:] = torch.from_numpy(scales).flatten()
+            held.append((api.MxFp4Matrix(rows, k, torch.from_numpy(Q.pack(numbers)).cuda(), odd.data_ptr() + 1), odd, Q.values(numbers, scales)))
+        y = torch.full((n, m), -77.0, device="cuda")
+        api.mul_mxfp4(held[0][0], held[1][0], params_of(S.F32), context, api.Matrix(S.F32, y, api.Layout(m, n, m, COL)))
+        assert torch.equal(y.double(), torch.from_numpy(held[1][2] @ held[0][2].T).cuda())
+        assert context.last_kernel_name() == "mxfp4_mfma"
+    finally:
+        context.force_tile(0, 0)
+
+
 @pytest.mark.parametrize("k", [512, 640, 768, 896, 1024, 1152, 1280, 1408, 1536, 2048, 2176, 2688, 4096, 4224, 7168])
 def test_the_largest_tile(context, k):
     """Odd and even numbers of steps and of pairs of steps, whole and cut short by one to three quarters of 512."""
@@ -385,7 +411,7 @@ def test_the_largest_tile(context, k):
 
 
 @pytest.mark.parametrize("m,n,k,offsets", [
-    (4200, 4352, 512, None), (4352, 4096, 640, None), (5120, 3700, 1152, None), (16384, 1100, 512, None),
+    (4200, 4352, 512, None), (4352, 4096, 640, None), (5120, 3700, 1152, None), (4352, 4090, 1120, None), (4352, 4096, 544, None), (16384, 1100, 512, None),
     (2048, 9000, 512, [0, 1874, 3199, 4281, 5218, 6056, 6821, 7530, 9000]), (4096, 4480, 768, [0, 0, 4400, 4401, 4480]),
     (512, 33300, 512, list(range(0, 33301, 333)))])
 def test_tiles_left_after_full_rounds(context, m, n, k, offsets):
