@@ -63,6 +63,15 @@ struct Unit {
 #pragma unroll
     for (int i = 0; i < kGranules; ++i) raw[i] = reinterpret_cast<const v4i_unaligned*>(row + first * Bytes(kType))[i];
   }
+  // Where the row ends `left` values behind `row` (maybe inside the unit, or in front of it): zeros behind. (It has 16 bytes; all lanes
+  // load at once, which those that end the row would not if they took its last values one by one.)
+  __device__ __forceinline__ void LoadEnd(const char* row, int first, int left) {
+#pragma unroll
+    for (int i = 0; i < kGranules; ++i)
+      raw[i] = granule::LoadGranule<false>(reinterpret_cast<const uint8_t*>(row), first * Bytes(kType) + i * 16, left * Bytes(kType));
+#pragma unroll
+    for (int i = 0; i < kGranules; ++i) raw[i] = granule::PlaceGranule(raw[i], first * Bytes(kType) + i * 16, left * Bytes(kType));
+  }
   __device__ __forceinline__ void Values(float (&v)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -112,11 +121,6 @@ __global__ __launch_bounds__(256) void QuantizeKernel(ConvertCall c, int segment
     float v[kUnits][8];
     uint32_t packed[kUnits];
     int scale[kUnits];
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[u][e] = 0;
-    }
     if (whole) {
       Unit<kType> held[kUnits];
 #pragma unroll
@@ -124,19 +128,13 @@ __global__ __launch_bounds__(256) void QuantizeKernel(ConvertCall c, int segment
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) held[u].Values(v[u]);
     } else {
+      const int64_t segment = int64_t(piece.segment) * (512 * kUnits);
+      Unit<kType> held[kUnits];
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int64_t first = (unit0 + u * 64) * 8;
-        if (first + 8 <= cols) {
-          Unit<kType> held;
-          held.Load(from, first);
-          held.Values(v[u]);
-        } else {
+      for (int u = 0; u < kUnits; ++u)
+        held[u].LoadEnd(from + segment * Bytes(kType), (u * 64 + lane) * 8, static_cast<int>(cols - segment));
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (first + e < cols) v[u][e] = LoadFloat(from, kType, first + e);
-        }
-      }
+      for (int u = 0; u < kUnits; ++u) held[u].Values(v[u]);
     }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
@@ -223,6 +221,78 @@ __global__ __launch_bounds__(256) void DequantizeKernel(ConvertCall c, int segme
   }
 }
 
+// ---- Rows of 256 values or less ----
+//
+// kLanes lanes have a row, a unit of 8 values each: 64 / kLanes rows to a wave. (100000 x 128 bfloat16 values, a wave to a row and so: 57 and 8 us,
+// back 72 and 8.6.)
+
+template <int kType, int kLanes>
+__global__ __launch_bounds__(256) void NarrowQuantizeKernel(ConvertCall c) {
+  const int cols = c.matrix.cols, mine = threadIdx.x & (kLanes - 1), first = mine * 8;
+  for (int64_t row0 = int64_t(blockIdx.x) * (256 / kLanes); row0 < c.rows; row0 += int64_t(gridDim.x) * (256 / kLanes)) {
+    const int64_t row = row0 + threadIdx.x / kLanes;
+    const bool there = row < c.rows && first < cols;  // (all lanes go through the exchanges)
+    const char* const from = static_cast<const char*>(c.data) + row * c.rs * Bytes(kType);
+    float v[8] = {};
+    if (there && cols * Bytes(kType) >= 16) {
+      Unit<kType> held;
+      held.LoadEnd(from, first, cols);
+      held.Values(v);
+    } else if (there) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (first + e < cols) v[e] = LoadFloat(from, kType, first + e);
+    }
+    uint32_t largest = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(v[e]) & 0x7fffffffu);
+    const int scale = ScaleOf(LargestOfFour(largest));
+    const float inverse = InverseOf(scale);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= inverse;
+    const uint32_t packed = scale == kNaNScale ? 0 : Round8(v);
+    if (!there) continue;
+    ForEachPlace(c, static_cast<int>(row), [&](int to) __attribute__((always_inline)) {
+      uint8_t* const data = c.matrix.data + to * c.matrix.row_bytes;
+      if ((mine & 3) == 0) c.matrix.scales[to * c.matrix.scale_stride + first / kBlock] = static_cast<uint8_t>(scale);
+      if (first + 8 <= cols) {
+        *reinterpret_cast<u32_unaligned*>(data + first / 2) = packed;
+      } else {
+        for (int b = 0; b < (cols - first + 1) / 2; ++b) data[first / 2 + b] = static_cast<uint8_t>(packed >> (8 * b));
+      }
+    });
+  }
+}
+
+template <int kType, int kLanes>
+__global__ __launch_bounds__(256) void NarrowDequantizeKernel(ConvertCall c) {
+  const int cols = c.matrix.cols, first = (threadIdx.x & (kLanes - 1)) * 8;
+  if (first >= cols) return;
+  for (int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes; row < c.rows; row += int64_t(gridDim.x) * (256 / kLanes)) {
+    const uint8_t* const data = c.matrix.data + row * c.matrix.row_bytes;
+    char* const to = static_cast<char*>(c.data) + row * c.rs * Bytes(kType);
+    const float power = PowerOf(c.matrix.scales[row * c.matrix.scale_stride + first / kBlock]);
+    uint32_t packed = 0;
+    if (first + 8 <= cols) {
+      packed = *reinterpret_cast<const u32_unaligned*>(data + first / 2);
+    } else {
+      for (int b = 0; b < 4; ++b)
+        if (first + 2 * b < cols) packed |= uint32_t(data[first / 2 + b]) << (8 * b);
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = ValueOf(packed >> (4 * e) & 15) * power;
+    if (first + 8 <= cols) {
+      Unit<kType> held;
+      held.Store(to, first, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (first + e < cols) StoreFloat(to, kType, first + e, v[e]);
+    }
+  }
+}
+
 // ---- Any order and stride ----
 
 __global__ __launch_bounds__(256) void GenericQuantizeKernel(ConvertCall c) {
@@ -268,28 +338,49 @@ unsigned BlocksFor(int64_t work, int threads) {
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((work + threads - 1) / threads, 1 << 20)));
 }
 
-// Segments of 64 * units units, and how many units: as many as leave every CU some waves.
+// Segments of 64 * units units, and how many units: no more than a row has, and as many as leave every CU some waves.
 template <class F>
 void WithUnits(const ConvertCall& c, int compute_units, F&& f) {
   const auto segments = [&](int units) { return (int64_t(c.matrix.cols) + 512 * units - 1) / (512 * units); };
   const auto launch = [&](auto units) { f(units, int(segments(units)), BlocksFor(c.rows * segments(units), 4)); };
-  if (c.rows * segments(4) >= int64_t(16) * compute_units) return launch(std::integral_constant<int, 4>());
+  const int64_t enough = int64_t(16) * compute_units;
+  if (c.matrix.cols > 1024 && c.rows * segments(4) >= enough) return launch(std::integral_constant<int, 4>());
+  if (c.matrix.cols > 512 && c.rows * segments(2) >= enough) return launch(std::integral_constant<int, 2>());
   launch(std::integral_constant<int, 1>());
+}
+// Lanes to a narrow row: f(lanes as a constant, blocks), or false for one that is not narrow.
+template <class F>
+bool WithLanes(const ConvertCall& c, F&& f) {
+  const auto launch = [&](auto lanes) { f(lanes, BlocksFor(int64_t(c.rows) * decltype(lanes)::value, 256)); };
+  if (c.matrix.cols > 256) return false;
+  if (c.matrix.cols > 128)
+    launch(std::integral_constant<int, 32>());
+  else if (c.matrix.cols > 64)
+    launch(std::integral_constant<int, 16>());
+  else
+    launch(std::integral_constant<int, 8>());
+  return true;
+}
+// f(type as a constant).
+template <class F>
+void WithType(int type, F&& f) {
+  if (type == RUYAMD_DTYPE_BF16) return f(std::integral_constant<int, RUYAMD_DTYPE_BF16>());
+  if (type == RUYAMD_DTYPE_F16) return f(std::integral_constant<int, RUYAMD_DTYPE_F16>());
+  f(std::integral_constant<int, RUYAMD_DTYPE_F32>());
 }
 
 }  // namespace
 
 bool LaunchQuantize(hipStream_t stream, const ConvertCall& c, int compute_units, hipError_t* status) {
   if (c.cs != 1 && c.matrix.cols != 1) return false;
-  WithUnits(c, compute_units, [&](auto units, int segments, unsigned blocks) {
-    constexpr int kUnits = decltype(units)::value;
-    const dim3 grid(blocks), block(256);
-    if (c.type == RUYAMD_DTYPE_BF16)
-      hipLaunchKernelGGL((QuantizeKernel<RUYAMD_DTYPE_BF16, kUnits>), grid, block, 0, stream, c, segments);
-    else if (c.type == RUYAMD_DTYPE_F16)
-      hipLaunchKernelGGL((QuantizeKernel<RUYAMD_DTYPE_F16, kUnits>), grid, block, 0, stream, c, segments);
-    else
-      hipLaunchKernelGGL((QuantizeKernel<RUYAMD_DTYPE_F32, kUnits>), grid, block, 0, stream, c, segments);
+  WithType(c.type, [&](auto type) {
+    constexpr int kType = decltype(type)::value;
+    const bool narrow = WithLanes(c, [&](auto lanes, unsigned blocks) {
+      hipLaunchKernelGGL((NarrowQuantizeKernel<kType, decltype(lanes)::value>), dim3(blocks), dim3(256), 0, stream, c);
+    });
+    if (!narrow) WithUnits(c, compute_units, [&](auto units, int segments, unsigned blocks) {
+      hipLaunchKernelGGL((QuantizeKernel<kType, decltype(units)::value>), dim3(blocks), dim3(256), 0, stream, c, segments);
+    });
   });
   *status = hipGetLastError();
   return true;
@@ -297,15 +388,14 @@ bool LaunchQuantize(hipStream_t stream, const ConvertCall& c, int compute_units,
 
 bool LaunchDequantize(hipStream_t stream, const ConvertCall& c, int compute_units, hipError_t* status) {
   if (c.cs != 1 && c.matrix.cols != 1) return false;
-  WithUnits(c, compute_units, [&](auto units, int segments, unsigned blocks) {
-    constexpr int kUnits = decltype(units)::value;
-    const dim3 grid(blocks), block(256);
-    if (c.type == RUYAMD_DTYPE_BF16)
-      hipLaunchKernelGGL((DequantizeKernel<RUYAMD_DTYPE_BF16, kUnits>), grid, block, 0, stream, c, segments);
-    else if (c.type == RUYAMD_DTYPE_F16)
-      hipLaunchKernelGGL((DequantizeKernel<RUYAMD_DTYPE_F16, kUnits>), grid, block, 0, stream, c, segments);
-    else
-      hipLaunchKernelGGL((DequantizeKernel<RUYAMD_DTYPE_F32, kUnits>), grid, block, 0, stream, c, segments);
+  WithType(c.type, [&](auto type) {
+    constexpr int kType = decltype(type)::value;
+    const bool narrow = WithLanes(c, [&](auto lanes, unsigned blocks) {
+      hipLaunchKernelGGL((NarrowDequantizeKernel<kType, decltype(lanes)::value>), dim3(blocks), dim3(256), 0, stream, c);
+    });
+    if (!narrow) WithUnits(c, compute_units, [&](auto units, int segments, unsigned blocks) {
+      hipLaunchKernelGGL((DequantizeKernel<kType, decltype(units)::value>), dim3(blocks), dim3(256), 0, stream, c, segments);
+    });
   });
   *status = hipGetLastError();
   return true;

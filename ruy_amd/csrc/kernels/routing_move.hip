@@ -168,6 +168,61 @@ __global__ __launch_bounds__(256) void CombineKernel(Call c, int segments) {
   }
 }
 
+// ---- The same for narrow tokens ----
+//
+// A token of so few units that kLanes lanes have one each: 64 / kLanes tokens to a wave. (us, 100000 tokens of 128 values in bfloat16 with two
+// places each, a wave to a token and these: to their places 24 and 10, added up 70 and 15, gradients 64 and 30; 12991 tokens of 151 values
+// in half added up 9.9 and 5.5.)
+
+template <int kBytes, int kLanes, bool kStreamed>
+__global__ __launch_bounds__(256) void NarrowDispatchKernel(Call c) {
+  const int64_t bytes = int64_t(c.width) * kBytes;
+  const int first = (threadIdx.x & (kLanes - 1)) * 16;
+  if (first >= bytes) return;
+  const int64_t at = min(int64_t(first), bytes - 16);
+  for (int64_t token = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes; token < c.tokens; token += int64_t(gridDim.x) * (256 / kLanes)) {
+    const v4i held =
+        *reinterpret_cast<const v4i_unaligned*>(static_cast<const char*>(c.token_side.data) + token * c.token_side.cs * kBytes + at);
+    for (int j = 0; j < c.top; ++j) {
+      const int place = PlaceOf(c, token, j);
+      if (place >= 0)
+        StoreGranule<kStreamed>(
+            reinterpret_cast<v4i_unaligned*>(static_cast<char*>(c.place_side.data) + place * c.place_side.cs * kBytes + at), held);
+    }
+  }
+}
+
+template <int kType, int kDstType, int kLanes, bool kStreamed>
+__global__ __launch_bounds__(256) void NarrowCombineKernel(Call c) {
+  constexpr int kValues = 16 / Bytes(kType), kAtOnce = 4;
+  const int first = (threadIdx.x & (kLanes - 1)) * kValues;
+  if (first >= c.width) return;
+  const int64_t at = min(first, c.width - kValues);
+  for (int64_t token = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes; token < c.tokens; token += int64_t(gridDim.x) * (256 / kLanes)) {
+    float sum[kValues] = {};
+    for (int j0 = 0; j0 < c.top; j0 += kAtOnce) {
+      v4i held[kAtOnce][1];
+      int place[kAtOnce];
+      float weight[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) place[j] = j0 + j < c.top ? PlaceOf(c, token, j0 + j) : -1;
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (place[j] < 0) continue;
+        weight[j] = WeightOf(c, token, j0 + j);
+        Load<kType, kValues>(c.place_side.data, place[j] * c.place_side.cs + at, held[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (place[j] < 0) continue;
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) sum[e] += weight[j] * Value<kType, kValues>(held[j], e);
+      }
+    }
+    Store<kDstType, kValues, kStreamed>(c.token_side.data, token * c.token_side.cs + at, sum);
+  }
+}
+
 // ---- The gradients of that sum ----
 
 // The lanes' values added up, in every lane, always in the same order: over 2, 4, 8 and 16 neighbours, then over the four rows of 16.
@@ -287,6 +342,69 @@ __global__ __launch_bounds__(64 * kMostWaves) void GradientsKernel(Call c, int w
   }
 }
 
+// Narrow tokens, kLanes lanes to each (as above).
+template <int kType, int kGradType, int kLanes, bool kStreamed>
+__global__ __launch_bounds__(256) void NarrowGradientsKernel(Call c) {
+  constexpr int kValues = 16 / Bytes(kType), kAtOnce = 4;
+  const int mine = threadIdx.x & (kLanes - 1), first = mine * kValues;
+  const bool active = first < c.width;  // (all lanes go through the sums)
+  const int64_t at = min(first, c.width - kValues);
+  const int again = static_cast<int>(min(int64_t(first) - at, int64_t(kValues)));  // values that the lane before has too
+  const bool rows = c.grad_src.data, weights = c.grad_weights.data;
+  const int64_t tokens_here = 256 / kLanes, stride = int64_t(gridDim.x) * tokens_here;
+  for (int64_t token0 = int64_t(blockIdx.x) * tokens_here; token0 < c.tokens; token0 += stride) {
+    const int64_t token = token0 + threadIdx.x / kLanes;
+    const bool there = active && token < c.tokens;
+    v4i raw[kValues * Bytes(kGradType) / 16];
+    float grad[kValues] = {};
+    if (there) {
+      Load<kGradType, kValues>(c.token_side.data, token * c.token_side.cs + at, raw);
+#pragma unroll
+      for (int e = 0; e < kValues; ++e) grad[e] = Value<kGradType, kValues>(raw, e);
+    }
+    for (int j0 = 0; j0 < c.top; j0 += kAtOnce) {
+      int place[kAtOnce];
+      v4i held[kAtOnce][1];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) place[j] = there && j0 + j < c.top ? PlaceOf(c, token, j0 + j) : -1;
+      if (weights) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+          if (place[j] >= 0) Load<kType, kValues>(c.place_side.data, place[j] * c.place_side.cs + at, held[j]);
+      }
+      if (rows) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          if (place[j] < 0) continue;
+          const float weight = WeightOf(c, token, j0 + j);
+          float v[kValues];
+#pragma unroll
+          for (int e = 0; e < kValues; ++e) v[e] = weight * grad[e];
+          Store<kType, kValues, kStreamed>(c.grad_src.data, place[j] * c.grad_src.cs + at, v);
+        }
+      }
+      if (weights) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          if (j0 + j >= c.top) break;
+          float dot = 0;
+          if (place[j] >= 0) {
+#pragma unroll
+            for (int e = 0; e < kValues; ++e) {
+              const float product = grad[e] * Value<kType, kValues>(held[j], e);
+              dot += e >= again ? product : 0.0f;
+            }
+          }
+#pragma unroll
+          for (int d = 1; d < kLanes; d *= 2) dot += __shfl_xor(dot, d);
+          if (mine == 0 && there)
+            StoreFloat(c.grad_weights.data, c.grad_weights.type, (j0 + j) * c.grad_weights.rs + token * c.grad_weights.cs, dot);
+        }
+      }
+    }
+  }
+}
+
 // ---- One value to a lane ----
 
 constexpr unsigned kMostBlocks = 1u << 20;
@@ -369,7 +487,8 @@ __global__ __launch_bounds__(256) void GenericWeightGradientsKernel(Call c) {
 // Whether a view's values of a token lie side by side (one value alone does).
 bool SideBySide(const Call& c, const View& v) { return !v.data || v.rs == 1 || c.width == 1; }
 
-// Segments of 64 * units units of 16 bytes, and how many units: as many as leave every CU some waves. f(units as a
+// Segments of 64 * units units of 16 bytes, and how many units: no more than a row has (100000 tokens of 512 values in bfloat16 added up with
+// four units 72.7 us, with one 49.7), and as many as leave every CU some waves. f(units as a
 // constant, segments, blocks).
 template <class F>
 void WithUnits(const Call& c, int type, int compute_units, F&& f) {
@@ -377,8 +496,8 @@ void WithUnits(const Call& c, int type, int compute_units, F&& f) {
   const auto segments = [&](int units) { return (c.width + unit * units - 1) / (unit * units); };
   const auto blocks = [&](int64_t s) { return BlocksFor(c.tokens * s, 4); };
   const int64_t enough = int64_t(16) * compute_units;
-  if (c.tokens * segments(4) >= enough) return f(std::integral_constant<int, 4>(), int(segments(4)), blocks(segments(4)));
-  if (c.tokens * segments(2) >= enough) return f(std::integral_constant<int, 2>(), int(segments(2)), blocks(segments(2)));
+  if (c.width > 2 * unit && c.tokens * segments(4) >= enough) return f(std::integral_constant<int, 4>(), int(segments(4)), blocks(segments(4)));
+  if (c.width > unit && c.tokens * segments(2) >= enough) return f(std::integral_constant<int, 2>(), int(segments(2)), blocks(segments(2)));
   f(std::integral_constant<int, 1>(), int(segments(1)), blocks(segments(1)));
 }
 
@@ -390,6 +509,20 @@ template <class F>
 void WithStores(int64_t bytes, F&& f) {
   if (bytes >= kStreamFrom) return f(std::true_type());
   f(std::false_type());
+}
+
+// Lanes to a narrow token: f(lanes as a constant), or false for one that is not narrow.
+template <class F>
+bool WithLanes(const Call& c, int type, F&& f) {
+  const int64_t units = (int64_t(c.width) * Bytes(type) + 15) / 16;
+  if (units > 32) return false;
+  if (units > 16)
+    f(std::integral_constant<int, 32>());
+  else if (units > 8)
+    f(std::integral_constant<int, 16>());
+  else
+    f(std::integral_constant<int, 8>());
+  return true;
 }
 
 // f(type of the rows, other type): the other is the rows' or fp32.
@@ -408,7 +541,18 @@ void WithTypes(int type, int other, F&& f) {
 bool LaunchDispatch(hipStream_t stream, const Call& c, int compute_units, hipError_t* status) {
   const int type = c.token_side.type;
   if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side)) return false;
-  WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
+  const bool narrow = WithLanes(c, type, [&](auto lanes) {
+    constexpr int kLanes = decltype(lanes)::value;
+    WithStores(int64_t(c.tokens) * c.top * c.width * Bytes(type), [&](auto streamed) {
+      constexpr bool kStreamed = decltype(streamed)::value;
+      const dim3 grid(BlocksFor(int64_t(c.tokens) * kLanes, 256));
+      if (type == RUYAMD_DTYPE_F32)
+        hipLaunchKernelGGL((NarrowDispatchKernel<4, kLanes, kStreamed>), grid, dim3(256), 0, stream, c);
+      else
+        hipLaunchKernelGGL((NarrowDispatchKernel<2, kLanes, kStreamed>), grid, dim3(256), 0, stream, c);
+    });
+  });
+  if (!narrow) WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
     constexpr int kUnits = decltype(units)::value;
     WithStores(int64_t(c.tokens) * c.top * c.width * Bytes(type), [&](auto streamed) {
       constexpr bool kStreamed = decltype(streamed)::value;
@@ -425,7 +569,16 @@ bool LaunchDispatch(hipStream_t stream, const Call& c, int compute_units, hipErr
 bool LaunchCombine(hipStream_t stream, const Call& c, int compute_units, hipError_t* status) {
   const int type = c.place_side.type;
   if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side)) return false;
-  WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
+  const bool narrow = WithLanes(c, type, [&](auto lanes) {
+    WithTypes(type, c.token_side.type, [&](auto t, auto dst) {
+      constexpr int kType = decltype(t)::value, kDst = decltype(dst)::value, kLanes = decltype(lanes)::value;
+      WithStores(int64_t(c.tokens) * c.width * Bytes(kDst), [&](auto streamed) {
+        hipLaunchKernelGGL((NarrowCombineKernel<kType, kDst, kLanes, decltype(streamed)::value>),
+                           dim3(BlocksFor(int64_t(c.tokens) * kLanes, 256)), dim3(256), 0, stream, c);
+      });
+    });
+  });
+  if (!narrow) WithUnits(c, type, compute_units, [&](auto units, int segments, unsigned blocks) {
     WithTypes(type, c.token_side.type, [&](auto t, auto dst) {
       constexpr int kType = decltype(t)::value, kDst = decltype(dst)::value, kUnits = decltype(units)::value;
       WithStores(int64_t(c.tokens) * c.width * Bytes(kDst), [&](auto streamed) {
@@ -441,6 +594,19 @@ bool LaunchGradients(hipStream_t stream, const Call& c, int compute_units, hipEr
   const int type = c.place_side.type;
   if (c.width < 16 / Bytes(type) || !SideBySide(c, c.token_side) || !SideBySide(c, c.place_side) || !SideBySide(c, c.grad_src))
     return false;
+  const bool narrow = WithLanes(c, type, [&](auto lanes) {
+    WithTypes(type, c.token_side.type, [&](auto t, auto grad) {
+      constexpr int kType = decltype(t)::value, kGrad = decltype(grad)::value, kLanes = decltype(lanes)::value;
+      WithStores(c.grad_src.data ? int64_t(c.tokens) * c.top * c.width * Bytes(kType) : 0, [&](auto streamed) {
+        hipLaunchKernelGGL((NarrowGradientsKernel<kType, kGrad, kLanes, decltype(streamed)::value>),
+                           dim3(BlocksFor(int64_t(c.tokens) * kLanes, 256)), dim3(256), 0, stream, c);
+      });
+    });
+  });
+  if (narrow) {
+    *status = hipGetLastError();
+    return true;
+  }
   // Waves to a token: as few as leave every CU 16, each with a unit at least.
   const int64_t units = (c.width + 64 * (16 / Bytes(type)) - 1) / (64 * (16 / Bytes(type)));
   int waves = 1;

@@ -96,7 +96,10 @@ def spread_values(rng, rows, cols, type_):
     return x
 
 
-CONVERTED = [(1, 1), (1, 32), (3, 31), (2, 33), (5, 7), (4, 64), (7, 515), (3, 2048), (2, 4104), (300, 2051), (40, 8192), (1, 16384)]
+CONVERTED = [(1, 1), (1, 32), (3, 31), (2, 33), (5, 7), (4, 64), (7, 515), (3, 2048), (2, 4104), (300, 2051), (40, 8192), (1, 16384),
+             # Several rows to a wave, and just not; rows that end in a unit, alone in a segment or not.
+             (700, 3), (701, 8), (333, 12), (515, 63), (1000, 96), (130, 129), (257, 250), (65, 256), (300, 257), (4100, 300), (5000, 600),
+             (4200, 1025), (2100, 2050), (4099, 770)]
 
 
 @pytest.mark.parametrize("type_", TYPES, ids=name_of)
@@ -183,7 +186,7 @@ def test_dequantize_of_every_number_and_scale(context, kernel, type_):
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(9, 8, 7), want.nan_to_num(9, 8, 7))
 
 
-@pytest.mark.parametrize("tokens,top,cols", [(1, 8, 2048), (40, 2, 515), (300, 4, 4096), (9, 3, 33)])
+@pytest.mark.parametrize("tokens,top,cols", [(1, 8, 2048), (40, 2, 515), (300, 4, 4096), (9, 3, 33), (500, 3, 100), (333, 2, 7), (70, 5, 255)])
 def test_quantize_into_places(context, kernel, tokens, top, cols):
     rng = np.random.default_rng(cols)
     n = tokens * top + 2

@@ -172,7 +172,9 @@ def held_places(places, columns):
 
 # Widths: shorter than 16 bytes, one unit, overlapping units, several segments.
 SHAPES = [(1, 1, 8), (1, 8, 2048), (5, 2, 1), (7, 3, 3), (16, 2, 64), (9, 5, 1111), (33, 9, 520), (300, 2, 4096), (40, 4, 8199),
-          (2500, 2, 65)]
+          (2500, 2, 65),
+          # Several tokens to a wave, and just not.
+          (1000, 5, 24), (333, 9, 100), (2001, 1, 128), (777, 6, 130), (101, 4, 255), (403, 2, 256), (55, 3, 257)]
 LAYOUTS = [((COL, 0, 0), (COL, 0, 0)), ((COL, 3, 1), (COL, 5, 1)), ((ROW, 0, 0), (COL, 1, 0)), ((COL, 0, 1), (ROW, 2, 0))]
 
 
@@ -404,6 +406,38 @@ def test_long_rows_and_far_columns(context):
     for t in range(3):
         for p in places[t]:
             assert torch.equal(rows[p], x[t])
+
+
+@pytest.mark.parametrize("width", [100, 250, 600])
+def test_many_narrow_tokens(context, width):
+    """More than the caches hold, several tokens to a wave and one. Small whole numbers: every sum is exact."""
+    tokens, top = 100000, 2
+    announce("many narrow tokens", width)
+    g = generator(width)
+    x = torch.randint(-3, 4, (tokens, width), generator=g, device="cuda").to(torch.bfloat16)
+    rows = torch.randint(-3, 4, (tokens * top + 3, width), generator=g, device="cuda").to(torch.bfloat16)
+    weights = torch.randint(-2, 3, (tokens, top), generator=g, device="cuda").float()
+    places = torch.randperm(tokens * top + 3, generator=g, device="cuda")[:tokens * top].reshape(tokens, top).int()
+    routing = api.Routing(tokens, top, 1, None, places)
+    at = places.long()
+
+    def col(t):
+        return api.Matrix({torch.bfloat16: S.BF16, torch.float32: S.F32}[t.dtype], t, api.Layout(t.shape[1], t.shape[0], t.shape[1], COL))
+
+    y, dw, moved, drows = torch.zeros(tokens, width, device="cuda"), torch.zeros_like(weights), torch.full_like(rows, 9), torch.full_like(rows, 9)
+    api.dispatch_tokens(col(x), routing, context, col(moved))
+    api.combine_tokens(col(rows), routing, col(weights), context, col(y))
+    api.combine_tokens_gradients(col(x), col(rows), routing, col(weights), context, col(drows), col(dw))
+    left = torch.ones(tokens * top + 3, dtype=torch.bool, device="cuda")
+    left[at.flatten()] = False
+    assert bool((moved[left] == 9).all()) and bool((drows[left] == 9).all())
+    want = torch.zeros_like(y)
+    for j in range(top):
+        assert torch.equal(moved[at[:, j]], x)
+        assert torch.equal(drows[at[:, j]], weights[:, j:j + 1].bfloat16() * x)
+        want += weights[:, j:j + 1] * rows[at[:, j]].float()
+        assert torch.equal(dw[:, j], (x.float() * rows[at[:, j]].float()).sum(1))
+    assert torch.equal(y, want)
 
 
 def test_the_most_tokens(context):
