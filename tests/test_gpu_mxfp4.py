@@ -634,3 +634,34 @@ def test_replayed_from_a_graph(context, m, n, k):
         step(*own)
         torch.cuda.synchronize()
         assert own[1].abs().sum() > 0 and torch.equal(own[1], recorded[1]), i
+
+
+def test_two_contexts_on_their_own_streams():
+    """Products of two contexts side by side, of every kind of kernel, again and again: always what each is alone."""
+    cases = [((16, 16, 0), 500, 20, 2048), ((64, 64, 0), 500, 300, 1024), ((64, 64, 1), 300, 200, 2080), ((128, 128, 0), 700, 500, 1024),
+             ((128, 128, 1), 700, 500, 1120), ((256, 128, 0), 900, 700, 1024), ((256, 256, 0), 900, 700, 1056), ((256, 256, 0), 4352, 4096, 512)]
+    contexts, streams = [api.Context() for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    for ctx, stream in zip(contexts, streams):
+        ctx.set_stream(stream.cuda_stream)
+        ctx.set_synchronous(False)
+    rng = np.random.default_rng(0)
+    sets = []
+    for tile, m, n, k in cases:
+        lhs, rhs = random_held(rng, m, k), random_held(rng, n, k)
+        sets.append((tile, lhs, rhs, [[torch.full((n, m), -77.0, device="cuda") for _ in range(3)] for _ in contexts], (m, n)))
+    torch.cuda.synchronize()
+    announce("two contexts")
+    for r in range(3):
+        for i in range(len(cases)):
+            for c, ctx in enumerate(contexts):
+                tile, lhs, rhs, out, (m, n) = sets[(i + 3 * c) % len(cases)]  # (other cases side by side)
+                ctx.force_tile(*tile)
+                api.mul_mxfp4(lhs.matrix(), rhs.matrix(), params_of(S.F32), ctx, api.Matrix(S.F32, out[c][r], api.Layout(m, n, m, COL)))
+    torch.cuda.synchronize()
+    for tile, lhs, rhs, out, _ in sets:
+        want = (rhs.values() @ lhs.values().t().contiguous()).float()
+        for c in range(2):
+            for r in range(3):
+                assert torch.equal(out[c][r], want), (tile, c, r)
+    for ctx in contexts:
+        ctx.close()
