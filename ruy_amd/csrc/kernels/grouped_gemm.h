@@ -28,6 +28,7 @@
 
 #include "granule.h"
 #include "grouped_device.h"
+#include "launch_geometry.h"
 
 namespace ruyamd {
 namespace grouped {
@@ -223,12 +224,11 @@ __device__ __forceinline__ int InclusiveSum(int v) {
 // group go in bands of kBand along the N side.
 // (Offsets that run backwards may have every other group take all columns. 64 groups have fewer than 2^31 tiles even so, as a
 // launch has fewer than 2^26 workgroups, and the search ends; their total may wrap round, and tiles are left out then.)
-// at_once: 0, or how many tiles an XCD makes at once. What is left of its share after full rounds of these goes to four
-// workgroups a tile then, where it is a quarter of a round at most (and there are full ones): *quarter is which one this is, or
-// -1 for a whole tile.
+// quarter: null, or where it goes which quarter of the tile this is, -1 for all of it, of tiles of which an XCD makes at_once at a
+// time (XcdPlaceOf).
 constexpr int kBand = 8;
 __device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int columns, int tile_n, int tiles_m,
-                                         TileOf* tile, Range* range, int at_once = 0, int* quarter = nullptr) {
+                                         TileOf* tile, Range* range, int at_once = 1, int* quarter = nullptr) {
   const int lane = threadIdx.x & 63;
   struct Lane {
     int begin, count, tiles;
@@ -247,13 +247,10 @@ __device__ __forceinline__ bool FindTile(const int32_t* offsets, int groups, int
   // (int64_t: tiles of many groups times those of many rows.)
   const int64_t all = int64_t(total) * tiles_m, per_xcd = (all + 7) / 8;
   int64_t place = blockIdx.x >> 3;
-  if (at_once) {
-    const int64_t full = per_xcd / at_once * at_once;
-    *quarter = -1;
-    if (full && place >= full && (per_xcd - full) * 4 <= at_once) {
-      *quarter = static_cast<int>(place - full) & 3;
-      place = full + (place - full) / 4;
-    }
+  if (quarter) {
+    const XcdPlace at = XcdPlaceOf(place, per_xcd, at_once);
+    place = at.tile;
+    *quarter = at.quarter;
   }
   const int64_t t = int64_t(blockIdx.x & 7) * per_xcd + place;
   if (place >= per_xcd || t >= all) return false;

@@ -50,6 +50,30 @@ inline bool TileOffsetsFit(int64_t runs, int64_t pitch, int64_t length) {
   return (runs - 1) * pitch + length <= int64_t(1) << 31;
 }
 
+// Tiles dealt to the eight XCDs, each of which makes so many at once (where it has no CU of its own, one): what is left of an XCD's
+// share after full rounds of these goes to four workgroups a tile where it is a quarter of a round at most. The host's
+// count of workgroups and the device's search go by these, whatever the number of CUs.
+constexpr int TilesAtOnce(int compute_units) { return compute_units < 8 ? 1 : compute_units / 8; }
+
+// What workgroup number `place` of an XCD that has `tiles` tiles makes: tile number `tile` of these (`tiles` and more: none), or
+// one quarter of it (-1: all of it).
+struct XcdPlace {
+  int64_t tile;
+  int quarter;
+};
+constexpr XcdPlace XcdPlaceOf(int64_t place, int64_t tiles, int at_once) {
+  const int64_t full = tiles / at_once * at_once;
+  if (!full || place < full || (tiles - full) * 4 > at_once) return {place, -1};
+  return {full + (place - full) / 4, static_cast<int>((place - full) & 3)};
+}
+
+// Workgroups that an XCD with `tiles` tiles (or_fewer: or any number below) needs at most.
+constexpr int64_t XcdWorkgroups(int64_t tiles, int at_once, bool or_fewer) {
+  if (tiles < at_once) return tiles;
+  const int64_t rest = tiles % at_once;
+  return tiles + 3 * (or_fewer ? at_once / 4 : rest * 4 <= at_once ? rest : 0);
+}
+
 }  // namespace ruyamd
 
 #endif  // RUY_AMD_CSRC_KERNELS_LAUNCH_GEOMETRY_H_

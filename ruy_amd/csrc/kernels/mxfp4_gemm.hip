@@ -131,9 +131,9 @@ Choice Choose(const MulCall& call) {
     const int64_t tiles_m = (int64_t(call.m) + t.m - 1) / t.m;
     const int64_t tiles = call.offsets ? tiles_m * (call.n / t.n + busy) : tiles_m * ((int64_t(call.n) + t.n - 1) / t.n);
     // (Of the largest tiles three more workgroups for each that may go to quarters.)
-    const int64_t at_once = std::max(1, call.compute_units / 8), each_xcd = (tiles + 7) / 8, rest = each_xcd % at_once;
-    if (t.tile != Tile::k256x256 || each_xcd < at_once) return each_xcd * 8;
-    return (each_xcd + (call.offsets ? at_once / 4 * 3 : rest * 4 <= at_once ? rest * 3 : 0)) * 8;
+    const int64_t each_xcd = (tiles + 7) / 8;
+    if (t.tile != Tile::k256x256) return each_xcd * 8;
+    return XcdWorkgroups(each_xcd, TilesAtOnce(call.compute_units), call.offsets != nullptr) * 8;
   };
   const auto usable = [&](const TileCost& t) { return timing_of(t).step != 0 && LaunchFits(blocks_of(t), kThreads); };
   const auto forced = [&](const TileCost& t) {

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256, 1) void MxFp4LargeKernel(MulCall c) {
   TileOf tile;
   Range range;
   int quarter;
-  if (!FindTile(c.offsets, c.groups, c.n, kTile, tiles_m, &tile, &range, c.compute_units / 8, &quarter)) return;
+  if (!FindTile(c.offsets, c.groups, c.n, kTile, tiles_m, &tile, &range, TilesAtOnce(c.compute_units), &quarter)) return;
   if (quarter >= 0) {
     tile.m = 2 * tile.m + (quarter & 1);
     tile.n = 2 * tile.n + (quarter >> 1);
