@@ -14,6 +14,7 @@ import pytest
 
 import test_gpu_mxfp4 as products
 import test_gpu_routing as routing
+import test_gpu_sort_launches as sort_tests
 from ruy_amd import _structs as S
 from ruy_amd import build
 
@@ -62,6 +63,13 @@ def test_both_ways_of_sorting_are_tested(launched):
     assert taken == [3 if s in routing.SORTS[-6:] else 1 for s in shapes]
     # With empty experts, of two contexts at once, and of many choices.
     assert sort_launches(launched, [(50, 2, 8), (20000, 8, 128), (9001, 7, 1000), (200000, 1, 4), (1 << 20, 2, 64)]) == [1, 3, 3, 3, 3]
+
+
+def test_sorts_in_three_launches_are_recorded(launched):
+    assert set(sort_launches(launched, sort_tests.THREE_LAUNCHES)) == {3}
+    marks = [m for m in sort_tests.test_many_experts_and_the_line_between_one_launch_and_three.pytestmark if m.name == "parametrize"]
+    shapes = next(m.args[1] for m in marks if "tokens" in m.args[0])
+    assert sort_launches(launched, shapes) == [1 if c > 16384 or (t, p, c) == (49152, 1, 4) else 3 for t, p, c in shapes]
 
 
 # ---- Products of 4-bit floats ----
