@@ -417,7 +417,8 @@ class Context:
         return ms.value, n.value
 
     def mfma_ceiling(self, instruction, operands_from_lds, random_operands, settle_ms=100.0):
-        """(TOP/s, ms per launch) of the bare int8 matrix-instruction loop."""
+        """(TOP/s, ms per launch) of a bare loop of matrix instructions (0 to 2:
+        int8, 3: 4-bit floats)."""
         tops, ms = C.c_double(0), C.c_double(0)
         self._check(lib.ruyamd_diag_mfma_ceiling(self._h, instruction, int(operands_from_lds),
                                                  int(random_operands), float(settle_ms),

@@ -1,5 +1,5 @@
-// ruyamd_diag_mfma_ceiling: measures what the int8 matrix instructions sustain
-// on this card with nothing else running (see kernels/diag.hip).
+// ruyamd_diag_mfma_ceiling: measures what the int8 and the 4-bit floating-point
+// matrix instructions sustain on this card with nothing else running (see kernels/diag.hip).
 // ruyamd_diag_tile_for: which tile the tiled kernels run a shape on.
 #include <chrono>
 #include <cstdint>
@@ -19,7 +19,7 @@ extern "C" int ruyamd_diag_mfma_ceiling(ruyamd_ctx* ctx, int instruction, int op
     ctx->last_error = msg;
     return code;
   };
-  if (!tera_ops_per_second || !ms_per_launch || instruction < 0 || instruction > 2 || settle_ms < 0)
+  if (!tera_ops_per_second || !ms_per_launch || instruction < 0 || instruction > 3 || settle_ms < 0)
     return fail(RUYAMD_E_INVALID, "bad argument");
   if (hipSetDevice(ctx->device) != hipSuccess) return fail(RUYAMD_E_HIP, "hipSetDevice failed");
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -72,7 +72,7 @@ extern "C" int ruyamd_diag_mfma_ceiling(ruyamd_ctx* ctx, int instruction, int op
   if (!ok || ms <= 0) return fail(RUYAMD_E_HIP, "timing the launches failed");
   *ms_per_launch = double(ms) / kTimedLaunches;
   *tera_ops_per_second =
-      kMfmaCeilingOpsPerWorkgroupIteration * kIterations * workgroups / (*ms_per_launch * 1e-3) / 1e12;
+      MfmaCeilingOpsPerWorkgroupIteration(instruction) * kIterations * workgroups / (*ms_per_launch * 1e-3) / 1e12;
   return RUYAMD_OK;
 }
 

@@ -1,4 +1,4 @@
-// Diagnostic kernels: what the int8 matrix cores sustain when nothing but
+// Diagnostic kernels: what the matrix cores sustain on int8 and on 4-bit floats when nothing but
 // matrix instructions (and, optionally, the LDS fragment reads that feed them)
 // is running. The tiled GEMM replaces the inner loop of
 // ruy/kernel_avx512.cc:251-317; this measures the ceiling that loop can reach
@@ -12,7 +12,8 @@
 //   instruction 1: 2 x (8 + 8 fragments), 64 pairs of v_mfma_i32_16x16x64_i8
 //     (the two depth halves of a block back to back on its accumulator)
 //   instruction 2: the same 128 instructions, one depth half after the other
-// i.e. 2 * 128^3 operations per wave and iteration in both forms, and the same
+//   instruction 3: as 1, v_mfma_scale_f32_16x16x128_f8f6f4 on 4-bit floats: twice the depth
+// i.e. 2 * 128^3 operations per wave and iteration in all forms, twice that in the last, and the same
 // 32 KiB of fragment bytes.
 #include <hip/hip_runtime.h>
 
@@ -25,6 +26,21 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 constexpr int kLdsBytes = 64 * 1024;
+
+// acc += a b of 16 rows by 16 columns, one half of an iteration's depth. (scales: of both operands, a byte to either half.)
+template <int kInstruction, int kHalf>
+__device__ __forceinline__ void Mma16(const v4i& a, const v4i& b, int scales, v4i& acc) {
+  if constexpr (kInstruction != 3)
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  else if constexpr (kHalf == 0)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %3 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                 : "+a"(acc)
+                 : "v"(a), "v"(b), "v"(scales));
+  else
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %3 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                 : "+a"(acc)
+                 : "v"(a), "v"(b), "v"(scales));
+}
 
 template <int kInstruction, bool kFromLds>
 __global__ __launch_bounds__(256) void MfmaCeilingKernel(const v4i* operands, int* sink, int iterations) {
@@ -87,6 +103,7 @@ __global__ __launch_bounds__(256) void MfmaCeilingKernel(const v4i* operands, in
     // one that costs the least power of those tried (on random bytes 5 % faster
     // than one depth half after the other).
     v4i a[2][8], b[2][8];
+    const int scales = 0x7f7f7f7f + 0x01010101 * (threadIdx.x & 1);  // (1 and 2 in turn)
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -106,14 +123,14 @@ __global__ __launch_bounds__(256) void MfmaCeilingKernel(const v4i* operands, in
       }
       // Accumulator tied to itself: with the builtin the compiler moves these
       // small accumulators between registers inside the loop.
-      if constexpr (kInstruction == 1) {
+      if constexpr (kInstruction != 2) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
           for (int ii = 0; ii < 8; ++ii) {
             const int i = (j & 1) ? 7 - ii : ii;
-            asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c[i][j]) : "v"(a[0][i]), "v"(b[0][j]));
-            asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c[i][j]) : "v"(a[1][i]), "v"(b[1][j]));
+            Mma16<kInstruction, 0>(a[0][i], b[0][j], scales, c[i][j]);
+            Mma16<kInstruction, 1>(a[1][i], b[1][j], scales, c[i][j]);
           }
       } else {
         // For comparison: one depth half after the other, every instruction
@@ -125,7 +142,7 @@ __global__ __launch_bounds__(256) void MfmaCeilingKernel(const v4i* operands, in
 #pragma unroll
             for (int ii = 0; ii < 8; ++ii) {
               const int i = (j & 1) ? 7 - ii : ii;
-              asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c[i][j]) : "v"(a[ks][i]), "v"(b[ks][j]));
+              Mma16<kInstruction, 0>(a[ks][i], b[ks][j], scales, c[i][j]);
             }
       }
       if constexpr (kFromLds) __syncthreads();
@@ -165,6 +182,9 @@ hipError_t LaunchMfmaCeiling(hipStream_t stream, int instruction, bool from_lds,
   if (instruction == 2)
     return from_lds ? LaunchOne<2, true>(stream, operands, sink, iterations, workgroups)
                     : LaunchOne<2, false>(stream, operands, sink, iterations, workgroups);
+  if (instruction == 3)
+    return from_lds ? LaunchOne<3, true>(stream, operands, sink, iterations, workgroups)
+                    : LaunchOne<3, false>(stream, operands, sink, iterations, workgroups);
   return hipErrorInvalidValue;
 }
 
