@@ -426,11 +426,14 @@ RUYAMD_API int ruyamd_dequantize_mxfp4(ruyamd_ctx* ctx,
  * NULL) the columns of dst, and with them the rows of rhs, are dealt to groups, each with
  * an lhs of its own, as in ruyamd_mul_grouped (whose matrix_stride is not looked
  * at here: lhs says where its matrices lie; rhs's are not looked at). dst: fp32, bfloat16 or half,
- * any order. A block's sum of products is exact; sums of blocks are fp32, in
+ * any order. A block's sum of products is exact (and has to stay in the range of fp32: an infinity or
+ * a NaN comes of those that do not); sums of blocks are fp32, in
  * which those below 2^-126 may be lost; the result is rounded once. Parameters,
  * memory and calls as in ruyamd_mul_grouped. Depths below 32 go to a kernel of one element to
  * a lane; rows that do not begin at multiples of 4 bytes, or are no whole number of blocks, cost
- * up to twice as much where columns are many. */
+ * up to twice as much where columns are many, and so does dst by rows, or nearly three times where the depth
+ * is small too (without groups and a bias, the product with lhs
+ * and rhs exchanged has the same dst by columns). */
 RUYAMD_API int ruyamd_mul_mxfp4(ruyamd_ctx* ctx, const ruyamd_mxfp4_mat* lhs,
                                 const ruyamd_mxfp4_mat* rhs,
                                 const ruyamd_groups* groups,

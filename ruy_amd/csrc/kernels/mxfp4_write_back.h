@@ -139,7 +139,9 @@ struct WriteBack {
     }
   }
 
-  // Anything else: value by value, out of LDS in a loop; lanes along the columns, which is how dst by rows lies.
+  // Anything else: value by value, out of LDS in a loop; lanes along the columns, which is how dst by rows lies. (us, bfloat16 by columns and
+  // by rows: 8192 x 8192 x 512 48 and 129, 4096 x 4096 x 4096 38 and 76, 8192 x 8192 x 8192 275 and 398; fp32 by columns, 4096 rows 43 and
+  // 4000, whose last tile is cut short, 59.)
   __device__ __forceinline__ void Each() const {
     constexpr int kBlocks = kColumns32 / 16;
     const float* const held = reinterpret_cast<const float*>(lds);
