@@ -54,7 +54,7 @@ struct MulCall {
   float clamp_min = 0, clamp_max = 0;
   int compute_units = 0;
   int forced_tile_rows = 0, forced_tile_cols = 0;  // 0: the fastest one
-  bool forced_deep = false;                        // of 64x64, the one with four stages
+  bool forced_deep = false;                        // of 64x64 and 128x128, those with four stages
 };
 // As in grouped.h.
 hipError_t LaunchGeneric(hipStream_t stream, const MulCall& call);

@@ -7,10 +7,11 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 cycles with 4-bit values on both sides, so a wave's step of 64x64 is 512 cycles of products, of 16 KB
 // out of LDS (a CU's four waves 512 cycles) and of 8 KB into it; a tile waits for what is not done beside its products. Few
-// tiles: four stages, and one workgroup to a CU (2048 x 2048 x 8192: 128x128 25.5 us, 2.7 PFLOP/s; with two stages 29.8). Many:
-// two workgroups of 128x128 to a CU, one of which multiplies while the other waits (2048 x 4096 x 4096 25.7 us, with
-// four stages 30.3), of 256x128 (mxfp4_wide.hip; 16384 x 3300 x 512 35.0 us, 128x128 49.5), or 256x256, which read half as much for a
-// product (4096 x 4096 x 4096 38.4 us, 128x128 50).
+// tiles: four stages, and one workgroup to a CU (2048 x 2048 x 8192: 128x128 26 to 28 us, 2.4 to 2.6 PFLOP/s; with two stages 30.5; the
+// matrix cores are busy in a third of a deeper product's cycles, and waves wait in 29 %). Many:
+// two workgroups of 128x128 to a CU, one of which multiplies while the other waits (2048 x 4096 x 4096, forced, 25.0 us, with
+// four stages 29.5), of 256x128 (mxfp4_wide.hip; 16384 x 3300 x 512 35.0 us, 128x128 49.5), or 256x256, which read half as much for a
+// product (4096 x 4096 x 4096 37.3 us, 128x128 46).
 #include "launch_geometry.h"
 #include "mxfp4_large.h"
 #include "mxfp4_tile.h"
@@ -41,7 +42,8 @@ bool IsDeep(Tile t) { return t == Tile::k64x64Deep || t == Tile::k128x128Deep; }
 // `last` of a full one, fixed + rounds * (steps + more) * step, a step being 256 positions of depth; a quarter of a round or less
 // of 256x256 tiles behind full ones, which is made in quarters, (steps + kQuarters.more) * kQuarters.step. Fitted to 551 shapes of 256 to
 // 16384 rows, 48 to 8192 columns and depths of 512 to 8192, bfloat16 destinations, to 5 to 10 % root mean square. Choosing by it
-// costs 0.9 % over the fastest kernel at each of these shapes (16 % at the worst, 256 x 6000, depth 4096: 12.0 us for 10.4).
+// costs 0.9 % over the fastest kernel at each of these shapes (16 % at the worst, 256 x 6000, depth 4096: 12.0 us for 10.4). Of sizes
+// that are not among them, 2048 x 4096 x 4096 goes to 256x128 and takes 29.5 us for the 25.0 of 128x128.
 struct Timing {
   int per_cu;
   float fixed, step, more, last;

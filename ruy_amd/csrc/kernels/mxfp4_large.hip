@@ -20,11 +20,13 @@
 // (mxfp4_tile.h, four stages): 4352 x 4096 x 2048, 272 tiles, 38.3 -> 33 us; 5120 x 4096 x 8192, 320 tiles, 104 -> 87. Of half a round two rounds of
 // quarters take longer than one of whole tiles (6144 x 4096 x 2048 44.5 us and 38.9).
 //
-// 8192 x 8192 x 8192: 240 to 252 us (from card to card), 4.4 to 4.6 PFLOP/s; a loop of these instructions alone, on random
-// values in registers, makes 7.1 and on zeros 9.7. What bounds it is the power that the card may take: over a deep
-// product (4096 x 4096 x 32768, 5.0 PFLOP/s) it runs at 1.68 of its 2.4 GHz, the matrix cores are busy in 68 % of the cycles, and
-// LDS has bank conflicts in 17 % of its own. A tile's first loads and its write-back take as long as 5.8 steps of 256 (kTiles in mxfp4_gemm.hip), which is
-// what bounds shallow products: 8 experts of 4096 x 2048 and 8192 tokens, 8 steps to a tile, 56 us, 2.5 PFLOP/s.
+// 8192 x 8192 x 8192: 238 to 257 us on most cards, 4.3 to 4.6 PFLOP/s (285 on one, of uniformly random bytes); a loop of these instructions
+// alone (ruyamd_diag_mfma_ceiling), on random values in registers, makes 7.7 to 7.8 and on zeros 9.7. What bounds it is the power that the
+// card may take: it runs at 1.9 of its 2.4 GHz with the matrix cores busy in 57 % of the cycles, over a deeper
+// product (4096 x 4096 x 32768, 5.1 PFLOP/s) at 1.7 to 1.8 with 66 to 68 %; LDS has bank conflicts in 17 % of its own cycles. What a tile
+// costs beside its steps of 256 (`more` in kTiles, mxfp4_gemm.hip: its first loads and its write-back) bounds shallow products: 8 experts of
+// 4096 x 2048 and 8192 tokens, 8 steps to a tile, 62 us where expert i has a share of (i + 1) ^ -0.5, 2.2 PFLOP/s at 2.4 GHz with the matrix
+// cores busy in 24 % of the cycles; 53 where all have one share, which leaves no part of a round.
 #include "mxfp4_large.h"
 #include "mxfp4_tile.h"
 #include "paired_schedule.h"

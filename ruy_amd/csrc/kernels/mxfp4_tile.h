@@ -4,7 +4,8 @@
 // Products, LDS reads and loads stand in the order in which they are issued: behind each product what there is of the
 // others, so that neither the matrix core nor the address unit waits for the end of a run of the other's. (Left to the compiler, products
 // sank behind the barrier: 2048 x 2048 x 8192 on 128x128, four stages 29.0 -> 25.2 us, two 34.9 -> 29.8.) A step of four stages still
-// takes 0.65 us at 2.2 GHz, in which the matrix cores are busy for a third; loads spread over both halves of a step gained nothing.
+// takes 0.65 us at 2.15 GHz, in which the matrix cores are busy for a third (four waves of 64x64 read every fragment out of LDS twice, and
+// wait for each other in every step); loads spread over both halves of a step gained nothing.
 #ifndef RUY_AMD_CSRC_KERNELS_MXFP4_TILE_H_
 #define RUY_AMD_CSRC_KERNELS_MXFP4_TILE_H_
 
@@ -91,7 +92,7 @@ constexpr int kStep = 8 * kBlock;  // depth positions to a step: 128 bytes
 // kDirect: rows of both sides begin at multiples of 4 bytes, which is what a load to LDS asks of an address, and are whole blocks, so
 // that tiles go to LDS without passing through registers. (8192 x 8192 x 8192, rows 4100 bytes apart: 263 us, through registers
 // 406; 4096 and 4112 apart 245 and 260.) Otherwise rows are read 16 bytes a lane from wherever they begin: 8192 x 8192 x
-// 8192, rows 4097 bytes apart 496 us. (Reading the five words that hold 16 bytes and shifting them takes 503, and 8 % longer at
+// 8192, rows 4097 bytes apart 496 to 580 us from card to card. (Reading the five words that hold 16 bytes and shifting them takes 503, and 8 % longer at
 // 4096 x 4096 x 4096.)
 // kStages: steps on their way to LDS (kDirect), two or four.
 // How scales come to LDS. Through registers, a pair of steps ahead: the waves wait for these loads, and for those of all steps with

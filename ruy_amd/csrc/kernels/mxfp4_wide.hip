@@ -7,7 +7,8 @@
 //
 // Scales are in LDS as they lie, 16 bytes of a row to four steps; a lane reads those of its rows and takes its column of the four words.
 //
-// 5120 x 8192 x 512: 27.0 us (256x256 and 128x128 35.6); 16384 x 8192 x 1024 104 (123 and 144); 8192 x 8192 x 2048 83.6 (80.5 and 90.9); 4096 x 4096
+// 5120 x 8192 x 512: 27.3 us (256x256 34.2, 128x128 33.2); 16384 x 8192 x 1024 104 to 115 (118 to 123 and 134 to 144; three calls in turn, whose
+// destinations of 268 MB no cache holds, 132 to 137); 8192 x 8192 x 2048 83.6 (80.5 and 90.9); 4096 x 4096
 // x 32768, where nothing but the steps counts, 296 (207 and 290). Its loads, of half a line of 16 rows each, take a CU longer than those of a line of
 // 8: without them the last one is 231.
 #include "mxfp4_large.h"

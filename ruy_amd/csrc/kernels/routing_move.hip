@@ -501,7 +501,7 @@ void WithUnits(const Call& c, int type, int compute_units, F&& f) {
   f(std::integral_constant<int, 1>(), int(segments(1)), blocks(segments(1)));
 }
 
-// Bytes written from which on they go past the caches: 32 MiB, which is what all L2s hold. (us, tokens of 4096 values in bfloat16 and two
+// Bytes written from which on they go past the caches: 32 MiB, which is what all L2s hold. (Rows that are whole lines; us, tokens of 4096 values in bfloat16 and two
 // places each, 17, 34, 67 and 134 MB dispatched: 6.7 10.1 24.3 41.8, past them 5.5 9.0 16.7 32.7; combined, 8, 17, 34 and 67 MB: 6.4 9.6 22.8
 // 41.5, past them 5.9 9.6 17.3 37.9; combined and dispatched again, 2048 tokens 18.8 and 21.0, 4096 44.7 and 40.0.)
 constexpr int64_t kStreamFrom = int64_t(1) << 25;
