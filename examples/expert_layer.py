@@ -44,17 +44,22 @@ def params(dtype, bias=None, relu=False):
     return p
 
 
+def on_current_stream(contexts):
+    """The one of `contexts`, which go by their streams, whose calls are enqueued on torch's current stream, without waiting."""
+    stream = torch.cuda.current_stream().cuda_stream
+    if stream not in contexts:
+        contexts[stream] = api.Context()
+        contexts[stream].set_stream(stream)
+        contexts[stream].set_synchronous(False)
+    return contexts[stream]
+
+
 _contexts = {}
 
 
 def shared_context():
-    """The context of calls that belong to no layer: on torch's current stream, without waiting."""
-    stream = torch.cuda.current_stream().cuda_stream
-    if stream not in _contexts:
-        _contexts[stream] = api.Context()
-        _contexts[stream].set_stream(stream)
-        _contexts[stream].set_synchronous(False)
-    return _contexts[stream]
+    """The context of calls that belong to no layer."""
+    return on_current_stream(_contexts)
 
 
 class Routing:
@@ -115,12 +120,17 @@ class Experts:
         self.w1 = torch.randn(experts, hidden, width, generator=g, device="cuda") * (2.0 / width) ** 0.5
         self.w2 = torch.randn(experts, width, hidden, generator=g, device="cuda") / hidden ** 0.5
         self.b1 = torch.zeros(experts, hidden, device="cuda")
-        self.context = api.Context()
-        self.context.set_stream(torch.cuda.current_stream().cuda_stream)
-        self.context.set_synchronous(False)
+        self._contexts = {}
+
+    @property
+    def context(self):
+        """The context of the layer's products: on torch's current stream, as what torch does between them."""
+        return on_current_stream(self._contexts)
 
     def close(self):
-        self.context.close()
+        for context in self._contexts.values():
+            context.close()
+        self._contexts.clear()
 
     def forward(self, x, routing):
         """The experts' answers, one row to each token and expert it goes to."""
@@ -188,9 +198,13 @@ class Server:
     """The trained experts in 4 bits."""
 
     def __init__(self, trained, group_size=64):
-        self.dtype, self.context, self.b1 = trained.dtype, trained.context, trained.b1
+        self.dtype, self.layer, self.b1 = trained.dtype, trained, trained.b1
         self.w1, self.w1_values = quantize(trained.w1, group_size)
         self.w2, self.w2_values = quantize(trained.w2, group_size)
+
+    @property
+    def context(self):
+        return self.layer.context
 
     def answer(self, x, routing):
         chosen = routing.dispatch(x.to(self.dtype))
@@ -207,9 +221,13 @@ class FloatServer:
     """The trained experts in 4-bit floats with a power of two to every 32, and tokens in the same."""
 
     def __init__(self, trained):
-        self.dtype, self.context, self.b1 = trained.dtype, trained.context, trained.b1
+        self.dtype, self.layer, self.b1 = trained.dtype, trained, trained.b1
         self.experts = trained.w1.shape[0]
         self.w1, self.w2 = self.quantize_weights(trained.w1), self.quantize_weights(trained.w2)
+
+    @property
+    def context(self):
+        return self.layer.context
 
     def empty(self, rows, cols):
         return (torch.empty(rows, (cols + 1) // 2, dtype=torch.uint8, device="cuda"),
