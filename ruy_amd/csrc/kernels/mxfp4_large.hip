@@ -20,7 +20,7 @@
 // (mxfp4_tile.h, four stages): 4352 x 4096 x 2048, 272 tiles, 38.3 -> 33 us; 5120 x 4096 x 8192, 320 tiles, 104 -> 87. Of half a round two rounds of
 // quarters take longer than one of whole tiles (6144 x 4096 x 2048 44.5 us and 38.9).
 //
-// 8192 x 8192 x 8192: 238 to 257 us on most cards, 4.3 to 4.6 PFLOP/s (285 on one, of uniformly random bytes); a loop of these instructions
+// 8192 x 8192 x 8192: 238 to 261 us on most cards, 4.2 to 4.6 PFLOP/s (285 on one, of uniformly random bytes); a loop of these instructions
 // alone (ruyamd_diag_mfma_ceiling), on random values in registers, makes 7.7 to 7.8 and on zeros 9.7. What bounds it is the power that the
 // card may take: it runs at 1.9 of its 2.4 GHz with the matrix cores busy in 57 % of the cycles, over a deeper
 // product (4096 x 4096 x 32768, 5.1 PFLOP/s) at 1.7 to 1.8 with 66 to 68 %; LDS has bank conflicts in 17 % of its own cycles. What a tile
